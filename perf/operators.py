@@ -211,7 +211,7 @@ def _run_qk(s):
         if c["dir"] != "fwd":
             dqkv = torch.empty_like(s["qkv"])
             dq, dk, dv = _split(dict(case=c, qkv=dqkv))
-            g = gn.qk_norm_rope_bwd(s["dq"], s["dk"], q, k, s["wq"], s["wk"], s["f"], dv=s["dv"], out=(dq, dk, dv), **kw)
+            g = gn.qk_norm_rope_bwd(s["dq"], s["dk"], q, k, s["wq"], s["wk"], s["f"], dyv=s["dv"], out=(dq, dk, dv), **kw)
             out["dwq"], out["dwk"], out["dqkv"] = g[-2], g[-1], dqkv
         return out
     cos, sin = _cos_sin(s["pos"], s["f"], 1.0)
