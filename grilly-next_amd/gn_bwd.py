@@ -23,6 +23,7 @@ RMS_STAT = {"rstd": 0, "meansq": RMS_STAT_MEANSQ, "rms": RMS_STAT_RMS}
 ACT = {"relu": 0, "gelu_tanh": 1, "gelu_erf": 2, "silu": 3, "tanh": 4, "sigmoid": 5}
 GLU = {"swiglu_up": 0, "swiglu_gate": 1, "geglu_up": 2, "geglu_gate": 3, "reglu_up": 4}
 ROPE = {"none": 0, "interleaved": 1, "half": 2}
+ROPE_SCALE = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 
 # exported symbols, in the order include/gn_bwd.h declares them
 SYMBOLS = [
@@ -40,6 +41,8 @@ SYMBOLS = [
     "gn_vsa_cosine_blend_bwd", "gn_surprise_momentum_step", "gn_linear_bwd_surprise_momentum",
     "gn_adamw_step", "gn_layernorm_fwd",
     "gn_rmsnorm_fwd", "gn_layernorm_fwd_ex", "gn_rmsnorm_fwd_ex", "gn_rmsnorm_fwd_stat", "gn_act_fwd", "gn_glu_fwd", "gn_linear_fwd", "gn_glu_linear_fwd", "gn_add_inplace", "gn_convert", "gn_zero",
+    "gn_linear_xent_fwd", "gn_linear_xent_bwd", "gn_linear_xent_workspace_bytes", "gn_rope_freqs", "gn_rope_fwd",
+    "gn_rope_bwd", "gn_qk_norm_rope_fwd", "gn_qk_norm_rope_bwd", "gn_qk_norm_rope_workspace_bytes",
 ]
 BIN = {"sub": 0, "mul": 1, "div": 2, "neg": 3}
 RED = {"sum": 0, "mean": 1}
@@ -66,6 +69,24 @@ class OptParam(ctypes.Structure):
 
 
 _OPTP = ctypes.POINTER(OptParam)
+
+
+class Heads(ctypes.Structure):
+    """gn_heads (include/gn_bwd.h): a [B, S, H, D] view, strides in elements."""
+    _fields_ = [("p", ctypes.c_void_p), ("sb", ctypes.c_int64), ("ss", ctypes.c_int64),
+                ("sh", ctypes.c_int64), ("H", ctypes.c_int)]
+
+
+class Rope(ctypes.Structure):
+    """gn_rope (include/gn_bwd.h): a rotation by position."""
+    _fields_ = [("freqs", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("pos_sb", ctypes.c_int64),
+                ("pos0", ctypes.c_int64), ("mscale", ctypes.c_float), ("rot", ctypes.c_int),
+                ("mode", ctypes.c_int)]
+
+
+_HEADSP = ctypes.POINTER(Heads)
+_ROPEP = ctypes.POINTER(Rope)
+_D = ctypes.c_double
 
 _SIGS = {
     "gn_last_error": ([], ctypes.c_char_p),
@@ -143,6 +164,17 @@ _SIGS = {
     "gn_linear_fwd": ([_P, _P, _P, _P, _I, _I, _I, _I, _P], _I),
     "gn_glu_linear_fwd": ([_I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P], _I),
     "gn_add_inplace": ([_P, _P, _L, _I, _P], _I),
+    "gn_linear_xent_fwd": ([_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _Z, _P], _I),
+    "gn_linear_xent_bwd": ([_P, _P, _P, _P, _P, _P, _F, _P, _P, _I, _I, _I, _I, _I, _U, _P, _Z, _P], _I),
+    "gn_linear_xent_workspace_bytes": ([_I, _I, _I, _I], _Z),
+    "gn_rope_freqs": ([_I, _D, _I, _D, _D, _D, _D, _P, ctypes.POINTER(_F)], _I),
+    "gn_rope_fwd": ([_HEADSP, _HEADSP, _ROPEP, _I, _I, _I, _I, _P], _I),
+    "gn_rope_bwd": ([_HEADSP, _HEADSP, _ROPEP, _I, _I, _I, _I, _P], _I),
+    "gn_qk_norm_rope_fwd": ([_HEADSP, _HEADSP, _HEADSP, _P, _P, _HEADSP, _HEADSP, _HEADSP, _ROPEP, _I, _I, _I, _F,
+                             _I, _P], _I),
+    "gn_qk_norm_rope_bwd": ([_HEADSP, _HEADSP, _HEADSP, _HEADSP, _HEADSP, _P, _P, _HEADSP, _HEADSP, _HEADSP, _P, _P,
+                             _ROPEP, _I, _I, _I, _F, _I, _U, _P, _Z, _P], _I),
+    "gn_qk_norm_rope_workspace_bytes": ([_I, _I, _I], _Z),
 }
 
 
@@ -815,6 +847,224 @@ def glu_linear_fwd(kind, X, Wg, Wu, bg=None, bu=None):
                                    _ptr(gate), _ptr(up), _ptr(out), M, H, K, _dt(X), _stream()),
            "gn_glu_linear_fwd")
     return gate, up, out
+
+
+# ---- linear head with cross entropy, without its logits -----------------------------------
+def _here(name, t, dtype=None, shape=None):
+    """Device address of an argument, or None: contiguous, on the current device (whose stream the
+    call goes to), of the dtype and shape that the call needs."""
+    if t is None:
+        return None
+    p = _ptr(t)
+    if t.device.index != torch._C._cuda_getDevice():
+        raise GnError(f"{name} is on {t.device}, not on the current device")
+    if dtype is not None and t.dtype != dtype:
+        raise GnError(f"{name} must be {dtype}, not {t.dtype}")
+    if shape is not None and t.shape != shape:
+        raise GnError(f"{name} must be {list(shape)}, not {list(t.shape)}")
+    return p
+
+
+def linear_xent_workspace_bytes(T, d, V, dtype):
+    return int(lib().gn_linear_xent_workspace_bytes(T, d, V, dtype))
+
+
+def _xent_args(h, E, targets, ws):
+    if h.dim() != 2 or E.dim() != 2 or h.shape[1] != E.shape[1]:
+        raise GnError(f"h [T, d] and E [V, d] expected, not {list(h.shape)} and {list(E.shape)}")
+    (T, d), V, dt = h.shape, E.shape[0], _dt(h)
+    args = (_here("h", h), _here("E", E, h.dtype), _here("targets", targets, torch.int32, (T,)))
+    if ws is None:
+        ws = workspace(linear_xent_workspace_bytes(T, d, V, dt), h.device)
+    return args, T, d, V, dt, ws  # the caller holds ws until its kernels are enqueued
+
+
+def linear_xent_fwd(h, E, targets, ws=None):
+    """(loss, lse), fp32 [T], of logits h E^T that are never stored: h [T, d], E [V, d] (f32 or
+    bf16), targets int32 [T]; a target outside [0, V) (-100, say) marks a row without one, whose
+    loss is 0.  ws: linear_xent_workspace_bytes(T, d, V, dtype), allocated here when None."""
+    args, T, d, V, dt, ws = _xent_args(h, E, targets, ws)
+    loss = torch.empty((T,), dtype=torch.float32, device=h.device)
+    lse = torch.empty((T,), dtype=torch.float32, device=h.device)
+    _check(lib().gn_linear_xent_fwd(*args, _ptr(loss), _ptr(lse), T, d, V, dt, _here("ws", ws),
+                                    ws.numel() * ws.element_size(), _stream()),
+           "gn_linear_xent_fwd")
+    return loss, lse
+
+
+def linear_xent_bwd(h, E, targets, lse, dloss=None, dlse=None, scale=1.0, need_dh=True, need_dE=True,
+                    dE=None, dE_dtype=torch.float32, accumulate=False, ws=None):
+    """(dh, dE) of linear_xent_fwd from its lse: upstream gradients dloss, dlse (fp32 [T], None: 1
+    and 0) times scale.  dh in h's dtype; dE fp32, or bf16 under bf16 inputs (dE_dtype, or dE's own
+    when it is given); accumulate adds onto a given fp32 dE."""
+    args, T, d, V, dt, ws = _xent_args(h, E, targets, ws)
+    f32 = torch.float32
+    dh = torch.empty_like(h) if need_dh else None
+    if need_dE and dE is None:
+        if accumulate:
+            raise GnError("accumulate needs the dE to add onto")
+        dE = torch.empty((V, d), dtype=dE_dtype, device=h.device)
+    dE = dE if need_dE else None
+    _check(lib().gn_linear_xent_bwd(*args, _here("lse", lse, f32, (T,)), _here("dloss", dloss, f32, (T,)),
+                                    _here("dlse", dlse, f32, (T,)), scale, _ptr(dh),
+                                    _here("dE", dE, None, (V, d)), F32 if dE is None else _dt(dE), T, d, V, dt,
+                                    ACCUMULATE if accumulate else 0, _here("ws", ws),
+                                    ws.numel() * ws.element_size(), _stream()), "gn_linear_xent_bwd")
+    return dh, dE
+
+
+# ---- rotary positions, per-head norms of queries and keys ---------------------------------
+def rope_freqs(rot, theta=10000.0, scaling="none", factor=1.0, trained=4096, fast=32.0, slow=1.0, device="cuda:0"):
+    """(freqs, mscale) for rope_fwd and qk_norm_rope_fwd: an fp64 tensor [rot / 2] of radians per
+    position, kept by the caller, and the factor on cos and sin.  scaling stretches a context of
+    `trained` positions `factor` times: "linear", "ntk" or "yarn" (with its fast and slow bounds)."""
+    f = (ctypes.c_double * max(1, rot // 2))()
+    m = ctypes.c_float()
+    _check(lib().gn_rope_freqs(rot, theta, ROPE_SCALE[scaling], factor, trained, fast, slow,
+                               ctypes.cast(f, _P), ctypes.byref(m)), "gn_rope_freqs")
+    return torch.tensor(list(f)[:rot // 2], dtype=torch.float64).to(device), m.value
+
+
+def _heads(name, t, shape=None, dtype=None, first=False):
+    """gn_heads of a [B, S, H, D] tensor ([B, H, S, D] when first) whose last dimension is
+    contiguous; other strides are free."""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise GnError(f"{name} is not on the GPU")
+    if t.device.index != torch._C._cuda_getDevice():
+        raise GnError(f"{name} is on {t.device}, not on the current device")
+    if t.dim() != 4:
+        raise GnError(f"{name} must have four dimensions, not {t.dim()}")
+    if first:
+        t = t.transpose(1, 2)
+    if dtype is not None and t.dtype != dtype:
+        raise GnError(f"{name} must be {dtype}, not {t.dtype}")
+    if shape is not None and t.shape != shape:
+        raise GnError(f"{name} must be {list(shape)} ([B, S, H, D]), not {list(t.shape)}")
+    if t.shape[3] > 1 and t.stride(3) != 1:
+        raise GnError(f"{name}: the elements of a head must be contiguous")
+    return Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2])
+
+
+def _rope(freqs, mode, positions, pos0, mscale, B, S):
+    if freqs is None:
+        return None
+    if freqs.dim() != 1:
+        raise GnError("freqs must have one dimension")
+    r = Rope(_here("freqs", freqs, torch.float64), None, 0, pos0, mscale, 2 * freqs.numel(), ROPE[mode])
+    if positions is not None:
+        r.positions = _here("positions", positions, torch.int32)
+        if positions.shape == (B, S):
+            r.pos_sb = S
+        elif positions.shape != (S,):
+            raise GnError(f"positions must be [{S}] or [{B}, {S}], not {list(positions.shape)}")
+    return r
+
+
+def _empty_heads(shape, like, first):
+    B, S, H, D = shape
+    return torch.empty((B, H, S, D) if first else (B, S, H, D), dtype=like.dtype, device=like.device)
+
+
+def _rope_call(fn, name, x, freqs, mode, positions, pos0, mscale, out):
+    xh = _heads("x", x)
+    B, S, H, D = x.shape
+    y = _empty_heads(x.shape, x, False) if out is None else out
+    r = _rope(freqs, mode, positions, pos0, mscale, B, S)
+    _check(fn(xh, _heads("out", y, x.shape, x.dtype), r, B, S, D, _dt(x), _stream()), name)
+    return y
+
+
+def rope_fwd(x, freqs, mode="half", positions=None, pos0=0, mscale=1.0, out=None):
+    """x [B, S, H, D] rotated by its positions: the first 2 * len(freqs) elements of each head, the
+    rest as they are.  freqs, mscale: rope_freqs.  positions: int32 [S] or [B, S]; None: pos0,
+    pos0 + 1, ...  x and out may be views (heads of fused rows, head-first tensors); out may be x."""
+    return _rope_call(lib().gn_rope_fwd, "gn_rope_fwd", x, freqs, mode, positions, pos0, mscale, out)
+
+
+def rope_bwd(dy, freqs, mode="half", positions=None, pos0=0, mscale=1.0, out=None):
+    """The gradient of rope_fwd's x: dy rotated back, times mscale."""
+    return _rope_call(lib().gn_rope_bwd, "gn_rope_bwd", dy, freqs, mode, positions, pos0, mscale, out)
+
+
+def qk_norm_rope_workspace_bytes(B, S, D):
+    return int(lib().gn_qk_norm_rope_workspace_bytes(B, S, D))
+
+
+def _qk(q, k, wq, wk):
+    """The shapes and checked views of q and k, and the weights."""
+    qh = _heads("q", q)
+    B, S, _, D = q.shape
+    ks = None if k is None else (B, S, k.shape[2] if k.dim() == 4 else 0, D)
+    kh = _heads("k", k, ks, q.dtype)
+    w = (_here("wq", wq, q.dtype, (D,)), _here("wk", wk, q.dtype, (D,)))
+    return B, S, D, tuple(q.shape), ks, qh, kh, w
+
+
+def qk_norm_rope_fwd(q, k, wq=None, wk=None, freqs=None, v=None, mode="half", positions=None, pos0=0, mscale=1.0,
+                     eps=1e-6, heads_first=False, out=None):
+    """(yq, yk), or (yq, yk, yv) when v is given: q and k [B, S, H, D] (views; k may have fewer heads,
+    or be None) normed per head, y = x rsqrt(mean(x^2) + eps) w, and rotated as by rope_fwd (freqs None: not);
+    v copied.  heads_first: the outputs are [B, H, S, D], as attn_fwd takes them; `out` gives them."""
+    B, S, D, qs, ks, qh, kh, w = _qk(q, k, wq, wk)
+    vh = _heads("v", v, None if v is None or k is None else ks, q.dtype)
+    vs = None if v is None else tuple(v.shape)
+    if v is not None and (vs[0], vs[1], vs[3]) != (B, S, D):
+        raise GnError(f"v must be [{B}, {S}, H, {D}], not {list(vs)}")
+    r = _rope(freqs, mode, positions, pos0, mscale, B, S)
+    if out is None:
+        out = tuple(None if s is None else _empty_heads(s, q, heads_first) for s in (qs, ks, vs))
+    out = tuple(out) + (None,) * (3 - len(out))
+    for name, o, s in (("yk", out[1], ks), ("yv", out[2], vs)):
+        if (o is None) != (s is None):
+            raise GnError(f"out: {name} goes with its input")
+    yh = [_heads(n, o, s, q.dtype, heads_first) for n, o, s in zip(("yq", "yk", "yv"), out, (qs, ks, vs))]
+    _check(lib().gn_qk_norm_rope_fwd(qh, kh, vh, *w, *yh, r, B, S, D, eps, _dt(q), _stream()), "gn_qk_norm_rope_fwd")
+    return out if v is not None else out[:2]
+
+
+def qk_norm_rope_bwd(dyq, dyk, q, k, wq=None, wk=None, freqs=None, dyv=None, mode="half", positions=None, pos0=0,
+                     mscale=1.0, eps=1e-6, heads_first=False, out=None, need_dw=True, dwq=None, dwk=None,
+                     accumulate=False, ws=None):
+    """(dq, dk, dv, dwq, dwk) of qk_norm_rope_fwd from its inputs q, k and the gradients dyq, dyk, dyv of its outputs
+    (heads_first: [B, H, S, D]).  dq, dk, dv [B, S, H, D], or the views in `out` (the parts of a fused
+    dqkv, say); dv is None without dyv.  dwq, dwk fp32 [D]; accumulate adds onto given ones; need_dw
+    False: neither."""
+    B, S, D, qs, ks, qh, kh, w = _qk(q, k, wq, wk)
+    if (k is None) != (dyk is None):
+        raise GnError("dyk goes with k")
+    vs = None
+    if dyv is not None:
+        if dyv.dim() != 4:
+            raise GnError(f"dyv must have four dimensions, not {dyv.dim()}")
+        vs = (B, S, dyv.shape[1 if heads_first else 2], D)
+    dyh = [_heads(n, t, s, q.dtype, heads_first) for n, t, s in (("dyq", dyq, qs), ("dyk", dyk, ks), ("dyv", dyv, vs))]
+    r = _rope(freqs, mode, positions, pos0, mscale, B, S)
+    if out is None:
+        out = tuple(None if s is None else _empty_heads(s, q, False) for s in (qs, ks, vs))
+    out = tuple(out) + (None,) * (3 - len(out))
+    for name, o, s in (("dk", out[1], ks), ("dv", out[2], vs)):
+        if (o is None) != (s is None):
+            raise GnError(f"out: {name} goes with its input")
+    dh = [_heads(n, o, s, q.dtype) for n, o, s in zip(("dq", "dk", "dv"), out, (qs, ks, vs))]
+    f32 = torch.float32
+    if need_dw:
+        if accumulate and (dwq is None or (k is not None and dwk is None)):
+            raise GnError("accumulate needs the dwq and dwk to add onto")
+        if dwq is None:
+            dwq = torch.empty((D,), dtype=f32, device=q.device)
+        if k is not None and dwk is None:
+            dwk = torch.empty((D,), dtype=f32, device=q.device)
+        if ws is None:
+            ws = workspace(qk_norm_rope_workspace_bytes(B, S, D), q.device)
+    else:
+        dwq = dwk = None
+    wsp, wsb = (None, 0) if ws is None else (_here("ws", ws), ws.numel() * ws.element_size())
+    _check(lib().gn_qk_norm_rope_bwd(*dyh, qh, kh, *w, *dh, _here("dwq", dwq, f32, (D,)), _here("dwk", dwk, f32, (D,)), r,
+                                     B, S, D, eps, _dt(q), ACCUMULATE if accumulate else 0, wsp, wsb, _stream()),
+           "gn_qk_norm_rope_bwd")
+    return (*out, dwq, dwk)
 
 
 def add_inplace(out, a):

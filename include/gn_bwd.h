@@ -294,6 +294,107 @@ int gn_softmax_bwd(const void* dY, const void* Y, void* dX, int rows, int C, int
 int gn_xent_bwd(const void* logits, const int32_t* targets, void* dLogits, int rows, int C,
                 float scale, int dtype, void* stream);
 
+/* Softmax cross entropy of a linear head without its logits (the reference binds a Linear and
+ * cross-entropy-backward.glsl:29-84 over stored logits): with l = h E^T,
+ *   lse[t] = log sum_v exp l[t, v],  loss[t] = lse[t] - l[t, targets[t]]
+ * h [T x d], E [V x d] in dtype; targets int32 [T]; loss, lse fp32 [T] (each may be NULL).  A target
+ * outside [0, V) (-100, say) marks a row without one: loss 0, and no gradient from dloss.
+ * The logits exist a tile or a piece of the vocabulary at a time, in fp32.
+ * ws: gn_linear_xent_workspace_bytes(T, d, V, dtype), 16-byte aligned. */
+int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* targets, float* loss, float* lse,
+                       int T, int d, int V, int dtype, void* ws, size_t ws_bytes, void* stream);
+
+/* Its gradients, with lse as the forward left it:
+ *   u[t] = scale dloss[t] (dloss NULL: scale; 0 in a row without a target),  z[t] = scale dlse[t]
+ *   (dlse NULL: 0),  G[t, v] = u (p - [v = target]) + z p,  p = exp(l - lse)
+ *   dh = G E [T x d] in dtype,  dE (+)= G^T h [V x d] in dE_dtype (GN_F32, or GN_BF16 on the bf16
+ *   path).  dh or dE may be NULL; GN_ACCUMULATE adds onto an fp32 dE (a tied embedding's
+ *   gradient, micro-batches), dh is overwritten.
+ * A piece of the vocabulary at a time, its logits formed again.  On the bf16 path G enters dh and
+ * a bf16 dE rounded to bf16, and an fp32 dE as two bf16 pieces (2^-17 of each element).  Every
+ * sum's order is fixed: the same bits every time.  ws as for the forward. */
+int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* targets, const float* lse,
+                       const float* dloss, const float* dlse, float scale, void* dh, void* dE,
+                       int dE_dtype, int T, int d, int V, int dtype, unsigned flags, void* ws,
+                       size_t ws_bytes, void* stream);
+size_t gn_linear_xent_workspace_bytes(int T, int d, int V, int dtype);
+
+/* ---- rotary positions, per-head norms of queries and keys --------------------------------- */
+/* The two operators between a QKV projection and the attention.  The reference rotates inside
+ * its attention only (flash-attention2-rope.glsl:101-141, rope.glsl:74-125: whole heads,
+ * positions 0..S-1, one theta) and has no per-head norm. */
+
+/* Heads of B x S tokens: element (b, s, h, j), j < D, at p[b*sb + s*ss + h*sh + j] (strides in
+ * elements, none negative; a head's D elements are contiguous).  [B,S,H,D], [B,H,S,D] and the
+ * q, k or v part of fused QKV rows are all such views.  Inputs may repeat memory (stride 0);
+ * an output may not overlap itself or another tensor of the call, except that it may be its
+ * own input (same address and strides). */
+typedef struct gn_heads {
+    void* p;
+    int64_t sb, ss, sh;
+    int H;
+} gn_heads;
+
+/* A rotation by position.  Pair i < rot/2 of a head turns by position * freqs[i] radians; its
+ * elements are (2i, 2i+1) (GN_ROPE_INTERLEAVED) or (i, i + rot/2) (GN_ROPE_HALF), and elements
+ * from rot on pass through.  cos and sin are multiplied by mscale (a gradient too).  The angle is
+ * formed in fp64 and reduced to one turn before cos and sin are taken in fp32, so far positions
+ * keep their accuracy.  position = positions[b*pos_sb + s] (int32, device), or pos0 + s when
+ * positions is NULL. */
+typedef struct gn_rope {
+    const double* freqs;      /* device, [rot/2] */
+    const int32_t* positions; /* device, or NULL */
+    int64_t pos_sb;           /* its batch stride (0: the same positions for every b) */
+    int64_t pos0;
+    float mscale;
+    int rot;                  /* even, 0..D; 0: no rotation */
+    int mode;
+} gn_rope;
+
+#define GN_ROPE_SCALE_NONE 0
+#define GN_ROPE_SCALE_LINEAR 1 /* positions divided by factor */
+#define GN_ROPE_SCALE_NTK 2    /* theta * factor^(rot/(rot-2)): the slowest pair slows by factor */
+#define GN_ROPE_SCALE_YARN 3   /* pairs that turn often within `trained` positions keep their frequency,
+                                  slow ones are divided by factor, a linear ramp between */
+/* freqs[i], i < rot/2, into host memory: theta^(-2i/rot), scaled for a context `factor` (>= 1) times
+ * the `trained` positions.  YARN: a pair that turns r times within `trained` positions keeps
+ * clamp((r - slow) / (fast - slow), 0, 1) of its own frequency (usual fast 32, slow 1), and
+ * *mscale = 0.1 ln(factor) + 1; otherwise *mscale = 1.  trained, fast and slow are read by YARN
+ * only. */
+int gn_rope_freqs(int rot, double theta, int scaling, double factor, double trained, double fast,
+                  double slow, double* freqs, float* mscale);
+
+/* y = x rotated; dx = dy rotated back (the transpose of the rotation, times mscale).  x, y, dy, dx:
+ * H heads of D elements (even, <= 512), f32 or bf16; B*S below 2^31, H <= 1024.  Heads of 16-byte
+ * aligned rows with rot and D multiples of 16 move in 16-byte pieces, others element by element. */
+int gn_rope_fwd(const gn_heads* x, const gn_heads* y, const gn_rope* rope, int B, int S, int D,
+                int dtype, void* stream);
+int gn_rope_bwd(const gn_heads* dy, const gn_heads* dx, const gn_rope* rope, int B, int S, int D,
+                int dtype, void* stream);
+
+/* Per-head RMS norm of queries and keys, rotated in the same pass; values copied along, so that the
+ * call also splits fused QKV rows into the [B,H,S,D] tensors gn_attn_fwd takes:
+ *   r = rsqrt(mean_j x_j^2 + eps) per token and head,  y = rotation(x r w),  yv = v
+ * wq, wk: [D] in dtype, shared by the heads (NULL: 1).  k (with yk) and v (with yv) may be NULL;
+ * rope NULL: no rotation.  q and k may differ in their number of heads, k and v may not. */
+int gn_qk_norm_rope_fwd(const gn_heads* q, const gn_heads* k, const gn_heads* v, const void* wq,
+                        const void* wk, const gn_heads* yq, const gn_heads* yk, const gn_heads* yv,
+                        const gn_rope* rope, int B, int S, int D, float eps, int dtype,
+                        void* stream);
+
+/* Its backward from the forward's inputs (the statistic is formed again from x, which is read
+ * anyway), with g = the rotation's transpose applied to dy:
+ *   dx = r (w g - x r^2 mean_j(w_j g_j x_j)),  dw = sum over tokens and heads of g x r,  dv = dyv
+ * dwq, dwk: fp32 [D], NULL: not wanted; GN_ACCUMULATE adds onto them (the others are
+ * overwritten).  The sums run in a fixed order: the same bits every time.
+ * ws: gn_qk_norm_rope_workspace_bytes, 16-byte aligned; not used without dwq and dwk. */
+int gn_qk_norm_rope_bwd(const gn_heads* dyq, const gn_heads* dyk, const gn_heads* dyv,
+                        const gn_heads* q, const gn_heads* k, const void* wq, const void* wk,
+                        const gn_heads* dq, const gn_heads* dk, const gn_heads* dv, float* dwq,
+                        float* dwk, const gn_rope* rope, int B, int S, int D, float eps, int dtype,
+                        unsigned flags, void* ws, size_t ws_bytes, void* stream);
+size_t gn_qk_norm_rope_workspace_bytes(int B, int S, int D);
+
 /* ---- attention ------------------------------------------------------------------------ */
 /* Attention backward (attention-backward.glsl:73-194 semantics; RoPE of
  * flash-attention2-rope.glsl:73-145 applied to Q and K inside; causal mask j <= i).
