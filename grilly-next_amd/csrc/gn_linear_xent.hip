@@ -1,27 +1,38 @@
 // gn_linear_xent.hip — softmax cross entropy of a linear head (l = h E^T) without its logits, forward
-// and backward, a piece of the vocabulary at a time.
+// and backward.
 //
-//   forward    per piece: l = h E_c^T (fp32, in the workspace); each row's running maximum and sum of
-//              exp take the piece in; the target's logit is picked up in passing
-//   backward   per piece: l again, G = u (exp(l - lse) - [target]) + z exp(l - lse),
-//              dE_c (+)= G^T h,  dh += G E_c
+// bf16.  The logits exist in the accumulators of the product's tiles only (gemm_stream, 256 x 128 or
+// 128 x 128 tiles, blocks that stay):
+//   forward    a finished tile leaves each row's maximum and sum of exp over 64 columns, 8 bytes for
+//              64 logits, and the target's logit where it comes by; row_stats joins them
+//   backward   a piece of the vocabulary at a time: a finished tile of the same product leaves
+//              G = u (exp(l - lse) - [target]) + z exp(l - lse) in bf16, then dE_c (+)= G^T h and
+//              dh += G E_c (fp32) from it
+// A lane holds 16 columns of one row of each 32 x 32 accumulator, so the row statistics take one
+// exchange between lanes.  For an fp32 dE, G is stored as two bf16 pieces hi + lo, whose products
+// with h are two k-segments of one product: |G - hi - lo| <= 2^-17 |G|, where bf16 alone (2^-8)
+// would be the gradient's largest error.  For dh, hi is enough but at the target: there the rounding
+// of a row's largest element, which shows in all of dh's row, is kept in fp32 and its product with
+// E[target] added when dh is rounded (dh_finish).
 //
-// The products are the library's own (gemm_run).  On the bf16 path G is stored as bf16, and for an
-// fp32 dE as two bf16 pieces, hi + lo, whose products with h are summed as two k-segments of one
-// product: |G - hi - lo| <= 2^-17 |G|, where bf16 alone (2^-9) would be the gradient's largest error.
+// fp32.  The pieces' logits are stored (fp32, in the workspace) between the library's fp32 products
+// and row kernels, G in their place.
+//
+// Widths, row counts and vocabularies that the products' vectors do not divide: h and E's piece are
+// laid out to multiples of q = 8 (bf16) or 4 (fp32) elements first; the last V % q columns go
+// through products of q rows and through dh_finish.
 #include <algorithm>
 #include <cmath>
 
-#include "gn_common.h"
-#include "gn_gemm_dma.h"
+#include "gn_gemm_stream_core.h"
 
 namespace gn {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// A part of a row: its maximum m and the sum s of exp2 about it, (-inf, 0) when it is empty.  A NaN
-// among the logits is in s only (m skips it) and stays there.
+// A part of a row: its maximum m and the sum s of exp2 about it (logits in units of log2), (-inf, 0) when
+// it is empty.  A NaN among the logits is in s only (m skips it) and stays there.
 // s about another maximum n >= m
 __device__ __forceinline__ float about(float s, float m, float n) {
     return s * __builtin_amdgcn_exp2f(m - (n == -INFINITY ? 0.f : n));
@@ -32,8 +43,214 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     m = n;
 }
 
-// A row's statistics over one piece, joined with those of the pieces before; the last piece
-// turns them into lse and loss.  Statistics in units of log2.
+// ---- bf16: epilogues of the logits' product -------------------------------------------------
+// Element r of a 32 x 32 accumulator: row lane % 32, column 8 (r / 4) + 4 (lane / 32) + r % 4.
+
+// Each row's statistics over the wave's 64 columns, and its target's logit.
+struct StatsTile {
+    const int32_t* tgt;
+    float* lt;      // [T] the target's logit
+    float2* part;   // [strips][T]
+    int v0;         // the vocabulary's column of column 0 here
+    template <int FM, int FN>
+    __device__ __forceinline__ void tile(const GemmDesc& g, const f32x16_t (&acc)[FM][FN], int m0, int n0,
+                                         unsigned char*, int lane) const {
+        static_assert(FN == 2, "64 columns a wave");
+        if (n0 >= g.N) return;
+        const int nh = 4 * (lane >> 5);
+        float2* const out = part + (size_t)((v0 + n0) >> 6) * g.M;
+        int c[FM];  // the target's column among the wave's
+#pragma unroll
+        for (int i = 0; i < FM; ++i) c[i] = tgt[min(m0 + i * 32 + (lane & 31), g.M - 1)] - v0 - n0;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            float v[32];
+            float m = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = acc[i][e >> 4][e & 15];
+            if (n0 + 64 > g.N) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (n0 + (e >> 4) * 32 + ((e >> 2) & 3) * 8 + nh + (e & 3) >= g.N) v[e] = -INFINITY;
+            }
+            const int row = m0 + i * 32 + (lane & 31);
+            if (__any((unsigned)c[i] < 64u)) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (c[i] == (e >> 4) * 32 + ((e >> 2) & 3) * 8 + nh + (e & 3) && row < g.M &&
+                        n0 + c[i] < g.N)
+                        lt[row] = v[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) m = fmaxf(m, v[e]);
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float b = m == -INFINITY ? 0.f : m * kLog2e;
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s += __builtin_amdgcn_exp2f(fmaf(v[e], kLog2e, -b));
+            s += __shfl_xor(s, 32);
+            if (lane < 32 && row < g.M) out[row] = make_float2(m * kLog2e, s);
+        }
+    }
+};
+
+// What a row's G takes: {lse in units of log2, u + z, u, the target's column (as bits; -1: none)}
+typedef float4 RowScale;
+
+// G of the tile, as bf16 hi and (LO) lo; columns from N up to ld are zeros.
+template <bool LO>
+struct GradTile {
+    const RowScale* rows;
+    bf16_t *hi, *lo;  // [T x ld]
+    float* resid;     // [T] what rounding the target's element to hi left
+    int ld, v0;
+    template <int FM, int FN>
+    __device__ __forceinline__ void tile(const GemmDesc& g, const f32x16_t (&acc)[FM][FN], int m0, int n0,
+                                         unsigned char* st, int lane) const {
+        static_assert(FN == 2, "64 columns a wave");
+        if (n0 >= ld) return;
+        const int mr = lane & 31, nh = 4 * (lane >> 5);
+        RowScale rs[FM];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) rs[i] = rows[min(m0 + i * 32 + mr, g.M - 1)];
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int mw = m0 + i * 32, row = mw + mr;
+            const int c = __float_as_int(rs[i].w) - v0 - n0;
+            const bool hit = __any((unsigned)c < 64u), edge = n0 + 64 > g.N;
+            uint2 low[LO ? 8 : 1];
+            wave_lds_sync();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {  // four columns: 8 k + nh
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[e] = rs[i].y * __builtin_amdgcn_exp2f(fmaf(acc[i][k >> 2][4 * (k & 3) + e], kLog2e, -rs[i].x));
+                if (hit) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (c == 8 * k + nh + e) {
+                            x[e] -= rs[i].z;
+                            if (row < g.M) resid[row] = x[e] - bf2f(f2bf(x[e]));
+                        }
+                }
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (n0 + 8 * k + nh + e >= g.N) x[e] = 0.f;
+                }
+                const uint2 h = make_uint2(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]));
+                *reinterpret_cast<uint2*>(st + mr * 128 + ((k ^ (mr & 7)) * 16) + nh * 2) = h;
+                if constexpr (LO)
+                    low[k] = make_uint2(pack_bf2(x[0] - __uint_as_float(h.x << 16), x[1] - __uint_as_float(h.x & 0xffff0000u)),
+                                        pack_bf2(x[2] - __uint_as_float(h.y << 16), x[3] - __uint_as_float(h.y & 0xffff0000u)));
+            }
+            wave_lds_sync();
+            flush(hi, g.M, mw, n0, st, lane);
+            if constexpr (LO) {
+                wave_lds_sync();
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    *reinterpret_cast<uint2*>(st + mr * 128 + ((k ^ (mr & 7)) * 16) + nh * 2) = low[k];
+                wave_lds_sync();
+                flush(lo, g.M, mw, n0, st, lane);
+            }
+        }
+    }
+    // 32 rows x 64 columns from the wave's LDS, as 128-byte row segments
+    __device__ __forceinline__ void flush(bf16_t* P, int M, int mw, int n0, const unsigned char* st, int lane) const {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = q * 8 + (lane >> 3), n = n0 + (lane & 7) * 8;
+            const uint4 v = *reinterpret_cast<const uint4*>(st + r * 128 + (((lane & 7) ^ (lane >> 3)) * 16));
+            if (mw + r < M && n < ld) *reinterpret_cast<uint4*>(P + (size_t)(mw + r) * ld + n) = v;
+        }
+    }
+};
+
+template <int BM, typename EPI>
+int launch_logits_tile(const GemmDesc& g, const EPI& epi, hipStream_t s) {
+    constexpr int BN = 128, STAGES = 3;
+    constexpr size_t smem = (size_t)STAGES * (BM + BN) * BK * sizeof(bf16_t) + 4 * 4096;
+    static_assert(smem <= 160 * 1024, "LDS per CU");
+    static const bool ok = allow_lds(gemm_stream<false, true, float, BM, BN, STAGES, EPI>, smem);
+    if (!ok) {
+        set_error("linear xent: cannot reserve %zu B of LDS", smem);
+        return GN_E_HIP;
+    }
+    const long tiles = (long)((g.M + BM - 1) / BM) * ((g.N + BN - 1) / BN);
+    const unsigned grid = (unsigned)std::min<long>(tiles, stream_blocks());
+    hipLaunchKernelGGL((gemm_stream<false, true, float, BM, BN, STAGES, EPI>), dim3(grid), dim3(512), smem, s, g, epi);
+    GN_LAUNCH_CHECK("linear xent (logits)");
+    return GN_OK;
+}
+
+// 256-row tiles, or 128-row ones where they need less (the streamed products' rule: a round of them
+// takes 0.6 of a round of the large)
+template <typename EPI>
+int launch_logits(const GemmDesc& g, const EPI& epi, hipStream_t s) {
+    const long blocks = stream_blocks(), tn = (g.N + 127) / 128;
+    const long r256 = ((g.M + 255) / 256 * tn + blocks - 1) / blocks, r128 = ((g.M + 127) / 128 * tn + blocks - 1) / blocks;
+    return 0.62 * (double)r128 < (double)r256 ? launch_logits_tile<128>(g, epi, s) : launch_logits_tile<256>(g, epi, s);
+}
+
+__device__ __forceinline__ void finish_row(int t, float m, float s, const int32_t* tgt, const float* lt, float* loss,
+                                           float* lse, int V) {
+    const float z = (m + __builtin_amdgcn_logf(s)) / kLog2e;
+    if (lse) lse[t] = z;
+    const int g = tgt[t];
+    if (loss) loss[t] = g >= 0 && g < V ? z - lt[t] : 0.f;
+}
+
+// lse and loss from the strips' statistics: 16 rows x 16 slices of the strips a block
+__global__ __launch_bounds__(256) void row_stats(const float2* __restrict__ part, int strips, int T,
+                                                 const int32_t* __restrict__ tgt, const float* __restrict__ lt,
+                                                 float* __restrict__ loss, float* __restrict__ lse, int V) {
+    __shared__ float2 sh[16][17];
+    const int r = threadIdx.x & 15, sl = threadIdx.x >> 4, t = blockIdx.x * 16 + r;
+    float m = -INFINITY, s = 0.f;
+    if (t < T) {
+        for (int k = sl; k < strips; k += 64) {
+            float2 p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                p[j] = k + 16 * j < strips ? part[(size_t)(k + 16 * j) * T + t] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) join(m, s, p[j].x, p[j].y);
+        }
+    }
+    sh[sl][r] = make_float2(m, s);
+    __syncthreads();
+    if (threadIdx.x < 16 && t < T) {
+        m = -INFINITY;
+        s = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) join(m, s, sh[k][r].x, sh[k][r].y);
+        finish_row(t, m, s, tgt, lt, loss, lse, V);
+    }
+}
+
+// Every row's scales, and no residual yet; rows from T up to Tp (the fp32 products' padding) have none.
+__global__ __launch_bounds__(256) void row_scales(RowScale* __restrict__ rows, float* __restrict__ resid, int T, int Tp,
+                                                  const int32_t* __restrict__ tgt, const float* __restrict__ lse,
+                                                  const float* __restrict__ dloss, const float* __restrict__ dlse,
+                                                  float scale, int V) {
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= Tp) return;
+    RowScale r = make_float4(0.f, 0.f, 0.f, __int_as_float(-1));
+    if (t < T) {
+        const int g = tgt[t];
+        const bool has = g >= 0 && g < V;
+        const float u = has ? (dloss ? scale * dloss[t] : scale) : 0.f;
+        r = make_float4(lse[t] * kLog2e, u + (dlse ? scale * dlse[t] : 0.f), u, __int_as_float(has ? g : -1));
+    }
+    rows[t] = r;
+    resid[t] = 0.f;
+}
+
+// ---- fp32: row kernels over a piece's stored logits -------------------------------------------
+// A row's statistics over one piece, joined with those of the pieces before (st); the last
+// piece's are turned into lse and loss.  ld and L are multiples of 4 elements and 16 bytes.
 __global__ __launch_bounds__(256) void piece_stats(const float* __restrict__ L, int ld, int v0, int nv,
                                                    const int32_t* __restrict__ tgt, float2* __restrict__ st,
                                                    float* __restrict__ lt, float* __restrict__ loss,
@@ -42,14 +259,26 @@ __global__ __launch_bounds__(256) void piece_stats(const float* __restrict__ L, 
     const int t = blockIdx.x;
     const float* row = L + (size_t)t * ld;
     float m = -INFINITY, s = 0.f;
-    for (int v = threadIdx.x; v < nv; v += 256) {
-        const float x = row[v] * kLog2e;
-        if (x > m) {
-            s = s * __builtin_amdgcn_exp2f(m - x) + 1.f;
-            m = x;
-        } else if (x != -INFINITY) {
-            s += __builtin_amdgcn_exp2f(x - m);
+    for (int v = 4 * threadIdx.x; v < nv; v += 4096) {
+        float x[16];
+        float n = m;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = v + 1024 * j;
+            const float4 q = c < nv ? *reinterpret_cast<const float4*>(row + c)
+                                    : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            x[4 * j] = q.x * kLog2e;
+            x[4 * j + 1] = c + 1 < nv ? q.y * kLog2e : -INFINITY;
+            x[4 * j + 2] = c + 2 < nv ? q.z * kLog2e : -INFINITY;
+            x[4 * j + 3] = c + 3 < nv ? q.w * kLog2e : -INFINITY;
         }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) n = fmaxf(n, x[e]);
+        const float b = n == -INFINITY ? 0.f : n;
+        s *= __builtin_amdgcn_exp2f(m - b);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(x[e] - b);
+        m = n;
     }
     const float mw = wave_max(m);
     s = wave_sum(about(s, m, mw));
@@ -66,80 +295,89 @@ __global__ __launch_bounds__(256) void piece_stats(const float* __restrict__ L, 
     for (int i = 0; i < 4; ++i) join(m, s, sm[i], ss[i]);
     const int g = tgt[t];
     if (g >= v0 && g < v0 + nv) lt[t] = row[g - v0];
-    if (!last) {
-        st[t] = make_float2(m, s);
-        return;
-    }
-    const float z = (m + __builtin_amdgcn_logf(s)) / kLog2e;
-    if (lse) lse[t] = z;
-    if (loss) loss[t] = g >= 0 && g < V ? z - lt[t] : 0.f;
+    if (last) finish_row(t, m, s, tgt, lt, loss, lse, V);
+    else st[t] = make_float2(m, s);
 }
 
-// u and z of a row
-__device__ __forceinline__ float2 row_scale(int t, const int32_t* tgt, const float* dloss, const float* dlse, float scale,
-                                            int V) {
-    const int g = tgt[t];
-    const float u = g >= 0 && g < V ? (dloss ? scale * dloss[t] : scale) : 0.f;
-    return make_float2(u, dlse ? scale * dlse[t] : 0.f);
-}
-
-// G of one piece: fp32 in place (hi == nullptr), or as bf16 hi and (lo != nullptr) lo
-__global__ __launch_bounds__(256) void piece_grad(float* __restrict__ L, bf16_t* __restrict__ hi, bf16_t* __restrict__ lo,
-                                                  int ld, int v0, int nv, const int32_t* __restrict__ tgt,
-                                                  const float* __restrict__ lse, const float* __restrict__ dloss,
-                                                  const float* __restrict__ dlse, float scale, int V) {
-    const int t = blockIdx.x, g = tgt[t] - v0;
-    const float2 uz = row_scale(t, tgt, dloss, dlse, scale, V);
-    const float a = uz.x + uz.y, b = lse[t] * kLog2e;
-    for (int v = blockIdx.y * 256 + threadIdx.x; v < nv; v += 256 * gridDim.y) {
-        const size_t i = (size_t)t * ld + v;
-        float x = a * __builtin_amdgcn_exp2f(L[i] * kLog2e - b);
-        if (v == g) x -= uz.x;
-        if (!hi) {
-            L[i] = x;
-        } else {
-            const bf16_t p = f2bf(x);
-            hi[i] = p;
-            if (lo) lo[i] = f2bf(x - bf2f(p));
+// G of one piece in its logits' place, zeros from nv up to the next multiple of 4
+__global__ __launch_bounds__(256) void piece_grad(float* __restrict__ L, int ld, int v0, int nv,
+                                                  const RowScale* __restrict__ rows) {
+    const RowScale r = rows[blockIdx.x];
+    float* const row = L + (size_t)blockIdx.x * ld;
+    const int g = __float_as_int(r.w) - v0;
+    for (int v = 4 * (blockIdx.y * 256 + threadIdx.x); v < nv; v += 1024 * gridDim.y) {
+        float4* p = reinterpret_cast<float4*>(row + v);
+        const float4 q = *p;
+        float x[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] = r.y * __builtin_amdgcn_exp2f(fmaf(x[e], kLog2e, -r.x));
+            if (v + e == g) x[e] -= r.z;
+            if (v + e >= nv) x[e] = 0.f;
         }
+        *p = make_float4(x[0], x[1], x[2], x[3]);
     }
 }
 
-__global__ __launch_bounds__(256) void round_rows(const float* __restrict__ a, bf16_t* __restrict__ o, int64_t n) {
-    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) o[i] = f2bf(a[i]);
+// ---- both ---------------------------------------------------------------------------------
+// dst [Rp x dp] = src [R x d], zeros around it
+template <typename T>
+__global__ __launch_bounds__(256) void lay_out(const T* __restrict__ src, T* __restrict__ dst, int R, int d, int Rp, int dp) {
+    const int64_t n = (int64_t)Rp * dp;
+    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int r = (int)(i / dp), c = (int)(i - (int64_t)r * dp);
+        dst[i] = r < R && c < d ? src[(size_t)r * d + c] : (T)0;
+    }
 }
 
-// The vocabulary's pieces: as many columns as keep a piece's fp32 logits at 256 MB, multiples of 64.
-int piece_columns(int T, int V) {
-    const int64_t c = std::max<int64_t>(256, ((int64_t)64 << 20) / std::max(T, 1) / 64 * 64);
-    return (int)std::min<int64_t>(c, ((int64_t)V + 63) / 64 * 64);
+// dst [R x d] (+)= src [R x dp]
+template <typename T>
+__global__ __launch_bounds__(256) void take_rows(const float* __restrict__ src, T* __restrict__ dst, int R, int d, int dp,
+                                                 int accumulate) {
+    const int64_t n = (int64_t)R * d;
+    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int r = (int)(i / d), c = (int)(i - (int64_t)r * d);
+        const float v = src[(size_t)r * dp + c];
+        io<T>::st(dst, i, accumulate ? v + io<T>::ld(dst, i) : v);
+    }
 }
 
-size_t up(size_t b) { return (b + 255) / 256 * 256; }
-
-// The workspace of both directions
-struct Layout {
-    int vc, pieces;
-    size_t logits, stats, target, hi, lo, acc, bytes;
-    Layout(int T, int d, int V, int dtype) {
-        vc = piece_columns(T, V);
-        pieces = (V + vc - 1) / vc;
-        size_t at = 0;
-        auto take = [&](size_t n) {
-            const size_t p = at;
-            at += up(n);
-            return p;
+// dh's rows from their fp32 sums (acc [T x dp], nullptr: nothing), the target's residual and the
+// last `tail` columns of the vocabulary (G [T x ld] from that column on, Et its rows of E)
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void dh_finish(const float* __restrict__ acc, int dp, const RowScale* __restrict__ rows,
+                                                 const float* __restrict__ resid, const T* __restrict__ E,
+                                                 const T* __restrict__ G, int ld, const T* __restrict__ Et, int tail,
+                                                 T* __restrict__ dh, int n, int d) {
+    constexpr int W = VEC ? 8 : 1;
+    const int per = d / W;
+    const int64_t all = (int64_t)n * per;
+    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+        const int t = (int)(i / per), c = (int)(i - (int64_t)t * per) * W;
+        float v[8], e[8];
+        auto add = [&](float f, const T* p) {
+            if constexpr (VEC) chunk8<T>::ld(p + c, e);
+            else e[0] = io<T>::ld(p, c);
+#pragma unroll
+            for (int j = 0; j < W; ++j) v[j] += f * e[j];
         };
-        const bool bf = dtype == GN_BF16;
-        logits = take((size_t)T * vc * 4);
-        stats = take((size_t)T * 8);
-        target = take((size_t)T * 4);
-        hi = take(bf ? (size_t)T * vc * 2 : 0);
-        lo = take(bf ? (size_t)T * vc * 2 : 0);
-        acc = take(bf ? (size_t)T * d * 4 : 0);
-        bytes = at;
+#pragma unroll
+        for (int j = 0; j < W; ++j) v[j] = 0.f;
+        if (acc) {
+            if constexpr (VEC) chunk8<float>::ld(acc + (size_t)t * dp + c, v);
+            else v[0] = acc[(size_t)t * dp + c];
+        }
+        const float f = resid[t];
+        if (f != 0.f) add(f, E + (size_t)__float_as_int(rows[t].w) * d);
+        for (int j = 0; j < tail; ++j) add(io<T>::ld(G, (size_t)t * ld + j), Et + (size_t)j * d);
+        if constexpr (VEC) chunk8<T>::st(dh + (size_t)t * d + c, v);
+        else io<T>::st(dh, (size_t)t * d + c, v[0]);
     }
-};
+}
+
+// ---- host -----------------------------------------------------------------------------------
+inline bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+inline int round_up(int n, int q) { return (n + q - 1) / q * q; }
 
 GemmDesc product(const void* A, int lda, const void* B, int ldb, int K, void* C, int ldc, int M, int N) {
     GemmDesc g{};
@@ -158,11 +396,82 @@ GemmDesc product(const void* A, int lda, const void* B, int ldb, int K, void* C,
     return g;
 }
 
-inline bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+// A call's shapes and its workspace.  lay: h, E's pieces and dE go through copies in the products'
+// layout (widths that are no multiple of q, or tensors off the 16-byte grid).
+struct Plan {
+    bool bf, lay;
+    int T, d, V, q, es, dp, Tp;
+    int vc, pieces;  // columns of a piece, a multiple of 128 (or all of a smaller vocabulary)
+    size_t h, E, Et, lt, rows, resid, stats, logits, hi, lo, acc, de, det, part, part_bytes, bytes;
+
+    Plan(int T_, int d_, int V_, int dtype, bool lay_) : bf(dtype == GN_BF16), lay(lay_), T(T_), d(d_), V(V_) {
+        q = bf ? 8 : 4;
+        es = bf ? 2 : 4;
+        lay = lay || d % q;
+        dp = round_up(d, q);
+        Tp = bf ? T : round_up(T, 4);
+        // A piece's G (hi + lo, or the fp32 logits it replaces) takes 4 bytes an element
+        const int64_t most = kPieceBytes / (lay ? 4 : 1) / 4 / std::max(Tp, 1);
+        vc = (int)std::min<int64_t>(round_up(V, 128), std::max<int64_t>(512, most / 128 * 128));
+        pieces = (V + vc - 1) / vc;
+        // the products' own split workspaces: of a whole piece and of the last one
+        part_bytes = 0;
+        const int last = (V - (pieces - 1) * vc) / q * q;
+        for (int nv : {pieces > 1 ? vc : last, last, V % q ? q : 0}) {
+            if (nv <= 0) continue;
+            GemmDesc a = product(nullptr, vc, nullptr, dp, Tp, nullptr, dp, nv, dp);
+            GemmDesc b = product(nullptr, vc, nullptr, dp, nv, nullptr, dp, Tp, dp);
+            if (bf) {
+                a.nseg = 2;
+                a.lda[1] = vc;
+                a.ldb[1] = dp;
+                a.Ks[1] = T;
+                part_bytes = std::max({part_bytes, gemm_dma_part_bytes(a, 1, GN_F32), gemm_dma_part_bytes(b, 0, GN_F32)});
+                a.accumulate = b.accumulate = 1;
+                part_bytes = std::max({part_bytes, gemm_dma_part_bytes(a, 1, GN_F32), gemm_dma_part_bytes(b, 0, GN_F32)});
+            } else {
+                const GemmDesc l = product(nullptr, dp, nullptr, dp, dp, nullptr, vc, Tp, nv);
+                part_bytes = std::max({part_bytes, gemm_f32_part_bytes(a), gemm_f32_part_bytes(b), gemm_f32_part_bytes(l)});
+            }
+        }
+        size_t at = 0;
+        auto take = [&](size_t n) {
+            const size_t p = at;
+            at += (n + 255) / 256 * 256;
+            return p;
+        };
+        h = take(lay || Tp != T ? (size_t)Tp * dp * es : 0);
+        E = take(lay ? (size_t)vc * dp * es : 0);
+        Et = take((size_t)q * dp * es);
+        lt = take((size_t)T * 4);
+        logits = take(bf ? 0 : (size_t)Tp * vc * 4);
+        part = take(part_bytes);
+        const size_t both = at;  // from here on the forward and the backward have their own
+        stats = take(bf ? (size_t)((V + 127) / 128 * 2) * T * 8 : (size_t)T * 8);
+        const size_t fwd = at;
+        at = both;
+        rows = take((size_t)Tp * sizeof(RowScale));
+        resid = take((size_t)Tp * 4);
+        hi = take(bf ? (size_t)T * vc * 2 : 0);
+        lo = take(bf ? (size_t)T * vc * 2 : 0);
+        acc = take((size_t)Tp * dp * 4);
+        de = take(lay ? (size_t)vc * dp * 4 : 0);
+        det = take((size_t)q * dp * 4);
+        bytes = std::max(fwd, at);
+    }
+    // A piece of 512 MB: two pieces an 8192 x 32000 vocabulary, eight 8192 x 128000.
+    static constexpr int64_t kPieceBytes = (int64_t)512 << 20;
+};
+
+size_t workspace_bytes(int T, int d, int V, int dtype) {
+    // what alignment will be is not known from the shape
+    return std::max(Plan(T, d, V, dtype, false).bytes, Plan(T, d, V, dtype, true).bytes);
+}
 
 int check(const char* who, const void* h, const void* E, const int32_t* tgt, int T, int d, int V, int dtype) {
     GN_REQUIRE(dtype == GN_F32 || dtype == GN_BF16, "%s: dtype %d not supported (f32, bf16)", who, dtype);
     GN_REQUIRE(T >= 0 && d >= 1 && V >= 1, "%s: bad shape", who);
+    GN_REQUIRE(T < (1 << 28) && d <= (1 << 20) && V < (1 << 30), "%s: T below 2^28, d up to 2^20, V below 2^30", who);
     GN_REQUIRE(T == 0 || (h && E && tgt), "%s: null pointer", who);
     const int es = dtype == GN_F32 ? 4 : 2;
     GN_REQUIRE((((uintptr_t)h | (uintptr_t)E) & (es - 1)) == 0 && ((uintptr_t)tgt & 3u) == 0,
@@ -170,13 +479,66 @@ int check(const char* who, const void* h, const void* E, const int32_t* tgt, int
     return GN_OK;
 }
 
-int check_ws(const char* who, const Layout& w, const void* ws, size_t ws_bytes) {
-    if (!ws || ws_bytes < w.bytes || !al16(ws)) {
-        set_error("%s: workspace of %zu bytes (16-byte aligned) required", who, w.bytes);
+int check_ws(const char* who, const Plan& w, int dtype, const void* ws, size_t ws_bytes) {
+    const size_t need = workspace_bytes(w.T, w.d, w.V, dtype);
+    if (!ws || ws_bytes < need || !al16(ws)) {
+        set_error("%s: workspace of %zu bytes (16-byte aligned) required", who, need);
         return GN_E_WORKSPACE;
     }
     return GN_OK;
 }
+
+// One call's tensors in the products' layout.
+struct Call {
+    const char* who;
+    const Plan& w;
+    char* base;
+    const void *h, *E;
+    hipStream_t s;
+    int dtype;
+    const void* hp = nullptr;  // [Tp x dp]
+
+    int copy(const void* src, size_t to, int R, int Rp) {
+        const unsigned grid = grid_for((int64_t)Rp * w.dp, 1024, 16384);
+        if (w.bf) lay_out<bf16_t><<<grid, 256, 0, s>>>((const bf16_t*)src, (bf16_t*)(base + to), R, w.d, Rp, w.dp);
+        else lay_out<float><<<grid, 256, 0, s>>>((const float*)src, (float*)(base + to), R, w.d, Rp, w.dp);
+        GN_LAUNCH_CHECK(who);
+        return GN_OK;
+    }
+    int start() {
+        hp = h;
+        if (!w.lay && w.Tp == w.T) return GN_OK;
+        hp = base + w.h;
+        return copy(h, w.h, w.T, w.Tp);
+    }
+    // rows v0 .. v0 + nv of E as the products take them
+    int piece(int v0, int nv, const void** Ec) {
+        *Ec = (const char*)E + (size_t)v0 * w.d * w.es;
+        if (!w.lay) return GN_OK;
+        const int rc = copy(*Ec, w.E, nv, std::min(round_up(nv, w.q), w.vc));
+        *Ec = base + w.E;
+        return rc;
+    }
+    void scratch(GemmDesc& g) {
+        g.part = (float*)(base + w.part);
+        g.part_cap = w.part_bytes;
+    }
+    // fp32: a piece's logits, the columns past its last multiple of 4 through four rows of their own
+    int logits32(const void* Ec, int nv) {
+        float* const L = (float*)(base + w.logits);
+        const int nq = nv / w.q * w.q, cols = w.lay ? round_up(nv, w.q) : nq;
+        if (cols) {
+            GemmDesc g = product(hp, w.dp, Ec, w.dp, w.dp, L, w.vc, w.Tp, cols);
+            scratch(g);
+            if (const int rc = gemm_run(g, 0, 1, dtype, GN_F32, s)) return rc;
+        }
+        if (cols >= nv) return GN_OK;
+        if (const int rc = copy((const char*)Ec + (size_t)nq * w.d * w.es, w.Et, nv - nq, w.q)) return rc;
+        GemmDesc g = product(hp, w.dp, base + w.Et, w.dp, w.dp, L + nq, w.vc, w.Tp, w.q);
+        scratch(g);
+        return gemm_run(g, 0, 1, dtype, GN_F32, s);
+    }
+};
 
 }  // namespace
 }  // namespace gn
@@ -185,7 +547,7 @@ using namespace gn;
 
 extern "C" size_t gn_linear_xent_workspace_bytes(int T, int d, int V, int dtype) {
     if (T <= 0 || d <= 0 || V <= 0 || (dtype != GN_F32 && dtype != GN_BF16)) return 0;
-    return Layout(T, d, V, dtype).bytes;
+    return workspace_bytes(T, d, V, dtype);
 }
 
 extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* targets, float* loss, float* lse, int T,
@@ -195,17 +557,30 @@ extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* t
     if (const int rc = check(who, h, E, targets, T, d, V, dtype)) return rc;
     GN_REQUIRE((((uintptr_t)loss | (uintptr_t)lse) & 3u) == 0, "%s: loss, lse must be aligned to 4 bytes", who);
     if (T == 0 || (!loss && !lse)) return GN_OK;
-    const Layout w(T, d, V, dtype);
-    if (const int rc = check_ws(who, w, ws, ws_bytes)) return rc;
-    hipStream_t s = as_stream(stream);
+    const Plan w(T, d, V, dtype, !al16(h) || !al16(E));
+    if (const int rc = check_ws(who, w, dtype, ws, ws_bytes)) return rc;
     char* const base = (char*)ws;
-    const int es = dtype == GN_F32 ? 4 : 2;
-    for (int p = 0; p < w.pieces; ++p) {
-        const int v0 = p * w.vc, nv = std::min(w.vc, V - v0);
-        const GemmDesc g = product(h, d, (const char*)E + (size_t)v0 * d * es, d, d, base + w.logits, w.vc, T, nv);
-        if (const int rc = gemm_run(g, 0, 1, dtype, GN_F32, s)) return rc;
-        piece_stats<<<T, 256, 0, s>>>((const float*)(base + w.logits), w.vc, v0, nv, targets, (float2*)(base + w.stats),
-                                      (float*)(base + w.target), loss, lse, V, p == 0, p == w.pieces - 1);
+    Call c{who, w, base, h, E, as_stream(stream), dtype};
+    if (const int rc = c.start()) return rc;
+    float* const lt = (float*)(base + w.lt);
+    const int step = w.bf && !w.lay ? V : w.vc;  // all at once where E is read as it lies
+    for (int v0 = 0; v0 < V; v0 += step) {
+        const int nv = std::min(step, V - v0);
+        const void* Ec;
+        if (const int rc = c.piece(v0, nv, &Ec)) return rc;
+        if (w.bf) {
+            const GemmDesc g = product(c.hp, w.dp, Ec, w.dp, w.dp, nullptr, 0, T, nv);
+            const StatsTile epi{targets, lt, (float2*)(base + w.stats), v0};
+            if (const int rc = launch_logits(g, epi, c.s)) return rc;
+        } else {
+            if (const int rc = c.logits32(Ec, nv)) return rc;
+            piece_stats<<<T, 256, 0, c.s>>>((const float*)(base + w.logits), w.vc, v0, nv, targets,
+                                            (float2*)(base + w.stats), lt, loss, lse, V, v0 == 0, v0 + nv == V);
+            GN_LAUNCH_CHECK(who);
+        }
+    }
+    if (w.bf) {
+        row_stats<<<(T + 15) / 16, 256, 0, c.s>>>((const float2*)(base + w.stats), (V + 63) / 64, T, targets, lt, loss, lse, V);
         GN_LAUNCH_CHECK(who);
     }
     return GN_OK;
@@ -221,13 +596,14 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
     GN_REQUIRE(dE_dtype == GN_F32 || (dE_dtype == GN_BF16 && dtype == GN_BF16), "%s: dE must be f32, or bf16 on the bf16 path", who);
     GN_REQUIRE((flags & ~GN_ACCUMULATE) == 0, "%s: unknown flags", who);
     const bool acc = flags & GN_ACCUMULATE;
+    const int des = dE_dtype == GN_F32 ? 4 : 2;
     GN_REQUIRE(!acc || dE_dtype == GN_F32, "%s: only an fp32 dE accumulates", who);
-    GN_REQUIRE(((uintptr_t)dE & (dE_dtype == GN_F32 ? 3u : 1u)) == 0 && ((uintptr_t)dh & (dtype == GN_F32 ? 3u : 1u)) == 0 &&
+    GN_REQUIRE(((uintptr_t)dE & (des - 1)) == 0 && ((uintptr_t)dh & (dtype == GN_F32 ? 3u : 1u)) == 0 &&
                    (((uintptr_t)lse | (uintptr_t)dloss | (uintptr_t)dlse) & 3u) == 0,
                "%s: a tensor is not aligned to its elements", who);
     hipStream_t s = as_stream(stream);
     if (T == 0) {  // no rows: dE is zero
-        if (dE && !acc && launch_zero(dE, (size_t)V * d * (dE_dtype == GN_F32 ? 4 : 2), s) != hipSuccess) {
+        if (dE && !acc && launch_zero(dE, (size_t)V * d * des, s) != hipSuccess) {
             set_error("%s: clear failed", who);
             return GN_E_HIP;
         }
@@ -235,47 +611,94 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
     }
     GN_REQUIRE(lse, "%s: null pointer", who);
     if (!dh && !dE) return GN_OK;
-    const Layout w(T, d, V, dtype);
-    if (const int rc = check_ws(who, w, ws, ws_bytes)) return rc;
+    const Plan w(T, d, V, dtype, !al16(h) || !al16(E) || !al16(dE));
+    if (const int rc = check_ws(who, w, dtype, ws, ws_bytes)) return rc;
     char* const base = (char*)ws;
-    const bool bf = dtype == GN_BF16;
-    const int es = bf ? 2 : 4;
-    float* const L = (float*)(base + w.logits);
-    bf16_t* const hi = bf ? (bf16_t*)(base + w.hi) : nullptr;
-    bf16_t* const lo = bf && dE && dE_dtype == GN_F32 ? (bf16_t*)(base + w.lo) : nullptr;
-    // dh of one piece is rounded by its product; of several it is summed in fp32 first
-    const bool direct = !bf || w.pieces == 1;
-    void* const sum = direct ? dh : base + w.acc;
-    for (int p = 0; p < w.pieces; ++p) {
-        const int v0 = p * w.vc, nv = std::min(w.vc, V - v0);
-        const char* Ec = (const char*)E + (size_t)v0 * d * es;
-        if (const int rc = gemm_run(product(h, d, Ec, d, d, L, w.vc, T, nv), 0, 1, dtype, GN_F32, s)) return rc;
-        piece_grad<<<dim3(T, std::min(64, (nv + 1023) / 1024)), 256, 0, s>>>(L, hi, lo, w.vc, v0, nv, targets, lse, dloss,
-                                                                            dlse, scale, V);
-        GN_LAUNCH_CHECK(who);
-        const void* G = bf ? (const void*)hi : L;
-        if (dE) {
-            GemmDesc g = product(G, w.vc, h, d, T, (char*)dE + (size_t)v0 * d * (dE_dtype == GN_F32 ? 4 : 2), d, nv, d);
-            if (lo) {
-                g.nseg = 2;
-                g.A[1] = lo;
-                g.lda[1] = w.vc;
-                g.B[1] = g.B[0];
-                g.ldb[1] = d;
-                g.Ks[1] = T;
-            }
-            g.accumulate = acc;
-            if (const int rc = gemm_run(g, 1, 0, dtype, dE_dtype, s)) return rc;
+    Call c{who, w, base, h, E, s, dtype};
+    if (const int rc = c.start()) return rc;
+    const bool two = w.bf && dE && dE_dtype == GN_F32;  // G in two pieces
+    RowScale* const rows = (RowScale*)(base + w.rows);
+    float* const resid = (float*)(base + w.resid);
+    char* const G = base + (w.bf ? w.hi : w.logits);
+    bf16_t* const lo = (bf16_t*)(base + w.lo);
+    row_scales<<<(w.Tp + 255) / 256, 256, 0, s>>>(rows, resid, T, w.Tp, targets, lse, dloss, dlse, scale, V);
+    GN_LAUNCH_CHECK(who);
+    // dst (+)= G's columns c0 .. c0 + M, transposed, times h: fp32 or in dE's own type
+    auto weight = [&](int c0, int M, void* dst, int c_dtype, bool add) {
+        GemmDesc g = product(G + (size_t)c0 * w.es, w.vc, c.hp, w.dp, w.Tp, dst, w.dp, M, w.dp);
+        if (two) {
+            g.nseg = 2;
+            g.A[1] = lo + c0;
+            g.lda[1] = w.vc;
+            g.B[1] = g.B[0];
+            g.ldb[1] = w.dp;
+            g.Ks[1] = T;
         }
-        if (dh) {
-            GemmDesc g = product(G, w.vc, Ec, d, nv, sum, d, T, d);
-            g.accumulate = p > 0;
-            if (const int rc = gemm_run(g, 0, 0, dtype, bf && direct ? GN_BF16 : GN_F32, s)) return rc;
+        g.accumulate = add;
+        if (c_dtype == GN_F32) c.scratch(g);
+        return gemm_run(g, 1, 0, dtype, c_dtype, s);
+    };
+    // rows v .. v + R of dE from an fp32 [R x dp]
+    auto rows_out = [&](size_t from, int v, int R) {
+        const unsigned grid = grid_for((int64_t)R * d, 1024, 16384);
+        char* dst = (char*)dE + (size_t)v * d * des;
+        if (des == 2) take_rows<bf16_t><<<grid, 256, 0, s>>>((const float*)(base + from), (bf16_t*)dst, R, d, w.dp, 0);
+        else take_rows<float><<<grid, 256, 0, s>>>((const float*)(base + from), (float*)dst, R, d, w.dp, acc);
+        GN_LAUNCH_CHECK(who);
+        return (int)GN_OK;
+    };
+    const int tail = V % w.q;
+    for (int v0 = 0; v0 < V; v0 += w.vc) {
+        const int nv = std::min(w.vc, V - v0), nq = nv / w.q * w.q;
+        const void* Ec;
+        if (const int rc = c.piece(v0, nv, &Ec)) return rc;
+        if (w.bf) {
+            const GemmDesc g = product(c.hp, w.dp, Ec, w.dp, w.dp, nullptr, 0, T, nv);
+            const int rc = two ? launch_logits(g, GradTile<true>{rows, (bf16_t*)G, lo, resid, w.vc, v0}, s)
+                               : launch_logits(g, GradTile<false>{rows, (bf16_t*)G, nullptr, resid, w.vc, v0}, s);
+            if (rc) return rc;
+        } else {
+            if (const int rc = c.logits32(Ec, nv)) return rc;
+            piece_grad<<<dim3(w.Tp, std::min(16, (nv + 4095) / 4096)), 256, 0, s>>>((float*)G, w.vc, v0, nv, rows);
+            GN_LAUNCH_CHECK(who);
+        }
+        if (dE && w.lay) {
+            const int M = round_up(nv, w.q);
+            if (const int rc = weight(0, M, base + w.de, GN_F32, false)) return rc;
+            if (const int rc = rows_out(w.de, v0, nv)) return rc;
+        } else if (dE) {
+            if (nq) {
+                if (const int rc = weight(0, nq, (char*)dE + (size_t)v0 * d * des, dE_dtype, acc)) return rc;
+            }
+            if (nv > nq) {
+                if (const int rc = weight(nq, w.q, base + w.det, GN_F32, false)) return rc;
+                if (const int rc = rows_out(w.det, v0 + nq, nv - nq)) return rc;
+            }
+        }
+        if (dh && nq) {
+            GemmDesc g = product(G, w.vc, Ec, w.dp, nq, base + w.acc, w.dp, w.Tp, w.dp);
+            g.accumulate = v0 > 0;
+            c.scratch(g);
+            if (const int rc = gemm_run(g, 0, 0, dtype, GN_F32, s)) return rc;
         }
     }
-    if (dh && !direct) {
-        const int64_t n = (int64_t)T * d;
-        round_rows<<<grid_for(n, 1024, 8192), 256, 0, s>>>((const float*)sum, (bf16_t*)dh, n);
+    if (dh) {
+        const float* sum = V >= w.q ? (const float*)(base + w.acc) : nullptr;
+        const size_t col = (size_t)((V - 1) % w.vc + 1 - tail) * w.es;  // the tail's first column in the last piece
+        const char* Et = (const char*)E + (size_t)(V - tail) * d * w.es;
+        const bool vec = d % 8 == 0 && al16(dh) && al16(E);
+        const unsigned grid = grid_for((int64_t)T * (vec ? d / 8 : d), 256, 16384);
+        auto go = [&](auto VEC_) {
+            constexpr bool VEC = decltype(VEC_)::value;
+            if (w.bf)
+                dh_finish<bf16_t, VEC><<<grid, 256, 0, s>>>(sum, w.dp, rows, resid, (const bf16_t*)E, (const bf16_t*)(G + col),
+                                                            w.vc, (const bf16_t*)Et, tail, (bf16_t*)dh, T, d);
+            else
+                dh_finish<float, VEC><<<grid, 256, 0, s>>>(sum, w.dp, rows, resid, (const float*)E, (const float*)(G + col),
+                                                           w.vc, (const float*)Et, tail, (float*)dh, T, d);
+        };
+        if (vec) go(std::true_type{});
+        else go(std::false_type{});
         GN_LAUNCH_CHECK(who);
     }
     return GN_OK;
