@@ -57,39 +57,33 @@ struct StatsTile {
                                          unsigned char*, int lane) const {
         static_assert(FN == 2, "64 columns a wave");
         if (n0 >= g.N) return;
+        asm volatile("" : "+v"(lane));  // opaque: addresses are formed here, not kept across the k loop
         const int nh = 4 * (lane >> 5);
         float2* const out = part + (size_t)((v0 + n0) >> 6) * g.M;
-        int c[FM];  // the target's column among the wave's
-#pragma unroll
-        for (int i = 0; i < FM; ++i) c[i] = tgt[min(m0 + i * 32 + (lane & 31), g.M - 1)] - v0 - n0;
+        const bool edge = n0 + 64 > g.N;
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            float v[32];
+            const int row = m0 + i * 32 + (lane & 31);
+            const int c = tgt[min(row, g.M - 1)] - v0 - n0;  // the target's column among the wave's
+            // column of element e, and the element with -inf past the vocabulary's end
+            auto col = [&](int e) { return (e >> 4) * 32 + ((e >> 2) & 3) * 8 + nh + (e & 3); };
+            auto at = [&](int e) { return edge && n0 + col(e) >= g.N ? -INFINITY : acc[i][e >> 4][e & 15]; };
             float m = -INFINITY;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = acc[i][e >> 4][e & 15];
-            if (n0 + 64 > g.N) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    if (n0 + (e >> 4) * 32 + ((e >> 2) & 3) * 8 + nh + (e & 3) >= g.N) v[e] = -INFINITY;
-            }
-            const int row = m0 + i * 32 + (lane & 31);
-            if (__any((unsigned)c[i] < 64u)) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    if (c[i] == (e >> 4) * 32 + ((e >> 2) & 3) * 8 + nh + (e & 3) && row < g.M &&
-                        n0 + c[i] < g.N)
-                        lt[row] = v[e];
-            }
-#pragma unroll
-            for (int e = 0; e < 32; ++e) m = fmaxf(m, v[e]);
+            for (int e = 0; e < 32; ++e) m = fmaxf(m, at(e));
             m = fmaxf(m, __shfl_xor(m, 32));
             const float b = m == -INFINITY ? 0.f : m * kLog2e;
             float s = 0.f;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) s += __builtin_amdgcn_exp2f(fmaf(v[e], kLog2e, -b));
+            for (int e = 0; e < 32; ++e) s += __builtin_amdgcn_exp2f(fmaf(at(e), kLog2e, -b));
             s += __shfl_xor(s, 32);
             if (lane < 32 && row < g.M) out[row] = make_float2(m * kLog2e, s);
+            if (__any((unsigned)c < 64u)) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    if (c == col(e) && row < g.M) lt[row] = acc[i][e >> 4][e & 15];
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
@@ -109,14 +103,15 @@ struct GradTile {
                                          unsigned char* st, int lane) const {
         static_assert(FN == 2, "64 columns a wave");
         if (n0 >= ld) return;
+        asm volatile("" : "+v"(lane));  // as above
         const int mr = lane & 31, nh = 4 * (lane >> 5);
-        RowScale rs[FM];
-#pragma unroll
-        for (int i = 0; i < FM; ++i) rs[i] = rows[min(m0 + i * 32 + mr, g.M - 1)];
+        RowScale next = rows[min(m0 + mr, g.M - 1)];
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
+            const RowScale rs = next;
+            if (i + 1 < FM) next = rows[min(m0 + (i + 1) * 32 + mr, g.M - 1)];
             const int mw = m0 + i * 32, row = mw + mr;
-            const int c = __float_as_int(rs[i].w) - v0 - n0;
+            const int c = __float_as_int(rs.w) - v0 - n0;
             const bool hit = __any((unsigned)c < 64u), edge = n0 + 64 > g.N;
             uint2 low[LO ? 8 : 1];
             wave_lds_sync();
@@ -125,12 +120,12 @@ struct GradTile {
                 float x[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    x[e] = rs[i].y * __builtin_amdgcn_exp2f(fmaf(acc[i][k >> 2][4 * (k & 3) + e], kLog2e, -rs[i].x));
+                    x[e] = rs.y * __builtin_amdgcn_exp2f(fmaf(acc[i][k >> 2][4 * (k & 3) + e], kLog2e, -rs.x));
                 if (hit) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (c == 8 * k + nh + e) {
-                            x[e] -= rs[i].z;
+                            x[e] -= rs.z;
                             if (row < g.M) resid[row] = x[e] - bf2f(f2bf(x[e]));
                         }
                 }
@@ -144,6 +139,7 @@ struct GradTile {
                 if constexpr (LO)
                     low[k] = make_uint2(pack_bf2(x[0] - __uint_as_float(h.x << 16), x[1] - __uint_as_float(h.x & 0xffff0000u)),
                                         pack_bf2(x[2] - __uint_as_float(h.y << 16), x[3] - __uint_as_float(h.y & 0xffff0000u)));
+                __builtin_amdgcn_sched_barrier(0);
             }
             wave_lds_sync();
             flush(hi, g.M, mw, n0, st, lane);
@@ -202,32 +198,40 @@ __device__ __forceinline__ void finish_row(int t, float m, float s, const int32_
     if (loss) loss[t] = g >= 0 && g < V ? z - lt[t] : 0.f;
 }
 
-// lse and loss from the strips' statistics: 16 rows x 16 slices of the strips a block
+// lse and loss from the strips' statistics: R rows x 256 / R slices of the strips a block
+template <int R>
 __global__ __launch_bounds__(256) void row_stats(const float2* __restrict__ part, int strips, int T,
                                                  const int32_t* __restrict__ tgt, const float* __restrict__ lt,
                                                  float* __restrict__ loss, float* __restrict__ lse, int V) {
-    __shared__ float2 sh[16][17];
-    const int r = threadIdx.x & 15, sl = threadIdx.x >> 4, t = blockIdx.x * 16 + r;
+    constexpr int SL = 256 / R;
+    __shared__ float2 sh[SL][R + 1];
+    const int r = threadIdx.x % R, sl = threadIdx.x / R, t = blockIdx.x * R + r;
     float m = -INFINITY, s = 0.f;
     if (t < T) {
-        for (int k = sl; k < strips; k += 64) {
-            float2 p[4];
+        for (int k = sl; k < strips; k += 8 * SL) {
+            float2 p[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                p[j] = k + 16 * j < strips ? part[(size_t)(k + 16 * j) * T + t] : make_float2(-INFINITY, 0.f);
+            for (int j = 0; j < 8; ++j)
+                p[j] = k + SL * j < strips ? part[(size_t)(k + SL * j) * T + t] : make_float2(-INFINITY, 0.f);
+            float n = m;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) join(m, s, p[j].x, p[j].y);
+            for (int j = 0; j < 8; ++j) n = fmaxf(n, p[j].x);
+            s = about(s, m, n);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s += about(p[j].y, p[j].x, n);
+            m = n;
         }
     }
     sh[sl][r] = make_float2(m, s);
-    __syncthreads();
-    if (threadIdx.x < 16 && t < T) {
-        m = -INFINITY;
-        s = 0.f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) join(m, s, sh[k][r].x, sh[k][r].y);
-        finish_row(t, m, s, tgt, lt, loss, lse, V);
+    for (int k = SL / 2; k > 0; k /= 2) {
+        __syncthreads();
+        if (sl < k) {
+            const float2 o = sh[sl + k][r];
+            join(m, s, o.x, o.y);
+            sh[sl][r] = make_float2(m, s);
+        }
     }
+    if (sl == 0 && t < T) finish_row(t, m, s, tgt, lt, loss, lse, V);
 }
 
 // Every row's scales, and no residual yet; rows from T up to Tp (the fp32 products' padding) have none.
@@ -404,7 +408,7 @@ struct Plan {
     int vc, pieces;  // columns of a piece, a multiple of 128 (or all of a smaller vocabulary)
     size_t h, E, Et, lt, rows, resid, stats, logits, hi, lo, acc, de, det, part, part_bytes, bytes;
 
-    Plan(int T_, int d_, int V_, int dtype, bool lay_) : bf(dtype == GN_BF16), lay(lay_), T(T_), d(d_), V(V_) {
+    Plan(int T_, int d_, int V_, int dtype, bool lay_, bool bwd) : bf(dtype == GN_BF16), lay(lay_), T(T_), d(d_), V(V_) {
         q = bf ? 8 : 4;
         es = bf ? 2 : 4;
         lay = lay || d % q;
@@ -417,8 +421,8 @@ struct Plan {
         // the products' own split workspaces: of a whole piece and of the last one
         part_bytes = 0;
         const int last = (V - (pieces - 1) * vc) / q * q;
-        for (int nv : {pieces > 1 ? vc : last, last, V % q ? q : 0}) {
-            if (nv <= 0) continue;
+        for (int nv : {pieces > 1 ? vc : 0, last, V % q ? q : 0}) {
+            if (nv <= 0 || (bf && !bwd)) continue;
             GemmDesc a = product(nullptr, vc, nullptr, dp, Tp, nullptr, dp, nv, dp);
             GemmDesc b = product(nullptr, vc, nullptr, dp, nv, nullptr, dp, Tp, dp);
             if (bf) {
@@ -446,10 +450,11 @@ struct Plan {
         lt = take((size_t)T * 4);
         logits = take(bf ? 0 : (size_t)Tp * vc * 4);
         part = take(part_bytes);
-        const size_t both = at;  // from here on the forward and the backward have their own
-        stats = take(bf ? (size_t)((V + 127) / 128 * 2) * T * 8 : (size_t)T * 8);
-        const size_t fwd = at;
-        at = both;
+        if (!bwd) {
+            stats = take(bf ? (size_t)((V + 127) / 128 * 2) * T * 8 : (size_t)T * 8);
+            bytes = at;
+            return;
+        }
         rows = take((size_t)Tp * sizeof(RowScale));
         resid = take((size_t)Tp * 4);
         hi = take(bf ? (size_t)T * vc * 2 : 0);
@@ -457,15 +462,18 @@ struct Plan {
         acc = take((size_t)Tp * dp * 4);
         de = take(lay ? (size_t)vc * dp * 4 : 0);
         det = take((size_t)q * dp * 4);
-        bytes = std::max(fwd, at);
+        bytes = at;
     }
     // A piece of 512 MB: two pieces an 8192 x 32000 vocabulary, eight 8192 x 128000.
     static constexpr int64_t kPieceBytes = (int64_t)512 << 20;
 };
 
+// of either direction, whatever the tensors' alignment
 size_t workspace_bytes(int T, int d, int V, int dtype) {
-    // what alignment will be is not known from the shape
-    return std::max(Plan(T, d, V, dtype, false).bytes, Plan(T, d, V, dtype, true).bytes);
+    size_t most = 0;
+    for (const bool lay : {false, true})
+        for (const bool bwd : {false, true}) most = std::max(most, Plan(T, d, V, dtype, lay, bwd).bytes);
+    return most;
 }
 
 int check(const char* who, const void* h, const void* E, const int32_t* tgt, int T, int d, int V, int dtype) {
@@ -480,7 +488,13 @@ int check(const char* who, const void* h, const void* E, const int32_t* tgt, int
 }
 
 int check_ws(const char* who, const Plan& w, int dtype, const void* ws, size_t ws_bytes) {
-    const size_t need = workspace_bytes(w.T, w.d, w.V, dtype);
+    // the query's answer for the shape at hand (four plans, some microseconds)
+    thread_local int of[4] = {0, 0, 0, 0};
+    thread_local size_t need = 0;
+    if (of[0] != w.T || of[1] != w.d || of[2] != w.V || of[3] != dtype) {
+        need = workspace_bytes(w.T, w.d, w.V, dtype);
+        of[0] = w.T, of[1] = w.d, of[2] = w.V, of[3] = dtype;
+    }
     if (!ws || ws_bytes < need || !al16(ws)) {
         set_error("%s: workspace of %zu bytes (16-byte aligned) required", who, need);
         return GN_E_WORKSPACE;
@@ -557,7 +571,7 @@ extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* t
     if (const int rc = check(who, h, E, targets, T, d, V, dtype)) return rc;
     GN_REQUIRE((((uintptr_t)loss | (uintptr_t)lse) & 3u) == 0, "%s: loss, lse must be aligned to 4 bytes", who);
     if (T == 0 || (!loss && !lse)) return GN_OK;
-    const Plan w(T, d, V, dtype, !al16(h) || !al16(E));
+    const Plan w(T, d, V, dtype, !al16(h) || !al16(E), false);
     if (const int rc = check_ws(who, w, dtype, ws, ws_bytes)) return rc;
     char* const base = (char*)ws;
     Call c{who, w, base, h, E, as_stream(stream), dtype};
@@ -580,7 +594,9 @@ extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* t
         }
     }
     if (w.bf) {
-        row_stats<<<(T + 15) / 16, 256, 0, c.s>>>((const float2*)(base + w.stats), (V + 63) / 64, T, targets, lt, loss, lse, V);
+        const float2* part = (const float2*)(base + w.stats);
+        if (T < 2048) row_stats<2><<<(T + 1) / 2, 256, 0, c.s>>>(part, (V + 63) / 64, T, targets, lt, loss, lse, V);
+        else row_stats<16><<<(T + 15) / 16, 256, 0, c.s>>>(part, (V + 63) / 64, T, targets, lt, loss, lse, V);
         GN_LAUNCH_CHECK(who);
     }
     return GN_OK;
@@ -611,7 +627,7 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
     }
     GN_REQUIRE(lse, "%s: null pointer", who);
     if (!dh && !dE) return GN_OK;
-    const Plan w(T, d, V, dtype, !al16(h) || !al16(E) || !al16(dE));
+    const Plan w(T, d, V, dtype, !al16(h) || !al16(E) || !al16(dE), true);
     if (const int rc = check_ws(who, w, dtype, ws, ws_bytes)) return rc;
     char* const base = (char*)ws;
     Call c{who, w, base, h, E, s, dtype};

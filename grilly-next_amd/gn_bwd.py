@@ -11,6 +11,7 @@ Function names and argument meaning mirror the reference's backward ops
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -850,22 +851,35 @@ def glu_linear_fwd(kind, X, Wg, Wu, bg=None, bu=None):
 
 
 # ---- linear head with cross entropy, without its logits -----------------------------------
+_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else (lambda: -1)
+
+
+def _place(name, t, dtype):
+    """Refuses a tensor off the current device (whose stream the call goes to) or of another dtype."""
+    if not t.is_cuda:
+        raise GnError(f"{name}: tensor is not on the GPU")
+    if t.get_device() != _device():
+        raise GnError(f"{name} is on {t.device}, not on the current device")
+    if dtype is not None and t.dtype is not dtype:
+        raise GnError(f"{name} must be {dtype}, not {t.dtype}")
+
+
 def _here(name, t, dtype=None, shape=None):
-    """Device address of an argument, or None: contiguous, on the current device (whose stream the
-    call goes to), of the dtype and shape that the call needs."""
+    """Device address of an argument, or None: contiguous, on the current device, of the dtype and
+    shape that the call needs."""
     if t is None:
         return None
-    p = _ptr(t)
-    if t.device.index != torch._C._cuda_getDevice():
-        raise GnError(f"{name} is on {t.device}, not on the current device")
-    if dtype is not None and t.dtype != dtype:
-        raise GnError(f"{name} must be {dtype}, not {t.dtype}")
+    _place(name, t, dtype)
+    if not t.is_contiguous():
+        raise GnError(f"{name}: tensor must be contiguous")
     if shape is not None and t.shape != shape:
         raise GnError(f"{name} must be {list(shape)}, not {list(t.shape)}")
-    return p
+    return t.data_ptr()
 
 
+@functools.lru_cache(maxsize=256)
 def linear_xent_workspace_bytes(T, d, V, dtype):
+    """Workspace of linear_xent_fwd and linear_xent_bwd; dtype: a GN_* code."""
     return int(lib().gn_linear_xent_workspace_bytes(T, d, V, dtype))
 
 
@@ -925,26 +939,25 @@ def rope_freqs(rot, theta=10000.0, scaling="none", factor=1.0, trained=4096, fas
     return torch.tensor(list(f)[:rot // 2], dtype=torch.float64).to(device), m.value
 
 
-def _heads(name, t, shape=None, dtype=None, first=False):
+def _heads(name, t, shape, dtype, first=False):
     """gn_heads of a [B, S, H, D] tensor ([B, H, S, D] when first) whose last dimension is
-    contiguous; other strides are free."""
+    contiguous; other strides are free.  shape: what it has to be as [B, S, H, D], None: any."""
     if t is None:
         return None
-    if not t.is_cuda:
-        raise GnError(f"{name} is not on the GPU")
-    if t.device.index != torch._C._cuda_getDevice():
-        raise GnError(f"{name} is on {t.device}, not on the current device")
+    _place(name, t, dtype)
     if t.dim() != 4:
         raise GnError(f"{name} must have four dimensions, not {t.dim()}")
     if first:
-        t = t.transpose(1, 2)
-    if dtype is not None and t.dtype != dtype:
-        raise GnError(f"{name} must be {dtype}, not {t.dtype}")
-    if shape is not None and t.shape != shape:
-        raise GnError(f"{name} must be {list(shape)} ([B, S, H, D]), not {list(t.shape)}")
-    if t.shape[3] > 1 and t.stride(3) != 1:
+        b, h, n, d = t.shape
+        sb, sh, ss, sd = t.stride()
+    else:
+        b, n, h, d = t.shape
+        sb, ss, sh, sd = t.stride()
+    if shape is not None and (b, n, h, d) != shape:
+        raise GnError(f"{name} must be {list(shape)} as [B, S, H, D], not {[b, n, h, d]}")
+    if sd != 1 and d > 1:
         raise GnError(f"{name}: the elements of a head must be contiguous")
-    return Heads(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2])
+    return Heads(t.data_ptr(), sb, ss, sh, h)
 
 
 def _rope(freqs, mode, positions, pos0, mscale, B, S):
@@ -952,27 +965,30 @@ def _rope(freqs, mode, positions, pos0, mscale, B, S):
         return None
     if freqs.dim() != 1:
         raise GnError("freqs must have one dimension")
-    r = Rope(_here("freqs", freqs, torch.float64), None, 0, pos0, mscale, 2 * freqs.numel(), ROPE[mode])
+    f, p, sb = _here("freqs", freqs, torch.float64), None, 0
     if positions is not None:
-        r.positions = _here("positions", positions, torch.int32)
+        p = _here("positions", positions, torch.int32)
         if positions.shape == (B, S):
-            r.pos_sb = S
+            sb = S
         elif positions.shape != (S,):
             raise GnError(f"positions must be [{S}] or [{B}, {S}], not {list(positions.shape)}")
-    return r
+    return Rope(f, p, sb, pos0, mscale, 2 * freqs.numel(), ROPE[mode])
 
 
 def _empty_heads(shape, like, first):
+    if shape is None:
+        return None
     B, S, H, D = shape
-    return torch.empty((B, H, S, D) if first else (B, S, H, D), dtype=like.dtype, device=like.device)
+    return torch.empty((B, H, S, D) if first else shape, dtype=like.dtype, device=like.device)
 
 
 def _rope_call(fn, name, x, freqs, mode, positions, pos0, mscale, out):
-    xh = _heads("x", x)
-    B, S, H, D = x.shape
-    y = _empty_heads(x.shape, x, False) if out is None else out
+    xh = _heads("x", x, None, None)
+    B, S, H, D = shape = tuple(x.shape)
+    y = _empty_heads(shape, x, False) if out is None else out
+    yh = _heads("out", y, shape, x.dtype)
     r = _rope(freqs, mode, positions, pos0, mscale, B, S)
-    _check(fn(xh, _heads("out", y, x.shape, x.dtype), r, B, S, D, _dt(x), _stream()), name)
+    _check(fn(xh, yh, r, B, S, D, _dt(x), _stream()), name)
     return y
 
 
@@ -994,12 +1010,23 @@ def qk_norm_rope_workspace_bytes(B, S, D):
 
 def _qk(q, k, wq, wk):
     """The shapes and checked views of q and k, and the weights."""
-    qh = _heads("q", q)
-    B, S, _, D = q.shape
+    dt = q.dtype
+    qh = _heads("q", q, None, dt)
+    qs = B, S, _, D = tuple(q.shape)
     ks = None if k is None else (B, S, k.shape[2] if k.dim() == 4 else 0, D)
-    kh = _heads("k", k, ks, q.dtype)
-    w = (_here("wq", wq, q.dtype, (D,)), _here("wk", wk, q.dtype, (D,)))
-    return B, S, D, tuple(q.shape), ks, qh, kh, w
+    return B, S, D, qs, ks, qh, _heads("k", k, ks, dt), _here("wq", wq, dt, (D,)), _here("wk", wk, dt, (D,))
+
+
+def _qk_out(out, shapes, like, first, names):
+    """The three outputs, allocated or given, and their checked views."""
+    if out is None:
+        out = tuple(_empty_heads(s, like, first) for s in shapes)
+    elif len(out) < 3:
+        out = tuple(out) + (None,) * (3 - len(out))
+    for name, o, s in zip(names, out, shapes):
+        if (o is None) != (s is None):
+            raise GnError(f"out: {name} goes with its input")
+    return out, [_heads(n, o, s, like.dtype, first) for n, o, s in zip(names, out, shapes)]
 
 
 def qk_norm_rope_fwd(q, k, wq=None, wk=None, freqs=None, v=None, mode="half", positions=None, pos0=0, mscale=1.0,
@@ -1007,20 +1034,13 @@ def qk_norm_rope_fwd(q, k, wq=None, wk=None, freqs=None, v=None, mode="half", po
     """(yq, yk), or (yq, yk, yv) when v is given: q and k [B, S, H, D] (views; k may have fewer heads,
     or be None) normed per head, y = x rsqrt(mean(x^2) + eps) w, and rotated as by rope_fwd (freqs None: not);
     v copied.  heads_first: the outputs are [B, H, S, D], as attn_fwd takes them; `out` gives them."""
-    B, S, D, qs, ks, qh, kh, w = _qk(q, k, wq, wk)
-    vh = _heads("v", v, None if v is None or k is None else ks, q.dtype)
-    vs = None if v is None else tuple(v.shape)
-    if v is not None and (vs[0], vs[1], vs[3]) != (B, S, D):
-        raise GnError(f"v must be [{B}, {S}, H, {D}], not {list(vs)}")
+    B, S, D, qs, ks, qh, kh, wqp, wkp = _qk(q, k, wq, wk)
+    vs = None if v is None else (B, S, v.shape[2] if v.dim() == 4 else 0, D)
+    vh = _heads("v", v, vs, q.dtype)
     r = _rope(freqs, mode, positions, pos0, mscale, B, S)
-    if out is None:
-        out = tuple(None if s is None else _empty_heads(s, q, heads_first) for s in (qs, ks, vs))
-    out = tuple(out) + (None,) * (3 - len(out))
-    for name, o, s in (("yk", out[1], ks), ("yv", out[2], vs)):
-        if (o is None) != (s is None):
-            raise GnError(f"out: {name} goes with its input")
-    yh = [_heads(n, o, s, q.dtype, heads_first) for n, o, s in zip(("yq", "yk", "yv"), out, (qs, ks, vs))]
-    _check(lib().gn_qk_norm_rope_fwd(qh, kh, vh, *w, *yh, r, B, S, D, eps, _dt(q), _stream()), "gn_qk_norm_rope_fwd")
+    out, yh = _qk_out(out, (qs, ks, vs), q, heads_first, ("yq", "yk", "yv"))
+    _check(lib().gn_qk_norm_rope_fwd(qh, kh, vh, wqp, wkp, *yh, r, B, S, D, eps, _dt(q), _stream()),
+           "gn_qk_norm_rope_fwd")
     return out if v is not None else out[:2]
 
 
@@ -1031,23 +1051,16 @@ def qk_norm_rope_bwd(dyq, dyk, q, k, wq=None, wk=None, freqs=None, dyv=None, mod
     (heads_first: [B, H, S, D]).  dq, dk, dv [B, S, H, D], or the views in `out` (the parts of a fused
     dqkv, say); dv is None without dyv.  dwq, dwk fp32 [D]; accumulate adds onto given ones; need_dw
     False: neither."""
-    B, S, D, qs, ks, qh, kh, w = _qk(q, k, wq, wk)
+    B, S, D, qs, ks, qh, kh, wqp, wkp = _qk(q, k, wq, wk)
     if (k is None) != (dyk is None):
         raise GnError("dyk goes with k")
-    vs = None
-    if dyv is not None:
-        if dyv.dim() != 4:
-            raise GnError(f"dyv must have four dimensions, not {dyv.dim()}")
-        vs = (B, S, dyv.shape[1 if heads_first else 2], D)
-    dyh = [_heads(n, t, s, q.dtype, heads_first) for n, t, s in (("dyq", dyq, qs), ("dyk", dyk, ks), ("dyv", dyv, vs))]
+    vs = None if dyv is None else (B, S, dyv.shape[1 if heads_first else 2] if dyv.dim() == 4 else 0, D)
+    dt = q.dtype
+    dyqh = _heads("dyq", dyq, qs, dt, heads_first)
+    dykh = _heads("dyk", dyk, ks, dt, heads_first)
+    dyvh = _heads("dyv", dyv, vs, dt, heads_first)
     r = _rope(freqs, mode, positions, pos0, mscale, B, S)
-    if out is None:
-        out = tuple(None if s is None else _empty_heads(s, q, False) for s in (qs, ks, vs))
-    out = tuple(out) + (None,) * (3 - len(out))
-    for name, o, s in (("dk", out[1], ks), ("dv", out[2], vs)):
-        if (o is None) != (s is None):
-            raise GnError(f"out: {name} goes with its input")
-    dh = [_heads(n, o, s, q.dtype) for n, o, s in zip(("dq", "dk", "dv"), out, (qs, ks, vs))]
+    out, dh = _qk_out(out, (qs, ks, vs), q, False, ("dq", "dk", "dv"))
     f32 = torch.float32
     if need_dw:
         if accumulate and (dwq is None or (k is not None and dwk is None)):
@@ -1061,8 +1074,8 @@ def qk_norm_rope_bwd(dyq, dyk, q, k, wq=None, wk=None, freqs=None, dyv=None, mod
     else:
         dwq = dwk = None
     wsp, wsb = (None, 0) if ws is None else (_here("ws", ws), ws.numel() * ws.element_size())
-    _check(lib().gn_qk_norm_rope_bwd(*dyh, qh, kh, *w, *dh, _here("dwq", dwq, f32, (D,)), _here("dwk", dwk, f32, (D,)), r,
-                                     B, S, D, eps, _dt(q), ACCUMULATE if accumulate else 0, wsp, wsb, _stream()),
+    _check(lib().gn_qk_norm_rope_bwd(dyqh, dykh, dyvh, qh, kh, wqp, wkp, *dh, _here("dwq", dwq, f32, (D,)),
+                                     _here("dwk", dwk, f32, (D,)), r, B, S, D, eps, _dt(q), ACCUMULATE if accumulate else 0, wsp, wsb, _stream()),
            "gn_qk_norm_rope_bwd")
     return (*out, dwq, dwk)
 
