@@ -90,7 +90,9 @@ struct KFeed {
     }
 };
 
-// EPI: none (C in type CT), or one object whose tile() takes each finished tile instead.
+// EPI: none (C in type CT), or one object whose tile() takes each finished tile instead; its begin() is
+// called before the tile's k-tiles, with the same 4 KB of LDS of the wave, which is its own
+// from then on.
 template <bool TA, bool TB, typename CT, int BM, int BN, int STAGES, typename... EPI>
 __global__ __launch_bounds__(512, 1) void gemm_stream(GemmDesc g, EPI... epi) {
     constexpr int NW = 4;
@@ -286,6 +288,11 @@ __global__ __launch_bounds__(512, 1) void gemm_stream(GemmDesc g, EPI... epi) {
     static_for<NR>([&](auto R_) { read_one(I1{}, R_, stage_ptr(0), 1); });
     int slot = 0;
     for (int i = 0; i < ntile; ++i) {
+        if constexpr (sizeof...(EPI) > 0) {
+            int m0, n0;
+            tile_at(i, m0, n0);
+            (epi.template begin<FM>(g, m0 + wm * WM, st, lane), ...);
+        }
 #pragma unroll
         for (int a = 0; a < FM; ++a)
 #pragma unroll

@@ -46,16 +46,45 @@ __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
 // ---- bf16: epilogues of the logits' product -------------------------------------------------
 // Element r of a 32 x 32 accumulator: row lane % 32, column 8 (r / 4) + 4 (lane / 32) + r % 4.
 
+// What the epilogue takes of each of the wave's rows is brought into the wave's LDS by DMA while the tile's
+// k-tiles run (loads at the tile's end would stand in its way, and registers over the k loop are
+// not to be had).  BYTES 4 or 16 a row, 32 FM rows; begin() starts it, wait() ends it.
+template <int FM, int BYTES>
+__device__ __forceinline__ void rows_begin(const void* src, int m0, int M, unsigned char* st, int lane) {
+    // the previous tile's reads of this LDS have returned
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(63) & 0xF0FFu);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_addr(st));
+#pragma unroll
+    for (int k = 0; k < (FM + 1) / 2; ++k) {  // 64 rows an instruction (32 FM of them are used)
+        const char* from = (const char*)src + (size_t)min(m0 + 64 * k + lane, M - 1) * BYTES;
+        if constexpr (BYTES == 16) {
+            dma16(from, to + 1024u * k);
+        } else {
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+                         : : "s"(to + 256u * k), "v"(from) : "memory", "m0");
+        }
+    }
+}
+__device__ __forceinline__ void rows_wait() {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    wave_lds_sync();
+}
+
 // Each row's statistics over the wave's 64 columns, and its target's logit.
 struct StatsTile {
     const int32_t* tgt;
     float* lt;      // [T] the target's logit
     float2* part;   // [strips][T]
     int v0;         // the vocabulary's column of column 0 here
+    template <int FM>
+    __device__ __forceinline__ void begin(const GemmDesc& g, int m0, unsigned char* st, int lane) const {
+        rows_begin<FM, 4>(tgt, m0, g.M, st, lane);
+    }
     template <int FM, int FN>
     __device__ __forceinline__ void tile(const GemmDesc& g, const f32x16_t (&acc)[FM][FN], int m0, int n0,
-                                         unsigned char*, int lane) const {
+                                         unsigned char* st, int lane) const {
         static_assert(FN == 2, "64 columns a wave");
+        rows_wait();
         if (n0 >= g.N) return;
         asm volatile("" : "+v"(lane));  // opaque: addresses are formed here, not kept across the k loop
         const int nh = 4 * (lane >> 5);
@@ -64,7 +93,7 @@ struct StatsTile {
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
             const int row = m0 + i * 32 + (lane & 31);
-            const int c = tgt[min(row, g.M - 1)] - v0 - n0;  // the target's column among the wave's
+            const int c = reinterpret_cast<const int*>(st)[i * 32 + (lane & 31)] - v0 - n0;  // the target's column among the wave's
             // column of element e, and the element with -inf past the vocabulary's end
             auto col = [&](int e) { return (e >> 4) * 32 + ((e >> 2) & 3) * 8 + nh + (e & 3); };
             auto at = [&](int e) { return edge && n0 + col(e) >= g.N ? -INFINITY : acc[i][e >> 4][e & 15]; };
@@ -98,18 +127,24 @@ struct GradTile {
     bf16_t *hi, *lo;  // [T x ld]
     float* resid;     // [T] what rounding the target's element to hi left
     int ld, v0;
+    template <int FM>
+    __device__ __forceinline__ void begin(const GemmDesc& g, int m0, unsigned char* st, int lane) const {
+        rows_begin<FM, 16>(rows, m0, g.M, st, lane);
+    }
     template <int FM, int FN>
     __device__ __forceinline__ void tile(const GemmDesc& g, const f32x16_t (&acc)[FM][FN], int m0, int n0,
                                          unsigned char* st, int lane) const {
         static_assert(FN == 2, "64 columns a wave");
+        rows_wait();
         if (n0 >= ld) return;
         asm volatile("" : "+v"(lane));  // as above
         const int mr = lane & 31, nh = 4 * (lane >> 5);
-        RowScale next = rows[min(m0 + mr, g.M - 1)];
+        RowScale scales[FM];  // out of the LDS that G then goes through
+#pragma unroll
+        for (int i = 0; i < FM; ++i) scales[i] = reinterpret_cast<const RowScale*>(st)[i * 32 + mr];
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            const RowScale rs = next;
-            if (i + 1 < FM) next = rows[min(m0 + (i + 1) * 32 + mr, g.M - 1)];
+            const RowScale rs = scales[i];
             const int mw = m0 + i * 32, row = mw + mr;
             const int c = __float_as_int(rs.w) - v0 - n0;
             const bool hit = __any((unsigned)c < 64u), edge = n0 + 64 > g.N;
@@ -139,7 +174,7 @@ struct GradTile {
                 if constexpr (LO)
                     low[k] = make_uint2(pack_bf2(x[0] - __uint_as_float(h.x << 16), x[1] - __uint_as_float(h.x & 0xffff0000u)),
                                         pack_bf2(x[2] - __uint_as_float(h.y << 16), x[3] - __uint_as_float(h.y & 0xffff0000u)));
-                __builtin_amdgcn_sched_barrier(0);
+                if (k & 1) __builtin_amdgcn_sched_barrier(0);
             }
             wave_lds_sync();
             flush(hi, g.M, mw, n0, st, lane);
@@ -164,9 +199,9 @@ struct GradTile {
     }
 };
 
-template <int BM, typename EPI>
+template <int BM, int STAGES, typename EPI>
 int launch_logits_tile(const GemmDesc& g, const EPI& epi, hipStream_t s) {
-    constexpr int BN = 128, STAGES = 3;
+    constexpr int BN = 128;
     constexpr size_t smem = (size_t)STAGES * (BM + BN) * BK * sizeof(bf16_t) + 4 * 4096;
     static_assert(smem <= 160 * 1024, "LDS per CU");
     static const bool ok = allow_lds(gemm_stream<false, true, float, BM, BN, STAGES, EPI>, smem);
@@ -182,12 +217,14 @@ int launch_logits_tile(const GemmDesc& g, const EPI& epi, hipStream_t s) {
 }
 
 // 256-row tiles, or 128-row ones where they need less (the streamed products' rule: a round of them
-// takes 0.6 of a round of the large)
+// takes 0.6 of a round of the large).  Up to 64 rows the product is a read of E: 64-row tiles leave the
+// LDS to six stages, 80 KB of E on its way to each compute unit.
 template <typename EPI>
 int launch_logits(const GemmDesc& g, const EPI& epi, hipStream_t s) {
     const long blocks = stream_blocks(), tn = (g.N + 127) / 128;
     const long r256 = ((g.M + 255) / 256 * tn + blocks - 1) / blocks, r128 = ((g.M + 127) / 128 * tn + blocks - 1) / blocks;
-    return 0.62 * (double)r128 < (double)r256 ? launch_logits_tile<128>(g, epi, s) : launch_logits_tile<256>(g, epi, s);
+    if (g.M <= 64) return launch_logits_tile<64, 6>(g, epi, s);
+    return 0.62 * (double)r128 < (double)r256 ? launch_logits_tile<128, 3>(g, epi, s) : launch_logits_tile<256, 3>(g, epi, s);
 }
 
 __device__ __forceinline__ void finish_row(int t, float m, float s, const int32_t* tgt, const float* lt, float* loss,
@@ -464,8 +501,9 @@ struct Plan {
         det = take((size_t)q * dp * 4);
         bytes = at;
     }
-    // A piece of 512 MB: two pieces an 8192 x 32000 vocabulary, eight 8192 x 128000.
-    static constexpr int64_t kPieceBytes = (int64_t)512 << 20;
+    // Measured (us, pieces of 128, 256, 512, 1024 MB): 8190 x 768 x 32000 2479, 2376, 2412, 2238; 2001 x 1024 x
+    // 50001 971, 931, 920, 918; 8192 x 2048 x 128000 19.7, 19.1, 20.1, 20.0 ms.
+    static constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 };
 
 // of either direction, whatever the tensors' alignment
@@ -595,7 +633,7 @@ extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* t
     }
     if (w.bf) {
         const float2* part = (const float2*)(base + w.stats);
-        if (T < 2048) row_stats<2><<<(T + 1) / 2, 256, 0, c.s>>>(part, (V + 63) / 64, T, targets, lt, loss, lse, V);
+        if (T < 256) row_stats<2><<<(T + 1) / 2, 256, 0, c.s>>>(part, (V + 63) / 64, T, targets, lt, loss, lse, V);
         else row_stats<16><<<(T + 15) / 16, 256, 0, c.s>>>(part, (V + 63) / 64, T, targets, lt, loss, lse, V);
         GN_LAUNCH_CHECK(who);
     }

@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kThreads = 256;
 
-enum Kind { kRotate, kNorm, kNormBwd };
+enum Kind { kRotate, kNorm };
 
 struct Group {
     const void *x, *dy, *w;  // input of the norm (or of the rotation); upstream gradient; weights
@@ -42,9 +42,11 @@ struct Args {
     const int32_t* pos;
     int64_t pos_sb, pos0;
     float mscale, sgn, eps;  // sgn: -1 turns back
-    int rot, S, D, tokens, TB, tiles;
-    float* part;    // [gridDim.x][2][D] partial dw, nullptr: not wanted
-    float* dw[2];   // a single block's dw goes straight here
+    int rot, S, D, tokens;
+    int TB[2], tiles[2];  // tokens of a tile and tiles: of all groups, or (backward) of q and of k, v
+    int nq, with_copy;    // backward: the blocks of q; whose blocks copy the values
+    float* part;          // [gridDim.x][D] partial dw, nullptr: not wanted
+    float* dw[2];         // where one block has all of a dw, it goes straight here
     int accumulate;
 };
 
@@ -91,13 +93,55 @@ struct Row {
     }
     __device__ __forceinline__ bool has(int i) const { return VEC ? on : 2 * (l + 64 * i) < D; }
 
-    __device__ __forceinline__ void ld(const T* p, bool live, float (&u)[NP], float (&w)[NP]) const {
+    // a lane's elements as they lie in memory
+    struct Raw {
+        static constexpr int Q = VEC ? 8 * (int)sizeof(T) / 16 : 1;
+        uint4 a[Q], b[Q];
+        T s[VEC ? 1 : 2 * NP];
+    };
+    __device__ __forceinline__ void raw(const T* p, bool live, Raw& r) const {
         if constexpr (VEC) {
-            float a[8] = {}, b[8] = {};
+#pragma unroll
+            for (int q = 0; q < Raw::Q; ++q) r.a[q] = r.b[q] = make_uint4(0, 0, 0, 0);
             if (live && on) {
-                chunk8<T>::ld(p + c0, a);
-                chunk8<T>::ld(p + c1, b);
+#pragma unroll
+                for (int q = 0; q < Raw::Q; ++q) {
+                    r.a[q] = reinterpret_cast<const uint4*>(p + c0)[q];
+                    r.b[q] = reinterpret_cast<const uint4*>(p + c1)[q];
+                }
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const bool ok = live && has(i);
+                r.s[2 * i] = ok ? p[first(i)] : (T)0;
+                r.s[2 * i + 1] = ok ? p[second(i)] : (T)0;
+            }
+        }
+    }
+    static __device__ __forceinline__ void widen8(const uint4* p, float (&v)[8]) {
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t w[4] = {p->x, p->y, p->z, p->w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                v[4 * q] = __uint_as_float(p[q].x);
+                v[4 * q + 1] = __uint_as_float(p[q].y);
+                v[4 * q + 2] = __uint_as_float(p[q].z);
+                v[4 * q + 3] = __uint_as_float(p[q].w);
+            }
+        }
+    }
+    __device__ __forceinline__ void widen(const Raw& r, float (&u)[NP], float (&w)[NP]) const {
+        if constexpr (VEC) {
+            float a[8], b[8];
+            widen8(r.a, a);
+            widen8(r.b, b);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 u[i] = HALF ? a[i] : (i < 4 ? a[(2 * i) & 7] : b[(2 * i) & 7]);
@@ -106,11 +150,15 @@ struct Row {
         } else {
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                const bool ok = live && has(i);
-                u[i] = ok ? io<T>::ld(p, first(i)) : 0.f;
-                w[i] = ok ? io<T>::ld(p, second(i)) : 0.f;
+                u[i] = io<T>::ld(r.s, 2 * i);
+                w[i] = io<T>::ld(r.s, 2 * i + 1);
             }
         }
+    }
+    __device__ __forceinline__ void ld(const T* p, bool live, float (&u)[NP], float (&w)[NP]) const {
+        Raw r;
+        raw(p, live, r);
+        widen(r, u, w);
     }
     __device__ __forceinline__ void st(T* p, bool live, const float (&u)[NP], const float (&w)[NP]) const {
         if constexpr (VEC) {
@@ -182,14 +230,12 @@ __device__ __forceinline__ void token_head(const Group& g, int r, int& tt, int& 
     h = r - tt * g.H;
 }
 
+// Forward: rows in flight, U a lane
 template <typename T, int LPR, bool VEC, bool HALF, int KIND>
 __device__ __forceinline__ void group(const Args& a, const Group& g, int n, const float* cosv, const float* sinv,
-                                      const int2* bs, const Row<T, LPR, VEC, HALF>& row,
-                                      float (&du)[Row<T, LPR, VEC, HALF>::NP],
-                                      float (&dv)[Row<T, LPR, VEC, HALF>::NP]) {
+                                      const int2* bs, const Row<T, LPR, VEC, HALF>& row) {
     using R = Row<T, LPR, VEC, HALF>;
-    constexpr int NP = R::NP, NG = R::NG;
-    constexpr int U = KIND == kNormBwd ? 1 : 2;  // rows in flight per lane
+    constexpr int NP = R::NP, NG = R::NG, U = 2;
     const int rows = n * g.H, mine = threadIdx.x / LPR;
     float wu[NP], ww[NP];
 #pragma unroll
@@ -197,7 +243,7 @@ __device__ __forceinline__ void group(const Args& a, const Group& g, int n, cons
     if (KIND != kRotate && g.w) row.ld((const T*)g.w, true, wu, ww);
     const float inv_d = 1.0f / (float)a.D;
     for (int base = 0; base < rows; base += NG * U) {
-        float u[U][NP], w[U][NP], gu[KIND == kNormBwd ? U : 1][NP], gw[KIND == kNormBwd ? U : 1][NP];
+        float u[U][NP], w[U][NP];
         int tt[U], h[U];
         bool live[U];
 #pragma unroll
@@ -206,52 +252,86 @@ __device__ __forceinline__ void group(const Args& a, const Group& g, int n, cons
             live[k] = r < rows;
             token_head(g, min(r, rows - 1), tt[k], h[k]);
             row.ld((const T*)g.x + at(g.xs, bs[tt[k]], h[k]), live[k], u[k], w[k]);
-            if constexpr (KIND == kNormBwd) row.ld((const T*)g.dy + at(g.ds, bs[tt[k]], h[k]), live[k], gu[k], gw[k]);
         }
 #pragma unroll
         for (int k = 0; k < U; ++k) {
             float c[NP], s[NP], yu[NP], yw[NP];
             row.angles(cosv, sinv, tt[k], c, s);
-            if constexpr (KIND == kNormBwd) {
-                float s2 = 0.f, sx = 0.f;
+            if constexpr (KIND == kNorm) {
+                float s2 = 0.f;
+#pragma unroll
+                for (int i = 0; i < NP; ++i) s2 += u[k][i] * u[k][i] + w[k][i] * w[k][i];
+                const float r = rsqrtf(R::sum(s2) * inv_d + a.eps);
 #pragma unroll
                 for (int i = 0; i < NP; ++i) {
-                    // dy turned back (sin carries the sign)
-                    yu[i] = gu[k][i] * c[i] - gw[k][i] * s[i];
-                    yw[i] = gw[k][i] * c[i] + gu[k][i] * s[i];
-                    s2 += u[k][i] * u[k][i] + w[k][i] * w[k][i];
-                    sx += wu[i] * yu[i] * u[k][i] + ww[i] * yw[i] * w[k][i];
+                    u[k][i] *= r * wu[i];
+                    w[k][i] *= r * ww[i];
                 }
-                s2 = R::sum(s2);
-                sx = R::sum(sx);
-                const float r = rsqrtf(s2 * inv_d + a.eps), q = r * r * sx * inv_d;
+            }
 #pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    du[i] += yu[i] * u[k][i] * r;
-                    dv[i] += yw[i] * w[k][i] * r;
-                    yu[i] = r * (wu[i] * yu[i] - u[k][i] * q);
-                    yw[i] = r * (ww[i] * yw[i] - w[k][i] * q);
-                }
-            } else {
-                if constexpr (KIND == kNorm) {
-                    float s2 = 0.f;
-#pragma unroll
-                    for (int i = 0; i < NP; ++i) s2 += u[k][i] * u[k][i] + w[k][i] * w[k][i];
-                    const float r = rsqrtf(R::sum(s2) * inv_d + a.eps);
-#pragma unroll
-                    for (int i = 0; i < NP; ++i) {
-                        u[k][i] *= r * wu[i];
-                        w[k][i] *= r * ww[i];
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < NP; ++i) {
-                    yu[i] = u[k][i] * c[i] - w[k][i] * s[i];
-                    yw[i] = w[k][i] * c[i] + u[k][i] * s[i];
-                }
+            for (int i = 0; i < NP; ++i) {
+                yu[i] = u[k][i] * c[i] - w[k][i] * s[i];
+                yw[i] = w[k][i] * c[i] + u[k][i] * s[i];
             }
             row.st((T*)g.y + at(g.ys, bs[tt[k]], h[k]), live[k], yu, yw);
         }
+    }
+}
+
+// Backward: the next row's x and dy are loaded, as they lie in memory, before a row is worked on.
+template <typename T, int LPR, bool VEC, bool HALF>
+__device__ __forceinline__ void group_bwd(const Args& a, const Group& g, int n, const float* cosv, const float* sinv,
+                                          const int2* bs, const Row<T, LPR, VEC, HALF>& row,
+                                          float (&du)[Row<T, LPR, VEC, HALF>::NP],
+                                          float (&dv)[Row<T, LPR, VEC, HALF>::NP]) {
+    using R = Row<T, LPR, VEC, HALF>;
+    constexpr int NP = R::NP, NG = R::NG;
+    const int rows = n * g.H, mine = threadIdx.x / LPR;
+    const float inv_d = 1.0f / (float)a.D;
+    typename R::Raw x, dy, wr;
+    int tt, h;
+    row.raw((const T*)g.w, g.w != nullptr, wr);
+    token_head(g, min(mine, rows - 1), tt, h);
+    row.raw((const T*)g.x + at(g.xs, bs[tt], h), mine < rows, x);
+    row.raw((const T*)g.dy + at(g.ds, bs[tt], h), mine < rows, dy);
+    for (int base = 0; base < rows; base += NG) {
+        const int r0 = base + mine, t0 = tt, h0 = h;
+        float u[NP], w[NP], yu[NP], yw[NP];
+        row.widen(x, u, w);
+        {
+            float gu[NP], gw[NP], c[NP], s[NP];
+            row.widen(dy, gu, gw);
+            if (base + NG < rows) {
+                token_head(g, min(r0 + NG, rows - 1), tt, h);
+                row.raw((const T*)g.x + at(g.xs, bs[tt], h), r0 + NG < rows, x);
+                row.raw((const T*)g.dy + at(g.ds, bs[tt], h), r0 + NG < rows, dy);
+            }
+            row.angles(cosv, sinv, t0, c, s);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {  // dy turned back (sin carries the sign)
+                yu[i] = gu[i] * c[i] - gw[i] * s[i];
+                yw[i] = gw[i] * c[i] + gu[i] * s[i];
+            }
+        }
+        float wu[NP], ww[NP], s2 = 0.f, sx = 0.f;
+        row.widen(wr, wu, ww);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            if (!g.w) wu[i] = ww[i] = 1.f;
+            s2 += u[i] * u[i] + w[i] * w[i];
+            sx += wu[i] * yu[i] * u[i] + ww[i] * yw[i] * w[i];
+        }
+        s2 = R::sum(s2);
+        sx = R::sum(sx);
+        const float r = rsqrtf(s2 * inv_d + a.eps), q = r * r * sx * inv_d;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            du[i] += yu[i] * u[i] * r;
+            dv[i] += yw[i] * w[i] * r;
+            yu[i] = r * (wu[i] * yu[i] - u[i] * q);
+            yw[i] = r * (ww[i] * yw[i] - w[i] * q);
+        }
+        row.st((T*)g.y + at(g.ys, bs[t0], h0), r0 < rows, yu, yw);
     }
 }
 
@@ -290,95 +370,109 @@ __device__ __forceinline__ void copy_group(const Group& g, int n, const int2* bs
     }
 }
 
+// A tile's places and angles
+__device__ __forceinline__ void tile_angles(const Args& a, int t0, int n, float* cosv, float* sinv, int2* bs) {
+    const int hr = a.rot >> 1;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const int b = (t0 + i) / a.S;
+        bs[i] = make_int2(b, t0 + i - b * a.S);
+    }
+    for (int i = threadIdx.x; i < n * hr; i += kThreads) {
+        const int tt = i / hr, p = i - tt * hr, b = (t0 + tt) / a.S, s = t0 + tt - b * a.S;
+        const double pos = a.pos ? (double)a.pos[b * a.pos_sb + s] : (double)(a.pos0 + s);
+        const double turns = pos * (a.freqs[p] * 0.15915494309189533577);
+        float sn, cs;
+        sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
+        cosv[i] = a.mscale * cs;
+        sinv[i] = a.mscale * a.sgn * sn;
+    }
+    __syncthreads();
+}
+
 template <typename T, int LPR, bool VEC, bool HALF, int KIND>
 __global__ __launch_bounds__(kThreads) void rope_kernel(Args a) {
+    extern __shared__ __align__(16) unsigned char smem[];
+    float* const cosv = reinterpret_cast<float*>(smem);
+    float* const sinv = cosv + a.TB[0] * (a.rot >> 1);
+    int2* const bs = reinterpret_cast<int2*>(sinv + a.TB[0] * (a.rot >> 1));
+    const Row<T, LPR, VEC, HALF> row(a.D, a.rot);
+    const int t0 = blockIdx.x * a.TB[0], n = min(a.TB[0], a.tokens - t0);
+    tile_angles(a, t0, n, cosv, sinv, bs);
+    group<T, LPR, VEC, HALF, KIND>(a, a.g[0], n, cosv, sinv, bs, row);
+    if (KIND != kRotate && a.ng > 1) group<T, LPR, VEC, HALF, KIND>(a, a.g[1], n, cosv, sinv, bs, row);
+    if (KIND != kRotate && a.copy.H) copy_group<T, LPR, VEC, HALF>(a.copy, n, bs, row);
+}
+
+// Backward: the first nq blocks take the queries, the others the keys and values (a block's dw is one
+// weight's: half the registers of both), each walking over its tiles.
+template <typename T, int LPR, bool VEC, bool HALF>
+__global__ __launch_bounds__(kThreads, 3) void norm_bwd_kernel(Args a) {
     using R = Row<T, LPR, VEC, HALF>;
     constexpr int NP = R::NP, NG = R::NG;
     extern __shared__ __align__(16) unsigned char smem[];
-    const int hr = a.rot >> 1;
+    const int k = (int)blockIdx.x >= a.nq;
+    const int TB = a.TB[k], first = k ? blockIdx.x - a.nq : blockIdx.x, step = k ? gridDim.x - a.nq : a.nq;
     float* const cosv = reinterpret_cast<float*>(smem);
-    float* const sinv = cosv + a.TB * hr;
-    int2* const bs = reinterpret_cast<int2*>(sinv + a.TB * hr);
+    float* const sinv = cosv + TB * (a.rot >> 1);
+    int2* const bs = reinterpret_cast<int2*>(sinv + TB * (a.rot >> 1));
     const R row(a.D, a.rot);
-    float du[2][NP], dv[2][NP];
+    float du[NP], dv[NP];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int i = 0; i < NP; ++i) du[k][i] = dv[k][i] = 0.f;
-
-    for (int tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-        const int t0 = tile * a.TB, n = min(a.TB, a.tokens - t0);
-        if (KIND == kNormBwd) __syncthreads();  // the tile before has been read
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const int b = (t0 + i) / a.S;
-            bs[i] = make_int2(b, t0 + i - b * a.S);
-        }
-        for (int i = threadIdx.x; i < n * hr; i += kThreads) {
-            const int tt = i / hr, p = i - tt * hr, b = (t0 + tt) / a.S, s = t0 + tt - b * a.S;
-            const double pos = a.pos ? (double)a.pos[b * a.pos_sb + s] : (double)(a.pos0 + s);
-            const double turns = pos * (a.freqs[p] * 0.15915494309189533577);
-            float sn, cs;
-            sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
-            cosv[i] = a.mscale * cs;
-            sinv[i] = a.mscale * a.sgn * sn;
-        }
-        __syncthreads();
-        group<T, LPR, VEC, HALF, KIND>(a, a.g[0], n, cosv, sinv, bs, row, du[0], dv[0]);
-        if (KIND != kRotate && a.ng > 1) group<T, LPR, VEC, HALF, KIND>(a, a.g[1], n, cosv, sinv, bs, row, du[1], dv[1]);
-        if (KIND != kRotate && a.copy.H) copy_group<T, LPR, VEC, HALF>(a.copy, n, bs, row);
+    for (int i = 0; i < NP; ++i) du[i] = dv[i] = 0.f;
+    for (int tile = first; tile < a.tiles[k]; tile += step) {
+        const int t0 = tile * TB, n = min(TB, a.tokens - t0);
+        __syncthreads();  // the tile before has been read
+        tile_angles(a, t0, n, cosv, sinv, bs);
+        if (a.g[k].H) group_bwd<T, LPR, VEC, HALF>(a, a.g[k], n, cosv, sinv, bs, row, du, dv);
+        if (k == a.with_copy && a.copy.H) copy_group<T, LPR, VEC, HALF>(a.copy, n, bs, row);
     }
-    if constexpr (KIND == kNormBwd) {
-        if (!a.part && !a.dw[0] && !a.dw[1]) return;
-        // the block's dw: its NG lane groups added in order
-        float* const red = reinterpret_cast<float*>(smem);
+    if (!a.part && !a.dw[k]) return;
+    // the block's dw: its NG lane groups added in order
+    float* const red = reinterpret_cast<float*>(smem);
+    __syncthreads();
+    float* mine = red + (threadIdx.x / LPR) * a.D;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (k >= a.ng) break;
-            __syncthreads();
-            float* mine = red + (threadIdx.x / LPR) * a.D;
-#pragma unroll
-            for (int i = 0; i < NP; ++i)
-                if (row.has(i)) {
-                    mine[row.first(i)] = du[k][i];
-                    mine[row.second(i)] = dv[k][i];
-                }
-            __syncthreads();
-            for (int j = threadIdx.x; j < a.D; j += kThreads) {
-                float v = 0.f;
-                for (int q = 0; q < NG; ++q) v += red[q * a.D + j];
-                if (a.part) a.part[((size_t)blockIdx.x * 2 + k) * a.D + j] = v;
-                else if (a.dw[k]) a.dw[k][j] = a.accumulate ? a.dw[k][j] + v : v;
-            }
+    for (int i = 0; i < NP; ++i)
+        if (row.has(i)) {
+            mine[row.first(i)] = du[i];
+            mine[row.second(i)] = dv[i];
         }
+    __syncthreads();
+    for (int j = threadIdx.x; j < a.D; j += kThreads) {
+        float v = 0.f;
+        for (int q = 0; q < NG; ++q) v += red[q * a.D + j];
+        if (a.part) a.part[(size_t)blockIdx.x * a.D + j] = v;
+        else a.dw[k][j] = a.accumulate ? a.dw[k][j] + v : v;
     }
 }
 
-// dw[k] (+)= sum over the blocks' partial rows: 32 columns x 8 row slices a block, the slices
-// added in order
-__global__ __launch_bounds__(256) void dw_finish(const float* __restrict__ part, int nb, int D, float* dwq, float* dwk,
-                                                 int accumulate) {
-    __shared__ float sh[8][32];
+// dw (+)= the sum of the partial rows, of the first nq blocks for q and of the others for k: 16 columns x
+// 64 slices of the rows a block, the slices added in order
+__global__ __launch_bounds__(1024) void dw_finish(const float* __restrict__ part, int nq, int nb, int D, float* dwq,
+                                                  float* dwk, int accumulate) {
+    __shared__ float sh[64][17];
     float* const dw = blockIdx.y ? dwk : dwq;
     if (!dw) return;
-    const int j = blockIdx.x * 32 + (threadIdx.x & 31), sl = threadIdx.x >> 5;
+    const int c = threadIdx.x & 15, sl = threadIdx.x >> 4, j = blockIdx.x * 16 + c;
+    const int end = blockIdx.y ? nb : nq;
     float v = 0.f;
     if (j < D) {
 #pragma unroll 8
-        for (int b = sl; b < nb; b += 8) v += part[((size_t)b * 2 + blockIdx.y) * D + j];
+        for (int b = (blockIdx.y ? nq : 0) + sl; b < end; b += 64) v += part[(size_t)b * D + j];
     }
-    sh[sl][threadIdx.x & 31] = v;
+    sh[sl][c] = v;
     __syncthreads();
-    if (threadIdx.x < 32 && j < D) {
+    if (threadIdx.x < 16 && j < D) {
         v = 0.f;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v += sh[q][threadIdx.x];
+        for (int q = 0; q < 64; ++q) v += sh[q][c];
         dw[j] = accumulate ? dw[j] + v : v;
     }
 }
 
 // ---- host -------------------------------------------------------------------------------
 constexpr int kMaxD = 512, kMaxH = 1024;
-constexpr int kBwdBlocks = 1024;  // partial dw rows at most
+constexpr int kBwdBlocks = 1536;  // partial dw rows at most: two rounds of three blocks a compute unit
 
 int lanes_for(int D) {  // of a row in 16-byte pieces
     int l = 2;
@@ -386,9 +480,14 @@ int lanes_for(int D) {  // of a row in 16-byte pieces
     return l;
 }
 
+constexpr int kBwd = 2;  // launch_kind: the backward
+
 template <typename T, int LPR, bool VEC, bool HALF, int KIND>
 int launch(const Args& a, int grid, size_t smem, hipStream_t s) {
-    hipLaunchKernelGGL((rope_kernel<T, LPR, VEC, HALF, KIND>), dim3(grid), dim3(kThreads), smem, s, a);
+    if constexpr (KIND == kBwd)
+        hipLaunchKernelGGL((norm_bwd_kernel<T, LPR, VEC, HALF>), dim3(grid), dim3(kThreads), smem, s, a);
+    else
+        hipLaunchKernelGGL((rope_kernel<T, LPR, VEC, HALF, KIND>), dim3(grid), dim3(kThreads), smem, s, a);
     GN_LAUNCH_CHECK("rope / qk norm");
     return GN_OK;
 }
@@ -538,18 +637,21 @@ void fill(Group& g, const gn_heads* x, const gn_heads* dy, const void* w, const 
     g.magic = g.H > 1 ? (uint32_t)(((1ull << 32) + g.H - 1) / g.H) : 0;
 }
 
-// Tokens of a tile: enough rows for a few rounds of the block's lane groups, cos and sin in 16 KB, and
+// Tokens of tile k: enough rows for a few rounds of the block's lane groups, cos and sin in 16 KB, and
 // at least a thousand tiles (four blocks a compute unit) before a tile gets a second token.
-void tile(Args& a, int heads, int rows_at_once, int rounds) {
+void tile(Args& a, int k, int heads, int rows_at_once, int rounds) {
     int tb = std::max(1, rows_at_once * rounds / std::max(heads, 1));
     tb = std::min(tb, 64);
     if (a.rot) tb = std::min(tb, std::max(1, 4096 / a.rot));
     tb = std::min(tb, std::max(1, a.tokens / 1024));
-    a.TB = tb;
-    a.tiles = (a.tokens + tb - 1) / tb;
+    a.TB[k] = tb;
+    a.tiles[k] = (a.tokens + tb - 1) / tb;
 }
 
-size_t tile_smem(const Args& a) { return (size_t)a.TB * a.rot * 4 + (size_t)a.TB * 8; }
+size_t tile_smem(const Args& a) {
+    const int tb = std::max(a.TB[0], a.TB[1]);
+    return (size_t)tb * a.rot * 4 + (size_t)tb * 8;
+}
 
 int rope_call(const char* who, const gn_heads* x, const gn_heads* y, const gn_rope* r, int B, int S, int D, int dtype,
               float sgn, void* stream) {
@@ -566,8 +668,8 @@ int rope_call(const char* who, const gn_heads* x, const gn_heads* y, const gn_ro
     fill(a.g[0], x, nullptr, nullptr, y);
     a.ng = 1;
     a.sgn = sgn;
-    tile(a, x->H, 2 * kThreads / (vec ? lanes_for(D) : 64), 2);
-    return launch_kind<kRotate>(a, dtype, mode, vec, a.tiles, tile_smem(a), as_stream(stream));
+    tile(a, 0, x->H, 2 * kThreads / (vec ? lanes_for(D) : 64), 2);
+    return launch_kind<kRotate>(a, dtype, mode, vec, a.tiles[0], tile_smem(a), as_stream(stream));
 }
 
 }  // namespace
@@ -648,13 +750,13 @@ extern "C" int gn_qk_norm_rope_fwd(const gn_heads* q, const gn_heads* k, const g
     a.ng = k ? 2 : 1;
     a.sgn = 1.f;
     a.eps = eps;
-    tile(a, heads, 2 * kThreads / (vec ? lanes_for(D) : 64), 2);
-    return launch_kind<kNorm>(a, dtype, mode, vec, a.tiles, tile_smem(a), as_stream(stream));
+    tile(a, 0, heads, 2 * kThreads / (vec ? lanes_for(D) : 64), 2);
+    return launch_kind<kNorm>(a, dtype, mode, vec, a.tiles[0], tile_smem(a), as_stream(stream));
 }
 
 extern "C" size_t gn_qk_norm_rope_workspace_bytes(int B, int S, int D) {
     if (B <= 0 || S <= 0 || D <= 0) return 0;
-    return (size_t)std::min<int64_t>(kBwdBlocks, (int64_t)B * S) * 2 * D * sizeof(float);
+    return (size_t)std::min<int64_t>(kBwdBlocks, 2 * (int64_t)B * S) * D * sizeof(float);
 }
 
 extern "C" int gn_qk_norm_rope_bwd(const gn_heads* dyq, const gn_heads* dyk, const gn_heads* dyv, const gn_heads* q,
@@ -712,11 +814,22 @@ extern "C" int gn_qk_norm_rope_bwd(const gn_heads* dyq, const gn_heads* dyk, con
     a.eps = eps;
     a.accumulate = acc;
     const int at_once = kThreads / (vec ? lanes_for(D) : 64);
-    tile(a, heads, at_once, 2);
-    const int grid = std::min(a.tiles, kBwdBlocks);
-    const bool want = dwq || dwk;
-    if (want && grid > 1) {
-        const size_t need = (size_t)grid * 2 * D * sizeof(float);
+    // the blocks by the bytes of each side: two reads and a write a row of q and k, one each of v; as
+    // with values also without them, so that dw has the same bits either way
+    const int hk = k ? k->H : 0, hv = dv ? dv->H : 0;
+    const bool second = hk > 0;  // values without keys go with the queries
+    a.with_copy = second;
+    tile(a, 0, q->H + (second ? 0 : hv), at_once, 4);
+    if (second) tile(a, 1, 2 * hk, at_once, 4);
+    int grid = std::min(a.tiles[0] + a.tiles[1], kBwdBlocks);
+    a.nq = grid;
+    if (second) {
+        const double share = 3.0 * q->H / (3.0 * q->H + 5.0 * hk);
+        a.nq = std::min(a.tiles[0], std::max(1, std::min(grid - 1, (int)(share * grid + 0.5))));
+        grid = a.nq + std::min(a.tiles[1], grid - a.nq);
+    }
+    if ((dwq && a.nq > 1) || (dwk && grid - a.nq > 1)) {
+        const size_t need = (size_t)grid * D * sizeof(float);
         if (!ws || ws_bytes < need || ((uintptr_t)ws & 15u)) {
             set_error("%s: workspace of %zu bytes (16-byte aligned) required", who, need);
             return GN_E_WORKSPACE;
@@ -725,10 +838,14 @@ extern "C" int gn_qk_norm_rope_bwd(const gn_heads* dyq, const gn_heads* dyk, con
     }
     a.dw[0] = dwq;
     a.dw[1] = dwk;
+    if (dwk && !second && !acc && launch_zero(dwk, (size_t)D * 4, s) != hipSuccess) {  // keys without heads
+        set_error("%s: clear failed", who);
+        return GN_E_HIP;
+    }
     const size_t smem = std::max(tile_smem(a), (size_t)at_once * D * sizeof(float));
-    if (const int rc = launch_kind<kNormBwd>(a, dtype, mode, vec, grid, smem, s)) return rc;
+    if (const int rc = launch_kind<kBwd>(a, dtype, mode, vec, grid, smem, s)) return rc;
     if (a.part) {
-        dw_finish<<<dim3((D + 31) / 32, 2), 256, 0, s>>>(a.part, grid, D, dwq, dwk, acc);
+        dw_finish<<<dim3((D + 15) / 16, 2), 1024, 0, s>>>(a.part, a.nq, grid, D, dwq, second ? dwk : nullptr, acc);
         GN_LAUNCH_CHECK("qk norm weight gradients");
     }
     return GN_OK;
