@@ -105,6 +105,8 @@ PYBIND11_MODULE(_grilly_core, m) {
         .value("VSACosineBlendLoss", OpType::VSACosineBlendLoss)
         .value("FusedGLU", OpType::FusedGLU)
         .value("Embedding", OpType::Embedding)
+        .value("Rope", OpType::Rope).value("QkNormRope", OpType::QkNormRope)
+        .value("LinearCrossEntropy", OpType::LinearCrossEntropy)
         .export_values();
 
     py::class_<TensorRef>(m, "TensorRef")

@@ -259,6 +259,9 @@ void BackwardEngine::dispatch(Node* n) {
         case OpType::RMSNorm: bwd_rmsnorm(n); break;
         case OpType::FlashAttention2: bwd_attention(n); break;
         case OpType::CrossEntropy: bwd_cross_entropy(n); break;
+        case OpType::Rope: bwd_rope(n); break;
+        case OpType::QkNormRope: bwd_qk_norm_rope(n); break;
+        case OpType::LinearCrossEntropy: bwd_linear_cross_entropy(n); break;
         case OpType::Add: bwd_add_sub(n, false); break;
         case OpType::Reshape: bwd_passthrough(n); break;
         case OpType::VSAUnpackProject: bwd_vsa_unpack_project(n); break;
@@ -618,6 +621,114 @@ void BackwardEngine::bwd_cross_entropy(Node* n) {
             "cross-entropy backward");
     stats_.shaders_dispatched++;
     n->grad_input_buffers[0] = dZ;
+}
+
+namespace {
+
+// The rotation of a Rope or QkNormRope node over S positions a sequence.
+gn_rope node_rope(const RopeNodeParams& p, uint64_t freqs, uint64_t positions, int S, const char* what) {
+    gn_rope r{};
+    if (!p.rot) return r;
+    if (!freqs) throw std::invalid_argument(std::string(what) + ": the saved slots must hold the frequencies");
+    r.freqs = (const double*)P(freqs);
+    r.positions = (const int32_t*)P(positions);
+    r.pos_sb = p.positions_per_row ? S : 0;
+    r.pos0 = p.pos0;
+    r.mscale = p.mscale != 0.f ? p.mscale : 1.f;
+    r.rot = (int)p.rot;
+    r.mode = (int)p.mode;
+    return r;
+}
+
+// heads [first, first + H) of rows of C elements
+gn_heads row_heads(void* rows, size_t es, int S, int64_t C, int first, int H, int D) {
+    return gn_heads{rows ? (char*)rows + (size_t)first * D * es : nullptr, S * C, C, D, H};
+}
+
+}  // namespace
+
+// Rope: dx = dy rotated back.
+void BackwardEngine::bwd_rope(Node* n) {
+    const TensorRef& x = n->inputs[0];
+    if (!x.requires_grad) return;
+    const RopeNodeParams p = params_of<RopeNodeParams>(n);
+    if (x.ndim != 3 || p.heads == 0 || x.shape[2] % p.heads || n->outputs[0].numel() != x.numel())
+        throw std::invalid_argument("Rope: input and output [B,S,heads*D], heads > 0");
+    const int B = (int)x.shape[0], S = (int)x.shape[1], H = (int)p.heads, D = (int)x.shape[2] / H;
+    const gn_rope r = node_rope(p, n->saved_buffer_ids[0], n->num_saved > 1 ? n->saved_buffer_ids[1] : 0, S, "Rope");
+    const size_t es = TensorRef::elem_size(x.dtype);
+    uint64_t dx = alloc_grad(x.size_bytes());
+    const gn_heads in = row_heads(const_cast<void*>(gout(n)), es, S, x.shape[2], 0, H, D);
+    const gn_heads out = row_heads(P(dx), es, S, x.shape[2], 0, H, D);
+    gn_call(gn_rope_bwd(&in, &out, &r, B, S, D, gn_dtype(x.dtype, "Rope"), dev_.stream()), "rope backward");
+    stats_.shaders_dispatched++;
+    n->grad_input_buffers[0] = dx;
+}
+
+// QkNormRope: the gradients of the fused rows and of the two norms' weights, from the rows as they were
+// before the norm.
+void BackwardEngine::bwd_qk_norm_rope(Node* n) {
+    const TensorRef& x = n->inputs[0];
+    const RopeNodeParams p = params_of<RopeNodeParams>(n);
+    const int H = (int)p.heads, K = (int)p.kv_heads;
+    if (x.ndim != 3 || H <= 0 || K <= 0 || x.shape[2] % (p.heads + 2 * p.kv_heads) ||
+        n->outputs[0].numel() != x.numel())
+        throw std::invalid_argument("QkNormRope: input and output [B,S,(heads + 2 kv_heads)*D], heads and kv_heads > 0");
+    if (n->outputs[0].buffer_id == x.buffer_id)
+        throw std::invalid_argument("QkNormRope: the backward reads its input, which an output in its place overwrites");
+    const int B = (int)x.shape[0], S = (int)x.shape[1], D = (int)x.shape[2] / (H + 2 * K);
+    const int64_t C = x.shape[2];
+    const uint64_t wq = n->saved_buffer_ids[0], wk = n->num_saved > 1 ? n->saved_buffer_ids[1] : 0;
+    const gn_rope r = node_rope(p, n->num_saved > 2 ? n->saved_buffer_ids[2] : 0,
+                                n->num_saved > 3 ? n->saved_buffer_ids[3] : 0, S, "QkNormRope");
+    const int dt = gn_dtype(x.dtype, "QkNormRope");
+    const size_t es = TensorRef::elem_size(x.dtype);
+    uint64_t dx = alloc_grad(x.size_bytes());
+    uint64_t dwq = wq ? alloc_grad((size_t)D * 4) : 0, dwk = wk ? alloc_grad((size_t)D * 4) : 0;
+    const size_t wsb = dwq || dwk ? gn_qk_norm_rope_workspace_bytes(B, S, D) : 0;
+    const uint64_t ws = split_ws(wsb);
+    void *g = const_cast<void*>(gout(n)), *xp = P(x.buffer_id), *dp = P(dx);
+    const gn_heads gq = row_heads(g, es, S, C, 0, H, D), gk = row_heads(g, es, S, C, H, K, D),
+                   gv = row_heads(g, es, S, C, H + K, K, D), q = row_heads(xp, es, S, C, 0, H, D),
+                   k = row_heads(xp, es, S, C, H, K, D), dq = row_heads(dp, es, S, C, 0, H, D),
+                   dk = row_heads(dp, es, S, C, H, K, D), dv = row_heads(dp, es, S, C, H + K, K, D);
+    gn_call(gn_qk_norm_rope_bwd(&gq, &gk, &gv, &q, &k, P(wq), P(wk), &dq, &dk, &dv, (float*)P(dwq), (float*)P(dwk),
+                                &r, B, S, D, p.eps != 0.f ? p.eps : 1e-6f, dt, 0, P(ws), wsb, dev_.stream()),
+            "query/key norm backward");
+    stats_.shaders_dispatched += dwq || dwk ? 2 : 1;
+    n->grad_input_buffers[0] = dx;
+    if (dwq) contribute(wq, dwq, 0, (size_t)D, true);
+    if (dwk) contribute(wk, dwk, 0, (size_t)D, true);
+}
+
+// LinearCrossEntropy: a root like CrossEntropy, or with an upstream gradient per row.  E's gradient
+// is added onto one that is already there (tied tables).
+void BackwardEngine::bwd_linear_cross_entropy(Node* n) {
+    const TensorRef& h = n->inputs[0];
+    const TensorRef& t = n->inputs[1];
+    if (n->params_size < sizeof(LinearCrossEntropyParams))
+        throw std::invalid_argument("LinearCrossEntropy: params must hold the vocabulary size and the scale");
+    const LinearCrossEntropyParams p = params_of<LinearCrossEntropyParams>(n);
+    const uint64_t E = n->saved_buffer_ids[0], lse = n->num_saved > 1 ? n->saved_buffer_ids[1] : 0;
+    if (!E || !lse) throw std::invalid_argument("LinearCrossEntropy: the saved slots must hold E and lse");
+    const int T = (int)h.rows(), d = (int)h.last(), V = (int)p.vocab;
+    if (t.numel() != (size_t)T || t.dtype != 3)
+        throw std::invalid_argument("LinearCrossEntropy: one int32 target per row");
+    const int dt = gn_dtype(h.dtype, "LinearCrossEntropy");
+    const size_t bytes = (size_t)V * d * 4;
+    GradEntry* e = find(E);
+    const bool into = e && e->grad_id && e->owned && e->dtype == 0 && e->grad_bytes == bytes;
+    uint64_t dh = h.requires_grad ? alloc_grad(h.size_bytes()) : 0;
+    uint64_t dE = into ? e->grad_id : alloc_grad(bytes);
+    const size_t wsb = gn_linear_xent_workspace_bytes(T, d, V, dt);
+    const uint64_t ws = split_ws(wsb);
+    const float* dloss = n->grad_output_buffer > 1 ? (const float*)P(n->grad_output_buffer) : nullptr;
+    gn_call(gn_linear_xent_bwd(P(h.buffer_id), P(E), (const int32_t*)P(t.buffer_id), (const float*)P(lse), dloss, nullptr,
+                               p.scale, P(dh), P(dE), GN_F32, T, d, V, dt, into ? GN_ACCUMULATE : 0u, P(ws), wsb,
+                               dev_.stream()), "linear cross-entropy backward");
+    stats_.shaders_dispatched++;
+    n->grad_input_buffers[0] = dh;
+    if (!into) contribute(E, dE, 0, (size_t)V * d, true);
 }
 
 // Add: both inputs receive the upstream gradient itself (borrowed, copied on fan-out).  An

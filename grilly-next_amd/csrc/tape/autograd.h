@@ -15,7 +15,8 @@
 //   * RMSNorm, Softmax, ReLU, SiLU, Tanh, Sigmoid, LayerNorm, FlashAttention2 and
 //     CrossEntropy have real handlers (stubs or missing in the reference,
 //     autograd.cpp:543-711), and FusedGLU (appended after VSACosineBlendLoss) carries the
-//     fused SwiGLU/GEGLU/ReGLU projection backward.
+//     fused SwiGLU/GEGLU/ReGLU projection backward; Rope, QkNormRope and LinearCrossEntropy
+//     carry the operators the reference has no node for.
 #pragma once
 
 #include <algorithm>
@@ -71,6 +72,9 @@ enum class OpType : uint8_t {
     VSAUnpackProject, VSASurrogateLoss, VSALoRAExpand, VSACosineBlendLoss,
     FusedGLU,   // added by this build: fused gate/up projection + GLU backward
     Embedding,  // added by this build: row gather (tied embeddings); backward scatter-adds
+    Rope,                // added by this build: heads rotated by position
+    QkNormRope,          // added by this build: per-head norms of q and k with the rotation, on fused QKV rows
+    LinearCrossEntropy,  // added by this build: the loss of a linear head whose logits are not kept
     _Count
 };
 static_assert(static_cast<int>(OpType::VSACosineBlendLoss) == 33, "OpType numbering");
@@ -109,6 +113,19 @@ struct AttentionParams {
 };
 struct CrossEntropyParams { float scale; uint32_t has_scale; };  // scale default 1 (no 1/B)
 struct FusedGLUParams { uint32_t kind; };                       // GN_GLU_* kind
+// Rope: inputs[0] [B,S,heads*D] -> outputs[0] alike; QkNormRope: fused QKV rows [B,S,(heads + 2
+// kv_heads)*D] -> rows alike, q and k normed and rotated, v copied.  rot 0: no rotation.  saved slots: Rope
+// {freqs, positions or 0}, QkNormRope {wq, wk, freqs, positions or 0} (wq, wk: 0 = weights of 1).
+struct RopeNodeParams {
+    uint32_t heads, kv_heads, rot, mode;
+    float mscale, eps;           // 0 -> 1, 1e-6
+    uint32_t positions_per_row;  // positions [B,S] (1) or [S] (0)
+    int32_t pos0;                // the first position, without positions
+};
+static_assert(sizeof(RopeNodeParams) == 32, "RopeNodeParams layout");
+// LinearCrossEntropy: inputs h [T,d] and targets int32 [T], outputs[0] loss fp32 [T]; saved slots {E
+// [vocab,d], lse}.  Without an upstream gradient every row's is `scale`.
+struct LinearCrossEntropyParams { uint32_t vocab; float scale; };
 struct MSELossParams { float scale; uint32_t has_scale; };      // scale default 1/n (mean)
 
 static constexpr uint32_t kMaxNodeIO = 8;
@@ -214,6 +231,9 @@ private:
     void bwd_rmsnorm(Node* n);
     void bwd_attention(Node* n);
     void bwd_cross_entropy(Node* n);
+    void bwd_rope(Node* n);
+    void bwd_qk_norm_rope(Node* n);
+    void bwd_linear_cross_entropy(Node* n);
     void bwd_add_sub(Node* n, bool sub);
     void bwd_passthrough(Node* n);
     void bwd_vsa_unpack_project(Node* n);

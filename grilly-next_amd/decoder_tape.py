@@ -10,6 +10,11 @@ write bf16, each bf16 branch output is added into it in fp32.  Carried in bf16, 
 gradient's rounding over the 12 layers reaches the LayerNorm gains' gradient (a sum that
 cancels heavily) at a few percent; in fp32 it stays within the bf16 tolerance.
 
+Two options replace parts of it: `qk_norm_rope` norms queries and keys per head (weights qn, kn
+[D]) and rotates them by position between the projection and the attention (gn_qk_norm_rope_fwd);
+`fused_loss` takes the loss from the last norm's output and E (gn_linear_xent_fwd): no logits and no
+gradient of them are kept.
+
 `Decoder.forward()` runs the forward on the GPU through this library's forward kernels
 (untimed: gn_layernorm_fwd saving mean/rstd, gn_linear_fwd, gn_glu_linear_fwd saving the
 gate/up caches, gn_attn_fwd saving the fp32 row logsumexp; torch only for the embedding
@@ -27,9 +32,9 @@ import gn_bwd as gn
 
 class Decoder:
     def __init__(self, layers=12, d=768, heads=12, ff=3072, vocab=32000, batch=8, seq=1024,
-                 seed=5, device="cuda:0", glu_epilogue=True):
+                 seed=5, device="cuda:0", glu_epilogue=True, qk_norm_rope=False, fused_loss=False):
         self.L, self.d, self.H, self.ff, self.V = layers, d, heads, ff, vocab
-        self.glu_epilogue = glu_epilogue
+        self.glu_epilogue, self.qk_norm_rope, self.fused_loss = glu_epilogue, qk_norm_rope, fused_loss
         self.B, self.S, self.T = batch, seq, batch * seq
         self.dev = torch.device(device)
         g = torch.Generator(device=self.dev)
@@ -48,6 +53,10 @@ class Decoder:
                             ln2_b=const(d, 0), Wg=w(ff, d), Wu=w(ff, d), bg=const(ff, 0),
                             bu=const(ff, 0), Wd=w(d, ff), bd=const(d, 0))
                        for _ in range(layers)]
+        if qk_norm_rope:
+            for p in self.layers:
+                p["qn"], p["kn"] = const(d // heads, 1), const(d // heads, 1)
+            self.freqs, self.mscale = gn.rope_freqs(d // heads, device=self.dev)
         self.lnf_g, self.lnf_b = const(d, 1), const(d, 0)
         ids = torch.randint(0, vocab, (batch, seq), device=self.dev, generator=g)
         self.ids = ids.reshape(-1).to(torch.int32).contiguous()
@@ -68,7 +77,14 @@ class Decoder:
             a = {"x": x}
             a["n1"], a["m1"], a["r1"] = gn.layernorm_fwd(x, p["ln1_g"], p["ln1_b"], out_dtype=bf)
             a["qkv"] = gn.linear_fwd(a["n1"], p["Wqkv"], p["bqkv"])
-            q, k, v = (t.contiguous() for t in a["qkv"].view(B, S, 3, H, D).permute(2, 0, 3, 1, 4))
+            if self.qk_norm_rope:
+                # the rows the attention's backward reads, and from them the forward's heads
+                a["rot"] = torch.empty_like(a["qkv"])
+                parts = [[t.view(B, S, 3, H, D)[:, :, i] for i in range(3)] for t in (a["qkv"], a["rot"])]
+                gn.qk_norm_rope_fwd(*parts[0][:2], p["qn"], p["kn"], self.freqs, v=parts[0][2], mscale=self.mscale,
+                                    out=parts[1])
+            rows = a["rot"] if self.qk_norm_rope else a["qkv"]
+            q, k, v = (t.contiguous() for t in rows.view(B, S, 3, H, D).permute(2, 0, 3, 1, 4))
             O, a["lse"] = gn.attn_fwd(q, k, v, causal=True, rope="none", ws=ws)
             a["o"] = O.permute(0, 2, 1, 3).reshape(T, d).contiguous()
             a["ao"] = gn.linear_fwd(a["o"], p["Wo"], p["bo"])
@@ -81,7 +97,10 @@ class Decoder:
             acts.append(a)
             x = a["x3"]
         self.nf, self.mf, self.rf = gn.layernorm_fwd(x, self.lnf_g, self.lnf_b, out_dtype=bf)
-        self.logits = gn.linear_fwd(self.nf, self.E)
+        if self.fused_loss:
+            self.row_loss, self.lse = gn.linear_xent_fwd(self.nf, self.E, self.tgt)
+        else:
+            self.logits = gn.linear_fwd(self.nf, self.E)
         self.acts = acts
         torch.cuda.synchronize()
 
@@ -98,7 +117,15 @@ class Decoder:
             tape.save_for_backward(n, [P(p["ln1_g"]), P(p["ln1_b"]), P(a["m1"]), P(a["r1"])])
             n = tape.record_op(op.Linear, [t(a["n1"], True)], [t(a["qkv"])])
             tape.save_for_backward(n, [P(p["Wqkv"]), P(p["bqkv"])])
-            qkv = gb.make_tensor_ref(P(a["qkv"]), (B, S, 3 * d), gb.DTYPE_BF16, True)
+            rows = a["qkv"]
+            if self.qk_norm_rope:
+                D = d // H
+                rows = a["rot"]
+                n = tape.record_op(op.QkNormRope, [gb.make_tensor_ref(P(a["qkv"]), (B, S, 3 * d), gb.DTYPE_BF16, True)],
+                                   [gb.make_tensor_ref(P(rows), (B, S, 3 * d), gb.DTYPE_BF16)],
+                                   gb.qk_norm_rope_params(H, H, D, mscale=self.mscale))
+                tape.save_for_backward(n, [P(p["qn"]), P(p["kn"]), P(self.freqs)])
+            qkv = gb.make_tensor_ref(P(rows), (B, S, 3 * d), gb.DTYPE_BF16, True)
             o = gb.make_tensor_ref(P(a["o"]), (B, S, d), gb.DTYPE_BF16)
             n = tape.record_op(op.FlashAttention2, [qkv], [o],
                                gb.attention_params(causal=True, rope="none", fused_qkv_heads=H))
@@ -118,6 +145,11 @@ class Decoder:
         last = self.acts[-1]["x3"]
         n = tape.record_op(op.LayerNorm, [t(last, True)], [t(self.nf)], gb.layernorm_params())
         tape.save_for_backward(n, [P(self.lnf_g), P(self.lnf_b), P(self.mf), P(self.rf)])
+        if self.fused_loss:
+            n = tape.record_op(op.LinearCrossEntropy, [t(self.nf, True), t(self.tgt)], [t(self.row_loss)],
+                               gb.linear_cross_entropy_params(self.V, 1.0 / self.T))
+            tape.save_for_backward(n, [P(self.E), P(self.lse)])
+            return n
         n = tape.record_op(op.Linear, [t(self.nf, True)], [t(self.logits)])
         tape.save_for_backward(n, [P(self.E)])
         return tape.record_op(op.CrossEntropy, [t(self.logits, True), t(self.tgt)], [t(self.loss)],

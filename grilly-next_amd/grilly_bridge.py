@@ -93,6 +93,25 @@ def cross_entropy_params(scale: float = 1.0) -> bytes:
     return struct.pack("<fI", scale, 1)
 
 
+def rope_params(heads: int, rot: int, mode: str = "half", mscale: float = 1.0, positions_per_row: bool = False,
+                pos0: int = 0, kv_heads: int = 0, eps: float = 0.0) -> bytes:
+    """Rope node: x [B, S, heads*D]; saved slots {freqs, positions (0: pos0, pos0 + 1, ...)}.
+    positions_per_row: positions are [B, S], else [S]."""
+    return struct.pack("<IIIIffIi", heads, kv_heads, rot, ROPE_MODE[mode], mscale, eps, int(positions_per_row), pos0)
+
+
+def qk_norm_rope_params(heads: int, kv_heads: int, rot: int, mode: str = "half", mscale: float = 1.0,
+                        eps: float = 1e-6, positions_per_row: bool = False, pos0: int = 0) -> bytes:
+    """QkNormRope node: fused QKV rows [B, S, (heads + 2 kv_heads)*D]; saved slots {wq, wk, freqs,
+    positions} (wq, wk 0: weights of 1; positions 0: pos0, pos0 + 1, ...)."""
+    return rope_params(heads, rot, mode, mscale, positions_per_row, pos0, kv_heads, eps)
+
+
+def linear_cross_entropy_params(vocab: int, scale: float = 1.0) -> bytes:
+    """LinearCrossEntropy node: h [T, d] and targets [T] -> loss [T]; saved slots {E, lse}."""
+    return struct.pack("<If", int(vocab), scale)
+
+
 def fused_glu_params(kind: str = "swiglu_up") -> bytes:
     return struct.pack("<I", GLU_KIND[kind])
 

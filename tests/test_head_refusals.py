@@ -213,3 +213,15 @@ def test_rope_freqs_refuses():
                dict(scaling="yarn", factor=2.0, trained=0), dict(scaling="yarn", factor=2.0, fast=1.0, slow=1.0)):
         with pytest.raises(gn.GnError):
             gn.rope_freqs(**{"rot": 64, "device": "cpu", **kw})
+
+
+def test_node_types_and_parameters():
+    """The tape's node types are appended to the numbering; their parameter blocks' layouts."""
+    import struct
+    grilly_core = pytest.importorskip("grilly_core")
+    import grilly_bridge as gb
+    assert [int(getattr(grilly_core.OpType, n)) for n in ("Embedding", "Rope", "QkNormRope", "LinearCrossEntropy")] == [
+        35, 36, 37, 38]
+    assert struct.unpack("<IIIIffIi", gb.rope_params(4, 32, "interleaved", 1.5, True, 7)) == (4, 0, 32, 1, 1.5, 0.0, 1, 7)
+    assert struct.unpack("<IIIIffIi", gb.qk_norm_rope_params(4, 2, 64, pos0=-1))[:4] == (4, 2, 64, 2)
+    assert struct.unpack("<If", gb.linear_cross_entropy_params(32000, 0.5)) == (32000, 0.5)
