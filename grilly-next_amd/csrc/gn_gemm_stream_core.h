@@ -312,6 +312,12 @@ __global__ __launch_bounds__(512, 1) void gemm_stream(GemmDesc g, EPI... epi) {
         tile_at(i, m0, n0);
         if constexpr (sizeof...(EPI) > 0) {
             (epi.tile(g, acc, m0 + wm * WM, n0 + wn * WN, st, lane), ...);
+            if constexpr ((EPI::kAgain || ...)) {
+                // the next tile's first fragments once more: not held through the epilogue, whose
+                // registers they would take
+                static_for<NR>([&](auto R_) { read_one(I0{}, R_, stage_ptr(slot), 0); });
+                static_for<NR>([&](auto R_) { read_one(I1{}, R_, stage_ptr(slot), 1); });
+            }
         } else if constexpr (sizeof(CT) == 4) {
             if (g.accumulate) store32(BT{}, m0, n0);
             else store32(BF{}, m0, n0);

@@ -72,6 +72,7 @@ __device__ __forceinline__ void rows_wait() {
 
 // Each row's statistics over the wave's 64 columns, and its target's logit.
 struct StatsTile {
+    static constexpr bool kAgain = false;
     const int32_t* tgt;
     float* lt;      // [T] the target's logit
     float2* part;   // [strips][T]
@@ -108,9 +109,10 @@ struct StatsTile {
             s += __shfl_xor(s, 32);
             if (lane < 32 && row < g.M) out[row] = make_float2(m * kLog2e, s);
             if (__any((unsigned)c < 64u)) {
+                float x = 0.f;
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    if (c == col(e) && row < g.M) lt[row] = acc[i][e >> 4][e & 15];
+                for (int e = 0; e < 32; ++e) x = c == col(e) ? acc[i][e >> 4][e & 15] : x;
+                if ((unsigned)c < 64u && (c & 4) == nh && row < g.M) lt[row] = x;
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -123,6 +125,7 @@ typedef float4 RowScale;
 // G of the tile, as bf16 hi and (LO) lo; columns from N up to ld are zeros.
 template <bool LO>
 struct GradTile {
+    static constexpr bool kAgain = LO;  // 44 registers spilled otherwise: 1.58 -> 1.45 ms, dE of 8190 x 768 x 32000
     const RowScale* rows;
     bf16_t *hi, *lo;  // [T x ld]
     float* resid;     // [T] what rounding the target's element to hi left
@@ -149,6 +152,7 @@ struct GradTile {
             const int c = __float_as_int(rs.w) - v0 - n0;
             const bool hit = __any((unsigned)c < 64u), edge = n0 + 64 > g.N;
             uint2 low[LO ? 8 : 1];
+            float left = 0.f;
             wave_lds_sync();
 #pragma unroll
             for (int k = 0; k < 8; ++k) {  // four columns: 8 k + nh
@@ -158,11 +162,11 @@ struct GradTile {
                     x[e] = rs.y * __builtin_amdgcn_exp2f(fmaf(acc[i][k >> 2][4 * (k & 3) + e], kLog2e, -rs.x));
                 if (hit) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (c == 8 * k + nh + e) {
-                            x[e] -= rs.z;
-                            if (row < g.M) resid[row] = x[e] - bf2f(f2bf(x[e]));
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        const bool at = c == 8 * k + nh + e;
+                        x[e] -= at ? rs.z : 0.f;
+                        left = at ? x[e] - bf2f(f2bf(x[e])) : left;
+                    }
                 }
                 if (edge) {
 #pragma unroll
@@ -176,6 +180,7 @@ struct GradTile {
                                         pack_bf2(x[2] - __uint_as_float(h.y << 16), x[3] - __uint_as_float(h.y & 0xffff0000u)));
                 if (k & 1) __builtin_amdgcn_sched_barrier(0);
             }
+            if (hit && (unsigned)c < 64u && (c & 4) == nh && row < g.M) resid[row] = left;
             wave_lds_sync();
             flush(hi, g.M, mw, n0, st, lane);
             if constexpr (LO) {
@@ -453,7 +458,10 @@ struct Plan {
         Tp = bf ? T : round_up(T, 4);
         // A piece's G (hi + lo, or the fp32 logits it replaces) takes 4 bytes an element
         const int64_t most = kPieceBytes / (lay ? 4 : 1) / 4 / std::max(Tp, 1);
-        vc = (int)std::min<int64_t>(round_up(V, 128), std::max<int64_t>(512, most / 128 * 128));
+        // whole rounds of 256 x 128 tiles of dE's product on the compute units, or what there is room for
+        const int64_t round = (int64_t)std::max(1, stream_blocks() / ((dp + 127) / 128)) * 256;
+        int64_t cols = most >= round ? most / round * round : 2 * most >= round ? round : most / 128 * 128;
+        vc = (int)std::min<int64_t>(round_up(V, 128), std::max<int64_t>(512, cols));
         pieces = (V + vc - 1) / vc;
         // the products' own split workspaces: of a whole piece and of the last one
         part_bytes = 0;
@@ -501,8 +509,10 @@ struct Plan {
         det = take((size_t)q * dp * 4);
         bytes = at;
     }
-    // Measured (us, pieces of 128, 256, 512, 1024 MB): 8190 x 768 x 32000 2479, 2376, 2412, 2238; 2001 x 1024 x
-    // 50001 971, 931, 920, 918; 8192 x 2048 x 128000 19.7, 19.1, 20.1, 20.0 ms.
+    // Measured (us, pieces of 128, 256, 512, 1024 MB in plain multiples of 128 columns): 8190 x 768 x
+    // 32000 2479, 2376, 2412, 2238; 2001 x 1024 x 50001 971, 931, 920, 918; 8192 x 2048 x 128000 19.7,
+    // 19.1, 20.1, 20.0 ms.  Whole rounds at 256 MB took the backward of the first 1821 -> 1793, of the
+    // second (bf16 dE) 709 -> 678.
     static constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 };
 
