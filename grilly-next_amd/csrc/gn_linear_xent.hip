@@ -9,11 +9,11 @@
 //              G = u (exp(l - lse) - [target]) + z exp(l - lse) in bf16, then dE_c (+)= G^T h and
 //              dh += G E_c (fp32) from it
 // A lane holds 16 columns of one row of each 32 x 32 accumulator, so the row statistics take one
-// exchange between lanes.  For an fp32 dE, G is stored as two bf16 pieces hi + lo, whose products
-// with h are two k-segments of one product: |G - hi - lo| <= 2^-17 |G|, where bf16 alone (2^-8)
-// would be the gradient's largest error.  For dh, hi is enough but at the target: there the rounding
-// of a row's largest element, which shows in all of dh's row, is kept in fp32 and its product with
-// E[target] added when dh is rounded (dh_finish).
+// exchange between lanes.  For an fp32 dE, G is stored as two or three bf16 pieces, whose products with h
+// are one product's longer k: two leave 2^-17 of an element, three nothing that fp32 holds, where
+// bf16 alone (2^-8) would be the gradient's largest error.  For dh the first piece is enough but at
+// the target: there the rounding of a row's largest element, which shows in all of dh's row, is
+// kept in fp32 and its product with E[target] added when dh is rounded (dh_finish).
 //
 // fp32.  The pieces' logits are stored (fp32, in the workspace) between the library's fp32 products
 // and row kernels, G in their place.
@@ -29,13 +29,18 @@
 namespace gn {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+constexpr float kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e);
 
-// A part of a row: its maximum m and the sum s of exp2 about it (logits in units of log2), (-inf, 0) when
-// it is empty.  A NaN among the logits is in s only (m skips it) and stays there.
+// exp(x - m) as exp2(x log2e - b) takes b = m log2e, whose rounding (2^-20 at 17) would go into every term
+// of a row alike: what it was off by
+__device__ __forceinline__ float off(float m, float b) { return fmaf(m, kLog2e, -b) + m * kLog2eRest; }
+
+// A part of a row: its maximum m and the sum s of exp about it, (-inf, 0) when it is empty.  A NaN among
+// the logits is in s only (m skips it) and stays there.
 // s about another maximum n >= m
 __device__ __forceinline__ float about(float s, float m, float n) {
-    return s * __builtin_amdgcn_exp2f(m - (n == -INFINITY ? 0.f : n));
+    return s * __builtin_amdgcn_exp2f((m - (n == -INFINITY ? 0.f : n)) * kLog2e);
 }
 __device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
     const float n = fmaxf(m, m2);
@@ -107,7 +112,8 @@ struct StatsTile {
 #pragma unroll
             for (int e = 0; e < 32; ++e) s += __builtin_amdgcn_exp2f(fmaf(at(e), kLog2e, -b));
             s += __shfl_xor(s, 32);
-            if (lane < 32 && row < g.M) out[row] = make_float2(m * kLog2e, s);
+            if (lane < 32 && row < g.M)
+                out[row] = make_float2(m, m == -INFINITY ? s : s * __builtin_amdgcn_exp2f(-off(m, b)));
             if (__any((unsigned)c < 64u)) {
                 float x = 0.f;
 #pragma unroll
@@ -119,24 +125,28 @@ struct StatsTile {
     }
 };
 
-// What a row's G takes: {lse in units of log2, u + z, u, the target's column (as bits; -1: none)}
+// What a row's G takes: {b = lse log2e, (u + z) corrected for b's rounding, u, the target's column (as bits;
+// -1: none)}
 typedef float4 RowScale;
 
-// G of the tile, as bf16 hi and (LO) lo; columns from N up to ld are zeros.
-template <bool LO>
+// G of the tile, as P bf16 pieces; columns from N up to ld are zeros.  G and then what a piece left of it
+// stay in the accumulators, and the next tile's fragments are read again after the epilogue of several
+// pieces: 44 registers spilled otherwise (dE of 8190 x 768 x 32000, two pieces, 1.58 -> 1.45 ms).
+template <int P>
 struct GradTile {
-    static constexpr bool kAgain = LO;  // 44 registers spilled otherwise: 1.58 -> 1.45 ms, dE of 8190 x 768 x 32000
+    static constexpr bool kAgain = P > 1;
     const RowScale* rows;
-    bf16_t *hi, *lo;  // [T x ld]
-    float* resid;     // [T] what rounding the target's element to hi left
+    bf16_t* G;      // P planes [T x ld]
+    size_t plane;
+    float* resid;   // [T] what rounding the target's element to the first piece left
     int ld, v0;
     template <int FM>
     __device__ __forceinline__ void begin(const GemmDesc& g, int m0, unsigned char* st, int lane) const {
         rows_begin<FM, 16>(rows, m0, g.M, st, lane);
     }
     template <int FM, int FN>
-    __device__ __forceinline__ void tile(const GemmDesc& g, const f32x16_t (&acc)[FM][FN], int m0, int n0,
-                                         unsigned char* st, int lane) const {
+    __device__ __forceinline__ void tile(const GemmDesc& g, f32x16_t (&acc)[FM][FN], int m0, int n0, unsigned char* st,
+                                         int lane) const {
         static_assert(FN == 2, "64 columns a wave");
         rows_wait();
         if (n0 >= ld) return;
@@ -151,55 +161,55 @@ struct GradTile {
             const int mw = m0 + i * 32, row = mw + mr;
             const int c = __float_as_int(rs.w) - v0 - n0;
             const bool hit = __any((unsigned)c < 64u), edge = n0 + 64 > g.N;
-            uint2 low[LO ? 8 : 1];
             float left = 0.f;
-            wave_lds_sync();
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {  // four columns: 8 k + nh
-                float x[4];
+            for (int p = 0; p < P; ++p) {
+                wave_lds_sync();
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    x[e] = rs.y * __builtin_amdgcn_exp2f(fmaf(acc[i][k >> 2][4 * (k & 3) + e], kLog2e, -rs.x));
-                if (hit) {
+                for (int k = 0; k < 8; ++k) {  // four columns: 8 k + nh
+                    float x[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const bool at = c == 8 * k + nh + e;
-                        x[e] -= at ? rs.z : 0.f;
-                        left = at ? x[e] - bf2f(f2bf(x[e])) : left;
+                    for (int e = 0; e < 4; ++e) x[e] = acc[i][k >> 2][4 * (k & 3) + e];
+                    if (p == 0) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = rs.y * __builtin_amdgcn_exp2f(fmaf(x[e], kLog2e, -rs.x));
+                        if (hit) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const bool at = c == 8 * k + nh + e;
+                                x[e] -= at ? rs.z : 0.f;
+                                left = at ? x[e] - bf2f(f2bf(x[e])) : left;
+                            }
+                        }
+                        if (edge) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (n0 + 8 * k + nh + e >= g.N) x[e] = 0.f;
+                        }
                     }
+                    const uint2 h = make_uint2(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]));
+                    *reinterpret_cast<uint2*>(st + mr * 128 + ((k ^ (mr & 7)) * 16) + nh * 2) = h;
+                    if (p + 1 < P) {
+                        acc[i][k >> 2][4 * (k & 3)] = x[0] - __uint_as_float(h.x << 16);
+                        acc[i][k >> 2][4 * (k & 3) + 1] = x[1] - __uint_as_float(h.x & 0xffff0000u);
+                        acc[i][k >> 2][4 * (k & 3) + 2] = x[2] - __uint_as_float(h.y << 16);
+                        acc[i][k >> 2][4 * (k & 3) + 3] = x[3] - __uint_as_float(h.y & 0xffff0000u);
+                    }
+                    if (k & 1) __builtin_amdgcn_sched_barrier(0);
                 }
-                if (edge) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (n0 + 8 * k + nh + e >= g.N) x[e] = 0.f;
-                }
-                const uint2 h = make_uint2(pack_bf2(x[0], x[1]), pack_bf2(x[2], x[3]));
-                *reinterpret_cast<uint2*>(st + mr * 128 + ((k ^ (mr & 7)) * 16) + nh * 2) = h;
-                if constexpr (LO)
-                    low[k] = make_uint2(pack_bf2(x[0] - __uint_as_float(h.x << 16), x[1] - __uint_as_float(h.x & 0xffff0000u)),
-                                        pack_bf2(x[2] - __uint_as_float(h.y << 16), x[3] - __uint_as_float(h.y & 0xffff0000u)));
-                if (k & 1) __builtin_amdgcn_sched_barrier(0);
-            }
-            if (hit && (unsigned)c < 64u && (c & 4) == nh && row < g.M) resid[row] = left;
-            wave_lds_sync();
-            flush(hi, g.M, mw, n0, st, lane);
-            if constexpr (LO) {
+                if (p == 0 && hit && (unsigned)c < 64u && (c & 4) == nh && row < g.M) resid[row] = left;
                 wave_lds_sync();
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    *reinterpret_cast<uint2*>(st + mr * 128 + ((k ^ (mr & 7)) * 16) + nh * 2) = low[k];
-                wave_lds_sync();
-                flush(lo, g.M, mw, n0, st, lane);
+                flush(G + p * plane, g.M, mw, n0, st, lane);
             }
         }
     }
     // 32 rows x 64 columns from the wave's LDS, as 128-byte row segments
-    __device__ __forceinline__ void flush(bf16_t* P, int M, int mw, int n0, const unsigned char* st, int lane) const {
+    __device__ __forceinline__ void flush(bf16_t* to, int M, int mw, int n0, const unsigned char* st, int lane) const {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const int r = q * 8 + (lane >> 3), n = n0 + (lane & 7) * 8;
             const uint4 v = *reinterpret_cast<const uint4*>(st + r * 128 + (((lane & 7) ^ (lane >> 3)) * 16));
-            if (mw + r < M && n < ld) *reinterpret_cast<uint4*>(P + (size_t)(mw + r) * ld + n) = v;
+            if (mw + r < M && n < ld) *reinterpret_cast<uint4*>(to + (size_t)(mw + r) * ld + n) = v;
         }
     }
 };
@@ -234,7 +244,7 @@ int launch_logits(const GemmDesc& g, const EPI& epi, hipStream_t s) {
 
 __device__ __forceinline__ void finish_row(int t, float m, float s, const int32_t* tgt, const float* lt, float* loss,
                                            float* lse, int V) {
-    const float z = (m + __builtin_amdgcn_logf(s)) / kLog2e;
+    const float z = m + __builtin_amdgcn_logf(s) * kLn2;
     if (lse) lse[t] = z;
     const int g = tgt[t];
     if (loss) loss[t] = g >= 0 && g < V ? z - lt[t] : 0.f;
@@ -288,7 +298,8 @@ __global__ __launch_bounds__(256) void row_scales(RowScale* __restrict__ rows, f
         const int g = tgt[t];
         const bool has = g >= 0 && g < V;
         const float u = has ? (dloss ? scale * dloss[t] : scale) : 0.f;
-        r = make_float4(lse[t] * kLog2e, u + (dlse ? scale * dlse[t] : 0.f), u, __int_as_float(has ? g : -1));
+        const float b = lse[t] * kLog2e, a = u + (dlse ? scale * dlse[t] : 0.f);
+        r = make_float4(b, a * __builtin_amdgcn_exp2f(-off(lse[t], b)), u, __int_as_float(has ? g : -1));
     }
     rows[t] = r;
     resid[t] = 0.f;
@@ -313,17 +324,17 @@ __global__ __launch_bounds__(256) void piece_stats(const float* __restrict__ L, 
             const int c = v + 1024 * j;
             const float4 q = c < nv ? *reinterpret_cast<const float4*>(row + c)
                                     : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            x[4 * j] = q.x * kLog2e;
-            x[4 * j + 1] = c + 1 < nv ? q.y * kLog2e : -INFINITY;
-            x[4 * j + 2] = c + 2 < nv ? q.z * kLog2e : -INFINITY;
-            x[4 * j + 3] = c + 3 < nv ? q.w * kLog2e : -INFINITY;
+            x[4 * j] = q.x;
+            x[4 * j + 1] = c + 1 < nv ? q.y : -INFINITY;
+            x[4 * j + 2] = c + 2 < nv ? q.z : -INFINITY;
+            x[4 * j + 3] = c + 3 < nv ? q.w : -INFINITY;
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) n = fmaxf(n, x[e]);
         const float b = n == -INFINITY ? 0.f : n;
-        s *= __builtin_amdgcn_exp2f(m - b);
+        s = about(s, m, n);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f(x[e] - b);
+        for (int e = 0; e < 16; ++e) s += __builtin_amdgcn_exp2f((x[e] - b) * kLog2e);
         m = n;
     }
     const float mw = wave_max(m);
@@ -365,14 +376,29 @@ __global__ __launch_bounds__(256) void piece_grad(float* __restrict__ L, int ld,
     }
 }
 
+// The last nv % 4 logits of a piece's rows: a wave's dot product each, L[t][nq + j] = h[t] . E[j];
+// zeros in the padding's rows
+__global__ __launch_bounds__(256) void tail_logits(const float* __restrict__ h, const float* __restrict__ E,
+                                                   float* __restrict__ L, int ld, int T, int Tp, int d, int tail) {
+    const int w = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int t = w / tail, j = w - t * tail;
+    if (t >= Tp) return;
+    float s = 0.f;
+    for (int k = lane; t < T && k < d; k += 64) s = fmaf(h[(size_t)t * d + k], E[(size_t)j * d + k], s);
+    s = wave_sum(s);
+    if (lane == 0) L[(size_t)t * ld + j] = s;
+}
+
 // ---- both ---------------------------------------------------------------------------------
-// dst [Rp x dp] = src [R x d], zeros around it
+// dst [Rp x dp] = src [R x d], zeros around it, `times` over
 template <typename T>
-__global__ __launch_bounds__(256) void lay_out(const T* __restrict__ src, T* __restrict__ dst, int R, int d, int Rp, int dp) {
+__global__ __launch_bounds__(256) void lay_out(const T* __restrict__ src, T* __restrict__ dst, int R, int d, int Rp, int dp,
+                                               int times) {
     const int64_t n = (int64_t)Rp * dp;
     for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int r = (int)(i / dp), c = (int)(i - (int64_t)r * dp);
-        dst[i] = r < R && c < d ? src[(size_t)r * d + c] : (T)0;
+        const T v = r < R && c < d ? src[(size_t)r * d + c] : (T)0;
+        for (int k = 0; k < times; ++k) dst[k * n + i] = v;
     }
 }
 
@@ -447,8 +473,9 @@ GemmDesc product(const void* A, int lda, const void* B, int ldb, int K, void* C,
 struct Plan {
     bool bf, lay;
     int T, d, V, q, es, dp, Tp;
+    int planes;      // bf16: pieces of G that an fp32 dE takes
     int vc, pieces;  // columns of a piece, a multiple of 128 (or all of a smaller vocabulary)
-    size_t h, E, Et, lt, rows, resid, stats, logits, hi, lo, acc, de, det, part, part_bytes, bytes;
+    size_t h, hs, E, lt, rows, resid, stats, logits, G, acc, de, det, part, part_bytes, bytes;
 
     Plan(int T_, int d_, int V_, int dtype, bool lay_, bool bwd) : bf(dtype == GN_BF16), lay(lay_), T(T_), d(d_), V(V_) {
         q = bf ? 8 : 4;
@@ -456,8 +483,9 @@ struct Plan {
         lay = lay || d % q;
         dp = round_up(d, q);
         Tp = bf ? T : round_up(T, 4);
-        // A piece's G (hi + lo, or the fp32 logits it replaces) takes 4 bytes an element
-        const int64_t most = kPieceBytes / (lay ? 4 : 1) / 4 / std::max(Tp, 1);
+        planes = T > kTwoPieces ? 2 : 3;
+        // a piece's G, or the fp32 logits it replaces
+        const int64_t most = kPieceBytes / (lay ? 4 : 1) / (bf ? 2 * planes : 4) / std::max(Tp, 1);
         // whole rounds of 256 x 128 tiles of dE's product on the compute units, or what there is room for
         const int64_t round = (int64_t)std::max(1, stream_blocks() / ((dp + 127) / 128)) * 256;
         int64_t cols = most >= round ? most / round * round : 2 * most >= round ? round : most / 128 * 128;
@@ -471,10 +499,14 @@ struct Plan {
             GemmDesc a = product(nullptr, vc, nullptr, dp, Tp, nullptr, dp, nv, dp);
             GemmDesc b = product(nullptr, vc, nullptr, dp, nv, nullptr, dp, Tp, dp);
             if (bf) {
-                a.nseg = 2;
-                a.lda[1] = vc;
-                a.ldb[1] = dp;
-                a.Ks[1] = T;
+                if (planes == 2) {
+                    a.nseg = 2;
+                    a.lda[1] = vc;
+                    a.ldb[1] = dp;
+                    a.Ks[1] = T;
+                } else {
+                    a.Ks[0] = 3 * T;
+                }
                 part_bytes = std::max({part_bytes, gemm_dma_part_bytes(a, 1, GN_F32), gemm_dma_part_bytes(b, 0, GN_F32)});
                 a.accumulate = b.accumulate = 1;
                 part_bytes = std::max({part_bytes, gemm_dma_part_bytes(a, 1, GN_F32), gemm_dma_part_bytes(b, 0, GN_F32)});
@@ -491,7 +523,6 @@ struct Plan {
         };
         h = take(lay || Tp != T ? (size_t)Tp * dp * es : 0);
         E = take(lay ? (size_t)vc * dp * es : 0);
-        Et = take((size_t)q * dp * es);
         lt = take((size_t)T * 4);
         logits = take(bf ? 0 : (size_t)Tp * vc * 4);
         part = take(part_bytes);
@@ -502,8 +533,8 @@ struct Plan {
         }
         rows = take((size_t)Tp * sizeof(RowScale));
         resid = take((size_t)Tp * 4);
-        hi = take(bf ? (size_t)T * vc * 2 : 0);
-        lo = take(bf ? (size_t)T * vc * 2 : 0);
+        hs = take(bf && planes == 3 ? (size_t)3 * T * dp * 2 : 0);
+        G = take(bf ? (size_t)planes * T * vc * 2 : 0);
         acc = take((size_t)Tp * dp * 4);
         de = take(lay ? (size_t)vc * dp * 4 : 0);
         det = take((size_t)q * dp * 4);
@@ -513,6 +544,9 @@ struct Plan {
     // 32000 2479, 2376, 2412, 2238; 2001 x 1024 x 50001 971, 931, 920, 918; 8192 x 2048 x 128000 19.7,
     // 19.1, 20.1, 20.0 ms.  Whole rounds at 256 MB took the backward of the first 1821 -> 1793, of the
     // second (bf16 dE) 709 -> 678.
+    // Rows from which an fp32 dE takes two pieces of G (2^-17 of an element): the fp32 sum over that many
+    // rows is itself no better (sqrt(4096) 2^-24 = 2^-18).  Below it takes three, as good as fp32.
+    static constexpr int kTwoPieces = 4096;
     static constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 };
 
@@ -560,10 +594,10 @@ struct Call {
     int dtype;
     const void* hp = nullptr;  // [Tp x dp]
 
-    int copy(const void* src, size_t to, int R, int Rp) {
+    int copy(const void* src, size_t to, int R, int Rp, int times = 1) {
         const unsigned grid = grid_for((int64_t)Rp * w.dp, 1024, 16384);
-        if (w.bf) lay_out<bf16_t><<<grid, 256, 0, s>>>((const bf16_t*)src, (bf16_t*)(base + to), R, w.d, Rp, w.dp);
-        else lay_out<float><<<grid, 256, 0, s>>>((const float*)src, (float*)(base + to), R, w.d, Rp, w.dp);
+        if (w.bf) lay_out<bf16_t><<<grid, 256, 0, s>>>((const bf16_t*)src, (bf16_t*)(base + to), R, w.d, Rp, w.dp, times);
+        else lay_out<float><<<grid, 256, 0, s>>>((const float*)src, (float*)(base + to), R, w.d, Rp, w.dp, times);
         GN_LAUNCH_CHECK(who);
         return GN_OK;
     }
@@ -585,7 +619,7 @@ struct Call {
         g.part = (float*)(base + w.part);
         g.part_cap = w.part_bytes;
     }
-    // fp32: a piece's logits, the columns past its last multiple of 4 through four rows of their own
+    // fp32: a piece's logits
     int logits32(const void* Ec, int nv) {
         float* const L = (float*)(base + w.logits);
         const int nq = nv / w.q * w.q, cols = w.lay ? round_up(nv, w.q) : nq;
@@ -595,10 +629,10 @@ struct Call {
             if (const int rc = gemm_run(g, 0, 1, dtype, GN_F32, s)) return rc;
         }
         if (cols >= nv) return GN_OK;
-        if (const int rc = copy((const char*)Ec + (size_t)nq * w.d * w.es, w.Et, nv - nq, w.q)) return rc;
-        GemmDesc g = product(hp, w.dp, base + w.Et, w.dp, w.dp, L + nq, w.vc, w.Tp, w.q);
-        scratch(g);
-        return gemm_run(g, 0, 1, dtype, GN_F32, s);
+        tail_logits<<<(w.Tp * (nv - nq) + 3) / 4, 256, 0, s>>>((const float*)h, (const float*)Ec + (size_t)nq * w.d, L + nq,
+                                                             w.vc, w.T, w.Tp, w.d, nv - nq);
+        GN_LAUNCH_CHECK(who);
+        return GN_OK;
     }
 };
 
@@ -680,19 +714,26 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
     char* const base = (char*)ws;
     Call c{who, w, base, h, E, s, dtype};
     if (const int rc = c.start()) return rc;
-    const bool two = w.bf && dE && dE_dtype == GN_F32;  // G in two pieces
+    const int planes = w.bf && dE && dE_dtype == GN_F32 ? w.planes : 1;
+    const size_t plane = (size_t)T * w.vc;
     RowScale* const rows = (RowScale*)(base + w.rows);
     float* const resid = (float*)(base + w.resid);
-    char* const G = base + (w.bf ? w.hi : w.logits);
-    bf16_t* const lo = (bf16_t*)(base + w.lo);
+    char* const G = base + (w.bf ? w.G : w.logits);
+    if (planes == 3) {  // three pieces are one k-segment of 3 T rows beside h three times
+        if (const int rc = c.copy(h, w.hs, T, T, 3)) return rc;
+    }
     row_scales<<<(w.Tp + 255) / 256, 256, 0, s>>>(rows, resid, T, w.Tp, targets, lse, dloss, dlse, scale, V);
     GN_LAUNCH_CHECK(who);
     // dst (+)= G's columns c0 .. c0 + M, transposed, times h: fp32 or in dE's own type
     auto weight = [&](int c0, int M, void* dst, int c_dtype, bool add) {
         GemmDesc g = product(G + (size_t)c0 * w.es, w.vc, c.hp, w.dp, w.Tp, dst, w.dp, M, w.dp);
-        if (two) {
+        if (planes == 3) {
+            g.B[0] = (const bf16_t*)(base + w.hs);
+            g.Ks[0] = 3 * T;
+        }
+        if (planes == 2) {
             g.nseg = 2;
-            g.A[1] = lo + c0;
+            g.A[1] = (const bf16_t*)G + plane + c0;
             g.lda[1] = w.vc;
             g.B[1] = g.B[0];
             g.ldb[1] = w.dp;
@@ -718,8 +759,10 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
         if (const int rc = c.piece(v0, nv, &Ec)) return rc;
         if (w.bf) {
             const GemmDesc g = product(c.hp, w.dp, Ec, w.dp, w.dp, nullptr, 0, T, nv);
-            const int rc = two ? launch_logits(g, GradTile<true>{rows, (bf16_t*)G, lo, resid, w.vc, v0}, s)
-                               : launch_logits(g, GradTile<false>{rows, (bf16_t*)G, nullptr, resid, w.vc, v0}, s);
+            bf16_t* const Gp = (bf16_t*)G;
+            const int rc = planes == 3   ? launch_logits(g, GradTile<3>{rows, Gp, plane, resid, w.vc, v0}, s)
+                           : planes == 2 ? launch_logits(g, GradTile<2>{rows, Gp, plane, resid, w.vc, v0}, s)
+                                         : launch_logits(g, GradTile<1>{rows, Gp, plane, resid, w.vc, v0}, s);
             if (rc) return rc;
         } else {
             if (const int rc = c.logits32(Ec, nv)) return rc;

@@ -310,9 +310,10 @@ int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* targets, flo
  *   dh = G E [T x d] in dtype,  dE (+)= G^T h [V x d] in dE_dtype (GN_F32, or GN_BF16 on the bf16
  *   path).  dh or dE may be NULL; GN_ACCUMULATE adds onto an fp32 dE (a tied embedding's
  *   gradient, micro-batches), dh is overwritten.
- * A piece of the vocabulary at a time, its logits formed again.  On the bf16 path G enters dh and
- * a bf16 dE rounded to bf16, and an fp32 dE as two bf16 pieces (2^-17 of each element).  Every
- * sum's order is fixed: the same bits every time.  ws as for the forward. */
+ * A piece of the vocabulary at a time, its logits formed again.  On the bf16 path G enters a bf16 dE and,
+ * but for its element at the target (fp32), dh rounded to bf16; an fp32 dE takes it as three bf16
+ * pieces, of more than 4096 rows as two (2^-17 of each element).  Every sum's order is fixed: the same
+ * bits every time.  ws as for the forward. */
 int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* targets, const float* lse,
                        const float* dloss, const float* dlse, float scale, void* dh, void* dE,
                        int dE_dtype, int T, int d, int V, int dtype, unsigned flags, void* ws,
