@@ -569,6 +569,11 @@ int check(const char* who, const void* h, const void* E, const int32_t* tgt, int
     return GN_OK;
 }
 
+// Whether two tensors share memory
+bool shared(const void* a, size_t na, const void* b, size_t nb) {
+    return a && b && (const char*)a < (const char*)b + nb && (const char*)b < (const char*)a + na;
+}
+
 int check_ws(const char* who, const Plan& w, int dtype, const void* ws, size_t ws_bytes) {
     // the query's answer for the shape at hand (four plans, some microseconds)
     thread_local int of[4] = {0, 0, 0, 0};
@@ -709,6 +714,10 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
     }
     GN_REQUIRE(lse, "%s: null pointer", who);
     if (!dh && !dE) return GN_OK;
+    const size_t es = dtype == GN_F32 ? 4 : 2, nh = (size_t)T * d * es, nE = (size_t)V * d * es, ndE = (size_t)V * d * des;
+    GN_REQUIRE(!shared(dh, nh, h, nh) && !shared(dh, nh, E, nE) && !shared(dE, ndE, h, nh) && !shared(dE, ndE, E, nE) &&
+                   !shared(dE, ndE, dh, nh),
+               "%s: dh and dE may not share memory with each other or the inputs", who);
     const Plan w(T, d, V, dtype, !al16(h) || !al16(E) || !al16(dE), true);
     if (const int rc = check_ws(who, w, dtype, ws, ws_bytes)) return rc;
     char* const base = (char*)ws;

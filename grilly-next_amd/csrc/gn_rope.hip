@@ -520,7 +520,7 @@ int64_t span(const gn_heads& t, int B, int S, int D) {
 }
 
 // Whether a and b may share an element.  Disjoint ranges do not; neither do parts of one buffer's
-// rows (equal token or batch strides, the two blocks apart within the period).
+// rows (equal head, token or batch strides, the two blocks apart within the period).
 bool overlap(const gn_heads& a, const gn_heads& b, int B, int S, int D, int es) {
     const char *pa = (const char*)a.p, *pb = (const char*)b.p;
     if (pa + span(a, B, S, D) * es <= pb || pb + span(b, B, S, D) * es <= pa) return false;
@@ -535,6 +535,10 @@ bool overlap(const gn_heads& a, const gn_heads& b, int B, int S, int D, int es) 
     const bool same_b = B == 1 || a.sb == b.sb, same_s = S == 1 || a.ss == b.ss;
     const int64_t ps = S > 1 ? a.ss : B > 1 ? a.sb : 0;
     if (same_b && same_s && (S == 1 || B == 1 || a.sb % a.ss == 0) && apart(ps, ha, hb)) return false;
+    const bool same_h = a.H == b.H && (a.H == 1 || a.sh == b.sh);
+    if (same_b && same_s && same_h && a.H > 1 && a.sh > 0 && (S == 1 || a.ss % a.sh == 0) &&
+        (B == 1 || a.sb % a.sh == 0) && apart(a.sh, D, D))
+        return false;
     if (same_b && B > 1 && apart(a.sb, ha + (S - 1) * a.ss, hb + (S - 1) * b.ss)) return false;
     return true;
 }
@@ -586,6 +590,8 @@ int check(const char* who, const gn_rope* r, int B, int S, int D, int dtype, con
         GN_REQUIRE(mode == GN_ROPE_HALF || mode == GN_ROPE_INTERLEAVED, "%s: unknown rope mode %d", who, mode);
         GN_REQUIRE(r->freqs, "%s: freqs is a null pointer", who);
         GN_REQUIRE(r->pos_sb >= 0, "%s: positions have a negative stride", who);
+        GN_REQUIRE(((uintptr_t)r->freqs & 7u) == 0 && ((uintptr_t)r->positions & 3u) == 0,
+                   "%s: freqs or positions are not aligned to their elements", who);
     }
     const int es = dtype == GN_F32 ? 4 : 2;
     vec = D % 16 == 0 && rot % 16 == 0;
@@ -645,7 +651,7 @@ void tile(Args& a, int k, int heads, int rows_at_once, int rounds) {
     if (a.rot) tb = std::min(tb, std::max(1, 4096 / a.rot));
     tb = std::min(tb, std::max(1, a.tokens / 1024));
     a.TB[k] = tb;
-    a.tiles[k] = (a.tokens + tb - 1) / tb;
+    a.tiles[k] = (int)(((int64_t)a.tokens + tb - 1) / tb);
 }
 
 size_t tile_smem(const Args& a) {

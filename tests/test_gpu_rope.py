@@ -215,6 +215,27 @@ def test_qk_norm_rope(gn, B, S, Hq, Hk, D, rot, mode, dtype):
     assert torch.equal(one, got[3] + 1)
 
 
+def test_qk_interleaved_heads_in_place(gn):
+    """q, k and v of a head side by side ([B, S, H, 3, D]), normed where they lie, and their gradients
+    in one tensor of that layout."""
+    g = gen(21)
+    B, S, H, D = 2, 19, 4, 64
+    x, dy = rand(g, B, S, H, 3, D), rand(g, B, S, H, 3, D)
+    w, f = rand(g, D), freqs(D)
+    a, b = gn.qk_norm_rope_fwd(x[:, :, :, 0].contiguous(), x[:, :, :, 1].contiguous(), w, w, f)
+    dq, dk, _, dwq, dwk = gn.qk_norm_rope_bwd(dy[:, :, :, 0].contiguous(), dy[:, :, :, 1].contiguous(), x[:, :, :, 0], x[:, :, :, 1],
+                                              w, w, f)
+    dx = torch.zeros_like(x)
+    got = gn.qk_norm_rope_bwd(dy[:, :, :, 0], dy[:, :, :, 1], x[:, :, :, 0], x[:, :, :, 1], w, w, f, dyv=dy[:, :, :, 2],
+                              out=[dx[:, :, :, i] for i in range(3)])
+    assert torch.equal(dx[:, :, :, 0], dq) and torch.equal(dx[:, :, :, 1], dk) and torch.equal(dx[:, :, :, 2], dy[:, :, :, 2])
+    assert torch.equal(got[3], dwq) and torch.equal(got[4], dwk)
+    keep = x.clone()
+    parts = [x[:, :, :, i] for i in range(3)]
+    gn.qk_norm_rope_fwd(*parts[:2], w, w, f, v=parts[2], out=parts)
+    assert torch.equal(x[:, :, :, 0], a) and torch.equal(x[:, :, :, 1], b) and torch.equal(x[:, :, :, 2], keep[:, :, :, 2])
+
+
 def test_qk_without_weights_keys_or_dw(gn):
     g = gen(2)
     q, dy = rand(g, 2, 9, 3, 64), rand(g, 2, 9, 3, 64)

@@ -49,6 +49,8 @@ def test_rope_refuses(entry):
     refused(fn(x, y, rope(mode=0), B, S, D, 4, None), "mode")
     refused(fn(x, y, rope(freqs=None), B, S, D, 4, None), "freqs")
     refused(fn(x, y, rope(pos_sb=-1), B, S, D, 4, None), "negative")
+    refused(fn(x, y, rope(freqs=BASE + 4), B, S, D, 4, None), "aligned")
+    refused(fn(x, y, rope(positions=BASE + 2), B, S, D, 4, None), "aligned")
     refused(fn(x, heads(MB, ss=-1), r, B, S, D, 4, None), "negative")
     refused(fn(heads(1), y, r, B, S, D, 4, None), "aligned")
     refused(fn(heads(2), y, r, B, S, D, 0, None), "aligned")
@@ -118,6 +120,14 @@ def test_fused_rows_may_be_written_part_by_part():
     bad = part(MB, 0)
     bad.sh = D + 2
     refused(go(bad), "overlaps")
+    # heads interleaved, q and k of a head side by side: rows of [H, 3, D]
+    C = 3 * 4 * D
+    turn = lambda off, i: gn.Heads(BASE + off + i * D * 2, S * C, C, 3 * D, 4)
+    go = lambda dq, dk: lib.gn_qk_norm_rope_bwd(dy[0], dy[1], dy[2], turn(0, 0), turn(0, 1), None, None, dq, dk,
+                                                turn(MB, 2), ctypes.c_void_p(BASE), None, rope(), B, S, D, 1e-6, 4, 0,
+                                                None, 0, None)
+    refused(go(turn(MB, 0), turn(MB, 1)), "workspace", -3)
+    refused(go(turn(MB, 0), gn.Heads(BASE + MB + D, S * C, C, 3 * D, 4)), "overlaps")
 
 
 def test_linear_xent_refuses():
@@ -159,6 +169,9 @@ def test_linear_xent_refuses():
     refused(bwd(dh=p(1)), "aligned")
     refused(bwd(dlse=p(2)), "aligned")
     refused(bwd(wsb=8), "workspace", -3)
+    refused(bwd(dh=p()), "share")
+    refused(bwd(dE=p(MB)), "share")
+    refused(bwd(dE=p(6 * MB + 64)), "share")
     assert bwd(dh=None, dE=None) == 0 and bwd(T=0, dE=None) == 0
     for bad in ((0, 64, 100, 4), (16, 0, 100, 4), (16, 64, 0, 4), (16, 64, 100, 1)):
         assert lib.gn_linear_xent_workspace_bytes(*bad) == 0
