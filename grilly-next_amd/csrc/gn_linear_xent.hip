@@ -214,6 +214,219 @@ struct GradTile {
     }
 };
 
+// ---- bf16, up to 32 rows --------------------------------------------------------------------
+// The product is then a read of E, and the tiles above read it 128 bytes of a row at a time (4.0 TB/s
+// where a whole-row reader reaches 6.0: 16 x 2048 x 32000, 33 us).  Here a stage is 32 rows of E, 512
+// bytes of each; eight stages (128 KB of LDS) run through, 112 KB of E on their way to each compute
+// unit.  The four waves share a stage's k, 64 each, and keep their part of h in registers for all of the
+// block's tiles (32 rows x NS 256 k: 16 NS registers); a tile's four partial 32 x 32 products are summed
+// in LDS in the waves' order.  Lane l then has row l % 32, and of the tile's columns wave w's
+// 8 w + 4 (l / 32) + 0..3.
+constexpr int kFewRows = 32, kFewStages = 8, kFewStage = 32 * 512;
+constexpr size_t kFewSmem = (size_t)kFewStages * kFewStage + 4 * 4096;
+
+template <int NS, typename EPI>
+__global__ __launch_bounds__(256, 1) void logits_few(const bf16_t* __restrict__ h, int T, const bf16_t* __restrict__ E,
+                                                     int V, EPI epi) {
+    constexpr int d = 256 * NS;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    const uint32_t lds0 = lds_addr(smem_raw);
+    float* const red = reinterpret_cast<float*>(smem_raw + kFewStages * kFewStage);
+    const int lane = threadIdx.x & 63, row = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles = (V + 31) / 32;
+    const int ntile = (tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+
+    // the stream of stages: tile fi of the block, its s-th 256 k
+    int fi = 0, fs = 0;
+    uint32_t vo[4];
+    const bf16_t* src;
+    auto place = [&]() __attribute__((always_inline)) {
+        const int r0 = ((int)blockIdx.x + fi * (int)gridDim.x) * 32;
+        src = E + (size_t)r0 * d;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int r = 2 * (4 * wave + q) + (lane >> 5);
+            vo[q] = (uint32_t)(min(r0 + r, V - 1) - r0) * (d * 2) + (uint32_t)((row ^ (r & 15)) * 16);
+        }
+    };
+    auto issue = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            dma16s(src + fs * 256, vo[q], lds0 + (uint32_t)(slot * kFewStage + (4 * wave + q) * 1024));
+        if (fs + 1 < NS) {
+            ++fs;
+        } else if (fi + 1 < ntile) {  // past the end: the last stage again
+            ++fi;
+            fs = 0;
+            place();
+        }
+    };
+    place();
+#pragma unroll
+    for (int k = 0; k < kFewStages - 1; ++k) issue(k);
+    bf16x8_t hf[NS][4];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks)
+            hf[s][ks] = ld_frag16(h + (size_t)min(row, T - 1) * d + 256 * s + 64 * wave + 16 * ks + 8 * (lane >> 5));
+    epi.start(T, row);
+    int fo[4];  // a fragment's place in a stage
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) fo[ks] = row * 512 + (((8 * wave + 2 * ks + (lane >> 5)) ^ (row & 15)) * 16);
+
+    int slot = 0;
+    for (int i = 0; i < ntile; ++i) {
+        f32x16_t acc;
+        zero16(acc);
+        static_for<NS>([&](auto S_) {
+            constexpr int s = decltype(S_)::value;
+            // this stage has landed (six may be on their way), and every wave has left the one before
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(4 * (kFewStages - 2)) & 0xF0FFu);
+            __syncthreads();
+            issue((slot + kFewStages - 1) & (kFewStages - 1));
+            const unsigned char* at = smem_raw + slot * kFewStage;
+            bf16x8_t e[4];
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) e[ks] = __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const uint4*>(at + fo[ks]));
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) acc = mfma32(e[ks], hf[s][ks], acc);
+            slot = (slot + 1) & (kFewStages - 1);
+        });
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4*>(red + ((wave * 4 + q) * 64 + lane) * 4) =
+                make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(63) & 0xF0FFu);
+        __syncthreads();
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float4 p = *reinterpret_cast<const float4*>(red + ((w * 4 + wave) * 64 + lane) * 4);
+            x[0] += p.x; x[1] += p.y; x[2] += p.z; x[3] += p.w;
+        }
+        epi.tile(((int)blockIdx.x + i * (int)gridDim.x) * 32 + 8 * wave + 4 * (lane >> 5), V, x);
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    __syncthreads();
+    epi.finish(red, wave, lane);
+}
+
+// A block's statistics of each row, one strip a block; c: the target's column
+struct StatsFew {
+    const int32_t* tgt;
+    float* lt;
+    float2* part;  // [gridDim.x][T]
+    int v0, strip0;
+    int T, t, c;
+    float m, s;
+    __device__ __forceinline__ void start(int T_, int row) {
+        T = T_;
+        t = row;
+        c = row < T ? tgt[row] - v0 : -1;
+        m = -INFINITY;
+        s = 0.f;
+    }
+    __device__ __forceinline__ void tile(int v, int V, const float (&x)[4]) {
+        float y[4], n = m;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            y[e] = v + e < V ? x[e] : -INFINITY;
+            n = fmaxf(n, y[e]);
+        }
+        const float b = n == -INFINITY ? 0.f : n;
+        s = about(s, m, n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            s += __builtin_amdgcn_exp2f((y[e] - b) * kLog2e);
+            if (v + e == c && v + e < V) lt[t] = x[e];
+        }
+        m = n;
+    }
+    __device__ __forceinline__ void finish(float* red, int wave, int lane) {
+        float2* const sh = reinterpret_cast<float2*>(red);
+        sh[(2 * wave + (lane >> 5)) * 32 + t] = make_float2(m, s);
+        __syncthreads();
+        if (wave || lane >= 32 || t >= T) return;
+#pragma unroll
+        for (int k = 1; k < 8; ++k) join(m, s, sh[k * 32 + t].x, sh[k * 32 + t].y);
+        part[(size_t)(strip0 + blockIdx.x) * T + t] = make_float2(m, s);
+    }
+};
+
+// G of the tile's columns (below ld), as P bf16 pieces
+template <int P>
+struct GradFew {
+    const RowScale* rows;
+    bf16_t* G;
+    size_t plane;
+    float* resid;
+    int ld, v0;
+    int T, t, c;
+    RowScale rs;
+    __device__ __forceinline__ void start(int T_, int row) {
+        T = T_;
+        t = row;
+        rs = rows[min(row, T - 1)];
+        c = row < T ? __float_as_int(rs.w) - v0 : -1;
+    }
+    __device__ __forceinline__ void tile(int v, int V, const float (&x)[4]) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            y[e] = rs.y * __builtin_amdgcn_exp2f(fmaf(x[e], kLog2e, -rs.x));
+            if (v + e == c) {
+                y[e] -= rs.z;
+                resid[t] = y[e] - bf2f(f2bf(y[e]));
+            }
+            if (v + e >= V) y[e] = 0.f;
+        }
+        if (t >= T || v >= ld) return;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const uint2 g = make_uint2(pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3]));
+            *reinterpret_cast<uint2*>(G + p * plane + (size_t)t * ld + v) = g;
+            y[0] -= __uint_as_float(g.x << 16);
+            y[1] -= __uint_as_float(g.x & 0xffff0000u);
+            y[2] -= __uint_as_float(g.y << 16);
+            y[3] -= __uint_as_float(g.y & 0xffff0000u);
+        }
+    }
+    __device__ __forceinline__ void finish(float*, int, int) {}
+};
+
+// whether logits_few takes a product, and its blocks (and strips of statistics) over N columns: no more than
+// the tiles' strips of 64, which the workspace has room for
+bool few_takes(const GemmDesc& g) { return g.M <= kFewRows && g.Ks[0] % 256 == 0 && g.Ks[0] <= 2048; }
+int few_blocks(int N) { return std::min((N + 63) / 64, stream_blocks()); }
+
+template <int NS, typename EPI>
+int launch_few(const GemmDesc& g, const EPI& epi, hipStream_t s) {
+    static const bool ok = allow_lds(logits_few<NS, EPI>, kFewSmem);
+    if (!ok) {
+        set_error("linear xent: cannot reserve %zu B of LDS", kFewSmem);
+        return GN_E_HIP;
+    }
+    hipLaunchKernelGGL((logits_few<NS, EPI>), dim3(few_blocks(g.N)), dim3(256), kFewSmem, s, g.A[0], g.M, g.B[0], g.N, epi);
+    GN_LAUNCH_CHECK("linear xent (logits of few rows)");
+    return GN_OK;
+}
+
+template <typename EPI>
+int launch_few(const GemmDesc& g, const EPI& epi, hipStream_t s) {
+    switch (g.Ks[0] / 256) {
+        case 1: return launch_few<1>(g, epi, s);
+        case 2: return launch_few<2>(g, epi, s);
+        case 3: return launch_few<3>(g, epi, s);
+        case 4: return launch_few<4>(g, epi, s);
+        case 5: return launch_few<5>(g, epi, s);
+        case 6: return launch_few<6>(g, epi, s);
+        case 7: return launch_few<7>(g, epi, s);
+        default: return launch_few<8>(g, epi, s);
+    }
+}
+
 template <int BM, int STAGES, typename EPI>
 int launch_logits_tile(const GemmDesc& g, const EPI& epi, hipStream_t s) {
     constexpr int BN = 128;
@@ -232,8 +445,7 @@ int launch_logits_tile(const GemmDesc& g, const EPI& epi, hipStream_t s) {
 }
 
 // 256-row tiles, or 128-row ones where they need less (the streamed products' rule: a round of them
-// takes 0.6 of a round of the large).  Up to 64 rows the product is a read of E: 64-row tiles leave the
-// LDS to six stages, 80 KB of E on its way to each compute unit.
+// takes 0.6 of a round of the large).  Up to 64 rows 64-row tiles, which leave the LDS to six stages.
 template <typename EPI>
 int launch_logits(const GemmDesc& g, const EPI& epi, hipStream_t s) {
     const long blocks = stream_blocks(), tn = (g.N + 127) / 128;
@@ -664,6 +876,7 @@ extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* t
     Call c{who, w, base, h, E, as_stream(stream), dtype};
     if (const int rc = c.start()) return rc;
     float* const lt = (float*)(base + w.lt);
+    int strips = 0;
     const int step = w.bf && !w.lay ? V : w.vc;  // all at once where E is read as it lies
     for (int v0 = 0; v0 < V; v0 += step) {
         const int nv = std::min(step, V - v0);
@@ -671,8 +884,11 @@ extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* t
         if (const int rc = c.piece(v0, nv, &Ec)) return rc;
         if (w.bf) {
             const GemmDesc g = product(c.hp, w.dp, Ec, w.dp, w.dp, nullptr, 0, T, nv);
-            const StatsTile epi{targets, lt, (float2*)(base + w.stats), v0};
-            if (const int rc = launch_logits(g, epi, c.s)) return rc;
+            float2* const part = (float2*)(base + w.stats);
+            const int rc = few_takes(g) ? launch_few(g, StatsFew{targets, lt, part, v0, strips}, c.s)
+                                        : launch_logits(g, StatsTile{targets, lt, part, v0}, c.s);
+            if (rc) return rc;
+            strips += few_takes(g) ? few_blocks(nv) : (nv + 63) / 64;
         } else {
             if (const int rc = c.logits32(Ec, nv)) return rc;
             piece_stats<<<T, 256, 0, c.s>>>((const float*)(base + w.logits), w.vc, v0, nv, targets,
@@ -682,8 +898,8 @@ extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* t
     }
     if (w.bf) {
         const float2* part = (const float2*)(base + w.stats);
-        if (T < 256) row_stats<2><<<(T + 1) / 2, 256, 0, c.s>>>(part, (V + 63) / 64, T, targets, lt, loss, lse, V);
-        else row_stats<16><<<(T + 15) / 16, 256, 0, c.s>>>(part, (V + 63) / 64, T, targets, lt, loss, lse, V);
+        if (T < 256) row_stats<2><<<(T + 1) / 2, 256, 0, c.s>>>(part, strips, T, targets, lt, loss, lse, V);
+        else row_stats<16><<<(T + 15) / 16, 256, 0, c.s>>>(part, strips, T, targets, lt, loss, lse, V);
         GN_LAUNCH_CHECK(who);
     }
     return GN_OK;
@@ -768,10 +984,17 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
         if (const int rc = c.piece(v0, nv, &Ec)) return rc;
         if (w.bf) {
             const GemmDesc g = product(c.hp, w.dp, Ec, w.dp, w.dp, nullptr, 0, T, nv);
-            bf16_t* const Gp = (bf16_t*)G;
-            const int rc = planes == 3   ? launch_logits(g, GradTile<3>{rows, Gp, plane, resid, w.vc, v0}, s)
-                           : planes == 2 ? launch_logits(g, GradTile<2>{rows, Gp, plane, resid, w.vc, v0}, s)
-                                         : launch_logits(g, GradTile<1>{rows, Gp, plane, resid, w.vc, v0}, s);
+            auto logits = [&](auto P_) {
+                constexpr int P = decltype(P_)::value;
+                bf16_t* const Gp = (bf16_t*)G;
+                if constexpr (P != 2) {  // two pieces: of many rows
+                    if (few_takes(g)) return launch_few(g, GradFew<P>{rows, Gp, plane, resid, w.vc, v0}, s);
+                }
+                return launch_logits(g, GradTile<P>{rows, Gp, plane, resid, w.vc, v0}, s);
+            };
+            const int rc = planes == 3   ? logits(std::integral_constant<int, 3>{})
+                           : planes == 2 ? logits(std::integral_constant<int, 2>{})
+                                         : logits(std::integral_constant<int, 1>{});
             if (rc) return rc;
         } else {
             if (const int rc = c.logits32(Ec, nv)) return rc;
