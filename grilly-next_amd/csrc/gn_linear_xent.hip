@@ -659,6 +659,68 @@ __global__ __launch_bounds__(256) void dh_finish(const float* __restrict__ acc, 
     }
 }
 
+// ---- bf16, up to 32 rows: dh ------------------------------------------------------------------
+// dh = G E over the whole vocabulary is a read of E too, with a long k and few outputs, which the products'
+// splits in eight left on 64 blocks (16 rows, 32000 x 2048: 70 us of dh alone).  Here a block takes 256
+// columns and one of S ranges of the vocabulary, 64 rows of E (512 bytes of each) and of G a stage,
+// four stages in LDS; its 32 x 256 partial sums go to plane blockIdx.y, added in order afterwards.
+constexpr int kFewDhStage = (256 + 32) * BK * 2, kFewDhStages = 4;
+constexpr size_t kFewDhSmem = (size_t)kFewDhStages * kFewDhStage;
+
+__global__ __launch_bounds__(256, 1) void dh_few(const bf16_t* __restrict__ G, int ldg, const bf16_t* __restrict__ E, int nv,
+                                                 int T, int N, int per, float* __restrict__ part) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    const uint32_t lds0 = lds_addr(smem_raw);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * 256, k0 = blockIdx.y * per, k1 = min(nv, k0 + per), KT = (k1 - k0 + BK - 1) / BK;
+    constexpr int ND = 256 / 32 + 1;  // DMA instructions of a wave a stage
+    // E's rows past the range's end are read as zeros, and G's past its columns (zeros up to a multiple of 8)
+    auto issue = [&](int t) __attribute__((always_inline)) {
+        const int k = k0 + min(t, KT - 1) * BK;
+        const uint32_t base = lds0 + (uint32_t)((t & (kFewDhStages - 1)) * kFewDhStage);
+        stage_tail<256, false, 4>(E, N, n0, N, k, k1, wave, base);
+        stage_tail<32, true, 4>(G, ldg, 0, T, k, (k1 + 7) & ~7, wave, base + 256 * BK * 2);
+    };
+    f32x16_t acc[2];
+    zero16(acc[0]);
+    zero16(acc[1]);
+#pragma unroll
+    for (int t = 0; t < kFewDhStages - 1; ++t) issue(t);
+    for (int t = 0; t < KT; ++t) {
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((kFewDhStages - 2) * ND) & 0xF0FFu);
+        __syncthreads();  // stage t has landed, and every wave has left the one before
+        issue(t + kFewDhStages - 1);
+        const bf16_t* e = reinterpret_cast<const bf16_t*>(smem_raw + (t & (kFewDhStages - 1)) * kFewDhStage);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+            const bf16x8_t a = frag<32, true>(e + 256 * BK, 0, ks);
+            acc[0] = mfma32(a, frag<256, false>(e, wave * 64, ks), acc[0]);
+            acc[1] = mfma32(a, frag<256, false>(e, wave * 64 + 32, ks), acc[1]);
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    float* const out = part + (size_t)blockIdx.y * T * N;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int n = n0 + wave * 64 + j * 32 + (lane & 31);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int t = 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+            if (t < T && n < N) out[(size_t)t * N + n] = acc[j][r];
+        }
+    }
+}
+
+// ranges of the vocabulary at most (two blocks a compute unit), the rows of one for nv in all (whole stages,
+// four at least), and their number, which is no more than few_dh_most(N) or nv / 256 rounded up
+int few_dh_most(int N) { return std::max(1, 2 * stream_blocks() / ((N + 255) / 256)); }
+int few_dh_rows(int nv, int N) {
+    const int most = few_dh_most(N);
+    return std::max(4 * BK, ((nv + most - 1) / most + BK - 1) / BK * BK);
+}
+int few_dh_ranges(int nv, int N) { return (nv + few_dh_rows(nv, N) - 1) / few_dh_rows(nv, N); }
+
 // ---- host -----------------------------------------------------------------------------------
 inline bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 inline int round_up(int n, int q) { return (n + q - 1) / q * q; }
@@ -727,6 +789,8 @@ struct Plan {
                 part_bytes = std::max({part_bytes, gemm_f32_part_bytes(a), gemm_f32_part_bytes(b), gemm_f32_part_bytes(l)});
             }
         }
+        if (bf && bwd && T <= kFewRows)
+            part_bytes = std::max(part_bytes, (size_t)std::min(few_dh_most(dp), (vc + 255) / 256) * T * dp * sizeof(float));
         size_t at = 0;
         auto take = [&](size_t n) {
             const size_t p = at;
@@ -977,7 +1041,8 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
         GN_LAUNCH_CHECK(who);
         return (int)GN_OK;
     };
-    const int tail = V % w.q;
+    const bool few = w.bf && T <= kFewRows;  // dh takes every column as it is
+    const int tail = few ? 0 : V % w.q;
     for (int v0 = 0; v0 < V; v0 += w.vc) {
         const int nv = std::min(w.vc, V - v0), nq = nv / w.q * w.q;
         const void* Ec;
@@ -1014,7 +1079,22 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
                 if (const int rc = rows_out(w.det, v0 + nq, nv - nq)) return rc;
             }
         }
-        if (dh && nq) {
+        if (dh && few) {
+            static const bool ok = allow_lds(dh_few, kFewDhSmem);
+            if (!ok) {
+                set_error("%s: cannot reserve %zu B of LDS", who, kFewDhSmem);
+                return GN_E_HIP;
+            }
+            GemmDesc g = product(G, w.vc, Ec, w.dp, nv, base + w.acc, w.dp, T, w.dp);
+            g.accumulate = v0 > 0;
+            g.ksplit = few_dh_ranges(nv, w.dp);
+            c.scratch(g);
+            dh_few<<<dim3((w.dp + 255) / 256, g.ksplit), 256, kFewDhSmem, s>>>((const bf16_t*)G, w.vc, (const bf16_t*)Ec, nv, T,
+                                                                             w.dp, few_dh_rows(nv, w.dp), g.part);
+            GN_LAUNCH_CHECK(who);
+            launch_split_reduce(g, s);
+            GN_LAUNCH_CHECK(who);
+        } else if (dh && nq) {
             GemmDesc g = product(G, w.vc, Ec, w.dp, nq, base + w.acc, w.dp, w.Tp, w.dp);
             g.accumulate = v0 > 0;
             c.scratch(g);
@@ -1022,7 +1102,7 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
         }
     }
     if (dh) {
-        const float* sum = V >= w.q ? (const float*)(base + w.acc) : nullptr;
+        const float* sum = few || V >= w.q ? (const float*)(base + w.acc) : nullptr;
         const size_t col = (size_t)((V - 1) % w.vc + 1 - tail) * w.es;  // the tail's first column in the last piece
         const char* Et = (const char*)E + (size_t)(V - tail) * d * w.es;
         const bool vec = d % 8 == 0 && al16(dh) && al16(E);
