@@ -659,67 +659,102 @@ __global__ __launch_bounds__(256) void dh_finish(const float* __restrict__ acc, 
     }
 }
 
-// ---- bf16, up to 32 rows: dh ------------------------------------------------------------------
+// ---- bf16, few rows: dh -----------------------------------------------------------------------
 // dh = G E over the whole vocabulary is a read of E too, with a long k and few outputs, which the products'
 // splits in eight left on 64 blocks (16 rows, 32000 x 2048: 70 us of dh alone).  Here a block takes 256
-// columns and one of S ranges of the vocabulary, 64 rows of E (512 bytes of each) and of G a stage,
-// four stages in LDS; its 32 x 256 partial sums go to plane blockIdx.y, added in order afterwards.
-constexpr int kFewDhStage = (256 + 32) * BK * 2, kFewDhStages = 4;
-constexpr size_t kFewDhSmem = (size_t)kFewDhStages * kFewDhStage;
+// columns, 32 RT rows and one of S ranges of the vocabulary, 64 rows of E (512 bytes of each) and of G a
+// stage, four stages in LDS; its partial sums go to plane blockIdx.y, added in order afterwards.
+constexpr int kFewDhStages = 4;
+template <int RT>
+constexpr size_t few_dh_smem = (size_t)kFewDhStages * (256 + 32 * RT) * BK * 2;
 
+template <int RT>
 __global__ __launch_bounds__(256, 1) void dh_few(const bf16_t* __restrict__ G, int ldg, const bf16_t* __restrict__ E, int nv,
                                                  int T, int N, int per, float* __restrict__ part) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     const uint32_t lds0 = lds_addr(smem_raw);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n0 = blockIdx.x * 256, k0 = blockIdx.y * per, k1 = min(nv, k0 + per), KT = (k1 - k0 + BK - 1) / BK;
-    constexpr int ND = 256 / 32 + 1;  // DMA instructions of a wave a stage
+    constexpr int kStage = (256 + 32 * RT) * BK * 2;
+    const int t0 = blockIdx.z * 32 * RT, n0 = blockIdx.x * 256;
+    const int k0 = blockIdx.y * per, k1 = min(nv, k0 + per), KT = (k1 - k0 + BK - 1) / BK;
+    constexpr int ND = 256 / 32 + RT;  // DMA instructions of a wave a stage
     // E's rows past the range's end are read as zeros, and G's past its columns (zeros up to a multiple of 8)
     auto issue = [&](int t) __attribute__((always_inline)) {
         const int k = k0 + min(t, KT - 1) * BK;
-        const uint32_t base = lds0 + (uint32_t)((t & (kFewDhStages - 1)) * kFewDhStage);
+        const uint32_t base = lds0 + (uint32_t)((t & (kFewDhStages - 1)) * kStage);
         stage_tail<256, false, 4>(E, N, n0, N, k, k1, wave, base);
-        stage_tail<32, true, 4>(G, ldg, 0, T, k, (k1 + 7) & ~7, wave, base + 256 * BK * 2);
+        stage_tail<32 * RT, true, 4>(G, ldg, t0, T, k, (k1 + 7) & ~7, wave, base + 256 * BK * 2);
     };
-    f32x16_t acc[2];
-    zero16(acc[0]);
-    zero16(acc[1]);
+    f32x16_t acc[RT][2];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+        zero16(acc[i][0]);
+        zero16(acc[i][1]);
+    }
 #pragma unroll
     for (int t = 0; t < kFewDhStages - 1; ++t) issue(t);
     for (int t = 0; t < KT; ++t) {
         __builtin_amdgcn_s_waitcnt(vmcnt_imm((kFewDhStages - 2) * ND) & 0xF0FFu);
         __syncthreads();  // stage t has landed, and every wave has left the one before
         issue(t + kFewDhStages - 1);
-        const bf16_t* e = reinterpret_cast<const bf16_t*>(smem_raw + (t & (kFewDhStages - 1)) * kFewDhStage);
+        const bf16_t* e = reinterpret_cast<const bf16_t*>(smem_raw + (t & (kFewDhStages - 1)) * kStage);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-            const bf16x8_t a = frag<32, true>(e + 256 * BK, 0, ks);
-            acc[0] = mfma32(a, frag<256, false>(e, wave * 64, ks), acc[0]);
-            acc[1] = mfma32(a, frag<256, false>(e, wave * 64 + 32, ks), acc[1]);
+            const bf16x8_t b0 = frag<256, false>(e, wave * 64, ks), b1 = frag<256, false>(e, wave * 64 + 32, ks);
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const bf16x8_t a = frag<32 * RT, true>(e + 256 * BK, 32 * i, ks);
+                acc[i][0] = mfma32(a, b0, acc[i][0]);
+                acc[i][1] = mfma32(a, b1, acc[i][1]);
+            }
         }
     }
     __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     float* const out = part + (size_t)blockIdx.y * T * N;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int n = n0 + wave * 64 + j * 32 + (lane & 31);
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int t = 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-            if (t < T && n < N) out[(size_t)t * N + n] = acc[j][r];
+        for (int j = 0; j < 2; ++j) {
+            const int n = n0 + wave * 64 + j * 32 + (lane & 31);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int t = t0 + 32 * i + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                if (t < T && n < N) out[(size_t)t * N + n] = acc[i][j][r];
+            }
         }
-    }
 }
 
+// Taken up to 128 rows from three million elements of E on.  dh alone, microseconds here and through the
+// library's products: 64 x 1024 x 50000 79 and 135, 128 x 1024 x 50000 96 and 130, 128 x 768 x 8000 32.5 and
+// 33.4, 64 x 512 x 8000 28 and 32; at 256 rows 111 and 103.  Below, the second launch costs more than the
+// ranges give: 64 x 512 x 4000 25 and 24, 16 x 256 x 2000 21 and 18.
+constexpr int kFewDhRows = 128;
+inline bool dh_few_takes(int T, int V, int N) { return T <= kFewDhRows && (size_t)V * N >= 3u << 20; }
+
 // ranges of the vocabulary at most (two blocks a compute unit), the rows of one for nv in all (whole stages,
-// four at least), and their number, which is no more than few_dh_most(N) or nv / 256 rounded up
-int few_dh_most(int N) { return std::max(1, 2 * stream_blocks() / ((N + 255) / 256)); }
-int few_dh_rows(int nv, int N) {
-    const int most = few_dh_most(N);
+// four at least), and their number, which is no more than few_dh_most or nv / 256 rounded up
+int few_dh_most(int T, int N) { return std::max(1, 2 * stream_blocks() / ((N + 255) / 256 * ((T + 63) / 64))); }
+int few_dh_rows(int nv, int T, int N) {
+    const int most = few_dh_most(T, N);
     return std::max(4 * BK, ((nv + most - 1) / most + BK - 1) / BK * BK);
 }
-int few_dh_ranges(int nv, int N) { return (nv + few_dh_rows(nv, N) - 1) / few_dh_rows(nv, N); }
+int few_dh_ranges(int nv, int T, int N) { return (nv + few_dh_rows(nv, T, N) - 1) / few_dh_rows(nv, T, N); }
+
+template <int RT>
+int launch_dh_few(const GemmDesc& g, hipStream_t s) {
+    static const bool ok = allow_lds(dh_few<RT>, few_dh_smem<RT>);
+    if (!ok) {
+        set_error("linear xent: cannot reserve %zu B of LDS", few_dh_smem<RT>);
+        return GN_E_HIP;
+    }
+    dh_few<RT><<<dim3((g.N + 255) / 256, g.ksplit, (g.M + 32 * RT - 1) / (32 * RT)), 256, few_dh_smem<RT>, s>>>(
+        g.A[0], g.lda[0], g.B[0], g.Ks[0], g.M, g.N, few_dh_rows(g.Ks[0], g.M, g.N), g.part);
+    GN_LAUNCH_CHECK("linear xent (dh of few rows)");
+    launch_split_reduce(g, s);
+    GN_LAUNCH_CHECK("linear xent (dh of few rows, sums)");
+    return GN_OK;
+}
 
 // ---- host -----------------------------------------------------------------------------------
 inline bool al16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
@@ -789,8 +824,8 @@ struct Plan {
                 part_bytes = std::max({part_bytes, gemm_f32_part_bytes(a), gemm_f32_part_bytes(b), gemm_f32_part_bytes(l)});
             }
         }
-        if (bf && bwd && T <= kFewRows)
-            part_bytes = std::max(part_bytes, (size_t)std::min(few_dh_most(dp), (vc + 255) / 256) * T * dp * sizeof(float));
+        if (bf && bwd && dh_few_takes(T, V, dp))
+            part_bytes = std::max(part_bytes, (size_t)std::min(few_dh_most(T, dp), (vc + 255) / 256) * T * dp * sizeof(float));
         size_t at = 0;
         auto take = [&](size_t n) {
             const size_t p = at;
@@ -1041,7 +1076,7 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
         GN_LAUNCH_CHECK(who);
         return (int)GN_OK;
     };
-    const bool few = w.bf && T <= kFewRows;  // dh takes every column as it is
+    const bool few = w.bf && dh_few_takes(T, V, w.dp);  // dh takes every column as it is
     const int tail = few ? 0 : V % w.q;
     for (int v0 = 0; v0 < V; v0 += w.vc) {
         const int nv = std::min(w.vc, V - v0), nq = nv / w.q * w.q;
@@ -1080,20 +1115,11 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
             }
         }
         if (dh && few) {
-            static const bool ok = allow_lds(dh_few, kFewDhSmem);
-            if (!ok) {
-                set_error("%s: cannot reserve %zu B of LDS", who, kFewDhSmem);
-                return GN_E_HIP;
-            }
             GemmDesc g = product(G, w.vc, Ec, w.dp, nv, base + w.acc, w.dp, T, w.dp);
             g.accumulate = v0 > 0;
-            g.ksplit = few_dh_ranges(nv, w.dp);
+            g.ksplit = few_dh_ranges(nv, T, w.dp);
             c.scratch(g);
-            dh_few<<<dim3((w.dp + 255) / 256, g.ksplit), 256, kFewDhSmem, s>>>((const bf16_t*)G, w.vc, (const bf16_t*)Ec, nv, T,
-                                                                             w.dp, few_dh_rows(nv, w.dp), g.part);
-            GN_LAUNCH_CHECK(who);
-            launch_split_reduce(g, s);
-            GN_LAUNCH_CHECK(who);
+            if (const int rc = T <= 32 ? launch_dh_few<1>(g, s) : launch_dh_few<2>(g, s)) return rc;
         } else if (dh && nq) {
             GemmDesc g = product(G, w.vc, Ec, w.dp, nq, base + w.acc, w.dp, w.Tp, w.dp);
             g.accumulate = v0 > 0;

@@ -99,6 +99,8 @@ def within(got, ref, bound):
 SIZES = [  # T, d, V
     (1, 8, 1), (1, 64, 50), (3, 72, 7), (2, 128, 64), (16, 64, 1000), (63, 72, 257), (65, 136, 4097), (129, 768, 2000),
     (200, 64, 33001), (257, 256, 1024), (5, 77, 131), (40, 33, 1000), (1, 770, 515), (300, 1000, 777),
+    # dh of few rows over ranges of the vocabulary
+    (1, 1024, 4097), (5, 520, 6200), (32, 2048, 1601), (64, 512, 6145), (97, 1024, 3401), (128, 264, 11917),
     # few rows, every width that is read in whole rows
     (1, 256, 3), (32, 512, 1003), (31, 768, 4096), (7, 1024, 129), (32, 1280, 8200), (2, 1536, 64), (17, 1792, 500),
     (16, 2048, 33000), (5, 2304, 300), (33, 256, 9000),
