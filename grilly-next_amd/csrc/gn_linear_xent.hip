@@ -10,8 +10,8 @@
 //              dh += G E_c (fp32) from it
 // A lane holds 16 columns of one row of each 32 x 32 accumulator, so the row statistics take one
 // exchange between lanes.  For an fp32 dE, G is stored as two or three bf16 pieces, whose products with h
-// are one product's longer k: two leave 2^-17 of an element, three nothing that fp32 holds, where
-// bf16 alone (2^-8) would be the gradient's largest error.  For dh the first piece is enough but at
+// are one product's longer k: two leave 2^-17 of an element (and target_rest takes the targets' rest),
+// three nothing that fp32 holds, where bf16 alone (2^-8) would be the gradient's largest error.  For dh the first piece is enough but at
 // the target: there the rounding of a row's largest element, which shows in all of dh's row, is
 // kept in fp32 and its product with E[target] added when dh is rounded (dh_finish).
 //
@@ -659,6 +659,77 @@ __global__ __launch_bounds__(256) void dh_finish(const float* __restrict__ acc, 
     }
 }
 
+// ---- bf16, an fp32 dE of two pieces -------------------------------------------------------------
+// What the pieces left of the target elements (resid less its rounding) times h, onto dE: the largest
+// elements of G by far while p is small, alike in every row of a mean, and so what the 2^-17 showed in (dE of
+// 8192 x 2048 x 128000 off by 3.5e-6 of its norm before and by 0.9e-6 now; fp32 torch products are by
+// 1.6e-6).  Block t has the tokens of t's target in their order, if t is the first of them; it finds them
+// by reading the targets through, 1024 at a time: latency, eight blocks a compute unit against it (63 us of
+// the 18.8 ms there, 5 blocks 80).
+template <bool VEC>
+__global__ __launch_bounds__(256, 8) void target_rest(const int32_t* __restrict__ tgt, const float* __restrict__ resid,
+                                                   const bf16_t* __restrict__ h, float* __restrict__ dE, int T, int d,
+                                                   int V) {
+    constexpr int W = VEC ? 8 : 1;
+    __shared__ int who[1024];
+    __shared__ float rest[1024];
+    __shared__ int count[16];
+    const int t = blockIdx.x, c = tgt[t];
+    if (c < 0 || c >= V) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i0 = 0; i0 < t; i0 += 1024) {
+        bool before = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = i0 + 256 * k + threadIdx.x;
+            before |= i < t && tgt[i] == c;
+        }
+        if (__syncthreads_or(before)) return;
+    }
+    for (int i0 = t; i0 < T; i0 += 1024) {
+        unsigned long long m[4], any = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = i0 + 256 * k + threadIdx.x;
+            m[k] = __ballot(i < T && tgt[i] == c);
+            any |= m[k];
+            if (lane == 0) count[4 * k + wave] = __popcll(m[k]);
+        }
+        if (!__syncthreads_or(any != 0)) continue;
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            if ((k & 3) == wave && (m[k >> 2] >> lane & 1)) {
+                const int j = n + __popcll(m[k >> 2] & ((1ull << lane) - 1)), i = i0 + 256 * (k >> 2) + threadIdx.x;
+                const float r = resid[i];
+                who[j] = i;
+                rest[j] = r - bf2f(f2bf(r));
+            }
+            n += count[k];
+        }
+        __syncthreads();
+        for (int j = threadIdx.x * W; j < d; j += 256 * W) {
+            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, e[8];
+#pragma unroll 4
+            for (int k = 0; k < n; ++k) {
+                const bf16_t* p = h + (size_t)who[k] * d + j;
+                if constexpr (VEC) chunk8<bf16_t>::ld(p, e);
+                else e[0] = bf2f(*p);
+#pragma unroll
+                for (int q = 0; q < W; ++q) v[q] = fmaf(rest[k], e[q], v[q]);
+            }
+            float* const to = dE + (size_t)c * d + j;
+            if constexpr (VEC) chunk8<float>::ld(to, e);
+            else e[0] = *to;
+#pragma unroll
+            for (int q = 0; q < W; ++q) e[q] += v[q];
+            if constexpr (VEC) chunk8<float>::st(to, e);
+            else *to = e[0];
+        }
+        __syncthreads();
+    }
+}
+
 // ---- bf16, few rows: dh -----------------------------------------------------------------------
 // dh = G E over the whole vocabulary is a read of E too, with a long k and few outputs, which the products'
 // splits in eight left on 64 blocks (16 rows, 32000 x 2048: 70 us of dh alone).  Here a block takes 256
@@ -856,8 +927,11 @@ struct Plan {
     // 19.1, 20.1, 20.0 ms.  Whole rounds at 256 MB took the backward of the first 1821 -> 1793, of the
     // second (bf16 dE) 709 -> 678.
     // Rows from which an fp32 dE takes two pieces of G (2^-17 of an element): the fp32 sum over that many
-    // rows is itself no better (sqrt(4096) 2^-24 = 2^-18).  Below it takes three, as good as fp32.
-    static constexpr int kTwoPieces = 4096;
+    // rows is itself no better (sqrt(4096) 2^-24 = 2^-18).  Below it takes three, as good as fp32 (of 8192 x
+    // 2048 x 128000 23.5 ms in place of 18.9, of 8190 x 768 x 32000 2.56 in place of 2.13).  Up to kTargets
+    // rows target_rest makes the target elements whole; its reading grows with the square of the rows, and
+    // beyond sqrt(16384) 2^-24 = 2^-17.
+    static constexpr int kTwoPieces = 4096, kTargets = 16384;
     static constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 };
 
@@ -1126,6 +1200,11 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
             c.scratch(g);
             if (const int rc = gemm_run(g, 0, 0, dtype, GN_F32, s)) return rc;
         }
+    }
+    if (planes == 2 && T <= Plan::kTargets) {
+        const auto rest = d % 8 == 0 && al16(h) && al16(dE) ? target_rest<true> : target_rest<false>;
+        rest<<<T, 256, 0, s>>>(targets, resid, (const bf16_t*)h, (float*)dE, T, d, V);
+        GN_LAUNCH_CHECK(who);
     }
     if (dh) {
         const float* sum = few || V >= w.q ? (const float*)(base + w.acc) : nullptr;

@@ -175,6 +175,35 @@ def test_far_logits(gn):
     within(dE, *r.dE)
 
 
+@pytest.mark.parametrize("T,d", [(4097, 64), (5001, 77), (16384, 264)])
+def test_target_elements_of_many_rows(gn, T, d):
+    """An fp32 dE of many rows, five of them with a weight and three of those with one target: G's target
+    elements are taken whole (2^-24, not the 2^-16 of two bf16 pieces; equal logits, p = 1 / V)."""
+    g = gen(T)
+    V = 520
+    h = guarded(g, T, d)
+    E = torch.zeros(V, d, device=DEV, dtype=BF)
+    t = torch.randint(0, V, (T,), device=DEV, generator=g).to(torch.int32)
+    at = torch.tensor([3, 700, 1500, T - 300, T - 1], device=DEV)
+    t[at] = torch.tensor([7, 100, 7, 7, V - 1], device=DEV, dtype=torch.int32)
+    u = torch.zeros(T, device=DEV)
+    u[at] = torch.rand(5, device=DEV, generator=g) + 0.1
+    lse = gn.linear_xent_fwd(h, E, t)[1]
+    _, dE = gn.linear_xent_bwd(h, E, t, lse, dloss=u)
+    one = torch.ones(V, d, device=DEV)
+    gn.linear_xent_bwd(h, E, t, lse, dloss=u, need_dh=False, dE=one, accumulate=True)
+    p = (u[at].double() / V)[:, None].expand(5, V)
+    G = p.clone()
+    G[torch.arange(5), t[at].long()] -= u[at].double()
+    x = h[at].double()
+    # p: its own rounding and lse's (2^-20 (1 + lse) and 2^-21 (lse + 1)), and two pieces where it is no target
+    dG = p * (2.0 ** -16 + 2.0 ** -19 * 8) + 2.0 ** -23 * G.abs()
+    ref = G.t() @ x
+    bound = dG.t() @ x.abs() + 8 * 2.0 ** -24 * (G.t().abs() @ x.abs()) + 1e-30
+    within(dE, ref, bound)
+    within(one, ref + 1, bound + 2 * 2.0 ** -24 * (1 + ref.abs() + bound))
+
+
 def test_no_row_has_a_target(gn):
     g = gen(10)
     h, E = guarded(g, 20, 64), guarded(g, 100, 64)
