@@ -11,12 +11,21 @@
 // A lane holds 16 columns of one row of each 32 x 32 accumulator, so the row statistics take one
 // exchange between lanes.  For an fp32 dE, G is stored as two or three bf16 pieces, whose products with h
 // are one product's longer k: two leave 2^-17 of an element (and target_rest takes the targets' rest),
-// three nothing that fp32 holds, where bf16 alone (2^-8) would be the gradient's largest error.  For dh the first piece is enough but at
-// the target: there the rounding of a row's largest element, which shows in all of dh's row, is
-// kept in fp32 and its product with E[target] added when dh is rounded (dh_finish).
+// three nothing that fp32 holds, where bf16 alone (2^-8) would be the gradient's largest error.  For dh the
+// first piece is enough but at the target: there the rounding of a row's largest element, which shows in
+// all of dh's row, is kept in fp32 and its product with E[target] added when dh is rounded (dh_finish).
 //
 // fp32.  The pieces' logits are stored (fp32, in the workspace) between the library's fp32 products
 // and row kernels, G in their place.
+//
+// Measured (rows x d x vocabulary): forward and both gradients of 8192 x 2048 x 128000 18.8 ms, of 8190 x
+// 768 x 32000 2.2 ms: five products where the formulas have three (the logits again, dE's second piece), 21.5
+// and 2.0 TFLOP at 1.14 and 0.92 PFLOP/s.  The matrix cores bound them, and on them the clock: the logits
+// with their statistics take 3.4-3.6 ms at 67 % of the matrix pipe and 1.65-1.75 GHz, the library's product
+// alone 3.3-3.9 at 76 % and 1.53.  256 x 256 tiles of four waves that issue their own loads took 2 % off
+// the larger and put 6 % onto smaller ones; staggered starts of the blocks gave nothing.  Few rows are a read
+// of E: 16 x 2048 x 32000 forward 26 us + 4 for 131 MB (5.0 TB/s).  fp32 of 1003 x 768 x 32000: 1.15-1.3 ms,
+// four products, 0.197 TFLOP at six bf16 ones each, 0.9-1.0 PFLOP/s of those.
 //
 // Widths, row counts and vocabularies that the products' vectors do not divide: h and E's piece are
 // laid out to multiples of q = 8 (bf16) or 4 (fp32) elements first; the last V % q columns go
@@ -396,7 +405,8 @@ struct GradFew {
     __device__ __forceinline__ void finish(float*, int, int) {}
 };
 
-// whether logits_few takes a product, and its blocks (and strips of statistics) over N columns: no more than
+// whether logits_few takes a product (h in registers: 32 rows of up to 2048; forward here and on the tiles: 16 x 2048 x
+// 32000 31 and 36 us, 1 x 2048 x 128000 94 and 110), and its blocks (and strips of statistics) over N columns: no more than
 // the tiles' strips of 64, which the workspace has room for
 bool few_takes(const GemmDesc& g) { return g.M <= kFewRows && g.Ks[0] % 256 == 0 && g.Ks[0] <= 2048; }
 int few_blocks(int N) { return std::min((N + 63) / 64, stream_blocks()); }
@@ -445,7 +455,8 @@ int launch_logits_tile(const GemmDesc& g, const EPI& epi, hipStream_t s) {
 }
 
 // 256-row tiles, or 128-row ones where they need less (the streamed products' rule: a round of them
-// takes 0.6 of a round of the large).  Up to 64 rows 64-row tiles, which leave the LDS to six stages.
+// takes 0.6 of a round of the large).  Up to 64 rows 64-row tiles, which leave the LDS to six stages: a
+// read of E again (64 x 1024 x 50000 forward 28.6 us).
 template <typename EPI>
 int launch_logits(const GemmDesc& g, const EPI& epi, hipStream_t s) {
     const long blocks = stream_blocks(), tn = (g.N + 127) / 128;
@@ -462,7 +473,8 @@ __device__ __forceinline__ void finish_row(int t, float m, float s, const int32_
     if (loss) loss[t] = g >= 0 && g < V ? z - lt[t] : 0.f;
 }
 
-// lse and loss from the strips' statistics: R rows x 256 / R slices of the strips a block
+// lse and loss from the strips' statistics: R rows x 256 / R slices of the strips a block.  2 below 256 rows
+// (500 strips of 16 rows: 3.8 us, with 16 5.5), 16 from there on (782 strips of 2001 rows: 9.5 us, with 2 16).
 template <int R>
 __global__ __launch_bounds__(256) void row_stats(const float2* __restrict__ part, int strips, int T,
                                                  const int32_t* __restrict__ tgt, const float* __restrict__ lt,
@@ -865,7 +877,8 @@ struct Plan {
         Tp = bf ? T : round_up(T, 4);
         planes = T > kTwoPieces ? 2 : 3;
         // a piece's G, or the fp32 logits it replaces
-        const int64_t most = kPieceBytes / (lay ? 4 : 1) / (bf ? 2 * planes : 4) / std::max(Tp, 1);
+        int64_t most = kPieceBytes / (lay ? 4 : 1) / (bf ? 2 * planes : 4) / std::max(Tp, 1);
+        if (lay) most = std::min(most, kPieceBytes / ((int64_t)dp * (es + 4)));  // the copies of E's and dE's piece
         // whole rounds of 256 x 128 tiles of dE's product on the compute units, or what there is room for
         const int64_t round = (int64_t)std::max(1, stream_blocks() / ((dp + 127) / 128)) * 256;
         int64_t cols = most >= round ? most / round * round : 2 * most >= round ? round : most / 128 * 128;
@@ -1042,6 +1055,7 @@ extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* t
     clear_error();
     if (const int rc = check(who, h, E, targets, T, d, V, dtype)) return rc;
     GN_REQUIRE((((uintptr_t)loss | (uintptr_t)lse) & 3u) == 0, "%s: loss, lse must be aligned to 4 bytes", who);
+    GN_REQUIRE(!shared(loss, (size_t)T * 4, lse, (size_t)T * 4), "%s: loss and lse may not share memory", who);
     if (T == 0 || (!loss && !lse)) return GN_OK;
     const Plan w(T, d, V, dtype, !al16(h) || !al16(E), false);
     if (const int rc = check_ws(who, w, dtype, ws, ws_bytes)) return rc;

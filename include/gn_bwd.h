@@ -297,7 +297,8 @@ int gn_xent_bwd(const void* logits, const int32_t* targets, void* dLogits, int r
 /* Softmax cross entropy of a linear head without its logits (the reference binds a Linear and
  * cross-entropy-backward.glsl:29-84 over stored logits): with l = h E^T,
  *   lse[t] = log sum_v exp l[t, v],  loss[t] = lse[t] - l[t, targets[t]]
- * h [T x d], E [V x d] in dtype; targets int32 [T]; loss, lse fp32 [T] (each may be NULL).  A target
+ * h [T x d], E [V x d] in dtype; targets int32 [T]; loss, lse fp32 [T] (each may be NULL; they
+ * may not share memory).  A target
  * outside [0, V) (-100, say) marks a row without one: loss 0, and no gradient from dloss.
  * The logits exist a tile or a piece of the vocabulary at a time, in fp32.
  * ws: gn_linear_xent_workspace_bytes(T, d, V, dtype), 16-byte aligned. */
@@ -387,7 +388,7 @@ int gn_qk_norm_rope_fwd(const gn_heads* q, const gn_heads* k, const gn_heads* v,
  * anyway), with g = the rotation's transpose applied to dy:
  *   dx = r (w g - x r^2 mean_j(w_j g_j x_j)),  dw = sum over tokens and heads of g x r,  dv = dyv
  * dwq, dwk: fp32 [D], NULL: not wanted; GN_ACCUMULATE adds onto them (the others are
- * overwritten).  The sums run in a fixed order: the same bits every time.
+ * overwritten; the two may not share memory).  The sums run in a fixed order: the same bits every time.
  * ws: gn_qk_norm_rope_workspace_bytes, 16-byte aligned; not used without dwq and dwk. */
 int gn_qk_norm_rope_bwd(const gn_heads* dyq, const gn_heads* dyk, const gn_heads* dyv,
                         const gn_heads* q, const gn_heads* k, const void* wq, const void* wk,

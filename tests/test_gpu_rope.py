@@ -102,6 +102,15 @@ def test_rope_far_positions(gn, first):
     near(gn.rope_fwd(x, f, positions=pos), turn(x.double(), pos, f, 1.0, "half"), 2.0 ** -19 * 2 * row_max(x.double()))
 
 
+@pytest.mark.parametrize("pos0", [2 ** 31 - 1, -(2 ** 31)])
+def test_rope_far_first_position(gn, pos0):
+    """A first position at the border of 32 bits counts on past it."""
+    x = rand(gen(4), 1, 3, 2, 64, dtype=F32)
+    f = freqs(64)
+    pos = pos0 + torch.arange(3, dtype=torch.int64, device=DEV)[None]
+    near(gn.rope_fwd(x, f, pos0=pos0), turn(x.double(), pos, f, 1.0, "half"), 2.0 ** -19 * 2 * row_max(x.double()))
+
+
 @pytest.mark.parametrize("mode", ["half", "interleaved"])
 def test_rope_views(gn, mode):
     """Heads of fused rows, head-first tensors, unaligned and broadcast views, in-place use; what

@@ -89,7 +89,7 @@ def test_qk_refuses():
     refused(fwd(yq=k), "overlaps")       # another tensor's input
     refused(fwd(yq=heads(128)), "overlaps q")
 
-    def bwd(dyq=yq, dyk=yk, dyv=yv, dq=heads(6 * MB), dk=heads(7 * MB), dv=heads(8 * MB), dwq=w, dwk=w, flags=0,
+    def bwd(dyq=yq, dyk=yk, dyv=yv, dq=heads(6 * MB), dk=heads(7 * MB), dv=heads(8 * MB), dwq=w, dwk=ctypes.c_void_p(BASE + 4 * D), flags=0,
             ws=ctypes.c_void_p(BASE), wsb=1 << 20, kk=k, S=S):
         return lib.gn_qk_norm_rope_bwd(dyq, dyk, dyv, q, kk, w, w, dq, dk, dv, dwq, dwk, r, B, S, D, 1e-6, 4, flags, ws,
                                        wsb, None)
@@ -100,6 +100,8 @@ def test_qk_refuses():
     refused(bwd(kk=None, dyk=None, dk=None), "dwk without k")
     refused(bwd(flags=8), "flags")
     refused(bwd(dwq=ctypes.c_void_p(BASE + 2)), "aligned")
+    refused(bwd(dwk=w), "share")
+    refused(bwd(dwk=ctypes.c_void_p(BASE + 4 * D - 4)), "share")
     refused(bwd(dq=heads(7 * MB)), "overlaps")
     refused(bwd(ws=None, wsb=0), "workspace", -3)
     refused(bwd(wsb=64), "workspace", -3)
@@ -150,6 +152,8 @@ def test_linear_xent_refuses():
     refused(fwd(h=p(1)), "aligned")
     refused(fwd(t=p(2 * MB + 2)), "aligned")
     refused(fwd(loss=p(2)), "aligned")
+    refused(fwd(lse=p(3 * MB)), "share")
+    refused(fwd(lse=p(3 * MB + 4 * T - 4)), "share")
     refused(fwd(ws=None), "workspace", -3)
     refused(fwd(wsb=need - 1), "workspace", -3)
     refused(fwd(ws=p(5 * MB + 8)), "workspace", -3)
