@@ -307,3 +307,43 @@ def test_on_another_stream_and_replayed(gn):
         torch.cuda.synchronize()
         for a, b in zip(both(None), held):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T", [16, 40])
+def test_offsets_past_32_bits(gn, T):
+    """A vocabulary whose E and dE have more than 2^31 elements, some rows' targets behind them."""
+    g = gen(T)
+    d, V = 2048, 1100001
+    h = guarded(g, T, d)
+    E = torch.empty(V, d, device=DEV, dtype=BF)
+    for v in range(0, V, 100000):
+        E[v:v + 100000].normal_(0, 0.02, generator=g)
+    t = torch.randint(0, V, (T,), device=DEV, generator=g).to(torch.int32)
+    t[:4] = torch.tensor([V - 1, 1048576, 1048577, 0], dtype=torch.int32)
+    hd = h.double()
+    l = torch.cat([hd @ E[v:v + 100000].double().t() for v in range(0, V, 100000)], 1)
+    el = d * 2.0 ** -24 * (hd.abs() @ E.float().abs().amax(0).double()[:, None])  # at least sum |h||E| of each logit
+    lse = torch.logsumexp(l, -1)
+    dlse = el[:, 0] + 2.0 ** -20 * (1 + l.abs().amax(-1))
+    rows = torch.arange(T, device=DEV)
+    loss, got = gn.linear_xent_fwd(h, E, t)
+    within(got, lse, dlse)
+    within(loss, lse - l[rows, t.long()], dlse + el[:, 0] + 2.0 ** -23 * lse.abs())
+    dh, dE = gn.linear_xent_bwd(h, E, t, got, scale=0.5)
+    p = 0.5 * torch.exp(l - lse[:, None])
+    dp = p * (el + dlse[:, None] + 2.0 ** -21 * (l.abs() + lse.abs()[:, None] + 1))
+    G = p
+    G[rows, t.long()] -= 0.5
+    dG = dp + 2.0 ** -22 * (G.abs() + 0.5)
+    ref, bound = torch.zeros(T, d, device=DEV, dtype=F64), torch.zeros(T, d, device=DEV, dtype=F64)
+    for v in range(0, V, 100000):
+        at = slice(v, v + 100000)
+        Ed = E[at].double()
+        ref += G[:, at] @ Ed
+        # G in bf16, the fp32 sum of V terms in ranges of a few thousand
+        bound += (dG[:, at] + (2.0 ** -8 + 2.0 ** -11) * G[:, at].abs()) @ Ed.abs()
+    within(dh, ref, bound + 2.0 ** -8 * ref.abs())
+    for at in (slice(0, 300), slice(1048500, 1048700), slice(V - 300, V)):
+        X = G[:, at].t()
+        within(dE[at], X @ hd, (dG[:, at].t() + (2.0 ** -16 + T * 2.0 ** -24) * X.abs()) @ hd.abs() + 1e-30)
+    assert bool(torch.isfinite(dE[::1000]).all())
