@@ -140,12 +140,13 @@ def test_linear_xent(gn, T, d, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T", [33, 4200])
 @pytest.mark.parametrize("offset", [1, 2])
-def test_unaligned(gn, offset, dtype):
+def test_unaligned(gn, offset, T, dtype):
     g = gen(offset)
-    h, E = guarded(g, 33, 64, dtype=dtype, offset=offset), guarded(g, 300, 64, dtype=dtype, offset=offset, std=0.3)
-    t = targets(g, 33, 300)
-    u = torch.ones(33, device=DEV)
+    h, E = guarded(g, T, 64, dtype=dtype, offset=offset), guarded(g, 300, 64, dtype=dtype, offset=offset, std=0.3)
+    t = targets(g, T, 300)
+    u = torch.ones(T, device=DEV)
     r = Ref(h, E, t, u)
     loss, lse = gn.linear_xent_fwd(h, E, t)
     within(lse, r.lse, r.dlse)
@@ -202,6 +203,28 @@ def test_target_elements_of_many_rows(gn, T, d):
     bound = dG.t() @ x.abs() + 8 * 2.0 ** -24 * (G.t().abs() @ x.abs()) + 1e-30
     within(dE, ref, bound)
     within(one, ref + 1, bound + 2 * 2.0 ** -24 * (1 + ref.abs() + bound))
+
+
+def test_two_calls_at_once(gn):
+    """Two streams, a workspace each: the bits of one call after the other."""
+    g = gen(17)
+    sets = []
+    for T, d, V in ((4200, 256, 9001), (3000, 256, 12001)):
+        h, E, t = guarded(g, T, d), guarded(g, V, d, std=0.2), targets(g, T, V)
+        loss, lse = gn.linear_xent_fwd(h, E, t)
+        sets.append((h, E, t, lse, gn.linear_xent_bwd(h, E, t, lse),
+                     gn.workspace(gn.linear_xent_workspace_bytes(T, d, V, gn.BF16), DEV)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(4):
+        for i, (h, E, t, lse, _, ws) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(gn.linear_xent_bwd(h, E, t, lse, ws=ws))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for dh, dE in got[i]:
+            assert torch.equal(dh, sets[i][4][0]) and torch.equal(dE, sets[i][4][1])
 
 
 def test_no_row_has_a_target(gn):
@@ -277,9 +300,9 @@ def test_against_the_framework_s_own_path(gn):
     assert float((dE - dE0).abs().max() / dE0.abs().max()) < 1e-5
 
 
-def test_on_another_stream_and_replayed(gn):
+@pytest.mark.parametrize("T,d,V", [(130, 128, 3001), (12, 512, 7000), (60, 1024, 4001), (4200, 128, 3001), (4200, 33, 700)])
+def test_on_another_stream_and_replayed(gn, T, d, V):
     g = gen(16)
-    T, d, V = 130, 128, 3001
     h, E = guarded(g, T, d).contiguous(), guarded(g, V, d, std=0.2).contiguous()
     t = targets(g, T, V)
     u = torch.rand(T, device=DEV, generator=g)
