@@ -17,8 +17,10 @@
 //
 // Measured (a large copy reaches 5.0 TB/s, an update in place 6.0): rotation of 307 MB in and out
 // 61.8 us (4.97 TB/s), fp32 of 49 MB 10.3 us (4.8); norms, rotation and head split of 403 MB 78.0 us
-// (5.2); their backward, 805 MB, 206 us (3.9: two dependent row sums between a row's loads and
-// its stores, and three waves a SIMD, no more, hold two rows each).  A token a sequence: 3.4 us of kernel,
+// (5.2); their backward, which reads x again, 570 MB 126 us (4.5: two dependent row sums between a row's
+// loads and its stores, and three waves a SIMD, no more, hold two rows each); both 206 us.  Stores past the
+// caches take 17 us off the two and add 10 to them with a reader behind, so they are ordinary ones.  A token
+// a sequence: 3.4 us of kernel,
 // under the call's host time of 8.7.  16-byte pieces against elements: bf16 rotation of 4 x 4096 x 32
 // heads, 128 wide 42.7 and 92.4 us, 64 wide 22.0 and 75.8; fp32 102 and 106, 48 and 84.
 #include <algorithm>
@@ -411,8 +413,8 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(Args a) {
 }
 
 // Backward: the first nq blocks take the queries, the others the keys and values (a block's dw is one
-// weight's: half the registers of both), each walking over its tiles.  Three waves a SIMD: the same 805 MB
-// took 208 us, with the registers of four 212, of five (spilling) 416.
+// weight's: half the registers of both), each walking over its tiles.  Three waves a SIMD: forward and
+// backward of the 570 MB took 208 us, with the registers of four 212, of five (spilling) 416.
 template <typename T, int LPR, bool VEC, bool HALF>
 __global__ __launch_bounds__(kThreads, 3) void norm_bwd_kernel(Args a) {
     using R = Row<T, LPR, VEC, HALF>;
@@ -481,7 +483,7 @@ __global__ __launch_bounds__(1024) void dw_finish(const float* __restrict__ part
 // ---- host -------------------------------------------------------------------------------
 constexpr int kMaxD = 512, kMaxH = 1024;
 constexpr int kBwdBlocks = 1536;  // partial dw rows at most: two rounds of three blocks a compute unit
-                                // (768, 1024, 2048 blocks: 209, 211, 208 us for 205)
+                                // (768, 1024, 2048: 209, 211, 208 us for 205)
 
 int lanes_for(int D) {  // of a row in 16-byte pieces
     int l = 2;
