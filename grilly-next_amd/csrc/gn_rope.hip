@@ -332,7 +332,8 @@ __device__ __forceinline__ void group_bwd(const Args& a, const Group& g, int n, 
         }
         s2 = R::sum(s2);
         sx = R::sum(sx);
-        const float r = rsqrtf(s2 * inv_d + a.eps), q = r * r * sx * inv_d;
+        // lanes past the tile's rows hold zeros, and with eps 0 their r would be inf: nothing into dw
+        const float r = r0 < rows ? rsqrtf(s2 * inv_d + a.eps) : 0.f, q = r * r * sx * inv_d;
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             du[i] += yu[i] * u[i] * r;

@@ -1,0 +1,43 @@
+"""GPU tests of the borders of rope, qk_norm_rope and linear_xent: a zero eps, infinities beside
+elements that pass through, confident rows, launches past a dimension's limit, chained nodes.
+
+Tolerances are those of test_gpu_rope.py and test_gpu_linear_xent.py where nothing else is said."""
+import pytest
+
+from test_gpu_rope import freqs, gen, grads, near, rand, row_max, turn
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+BF, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def gn(gpu):
+    import gn_bwd
+    gn_bwd.lib()
+    return gn_bwd
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("mode", ["half", "interleaved"])
+@pytest.mark.parametrize("B,S,Hq,Hk,D,rot", [(1, 1, 8, 2, 128, 128), (3, 7, 5, 1, 64, 32), (2, 9, 3, 1, 80, 26),
+                                             (1, 1, 1, 1, 34, 0), (1, 2100, 3, 3, 96, 48)])
+def test_norms_without_eps(gn, B, S, Hq, Hk, D, rot, mode, dtype):
+    """eps = 0 over rows that are not zero, in tiles whose rows do not fill the block."""
+    g = gen(B + S + D)
+    q, k = rand(g, B, S, Hq, D, dtype=dtype), rand(g, B, S, Hk, D, dtype=dtype)
+    dyq, dyk = rand(g, B, S, Hq, D, dtype=dtype), rand(g, B, S, Hk, D, dtype=dtype)
+    wq, wk = rand(g, D, dtype=dtype), rand(g, D, dtype=dtype)
+    f = freqs(rot) if rot else None
+    pos = torch.arange(S, device=DEV)[None].expand(B, S)
+    y = gn.qk_norm_rope_fwd(q, k, wq, wk, f, mode=mode, eps=0.0)
+    dq, dk, _, dwq, dwk = gn.qk_norm_rope_bwd(dyq, dyk, q, k, wq, wk, f, mode=mode, eps=0.0)
+    chain = (B * S * max(Hq, Hk) // 4 + 400) * 2.0 ** -24
+    for x, w, dy, got, dx, dw in ((q, wq, dyq, y[0], dq, dwq), (k, wk, dyk, y[1], dk, dwk)):
+        n = x.double() * x.double().square().mean(-1, keepdim=True).rsqrt() * w.double()
+        near(got, n if f is None else turn(n, pos, f, 1.0, mode), 2.0 ** -16 * 2 * row_max(n))
+        ref, rw, size, sw = grads(x, w, dy, pos, f, 1.0, mode, eps=0.0)
+        near(dx, ref, 2.0 ** -16 * size)
+        assert bool(((dw.double() - rw).abs() <= (2.0 ** -16 + chain) * sw).all())
