@@ -101,6 +101,8 @@ struct Row {
         return HALF ? p + (rot >> 1) : 2 * p + 1;
     }
     __device__ __forceinline__ bool has(int i) const { return VEC ? on : 2 * (l + 64 * i) < D; }
+    // whether pair i is rotated; the others are taken as they are (0 times an infinite partner is NaN)
+    __device__ __forceinline__ bool turns(int i) const { return VEC ? turn : 2 * (l + 64 * i) < rot; }
 
     // a lane's elements as they lie in memory
     struct Raw {
@@ -279,8 +281,8 @@ __device__ __forceinline__ void group(const Args& a, const Group& g, int n, cons
             }
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
-                yu[i] = u[k][i] * c[i] - w[k][i] * s[i];
-                yw[i] = w[k][i] * c[i] + u[k][i] * s[i];
+                yu[i] = row.turns(i) ? u[k][i] * c[i] - w[k][i] * s[i] : u[k][i];
+                yw[i] = row.turns(i) ? w[k][i] * c[i] + u[k][i] * s[i] : w[k][i];
             }
             row.st((T*)g.y + at(g.ys, bs[tt[k]], h[k]), live[k], yu, yw);
         }
@@ -318,8 +320,8 @@ __device__ __forceinline__ void group_bwd(const Args& a, const Group& g, int n, 
             row.angles(cosv, sinv, t0, c, s);
 #pragma unroll
             for (int i = 0; i < NP; ++i) {  // dy turned back (sin carries the sign)
-                yu[i] = gu[i] * c[i] - gw[i] * s[i];
-                yw[i] = gw[i] * c[i] + gu[i] * s[i];
+                yu[i] = row.turns(i) ? gu[i] * c[i] - gw[i] * s[i] : gu[i];
+                yw[i] = row.turns(i) ? gw[i] * c[i] + gu[i] * s[i] : gw[i];
             }
         }
         float wu[NP], ww[NP], s2 = 0.f, sx = 0.f;

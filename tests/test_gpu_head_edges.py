@@ -41,3 +41,25 @@ def test_norms_without_eps(gn, B, S, Hq, Hk, D, rot, mode, dtype):
         ref, rw, size, sw = grads(x, w, dy, pos, f, 1.0, mode, eps=0.0)
         near(dx, ref, 2.0 ** -16 * size)
         assert bool(((dw.double() - rw).abs() <= (2.0 ** -16 + chain) * sw).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("mode", ["half", "interleaved"])
+@pytest.mark.parametrize("D,rot", [(64, 32), (80, 26), (128, 0), (34, 2)])
+def test_elements_behind_the_rotation_pass_as_they_are(gn, D, rot, mode, dtype):
+    """Bit for bit, beside infinities, NaN and negative zeros too."""
+    g = gen(D)
+    x = rand(g, 2, 9, 3, D, dtype=dtype)
+    x[0, :, :, rot::5] = float("inf")
+    x[1, 2, :, rot + 1::7] = float("nan")
+    x[1, 3, :, rot::2] = -0.0
+    bits = torch.int16 if dtype is BF else torch.int32
+    f = freqs(rot)
+    for fn in (gn.rope_fwd, gn.rope_bwd):
+        y = fn(x, f, mode=mode, pos0=3)
+        assert torch.equal(y[..., rot:].contiguous().view(bits), x[..., rot:].contiguous().view(bits))
+        assert bool(torch.isfinite(y[..., :rot]).all())
+    # the norm of a row with an infinity: r = 0, so its finite elements become 0, and no neighbour NaN
+    y, _ = gn.qk_norm_rope_fwd(x[:1], None, freqs=f, mode=mode)
+    fine = torch.isfinite(x[:1])
+    assert bool((y[fine] == 0).all()) and bool(torch.isnan(y[~fine]).all())
