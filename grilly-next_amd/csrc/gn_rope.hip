@@ -408,7 +408,9 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(Args a) {
     float* const sinv = cosv + a.TB[0] * (a.rot >> 1);
     int2* const bs = reinterpret_cast<int2*>(sinv + a.TB[0] * (a.rot >> 1));
     const Row<T, LPR, VEC, HALF> row(a.D, a.rot);
-    const int t0 = blockIdx.x * a.TB[0], n = min(a.TB[0], a.tokens - t0);
+    const unsigned tile = blockIdx.y * gridDim.x + blockIdx.x;
+    if (tile >= (unsigned)a.tiles[0]) return;
+    const int t0 = (int)tile * a.TB[0], n = min(a.TB[0], a.tokens - t0);
     tile_angles(a, t0, n, cosv, sinv, bs);
     group<T, LPR, VEC, HALF, KIND>(a, a.g[0], n, cosv, sinv, bs, row);
     if (KIND != kRotate && a.ng > 1) group<T, LPR, VEC, HALF, KIND>(a, a.g[1], n, cosv, sinv, bs, row);
@@ -495,13 +497,17 @@ int lanes_for(int D) {  // of a row in 16-byte pieces
 }
 
 constexpr int kBwd = 2;  // launch_kind: the backward
+// Tiles along x: a launch's threads in one dimension are counted in 32 bits, which one token a tile and 256
+// threads would pass at 2^24 tokens.
+constexpr int kTilesX = 1 << 22;
 
 template <typename T, int LPR, bool VEC, bool HALF, int KIND>
 int launch(const Args& a, int grid, size_t smem, hipStream_t s) {
     if constexpr (KIND == kBwd)
         hipLaunchKernelGGL((norm_bwd_kernel<T, LPR, VEC, HALF>), dim3(grid), dim3(kThreads), smem, s, a);
     else
-        hipLaunchKernelGGL((rope_kernel<T, LPR, VEC, HALF, KIND>), dim3(grid), dim3(kThreads), smem, s, a);
+        hipLaunchKernelGGL((rope_kernel<T, LPR, VEC, HALF, KIND>),
+                           dim3(std::min(grid, kTilesX), (grid - 1) / kTilesX + 1), dim3(kThreads), smem, s, a);
     GN_LAUNCH_CHECK("rope / qk norm");
     return GN_OK;
 }

@@ -63,3 +63,27 @@ def test_elements_behind_the_rotation_pass_as_they_are(gn, D, rot, mode, dtype):
     y, _ = gn.qk_norm_rope_fwd(x[:1], None, freqs=f, mode=mode)
     fine = torch.isfinite(x[:1])
     assert bool((y[fine] == 0).all()) and bool(torch.isnan(y[~fine]).all())
+
+
+@pytest.mark.parametrize("tokens", [2 ** 24 + 5, 2 ** 22 + 1])
+def test_more_tiles_than_a_dimension_launches(gn, tokens):
+    """One token a tile, more than 2^32 threads: every token is reached (rotation, and the norm)."""
+    g = gen(1)
+    H, D = 17, 2  # 34 elements a token: element by element, a tile is one token
+    x = torch.randn(1, tokens, H, D, device=DEV, dtype=BF, generator=g)
+    f = freqs(D)
+    y = torch.full_like(x, float("nan"))
+    gn.rope_fwd(x, f, out=y)
+    back = gn.rope_bwd(y, f)
+    # two roundings to bf16 of a pair's elements
+    size = (2.0 ** -7 + 2.0 ** -18) * row_max(x.float())
+    assert bool(((back.float() - x.float()).abs() <= size).all())
+    at = [0, 1, tokens // 2, tokens - 6, tokens - 5, tokens - 1]
+    near(y[:, at], turn(x[:, at].double(), torch.tensor([at], device=DEV), f, 1.0, "half"),
+         2.0 ** -20 * 2 * row_max(x[:, at].double()))
+    y.fill_(float("nan"))
+    gn.qk_norm_rope_fwd(x, None, freqs=f, out=(y, None))
+    norm = y.float().square().mean(-1)
+    # each element of a pair off by 2^-8 of it, the norm by 2^-7; eps 1e-6 against mean(x^2)
+    fine = x.float().square().mean(-1) > 2e-4
+    assert bool(((norm - 1).abs() <= 2.0 ** -7 + 2.0 ** -7)[fine].all()) and bool(torch.isfinite(norm).all())
