@@ -530,14 +530,21 @@ __global__ __launch_bounds__(256) void row_scales(RowScale* __restrict__ rows, f
 }
 
 // ---- fp32: row kernels over a piece's stored logits -------------------------------------------
+// A launch's threads in one dimension are counted in 32 bits, which a row a block of 256 would pass at
+// 2^24 rows: blocks go on in another dimension from 2^22 on.
+constexpr int kRowsX = 1 << 22;
+inline dim3 blocks_of(int n, int y = 1) { return dim3(std::min(n, kRowsX), y, (n - 1) / kRowsX + 1); }
+__device__ __forceinline__ int block_of() { return blockIdx.z * gridDim.x + blockIdx.x; }
+
 // A row's statistics over one piece, joined with those of the pieces before (st); the last
 // piece's are turned into lse and loss.  ld and L are multiples of 4 elements and 16 bytes.
-__global__ __launch_bounds__(256) void piece_stats(const float* __restrict__ L, int ld, int v0, int nv,
+__global__ __launch_bounds__(256) void piece_stats(const float* __restrict__ L, int ld, int T, int v0, int nv,
                                                    const int32_t* __restrict__ tgt, float2* __restrict__ st,
                                                    float* __restrict__ lt, float* __restrict__ loss,
                                                    float* __restrict__ lse, int V, int first, int last) {
     __shared__ float sm[4], ss[4];
-    const int t = blockIdx.x;
+    const int t = block_of();
+    if (t >= T) return;
     const float* row = L + (size_t)t * ld;
     float m = -INFINITY, s = 0.f;
     for (int v = 4 * threadIdx.x; v < nv; v += 4096) {
@@ -581,10 +588,12 @@ __global__ __launch_bounds__(256) void piece_stats(const float* __restrict__ L, 
 }
 
 // G of one piece in its logits' place, zeros from nv up to the next multiple of 4
-__global__ __launch_bounds__(256) void piece_grad(float* __restrict__ L, int ld, int v0, int nv,
+__global__ __launch_bounds__(256) void piece_grad(float* __restrict__ L, int ld, int Tp, int v0, int nv,
                                                   const RowScale* __restrict__ rows) {
-    const RowScale r = rows[blockIdx.x];
-    float* const row = L + (size_t)blockIdx.x * ld;
+    const int t = block_of();
+    if (t >= Tp) return;
+    const RowScale r = rows[t];
+    float* const row = L + (size_t)t * ld;
     const int g = __float_as_int(r.w) - v0;
     for (int v = 4 * (blockIdx.y * 256 + threadIdx.x); v < nv; v += 1024 * gridDim.y) {
         float4* p = reinterpret_cast<float4*>(row + v);
@@ -604,8 +613,8 @@ __global__ __launch_bounds__(256) void piece_grad(float* __restrict__ L, int ld,
 // zeros in the padding's rows
 __global__ __launch_bounds__(256) void tail_logits(const float* __restrict__ h, const float* __restrict__ E,
                                                    float* __restrict__ L, int ld, int T, int Tp, int d, int tail) {
-    const int w = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int t = w / tail, j = w - t * tail;
+    const int64_t w = block_of() * (int64_t)4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, t = (int)(w / tail), j = (int)(w - (int64_t)t * tail);
     if (t >= Tp) return;
     float s = 0.f;
     for (int k = lane; t < T && k < d; k += 64) s = fmaf(h[(size_t)t * d + k], E[(size_t)j * d + k], s);
@@ -960,6 +969,8 @@ int check(const char* who, const void* h, const void* E, const int32_t* tgt, int
     GN_REQUIRE(dtype == GN_F32 || dtype == GN_BF16, "%s: dtype %d not supported (f32, bf16)", who, dtype);
     GN_REQUIRE(T >= 0 && d >= 1 && V >= 1, "%s: bad shape", who);
     GN_REQUIRE(T < (1 << 28) && d <= (1 << 20) && V < (1 << 30), "%s: T below 2^28, d up to 2^20, V below 2^30", who);
+    // the products count their tiles, and a block its k-tiles, in 31 bits
+    GN_REQUIRE((int64_t)T * V < (1ll << 43) && (double)T * V * d < 0x1p58, "%s: T * V below 2^43, T * V * d below 2^58", who);
     GN_REQUIRE(T == 0 || (h && E && tgt), "%s: null pointer", who);
     const int es = dtype == GN_F32 ? 4 : 2;
     GN_REQUIRE((((uintptr_t)h | (uintptr_t)E) & (es - 1)) == 0 && ((uintptr_t)tgt & 3u) == 0,
@@ -1032,7 +1043,7 @@ struct Call {
             if (const int rc = gemm_run(g, 0, 1, dtype, GN_F32, s)) return rc;
         }
         if (cols >= nv) return GN_OK;
-        tail_logits<<<(w.Tp * (nv - nq) + 3) / 4, 256, 0, s>>>((const float*)h, (const float*)Ec + (size_t)nq * w.d, L + nq,
+        tail_logits<<<blocks_of((w.Tp * (nv - nq) + 3) / 4), 256, 0, s>>>((const float*)h, (const float*)Ec + (size_t)nq * w.d, L + nq,
                                                              w.vc, w.T, w.Tp, w.d, nv - nq);
         GN_LAUNCH_CHECK(who);
         return GN_OK;
@@ -1078,8 +1089,8 @@ extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* t
             strips += few_takes(g) ? few_blocks(nv) : (nv + 63) / 64;
         } else {
             if (const int rc = c.logits32(Ec, nv)) return rc;
-            piece_stats<<<T, 256, 0, c.s>>>((const float*)(base + w.logits), w.vc, v0, nv, targets,
-                                            (float2*)(base + w.stats), lt, loss, lse, V, v0 == 0, v0 + nv == V);
+            piece_stats<<<blocks_of(T), 256, 0, c.s>>>((const float*)(base + w.logits), w.vc, T, v0, nv, targets,
+                                                       (float2*)(base + w.stats), lt, loss, lse, V, v0 == 0, v0 + nv == V);
             GN_LAUNCH_CHECK(who);
         }
     }
@@ -1186,7 +1197,7 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
             if (rc) return rc;
         } else {
             if (const int rc = c.logits32(Ec, nv)) return rc;
-            piece_grad<<<dim3(w.Tp, std::min(16, (nv + 4095) / 4096)), 256, 0, s>>>((float*)G, w.vc, v0, nv, rows);
+            piece_grad<<<blocks_of(w.Tp, std::min(16, (nv + 4095) / 4096)), 256, 0, s>>>((float*)G, w.vc, w.Tp, v0, nv, rows);
             GN_LAUNCH_CHECK(who);
         }
         if (dE && w.lay) {

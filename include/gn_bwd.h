@@ -300,7 +300,8 @@ int gn_xent_bwd(const void* logits, const int32_t* targets, void* dLogits, int r
  * h [T x d], E [V x d] in dtype; targets int32 [T]; loss, lse fp32 [T] (each may be NULL; they
  * may not share memory).  A target
  * outside [0, V) (-100, say) marks a row without one: loss 0, and no gradient from dloss.
- * The logits exist a tile or a piece of the vocabulary at a time, in fp32.
+ * The logits exist a tile or a piece of the vocabulary at a time, in fp32.  T below 2^28, d up to
+ * 2^20, V below 2^30, T * V below 2^43, T * V * d below 2^58.
  * ws: gn_linear_xent_workspace_bytes(T, d, V, dtype), 16-byte aligned. */
 int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* targets, float* loss, float* lse,
                        int T, int d, int V, int dtype, void* ws, size_t ws_bytes, void* stream);

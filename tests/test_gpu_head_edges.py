@@ -87,3 +87,72 @@ def test_more_tiles_than_a_dimension_launches(gn, tokens):
     # each element of a pair off by 2^-8 of it, the norm by 2^-7; eps 1e-6 against mean(x^2)
     fine = x.float().square().mean(-1) > 2e-4
     assert bool(((norm - 1).abs() <= 2.0 ** -7 + 2.0 ** -7)[fine].all()) and bool(torch.isfinite(norm).all())
+
+
+def some_rows(gn, h, E, t, at):
+    """Gradients of a loss over the rows `at` (none twice) alone, the same in fp64 from those rows, and lse."""
+    T = h.shape[0]
+    assert len(at) == len(at.unique())
+    u = torch.zeros(T, device=DEV)
+    u[at] = torch.rand(len(at), device=DEV, generator=gen(3)) + 0.5
+    loss, lse = gn.linear_xent_fwd(h, E, t)
+    dh, dE = gn.linear_xent_bwd(h, E, t, lse, dloss=u)
+    x, Ed = h[at].double(), E.double()
+    l = x @ Ed.t()
+    p = torch.softmax(l, -1)
+    G = p.clone()
+    G[torch.arange(len(at)), t[at].long()] -= 1
+    G *= u[at].double()[:, None]
+    size = torch.logsumexp(l, -1), (x.abs() @ Ed.abs().t()).amax(-1)
+    # p: the logits' error and 2^-20 (1 + |l| + |lse|); 2^-24 of each of d terms
+    d = h.shape[1]
+    dp = p * (2 * (d * 2.0 ** -24 + 2.0 ** -22) * size[1] + 2.0 ** -20 * (2 + 2 * l.abs().amax(-1) + size[0].abs()))[:, None]
+    dG = u[at].double()[:, None] * (dp + 2.0 ** -22)
+    return loss, lse, dh, dE, l, G, dG, x, Ed
+
+
+def test_rows_past_a_dimension_of_blocks(gn):
+    """fp32, more than 2^24 rows (a row a block): the last ones' loss and gradients, and a tail of the
+    vocabulary."""
+    g = gen(2)
+    T, d, V = 2 ** 24 + 9, 4, 5
+    h = torch.randn(T, d, device=DEV, generator=g)
+    E = torch.randn(V, d, device=DEV, generator=g)
+    t = torch.randint(0, V, (T,), device=DEV, generator=g).to(torch.int32)
+    at = torch.tensor([0, 5, 2 ** 22, 2 ** 24 - 1, T - 9, T - 1], device=DEV)
+    loss, lse, dh, dE, l, G, dG, x, Ed = some_rows(gn, h, E, t, at)
+    logits = h.double() @ Ed.t()
+    ref = torch.logsumexp(logits, -1)
+    # 4 terms a logit, and exp, sum and log
+    assert bool(((lse.double() - ref).abs() <= 2.0 ** -20 * (2 + logits.abs().amax(-1))).all())
+    ref = ref - logits.gather(1, t.long()[:, None])[:, 0]
+    assert bool(((loss.double() - ref).abs() <= 2.0 ** -19 * (2 + logits.abs().amax(-1))).all())
+    bound = dG @ Ed.abs() + 2.0 ** -21 * (G.abs() @ Ed.abs())
+    assert bool(((dh[at].double() - G @ Ed).abs() <= bound).all())
+    rest = torch.ones(T, dtype=torch.bool, device=DEV)
+    rest[at] = False
+    assert bool((dh[rest] == 0).all())
+    assert bool(((dE.double() - G.t() @ x).abs() <= dG.t() @ x.abs() + 2.0 ** -20 * (G.t().abs() @ x.abs())).all())
+
+
+def test_h_past_32_bits(gn):
+    """bf16, an h and a dh of more than 2^31 elements."""
+    g = gen(5)
+    T, d, V = 2 ** 21 + 37, 1032, 300
+    h = torch.empty(T, d, device=DEV, dtype=BF)
+    for i in range(0, T, 2 ** 18):
+        h[i:i + 2 ** 18].normal_(0, 1, generator=g)
+    E = rand(g, V, d, std=0.05)
+    t = torch.randint(0, V, (T,), device=DEV, generator=g).to(torch.int32)
+    at = torch.tensor([0, 1, 2 ** 20, T - 300, T - 2, T - 1], device=DEV)
+    loss, lse, dh, dE, l, G, dG, x, Ed = some_rows(gn, h, E, t, at)
+    ref = torch.logsumexp(l, -1)
+    el = d * 2.0 ** -24 * (x.abs() @ Ed.abs().t()).amax(-1) + 2.0 ** -20 * (1 + l.abs().amax(-1))
+    assert bool(((lse[at].double() - ref).abs() <= el).all())
+    ref = ref - l.gather(1, t[at].long()[:, None])[:, 0]
+    assert bool(((loss[at].double() - ref).abs() <= 2 * el).all())
+    ref = G @ Ed  # G in bf16 but at the target, dh's own rounding, and a sum of 300 terms
+    assert bool(((dh[at].double() - ref).abs() <= (dG + (2.0 ** -8 + 2.0 ** -15) * G.abs()) @ Ed.abs() + 2.0 ** -8 * ref.abs()).all())
+    ref = G.t() @ x  # two pieces of G
+    assert bool(((dE.double() - ref).abs() <= (dG.t() + 2.0 ** -16 * G.t().abs()) @ x.abs()).all())
+    assert bool((dh[2:2 ** 20] == 0).all()) and bool((dh[2 ** 20 + 1:T - 300] == 0).all())
