@@ -39,11 +39,11 @@ namespace gn {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
-constexpr float kLog2eRest = (float)(1.4426950408889634 - (double)kLog2e);
 
-// exp(x - m) as exp2(x log2e - b) takes b = m log2e, whose rounding (2^-20 at 17) would go into every term
-// of a row alike: what it was off by
-__device__ __forceinline__ float off(float m, float b) { return fmaf(m, kLog2e, -b) + m * kLog2eRest; }
+// exp(x - m) as exp2(x kLog2e - b) takes b = m kLog2e, whose rounding (2^-20 at 17) would go into every term
+// of a row alike: what it was off by, without log2e's own rounding, which x kLog2e has too (it cancels
+// where x is near m: x = m gives exactly 1)
+__device__ __forceinline__ float off(float m, float b) { return fmaf(m, kLog2e, -b); }
 
 // A part of a row: its maximum m and the sum s of exp about it, (-inf, 0) when it is empty.  A NaN among
 // the logits is in s only (m skips it) and stays there.

@@ -156,3 +156,31 @@ def test_h_past_32_bits(gn):
     ref = G.t() @ x  # two pieces of G
     assert bool(((dE.double() - ref).abs() <= (dG.t() + 2.0 ** -16 * G.t().abs()) @ x.abs()).all())
     assert bool((dh[2:2 ** 20] == 0).all()) and bool((dh[2 ** 20 + 1:T - 300] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,d", [(3, 64), (20, 256), (70, 64), (300, 40), (4100, 64)])
+@pytest.mark.parametrize("V", [1, 40])
+def test_a_certain_row_has_no_gradient(gn, T, d, V, dtype):
+    """The target's logit is 300 (exact in either type and in lse) and nothing beside it: p = 1, no loss
+    and no gradient.  exp2's argument is off by half a step of 300 log2e at most before it is put right, its
+    value by 2^-22."""
+    h, E = torch.zeros(T, d, device=DEV, dtype=dtype), torch.zeros(V, d, device=DEV, dtype=dtype)
+    h[:, 0], E[0, 0] = 256, 1.171875
+    t = torch.zeros(T, device=DEV, dtype=torch.int32)
+    loss, lse = gn.linear_xent_fwd(h, E, t)
+    assert bool((lse == 300).all()) and bool((loss.abs() <= 2.0 ** -22).all())
+    dh, dE = gn.linear_xent_bwd(h, E, t, lse)
+    # G <= 2^-22 at the target, times E and h (and summed over the rows)
+    assert bool((dh.float().abs() <= 2.0 ** -22 * 1.171875).all())
+    assert bool((dE.abs() <= 2.0 ** -22 * 256 * T).all())
+    # a row twice as certain of two equal columns: p = 1/2 each
+    if V > 1:
+        E[V - 1] = E[0]
+        l = torch.full((T,), 300.0, device=DEV, dtype=F64)
+        loss, lse = gn.linear_xent_fwd(h, E, t)
+        ref = l + torch.log(torch.tensor(2.0, dtype=F64))
+        assert bool(((lse.double() - ref).abs() <= 2.0 ** -16).all())  # half a step of 300
+        dh, dE = gn.linear_xent_bwd(h, E, t, torch.full_like(lse, 300.0))  # lse as it was: p = 1 each
+        assert bool((dE[0].abs() <= 2.0 ** -22 * 256 * T).all())
+        assert bool(((dE[V - 1] - h.float().sum(0)).abs() <= 2.0 ** -22 * 256 * T).all())
