@@ -465,12 +465,14 @@ int launch_logits(const GemmDesc& g, const EPI& epi, hipStream_t s) {
     return 0.62 * (double)r128 < (double)r256 ? launch_logits_tile<128, 3>(g, epi, s) : launch_logits_tile<256, 3>(g, epi, s);
 }
 
+// The loss is (m - target's logit) + ln s, not lse less the logit: of far logits lse has lost a confident row's
+// loss to its rounding (2^-16 at 300).
 __device__ __forceinline__ void finish_row(int t, float m, float s, const int32_t* tgt, const float* lt, float* loss,
                                            float* lse, int V) {
-    const float z = m + __builtin_amdgcn_logf(s) * kLn2;
-    if (lse) lse[t] = z;
+    const float ln = __builtin_amdgcn_logf(s) * kLn2;
+    if (lse) lse[t] = m + ln;
     const int g = tgt[t];
-    if (loss) loss[t] = g >= 0 && g < V ? z - lt[t] : 0.f;
+    if (loss) loss[t] = g >= 0 && g < V ? (m - lt[t]) + ln : 0.f;
 }
 
 // lse and loss from the strips' statistics: R rows x 256 / R slices of the strips a block.  2 below 256 rows

@@ -184,3 +184,22 @@ def test_a_certain_row_has_no_gradient(gn, T, d, V, dtype):
         dh, dE = gn.linear_xent_bwd(h, E, t, torch.full_like(lse, 300.0))  # lse as it was: p = 1 each
         assert bool((dE[0].abs() <= 2.0 ** -22 * 256 * T).all())
         assert bool(((dE[V - 1] - h.float().sum(0)).abs() <= 2.0 ** -22 * 256 * T).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("T,d,V", [(7, 64, 900), (16, 256, 3000), (70, 64, 900), (300, 64, 901), (1003, 72, 2000)])
+def test_small_losses_of_far_logits(gn, T, d, V, dtype):
+    """Logits of some hundreds, whole numbers and so exact, the target the largest or the next: the loss
+    keeps what lse has to round away.  s is good to 2^-19 (V terms of 2^-22 joined a few dozen times), ln s
+    to that and 2^-22, and the sum is rounded once."""
+    g = gen(T + V)
+    h = torch.randint(-8, 9, (T, d), device=DEV, generator=g).to(dtype)
+    E = torch.randint(-4, 5, (V, d), device=DEV, generator=g).to(dtype)
+    l = h.double() @ E.double().t()
+    best = l.topk(2, -1)
+    t = best.indices.gather(1, (torch.arange(T, device=DEV) % 3 == 0).long()[:, None])[:, 0].to(torch.int32)
+    loss, lse = gn.linear_xent_fwd(h, E, t)
+    top = best.values[:, :1]
+    ref = torch.logsumexp(l - top, -1) + top[:, 0] - l.gather(1, t.long()[:, None])[:, 0]
+    assert float(lse.max()) > 200
+    assert bool(((loss.double() - ref).abs() <= 2.0 ** -19 + 2.0 ** -22 + 2.0 ** -24 * ref).all())
