@@ -2,6 +2,7 @@
 #include "autograd.h"
 
 #include <cmath>
+#include <cstddef>
 #include <string>
 
 #include "gn_bwd.h"
@@ -625,6 +626,15 @@ void BackwardEngine::bwd_cross_entropy(Node* n) {
 
 namespace {
 
+// A Rope or QkNormRope node's parameters.  The forward takes an eps or mscale of 0 at its word, so zeros
+// are no defaults here.
+RopeNodeParams rope_params(const Node* n) {
+    RopeNodeParams p = params_of<RopeNodeParams>(n);
+    if (n->params_size < offsetof(RopeNodeParams, mscale) + sizeof(float)) p.mscale = 1.f;
+    if (n->params_size < offsetof(RopeNodeParams, eps) + sizeof(float)) p.eps = 1e-6f;
+    return p;
+}
+
 // The rotation of a Rope or QkNormRope node over S positions a sequence.
 gn_rope node_rope(const RopeNodeParams& p, uint64_t freqs, uint64_t positions, int S, const char* what) {
     gn_rope r{};
@@ -634,7 +644,7 @@ gn_rope node_rope(const RopeNodeParams& p, uint64_t freqs, uint64_t positions, i
     r.positions = (const int32_t*)P(positions);
     r.pos_sb = p.positions_per_row ? S : 0;
     r.pos0 = p.pos0;
-    r.mscale = p.mscale != 0.f ? p.mscale : 1.f;
+    r.mscale = p.mscale;
     r.rot = (int)p.rot;
     r.mode = (int)p.mode;
     return r;
@@ -651,7 +661,7 @@ gn_heads row_heads(void* rows, size_t es, int S, int64_t C, int first, int H, in
 void BackwardEngine::bwd_rope(Node* n) {
     const TensorRef& x = n->inputs[0];
     if (!x.requires_grad) return;
-    const RopeNodeParams p = params_of<RopeNodeParams>(n);
+    const RopeNodeParams p = rope_params(n);
     if (x.ndim != 3 || p.heads == 0 || x.shape[2] % p.heads || n->outputs[0].numel() != x.numel())
         throw std::invalid_argument("Rope: input and output [B,S,heads*D], heads > 0");
     const int B = (int)x.shape[0], S = (int)x.shape[1], H = (int)p.heads, D = (int)x.shape[2] / H;
@@ -669,7 +679,7 @@ void BackwardEngine::bwd_rope(Node* n) {
 // before the norm.
 void BackwardEngine::bwd_qk_norm_rope(Node* n) {
     const TensorRef& x = n->inputs[0];
-    const RopeNodeParams p = params_of<RopeNodeParams>(n);
+    const RopeNodeParams p = rope_params(n);
     const int H = (int)p.heads, K = (int)p.kv_heads;
     if (x.ndim != 3 || H <= 0 || K <= 0 || x.shape[2] % (p.heads + 2 * p.kv_heads) ||
         n->outputs[0].numel() != x.numel())
@@ -693,7 +703,7 @@ void BackwardEngine::bwd_qk_norm_rope(Node* n) {
                    k = row_heads(xp, es, S, C, H, K, D), dq = row_heads(dp, es, S, C, 0, H, D),
                    dk = row_heads(dp, es, S, C, H, K, D), dv = row_heads(dp, es, S, C, H + K, K, D);
     gn_call(gn_qk_norm_rope_bwd(&gq, &gk, &gv, &q, &k, P(wq), P(wk), &dq, &dk, &dv, (float*)P(dwq), (float*)P(dwk),
-                                &r, B, S, D, p.eps != 0.f ? p.eps : 1e-6f, dt, 0, P(ws), wsb, dev_.stream()),
+                                &r, B, S, D, p.eps, dt, 0, P(ws), wsb, dev_.stream()),
             "query/key norm backward");
     stats_.shaders_dispatched += dwq || dwk ? 2 : 1;
     n->grad_input_buffers[0] = dx;

@@ -118,7 +118,7 @@ struct FusedGLUParams { uint32_t kind; };                       // GN_GLU_* kind
 // {freqs, positions or 0}, QkNormRope {wq, wk, freqs, positions or 0} (wq, wk: 0 = weights of 1).
 struct RopeNodeParams {
     uint32_t heads, kv_heads, rot, mode;
-    float mscale, eps;           // 0 -> 1, 1e-6
+    float mscale, eps;           // taken as they are, zeros too; 1 and 1e-6 in a block that ends before them
     uint32_t positions_per_row;  // positions [B,S] (1) or [S] (0)
     int32_t pos0;                // the first position, without positions
 };

@@ -203,3 +203,68 @@ def test_small_losses_of_far_logits(gn, T, d, V, dtype):
     ref = torch.logsumexp(l - top, -1) + top[:, 0] - l.gather(1, t.long()[:, None])[:, 0]
     assert float(lse.max()) > 200
     assert bool(((loss.double() - ref).abs() <= 2.0 ** -19 + 2.0 ** -22 + 2.0 ** -24 * ref).all())
+
+
+# ---- nodes of the tape ------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def tape_env(gn):
+    import grilly_bridge as gb
+    import grilly_core
+    dev = grilly_core.Device(0)
+    gb.attach_torch_stream(dev)
+    return grilly_core, gb, dev
+
+
+def node_grads(tape_env, op, ins, outs, params, saved, up, wanted):
+    """The gradients (as fp32 host tensors) of `wanted` [(tensor, dtype code or None)] after one node."""
+    gc, gb, dev = tape_env
+    tape = gb.create_tape_context(dev)
+    tape.begin()
+    n = tape.record_op(getattr(gc.OpType, op), ins, outs, params)
+    tape.save_for_backward(n, saved)
+    tape.backward(n, up.data_ptr())
+    got = []
+    for t, dt in wanted:
+        gid = tape.get_grad_buffer(t.data_ptr())
+        got.append(torch.from_numpy(gb.download(dev, gid, t.shape, gb.dtype_code(t) if dt is None else dt)))
+    tape.end()
+    return got
+
+
+@pytest.mark.parametrize("eps,mscale", [(0.0, 1.0), (0.0, 0.0), (1e-6, 0.0), (1e-3, 2.0)])
+def test_nodes_take_zeros_at_their_word(gn, tape_env, eps, mscale):
+    """An eps or an mscale of 0 in a node's parameters is the forward's, not a default (rows whose mean square
+    is about 1e-6, where an eps of 1e-6 halves the norm)."""
+    gc, gb, dev = tape_env
+    g = gen(8)
+    B, S, H, K, D, rot = 1, 5, 3, 1, 64, 32
+    C = (H + 2 * K) * D
+    x, dy = rand(g, B, S, C, dtype=F32, std=1e-3), rand(g, B, S, C, dtype=F32)
+    wq, wk, f = rand(g, D, dtype=F32), rand(g, D, dtype=F32), freqs(rot)
+    part = lambda t: (t.view(B, S, -1, D)[:, :, :H], t.view(B, S, -1, D)[:, :, H:H + K], t.view(B, S, -1, D)[:, :, H + K:])
+    y, want = torch.empty_like(x), torch.empty_like(x)
+    gn.qk_norm_rope_fwd(*part(x)[:2], wq, wk, f, v=part(x)[2], out=part(y), eps=eps, mscale=mscale)
+    direct = gn.qk_norm_rope_bwd(*part(dy)[:2], *part(x)[:2], wq, wk, f, dyv=part(dy)[2], out=part(want), eps=eps,
+                                 mscale=mscale)
+    got = node_grads(tape_env, "QkNormRope", [gb.tref(x, True)], [gb.tref(y)],
+                     gb.qk_norm_rope_params(H, K, rot, eps=eps, mscale=mscale), [wq.data_ptr(), wk.data_ptr(), f.data_ptr()],
+                     dy, [(x, None), (wq, gb.DTYPE_F32), (wk, gb.DTYPE_F32)])
+    for a, b in zip(got, (want, direct[3], direct[4])):
+        assert torch.equal(a, b.cpu()) and bool(torch.isfinite(a).all())
+    z, dz = rand(g, B, S, H * D, dtype=F32), rand(g, B, S, H * D, dtype=F32)
+    back = gn.rope_bwd(dz.view(B, S, H, D), f, mscale=mscale).view_as(dz)
+    got = node_grads(tape_env, "Rope", [gb.tref(z, True)], [gb.tref(torch.empty_like(z))],
+                     gb.rope_params(H, rot, mscale=mscale), [f.data_ptr()], dz, [(z, None)])
+    assert torch.equal(got[0], back.cpu())
+
+
+def test_parameter_blocks_that_end_early(gn, tape_env):
+    """A block of heads, kv_heads, rot and mode alone: mscale 1, eps 1e-6."""
+    gc, gb, dev = tape_env
+    g = gen(9)
+    x, dy = rand(g, 1, 4, 3 * 64, dtype=F32, std=1e-3), rand(g, 1, 4, 3 * 64, dtype=F32)
+    f, y = freqs(64), torch.empty(1, 4, 3 * 64, device=DEV)
+    full = gb.qk_norm_rope_params(1, 1, 64)
+    a = node_grads(tape_env, "QkNormRope", [gb.tref(x, True)], [gb.tref(y)], full[:16], [0, 0, f.data_ptr()], dy, [(x, None)])
+    b = node_grads(tape_env, "QkNormRope", [gb.tref(x, True)], [gb.tref(y)], full, [0, 0, f.data_ptr()], dy, [(x, None)])
+    assert torch.equal(a[0], b[0])
