@@ -263,6 +263,22 @@ PYBIND11_MODULE(_grilly_core, m) {
         .def("save", [](const TapeArena& a) { return a.save().offset; })
         .def("restore", [](TapeArena& a, size_t off) { a.restore({off, nullptr}); });
     m.attr("NODE_BYTES") = sizeof(Node);
+    m.def("_check_node",
+          [](OpType op, const std::vector<TensorRef>& inputs, const std::vector<TensorRef>& outputs, py::bytes params,
+             bool upstream) {
+              Node n{};
+              n.op = op;
+              n.num_inputs = (uint32_t)std::min<size_t>(inputs.size(), kMaxNodeIO);
+              n.num_outputs = (uint32_t)std::min<size_t>(outputs.size(), kMaxNodeIO);
+              std::copy_n(inputs.begin(), n.num_inputs, n.inputs);
+              std::copy_n(outputs.begin(), n.num_outputs, n.outputs);
+              const std::string p = params;
+              n.params_size = (uint32_t)std::min(p.size(), sizeof(n.params));
+              std::copy_n(p.data(), n.params_size, n.params);
+              check_node(&n, upstream);
+          },
+          py::arg("op"), py::arg("inputs"), py::arg("outputs"), py::arg("params") = py::bytes(), py::arg("upstream") = false,
+          "The backward's check of a node's types and sizes, without a device");
 
     // ---- GRLY v3 hypernetwork checkpoint (bindings.cpp:2965-3039) + optimizer section ----
     // dims = (d_model, vsa_dim, K, router_hidden); opt = None or dict(kind, n_states, step,

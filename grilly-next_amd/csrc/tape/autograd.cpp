@@ -245,7 +245,35 @@ void BackwardEngine::flush_norms() {
     norm_pending_.clear();
 }
 
+void check_node(const Node* n, bool upstream) {
+    const TensorRef &x = n->inputs[0], &y = n->outputs[0];
+    auto alike = [](const TensorRef& a, const TensorRef& b) { return a.dtype == b.dtype && a.numel() == b.numel(); };
+    switch (n->op) {
+        case OpType::FlashAttention2:
+            // the kernels take one size and type for all of them
+            if (params_of<AttentionParams>(n).layout == 1) {
+                if (y.dtype != x.dtype || x.numel() != 3 * y.numel())
+                    throw std::invalid_argument("FlashAttention2 (fused QKV): O must have qkv's type and a third of its elements");
+            } else if (n->num_inputs < 3 || !alike(n->inputs[1], x) || !alike(n->inputs[2], x) || !alike(y, x)) {
+                throw std::invalid_argument("FlashAttention2: K, V and O must have Q's type and size (fewer key and value "
+                                            "heads are repeated first)");
+            }
+            break;
+        case OpType::Rope:
+        case OpType::QkNormRope:
+            if (y.dtype != x.dtype)
+                throw std::invalid_argument("Rope, QkNormRope: the output must have the input's type");
+            break;
+        case OpType::LinearCrossEntropy:
+            if (upstream && (y.dtype != 0 || y.numel() != x.rows()))
+                throw std::invalid_argument("LinearCrossEntropy: an upstream gradient goes with a loss of fp32 [T]");
+            break;
+        default: break;
+    }
+}
+
 void BackwardEngine::dispatch(Node* n) {
+    check_node(n, n->grad_output_buffer > 1);
     switch (n->op) {
         case OpType::Linear: bwd_linear(n); break;
         case OpType::ReLU: bwd_act(n, GN_ACT_RELU, false); break;

@@ -155,6 +155,10 @@ T* TapeArena::allocate_node(Args&&... args) {
     return node;
 }
 
+// Throws where the types or sizes of an attention, Rope, QkNormRope or LinearCrossEntropy node's tensors are
+// not what its backward reads and writes by (upstream: it is given a gradient of its output).  No device call.
+void check_node(const Node* n, bool upstream);
+
 class BackwardEngine {
 public:
     explicit BackwardEngine(Device& dev);
