@@ -519,13 +519,23 @@ def attn_workspace_bytes(B, H, S, D, dtype=None):
     return int(lib().gn_attn_workspace_bytes_dtype(B, H, S, D, code))
 
 
+def _attn_like(Q, **others):
+    """The kernels read and write every tensor by Q's type and size."""
+    for name, t in others.items():
+        if t is not None and (t.dtype is not Q.dtype or t.shape != Q.shape):
+            raise GnError(f"{name} {list(t.shape)} {t.dtype} must be as Q, {list(Q.shape)} {Q.dtype}"
+                          + (" (fewer key and value heads are repeated first)" if name in "KV" else ""))
+
+
 def attn_bwd(Q, K, V, O, dO, LSE, scale=None, causal=True, rope="interleaved", theta=10000.0,
              ws=None, out=None, mask=None):
-    """(dQ, dK, dV).  mask: fp32 [B, S] key-padding mask (1 keep, 0 masked), or None."""
+    """(dQ, dK, dV).  K and V have Q's heads; mask: fp32 [B, S] key-padding mask (1 keep, 0 masked), or None."""
     B, H, S, D = Q.shape
+    _attn_like(Q, K=K, V=V, O=O, dO=dO)
     scale = D ** -0.5 if scale is None else scale
     dQ, dK, dV = out if out is not None else (torch.empty_like(Q), torch.empty_like(K),
                                               torch.empty_like(V))
+    _attn_like(Q, dQ=dQ, dK=dK, dV=dV)
     if ws is None:
         ws = workspace(attn_workspace_bytes(B, H, S, D, Q.dtype), Q.device)
     if mask is None:
@@ -564,8 +574,10 @@ def attn_bwd_qkv(qkv, O, dO, LSE, heads, scale=None, causal=True, rope="none", t
 
 def attn_fwd(Q, K, V, scale=None, causal=True, rope="interleaved", theta=10000.0, ws=None,
              mask=None):
-    """(O, LSE).  mask: fp32 [B, S] key-padding mask (1 keep, 0 masked), or None."""
+    """(O, LSE).  K and V have Q's heads (fewer are repeated first: K.repeat_interleave(n, 1)); mask: fp32
+    [B, S] key-padding mask (1 keep, 0 masked), or None."""
     B, H, S, D = Q.shape
+    _attn_like(Q, K=K, V=V)
     scale = D ** -0.5 if scale is None else scale
     O = torch.empty_like(Q)
     LSE = torch.empty((B, H, S), dtype=torch.float32, device=Q.device)
@@ -1033,7 +1045,8 @@ def qk_norm_rope_fwd(q, k, wq=None, wk=None, freqs=None, v=None, mode="half", po
                      eps=1e-6, heads_first=False, out=None):
     """(yq, yk), or (yq, yk, yv) when v is given: q and k [B, S, H, D] (views; k may have fewer heads,
     or be None) normed per head, y = x rsqrt(mean(x^2) + eps) w, and rotated as by rope_fwd (freqs None: not);
-    v copied.  heads_first: the outputs are [B, H, S, D], as attn_fwd takes them; `out` gives them."""
+    v copied.  heads_first: the outputs are [B, H, S, D], attn_fwd's layout (which takes k and v of q's heads:
+    fewer are repeated first); `out` gives them."""
     B, S, D, qs, ks, qh, kh, wqp, wkp = _qk(q, k, wq, wk)
     vs = None if v is None else (B, S, v.shape[2] if v.dim() == 4 else 0, D)
     vh = _heads("v", v, vs, q.dtype)

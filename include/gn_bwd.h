@@ -376,7 +376,8 @@ int gn_rope_bwd(const gn_heads* dy, const gn_heads* dx, const gn_rope* rope, int
                 int dtype, void* stream);
 
 /* Per-head RMS norm of queries and keys, rotated in the same pass; values copied along, so that the
- * call also splits fused QKV rows into the [B,H,S,D] tensors gn_attn_fwd takes:
+ * call also splits fused QKV rows into [B,H,S,D] tensors, gn_attn_fwd's layout (which takes k and v of
+ * q's heads: fewer are repeated first):
  *   r = rsqrt(mean_j x_j^2 + eps) per token and head,  y = rotation(x r w),  yv = v
  * wq, wk: [D] in dtype, shared by the heads (NULL: 1).  k (with yk) and v (with yv) may be NULL;
  * rope NULL: no rotation.  q and k may differ in their number of heads, k and v may not. */

@@ -268,3 +268,44 @@ def test_parameter_blocks_that_end_early(gn, tape_env):
     a = node_grads(tape_env, "QkNormRope", [gb.tref(x, True)], [gb.tref(y)], full[:16], [0, 0, f.data_ptr()], dy, [(x, None)])
     b = node_grads(tape_env, "QkNormRope", [gb.tref(x, True)], [gb.tref(y)], full, [0, 0, f.data_ptr()], dy, [(x, None)])
     assert torch.equal(a[0], b[0])
+
+
+def test_grouped_heads_through_the_attention(gn):
+    """The documented run: fused rows of 4 + 2 + 2 heads, norms and rotation head first, k and v repeated for
+    the attention, and back; fp32, against fp64 autograd within the 1e-4 of the largest element that the
+    fp32 attention's own tests have (two-piece products, 2^-16 a term)."""
+    g = gen(31)
+    B, S, Hq, Hk, D = 2, 65, 4, 2, 64
+    qkv = rand(g, B, S, (Hq + 2 * Hk) * D, dtype=F32)
+    wq, wk, dO = rand(g, D, dtype=F32), rand(g, D, dtype=F32), rand(g, B, Hq, S, D, dtype=F32)
+    pos = torch.randint(0, 900, (B, S), device=DEV, generator=g).to(torch.int32)
+    f, m = gn.rope_freqs(D, theta=1e6, scaling="yarn", factor=4.0, trained=8192)
+    q, k, v = (t.view(B, S, -1, D) for t in qkv.split((Hq * D, Hk * D, Hk * D), dim=-1))
+    n = Hq // Hk
+    yq, yk, yv = gn.qk_norm_rope_fwd(q, k, wq, wk, f, v=v, positions=pos, mscale=m, heads_first=True)
+    rk, rv = yk.repeat_interleave(n, 1), yv.repeat_interleave(n, 1)
+    O, lse = gn.attn_fwd(yq, rk, rv, rope="none")
+    dyq, dyk, dyv = gn.attn_bwd(yq, rk, rv, O, dO, lse, rope="none")
+    dyk, dyv = (t.view(B, Hk, n, S, D).float().sum(2).to(t.dtype) for t in (dyk, dyv))
+    dq, dk, dv, dwq, dwk = gn.qk_norm_rope_bwd(dyq, dyk, q, k, wq, wk, f, dyv=dyv, positions=pos, mscale=m,
+                                               heads_first=True)
+    x = qkv.cpu().double().requires_grad_()
+    w = [t.cpu().double().requires_grad_() for t in (wq, wk)]
+    a = x.view(B, S, -1, D)
+    a, b, c = a[:, :, :Hq], a[:, :, Hq:Hq + Hk], a[:, :, Hq + Hk:]
+    ang = pos.cpu().double()[:, :, None, None] * f.cpu()
+    cos, sin = m * torch.cos(ang), m * torch.sin(ang)
+
+    def norm_turn(t, w):
+        t = t * (t.square().mean(-1, keepdim=True) + 1e-6).rsqrt() * w
+        u, y = t.chunk(2, -1)
+        return torch.cat((u * cos - y * sin, y * cos + u * sin), -1).transpose(1, 2)
+
+    a, b, c = norm_turn(a, w[0]), norm_turn(b, w[1]).repeat_interleave(n, 1), c.transpose(1, 2).repeat_interleave(n, 1)
+    s = (a @ b.transpose(-1, -2).contiguous()) * D ** -0.5
+    s = s.masked_fill(torch.triu(torch.ones(S, S, dtype=torch.bool), 1), float("-inf"))
+    o = torch.softmax(s, -1) @ c
+    (o * dO.cpu().double()).sum().backward()
+    got = torch.cat([t.reshape(B, S, -1) for t in (dq, dk, dv)], -1)
+    for have, want in ((O, o.detach()), (got, x.grad), (dwq, w[0].grad), (dwk, w[1].grad)):
+        assert float((have.cpu().double() - want).abs().max() / want.abs().max()) < 1e-4

@@ -63,3 +63,23 @@ def test_nodes_check_their_tensors():
     gc._check_node(op.LinearCrossEntropy, [h, t], [ref(F, 1)], b"", False)
     bad("upstream", op.LinearCrossEntropy, [h, t], [ref(F, 1)], b"", True)
     bad("upstream", op.LinearCrossEntropy, [h, t], [ref(H, 16)], b"", True)
+
+
+def test_attention_takes_one_size():
+    """K and V of fewer heads than Q would be read past their end."""
+    torch = pytest.importorskip("torch")
+    q, k = torch.zeros(2, 4, 64, 32), torch.zeros(2, 2, 64, 32)
+    lse = torch.zeros(2, 4, 64)
+    for args in ((k, k), (q, k), (k, q), (q.bfloat16(), q), (q[:, :, :32], q)):
+        with pytest.raises(gn.GnError, match="as Q"):
+            gn.attn_fwd(q, *args)
+        with pytest.raises(gn.GnError, match="as Q"):
+            gn.attn_bwd(q, *args, q, q, lse)
+    with pytest.raises(gn.GnError, match="repeated"):
+        gn.attn_fwd(q, k, k)
+    with pytest.raises(gn.GnError, match="as Q"):
+        gn.attn_bwd(q, q, q, q, k, lse)
+    with pytest.raises(gn.GnError, match="as Q"):
+        gn.attn_bwd(q, q, q, q, q, lse, out=(q, k, q))
+    with pytest.raises(gn.GnError, match="not on the GPU"):  # of one size: on to the next check
+        gn.attn_fwd(q, q, q)
