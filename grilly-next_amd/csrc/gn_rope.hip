@@ -563,6 +563,31 @@ bool overlap(const gn_heads& a, const gn_heads& b, int B, int S, int D, int es) 
     return true;
 }
 
+// Whether one of t's elements lies in [lo, hi): the heads' rows are searched by their strides, the largest
+// first; of views that overlap themselves it may say so without one.
+bool holds(const gn_heads& t, int B, int S, int D, int es, const void* lo, const void* hi) {
+    if (!lo || t.H == 0 || B == 0 || S == 0) return false;
+    const int64_t n[3] = {B, S, t.H}, st[3] = {t.sb * es, t.ss * es, t.sh * es};
+    int order[3] = {0, 1, 2};
+    std::sort(order, order + 3, [&](int i, int j) { return st[i] > st[j]; });
+    int64_t inner[4];  // bytes that the dimensions from the k-th on span
+    inner[3] = (int64_t)D * es;
+    for (int k = 2; k >= 0; --k) inner[k] = inner[k + 1] + (n[order[k]] - 1) * st[order[k]];
+    auto search = [&](auto& self, int k, const char* at) -> bool {
+        if (at + inner[k] <= (const char*)lo || (const char*)hi <= at) return false;
+        if (k == 3) return true;
+        const int64_t s = st[order[k]], most = n[order[k]] - 1;
+        if (s == 0 || most == 0) return self(self, k + 1, at);
+        const int64_t before = (const char*)lo - at - inner[k + 1];  // i s > before, at + i s < hi
+        const int64_t i0 = before < 0 ? 0 : before / s + 1, i1 = std::min(most, ((const char*)hi - at - 1) / s);
+        if (i1 - i0 > 1024) return true;
+        for (int64_t i = i0; i <= i1; ++i)
+            if (self(self, k + 1, at + i * s)) return true;
+        return false;
+    };
+    return search(search, 0, (const char*)t.p);
+}
+
 // whether an output's elements are all different ones
 bool writable(const gn_heads& t, int B, int S, int D) {
     int64_t n[3] = {B, S, t.H}, st[3] = {t.sb, t.ss, t.sh};
@@ -593,11 +618,49 @@ int check_heads(const char* who, const char* name, const gn_heads* t, int es, bo
     return GN_OK;
 }
 
-// The shapes, the rotation and the tensors' places; fills a's common part.
 struct Named {
     const gn_heads* t;
     const char* name;
 };
+
+// Memory of a call beside its heads: weights, frequencies, positions, weight gradients, the workspace
+struct Flat {
+    const void* p;
+    int64_t bytes;
+    const char* name;
+    bool written;
+};
+
+// What is written may share no memory with anything else of the call.
+int check_flat(const char* who, const Named* in, int ni, const Named* out, int no, const Flat* f, int nf, int B, int S,
+               int D, int dtype) {
+    const int es = dtype == GN_F32 ? 4 : 2;
+    auto end = [](const Flat& x) { return (const char*)x.p + x.bytes; };
+    for (int i = 0; i < nf; ++i) {
+        if (!f[i].p || f[i].bytes <= 0) continue;
+        for (int j = 0; j < no; ++j)
+            GN_REQUIRE(!holds(*out[j].t, B, S, D, es, f[i].p, end(f[i])), "%s: %s shares memory with %s", who, out[j].name,
+                       f[i].name);
+        if (!f[i].written) continue;
+        for (int j = 0; j < ni; ++j)
+            GN_REQUIRE(!holds(*in[j].t, B, S, D, es, f[i].p, end(f[i])), "%s: %s shares memory with %s", who, f[i].name,
+                       in[j].name);
+        for (int j = 0; j < nf; ++j)
+            GN_REQUIRE(j == i || !f[j].p || (const char*)f[j].p >= end(f[i]) || (const char*)f[i].p >= end(f[j]),
+                       "%s: %s and %s may not share memory", who, f[i].name, f[j].name);
+    }
+    return GN_OK;
+}
+
+// the rotation's frequencies and positions
+int add_rope(Flat* f, int n, const gn_rope* r, int B, int S) {
+    if (!r || r->rot == 0) return n;
+    f[n++] = {r->freqs, (int64_t)r->rot / 2 * 8, "freqs", false};
+    f[n++] = {r->positions, ((int64_t)(B - 1) * r->pos_sb + S) * 4, "positions", false};
+    return n;
+}
+
+// The shapes, the rotation and the tensors' places; fills a's common part.
 int check(const char* who, const gn_rope* r, int B, int S, int D, int dtype, const Named* in, int ni, const Named* out,
           int no, const int* own, Args& a, bool& vec, int& mode) {
     GN_REQUIRE(dtype == GN_F32 || dtype == GN_BF16, "%s: dtype %d not supported (f32, bf16)", who, dtype);
@@ -692,6 +755,8 @@ int rope_call(const char* who, const gn_heads* x, const gn_heads* y, const gn_ro
     const int own = 0;
     if (const int rc = check(who, r, B, S, D, dtype, &in, 1, &out, 1, &own, a, vec, mode)) return rc;
     if (a.tokens == 0 || x->H == 0) return GN_OK;
+    Flat flat[2];
+    if (const int rc = check_flat(who, &in, 1, &out, 1, flat, add_rope(flat, 0, r, B, S), B, S, D, dtype)) return rc;
     fill(a.g[0], x, nullptr, nullptr, y);
     a.ng = 1;
     a.sgn = sgn;
@@ -771,6 +836,8 @@ extern "C" int gn_qk_norm_rope_fwd(const gn_heads* q, const gn_heads* k, const g
     vec = vec && (((uintptr_t)wq | (uintptr_t)wk) & 15u) == 0;
     const int heads = q->H + (k ? k->H : 0) + (v ? v->H : 0);
     if (a.tokens == 0 || heads == 0) return GN_OK;
+    Flat flat[4] = {{wq, (int64_t)D * es, "wq", false}, {wk, (int64_t)D * es, "wk", false}};
+    if (const int rc = check_flat(who, in, n, out, n, flat, add_rope(flat, 2, rope, B, S), B, S, D, dtype)) return rc;
     fill(a.g[0], q, nullptr, wq, yq);
     if (k) fill(a.g[1], k, nullptr, wk, yk);
     if (v) fill(a.copy, v, nullptr, nullptr, yv);
@@ -864,6 +931,12 @@ extern "C" int gn_qk_norm_rope_bwd(const gn_heads* dyq, const gn_heads* dyk, con
         }
         a.part = (float*)ws;
     }
+    Flat flat[7] = {{wq, (int64_t)D * es, "wq", false},
+                    {wk, (int64_t)D * es, "wk", false},
+                    {dwq, (int64_t)D * 4, "dwq", true},
+                    {dwk, (int64_t)D * 4, "dwk", true},
+                    {a.part, (int64_t)grid * D * 4, "the workspace", true}};
+    if (const int rc = check_flat(who, in, ni, out, no, flat, add_rope(flat, 5, rope, B, S), B, S, D, dtype)) return rc;
     a.dw[0] = dwq;
     a.dw[1] = dwk;
     if (dwk && !second && !acc && launch_zero(dwk, (size_t)D * 4, s) != hipSuccess) {  // keys without heads

@@ -330,8 +330,8 @@ size_t gn_linear_xent_workspace_bytes(int T, int d, int V, int dtype);
 /* Heads of B x S tokens: element (b, s, h, j), j < D, at p[b*sb + s*ss + h*sh + j] (strides in
  * elements, none negative; a head's D elements are contiguous).  [B,S,H,D], [B,H,S,D] and the
  * q, k or v part of fused QKV rows are all such views.  Inputs may repeat memory (stride 0);
- * an output may not overlap itself or another tensor of the call, except that it may be its
- * own input (same address and strides). */
+ * an output may not overlap itself or another tensor of the call (weights, frequencies and positions
+ * among them), except that it may be its own input (same address and strides). */
 typedef struct gn_heads {
     void* p;
     int64_t sb, ss, sh;
@@ -390,7 +390,8 @@ int gn_qk_norm_rope_fwd(const gn_heads* q, const gn_heads* k, const gn_heads* v,
  * anyway), with g = the rotation's transpose applied to dy:
  *   dx = r (w g - x r^2 mean_j(w_j g_j x_j)),  dw = sum over tokens and heads of g x r,  dv = dyv
  * dwq, dwk: fp32 [D], NULL: not wanted; GN_ACCUMULATE adds onto them (the others are
- * overwritten; the two may not share memory).  The sums run in a fixed order: the same bits every time.
+ * overwritten).  The sums run in a fixed order: the same bits every time.  dwq, dwk and the workspace, like
+ * the outputs, may share memory with nothing else of the call.
  * ws: gn_qk_norm_rope_workspace_bytes, 16-byte aligned; not used without dwq and dwk. */
 int gn_qk_norm_rope_bwd(const gn_heads* dyq, const gn_heads* dyk, const gn_heads* dyv,
                         const gn_heads* q, const gn_heads* k, const void* wq, const void* wk,

@@ -83,3 +83,79 @@ def test_attention_takes_one_size():
         gn.attn_bwd(q, q, q, q, q, lse, out=(q, k, q))
     with pytest.raises(gn.GnError, match="not on the GPU"):  # of one size: on to the next check
         gn.attn_fwd(q, q, q)
+
+
+B, S, D = 2, 8, 64
+
+
+def heads(off=0, H=2, sb=None, ss=None, sh=None):
+    ss = H * D if ss is None else ss
+    return gn.Heads(BASE + off, S * ss if sb is None else sb, ss, D if sh is None else sh, H)
+
+
+def turn(**kw):
+    r = gn.Rope(BASE >> 1, None, 0, 0, 1.0, D, 2)
+    for k, v in kw.items():
+        setattr(r, k, v)
+    return r
+
+
+def test_rope_output_over_its_tables():
+    """An output may not lie over the frequencies or the positions (rows of 128 bytes a head, 4096 in all)."""
+    for fn in (gn.lib().gn_rope_fwd, gn.lib().gn_rope_bwd):
+        for off in (-248, 0, 100 * 8, 4088):
+            refused(fn(heads(), heads(MB), turn(freqs=BASE + MB + off), B, S, D, 4, None), "freqs")
+        refused(fn(heads(), heads(), turn(positions=BASE + 4092), B, S, D, 4, None), "positions")
+        refused(fn(heads(), heads(MB), turn(positions=BASE + MB - 36, pos_sb=2), B, S, D, 4, None), "positions")
+        # a table between an output's heads, and into the next one by its last 8 bytes
+        far = heads(MB, sb=64 * S * D, ss=64 * D, sh=32 * D)
+        refused(fn(heads(), far, turn(freqs=BASE + MB + 33 * 128 - 248 + 31 * 128), B, S, D, 4, None), "freqs")
+
+
+def test_qk_weight_gradients_and_workspace_stand_alone():
+    lib = gn.lib()
+    q, k, dyq, dyk, dyv = (heads(i * MB) for i in range(5))
+    dq, dk, dv = (heads(i * MB) for i in range(5, 8))
+    w, ws = p(8 * MB), p(9 * MB)
+    dw = [p(10 * MB), p(11 * MB)]
+
+    def bwd(dwq=dw[0], dwk=dw[1], ws=ws, wq=w, r=turn()):
+        return lib.gn_qk_norm_rope_bwd(dyq, dyk, dyv, q, k, wq, w, dq, dk, dv, dwq, dwk, r, B, S, D, 1e-6, 4, 0, ws, 1 << 20,
+                                       None)
+
+    for i in range(8):
+        refused(bwd(dwq=p(i * MB)), "shares memory")
+        refused(bwd(dwk=p(i * MB + 4096 - 4)), "shares memory")
+        refused(bwd(ws=p(i * MB + 4096 - 16)), "shares memory")
+    refused(bwd(dwq=p(8 * MB + 124)), "may not share")     # the weights' last bytes
+    refused(bwd(dwk=p(9 * MB)), "may not share")           # the workspace
+    refused(bwd(r=turn(freqs=BASE + 9 * MB)), "may not share")
+    refused(bwd(dwq=w), "may not share")
+    refused(bwd(wq=p(5 * MB + 16)), "dq shares memory with wq")
+
+    def fwd(wq=w, wk=w, r=turn()):
+        return lib.gn_qk_norm_rope_fwd(q, k, dyv, wq, wk, dq, dk, dv, r, B, S, D, 1e-6, 4, None)
+
+    refused(fwd(wq=p(6 * MB)), "yk shares memory with wq")
+    refused(fwd(wk=p(7 * MB + 4094)), "yv shares memory with wk")
+    refused(fwd(r=turn(freqs=BASE + 5 * MB)), "yq shares memory with freqs")
+
+
+def test_between_the_heads_is_free():
+    """A weight gradient in the gap between the parts of fused rows touches none of them: on to the check of
+    the workspace; one element further it is refused."""
+    lib = gn.lib()
+    C = 1024  # q, k, v of two heads, then 640 elements of something else
+    part = lambda off, i: gn.Heads(BASE + off + i * 2 * D * 2, S * C, C, D, 2)
+    d = [part(MB, i) for i in range(3)]
+    dy = [heads((3 + i) * MB) for i in range(3)]
+    gap = BASE + MB + 3 * C * 2 + 6 * D * 2  # behind row 3's heads
+
+    def go(dwq, ws, wsb=1 << 20):
+        return lib.gn_qk_norm_rope_bwd(dy[0], dy[1], dy[2], part(0, 0), part(0, 1), None, None, *d, ctypes.c_void_p(dwq), None,
+                                       turn(), B, S, D, 1e-6, 4, 0, ws, wsb, None)
+
+    refused(go(gap, None, 0), "workspace", -3)
+    refused(go(gap, p(4 * MB)), "the workspace shares memory with dyk")  # dwq itself passed
+    refused(go(gap - 4, p(9 * MB)), "dv shares memory with dwq")
+    refused(go(gap + 640 * 2 - 4 * D + 4, p(9 * MB)), "dq shares memory with dwq")
