@@ -980,9 +980,23 @@ int check(const char* who, const void* h, const void* E, const int32_t* tgt, int
     return GN_OK;
 }
 
-// Whether two tensors share memory
-bool shared(const void* a, size_t na, const void* b, size_t nb) {
-    return a && b && (const char*)a < (const char*)b + nb && (const char*)b < (const char*)a + na;
+// A tensor of a call, or its workspace
+struct Span {
+    const void* p;
+    size_t bytes;
+    const char* name;
+    bool written;
+};
+
+// What is written may share no memory with anything else of the call.
+template <int N>
+int check_spans(const char* who, const Span (&t)[N]) {
+    for (int i = 0; i < N; ++i)
+        for (int j = 0; j < N && t[i].written; ++j)
+            GN_REQUIRE(i == j || !t[i].p || !t[j].p || (const char*)t[i].p >= (const char*)t[j].p + t[j].bytes ||
+                           (const char*)t[j].p >= (const char*)t[i].p + t[i].bytes,
+                       "%s: %s and %s may not share memory", who, t[i].name, t[j].name);
+    return GN_OK;
 }
 
 int check_ws(const char* who, const Plan& w, int dtype, const void* ws, size_t ws_bytes) {
@@ -1068,9 +1082,12 @@ extern "C" int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* t
     clear_error();
     if (const int rc = check(who, h, E, targets, T, d, V, dtype)) return rc;
     GN_REQUIRE((((uintptr_t)loss | (uintptr_t)lse) & 3u) == 0, "%s: loss, lse must be aligned to 4 bytes", who);
-    GN_REQUIRE(!shared(loss, (size_t)T * 4, lse, (size_t)T * 4), "%s: loss and lse may not share memory", who);
     if (T == 0 || (!loss && !lse)) return GN_OK;
     const Plan w(T, d, V, dtype, !al16(h) || !al16(E), false);
+    const size_t es = dtype == GN_F32 ? 4 : 2, row = (size_t)T * 4;
+    const Span spans[] = {{h, (size_t)T * d * es, "h", false}, {E, (size_t)V * d * es, "E", false}, {targets, row, "targets", false},
+                          {loss, row, "loss", true}, {lse, row, "lse", true}, {ws, w.bytes, "the workspace", true}};
+    if (const int rc = check_spans(who, spans)) return rc;
     if (const int rc = check_ws(who, w, dtype, ws, ws_bytes)) return rc;
     char* const base = (char*)ws;
     Call c{who, w, base, h, E, as_stream(stream), dtype};
@@ -1130,11 +1147,12 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
     }
     GN_REQUIRE(lse, "%s: null pointer", who);
     if (!dh && !dE) return GN_OK;
-    const size_t es = dtype == GN_F32 ? 4 : 2, nh = (size_t)T * d * es, nE = (size_t)V * d * es, ndE = (size_t)V * d * des;
-    GN_REQUIRE(!shared(dh, nh, h, nh) && !shared(dh, nh, E, nE) && !shared(dE, ndE, h, nh) && !shared(dE, ndE, E, nE) &&
-                   !shared(dE, ndE, dh, nh),
-               "%s: dh and dE may not share memory with each other or the inputs", who);
     const Plan w(T, d, V, dtype, !al16(h) || !al16(E) || !al16(dE), true);
+    const size_t es = dtype == GN_F32 ? 4 : 2, nh = (size_t)T * d * es, nE = (size_t)V * d, row = (size_t)T * 4;
+    const Span spans[] = {{h, nh, "h", false}, {E, nE * es, "E", false}, {targets, row, "targets", false}, {lse, row, "lse", false},
+                          {dloss, row, "dloss", false}, {dlse, row, "dlse", false}, {dh, nh, "dh", true},
+                          {dE, nE * des, "dE", true}, {ws, w.bytes, "the workspace", true}};
+    if (const int rc = check_spans(who, spans)) return rc;
     if (const int rc = check_ws(who, w, dtype, ws, ws_bytes)) return rc;
     char* const base = (char*)ws;
     Call c{who, w, base, h, E, s, dtype};

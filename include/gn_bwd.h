@@ -297,8 +297,8 @@ int gn_xent_bwd(const void* logits, const int32_t* targets, void* dLogits, int r
 /* Softmax cross entropy of a linear head without its logits (the reference binds a Linear and
  * cross-entropy-backward.glsl:29-84 over stored logits): with l = h E^T,
  *   lse[t] = log sum_v exp l[t, v],  loss[t] = lse[t] - l[t, targets[t]]
- * h [T x d], E [V x d] in dtype; targets int32 [T]; loss, lse fp32 [T] (each may be NULL; they
- * may not share memory).  A target
+ * h [T x d], E [V x d] in dtype; targets int32 [T]; loss, lse fp32 [T] (each may be NULL).  Outputs and the
+ * workspace, here and in the backward, may share memory with nothing else of the call.  A target
  * outside [0, V) (-100, say) marks a row without one: loss 0, and no gradient from dloss.
  * The logits exist a tile or a piece of the vocabulary at a time, in fp32.  T below 2^28, d up to
  * 2^20, V below 2^30, T * V below 2^43, T * V * d below 2^58.

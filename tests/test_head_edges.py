@@ -159,3 +159,33 @@ def test_between_the_heads_is_free():
     refused(go(gap, p(4 * MB)), "the workspace shares memory with dyk")  # dwq itself passed
     refused(go(gap - 4, p(9 * MB)), "dv shares memory with dwq")
     refused(go(gap + 640 * 2 - 4 * D + 4, p(9 * MB)), "dq shares memory with dwq")
+
+
+def test_linear_xent_outputs_and_workspace_stand_alone():
+    lib = gn.lib()
+    T, d, V = 16, 64, 100
+    need = lib.gn_linear_xent_workspace_bytes(T, d, V, 4)
+    GB = 1 << 30
+
+    def fwd(loss=p(3 * MB), lse=p(4 * MB), ws=p(GB)):
+        return lib.gn_linear_xent_fwd(p(), p(MB), p(2 * MB), loss, lse, T, d, V, 4, ws, need, None)
+
+    last = {0: T * d * 2, 1: V * d * 2, 2: T * 4}  # bytes of h, E, targets
+    for i, n in last.items():
+        refused(fwd(loss=p(i * MB + n - 4)), "loss and")
+        refused(fwd(lse=p(i * MB)), "lse and")
+        refused(fwd(ws=p(i * MB)), "workspace")
+        refused(fwd(ws=p(i * MB + n - 16)), "may not share")
+    refused(fwd(ws=p(3 * MB)), "loss and the workspace")
+    refused(fwd(lse=p(GB)), "lse and the workspace")
+
+    def bwd(lse=p(3 * MB), dloss=p(4 * MB), dlse=p(5 * MB), dh=p(6 * MB), dE=p(7 * MB), ws=p(GB)):
+        return lib.gn_linear_xent_bwd(p(), p(MB), p(2 * MB), lse, dloss, dlse, 1.0, dh, dE, 0, T, d, V, 4, 0, ws, need, None)
+
+    last.update({3: T * 4, 4: T * 4, 5: T * 4})
+    for i, n in last.items():
+        refused(bwd(dh=p(i * MB + n - 4)), "dh and")
+        refused(bwd(dE=p(i * MB + n - 4)), "dE and")
+        refused(bwd(ws=p(i * MB)), "may not share")
+    refused(bwd(ws=p(7 * MB + V * d * 4 - 16)), "dE and the workspace")
+    refused(bwd(ws=p(6 * MB)), "dh and the workspace")
