@@ -876,6 +876,15 @@ def _place(name, t, dtype):
         raise GnError(f"{name} must be {dtype}, not {t.dtype}")
 
 
+_INT = 2 ** 31 - 1
+
+
+def _int32(name, t):
+    """The entries take sizes as ints, which ctypes would cut off without a word."""
+    if t.numel() > _INT and max(t.shape) > _INT:
+        raise GnError(f"{name}: a size of {max(t.shape)} is past 31 bits")
+
+
 def _here(name, t, dtype=None, shape=None):
     """Device address of an argument, or None: contiguous, on the current device, of the dtype and
     shape that the call needs."""
@@ -899,6 +908,8 @@ def _xent_args(h, E, targets, ws):
     if h.dim() != 2 or E.dim() != 2 or h.shape[1] != E.shape[1]:
         raise GnError(f"h [T, d] and E [V, d] expected, not {list(h.shape)} and {list(E.shape)}")
     (T, d), V, dt = h.shape, E.shape[0], _dt(h)
+    _int32("h", h)
+    _int32("E", E)
     args = (_here("h", h), _here("E", E, h.dtype), _here("targets", targets, torch.int32, (T,)))
     if ws is None:
         ws = workspace(linear_xent_workspace_bytes(T, d, V, dt), h.device)
@@ -967,6 +978,8 @@ def _heads(name, t, shape, dtype, first=False):
         sb, ss, sh, sd = t.stride()
     if shape is not None and (b, n, h, d) != shape:
         raise GnError(f"{name} must be {list(shape)} as [B, S, H, D], not {[b, n, h, d]}")
+    if h > _INT or (shape is None and (b > _INT or n > _INT or d > _INT)):  # (b, n and d: shape's)
+        _int32(name, t)
     if sd != 1 and d > 1:
         raise GnError(f"{name}: the elements of a head must be contiguous")
     return Heads(t.data_ptr(), sb, ss, sh, h)
@@ -977,6 +990,8 @@ def _rope(freqs, mode, positions, pos0, mscale, B, S):
         return None
     if freqs.dim() != 1:
         raise GnError("freqs must have one dimension")
+    if not -(1 << 63) <= pos0 < 1 << 63:
+        raise GnError(f"pos0 {pos0} is past 64 bits")
     f, p, sb = _here("freqs", freqs, torch.float64), None, 0
     if positions is not None:
         p = _here("positions", positions, torch.int32)

@@ -309,3 +309,11 @@ def test_grouped_heads_through_the_attention(gn):
     got = torch.cat([t.reshape(B, S, -1) for t in (dq, dk, dv)], -1)
     for have, want in ((O, o.detach()), (got, x.grad), (dwq, w[0].grad), (dwk, w[1].grad)):
         assert float((have.cpu().double() - want).abs().max() / want.abs().max()) < 1e-4
+
+
+def test_sizes_past_31_bits_are_refused(gn):
+    x = torch.zeros(1, 1, 1, 2, device=DEV).expand(2 ** 32 + 2, 1, 1, 2)
+    with pytest.raises(gn.GnError, match="31 bits"):
+        gn.rope_fwd(x, freqs(2))
+    with pytest.raises(gn.GnError, match="31 bits"):
+        gn.qk_norm_rope_fwd(x, None)

@@ -189,3 +189,20 @@ def test_linear_xent_outputs_and_workspace_stand_alone():
         refused(bwd(ws=p(i * MB)), "may not share")
     refused(bwd(ws=p(7 * MB + V * d * 4 - 16)), "dE and the workspace")
     refused(bwd(ws=p(6 * MB)), "dh and the workspace")
+
+
+def test_sizes_past_31_bits():
+    """Sizes that the entries' ints would cut off: [2^32 + 2, ...] is not [2, ...]."""
+    torch = pytest.importorskip("torch")
+    n = 2 ** 32 + 2
+    long = torch.zeros(1).expand(n, 1)
+    short, t = torch.zeros(2, 1), torch.zeros(2, dtype=torch.int32)
+    for h, E in ((long, short), (short, long), (long.t(), long.t())):
+        with pytest.raises(gn.GnError, match="31 bits"):
+            gn.linear_xent_fwd(h, E, t)
+        with pytest.raises(gn.GnError, match="31 bits"):
+            gn.linear_xent_bwd(h, E, t, t)
+    with pytest.raises(gn.GnError, match="31 bits"):
+        gn._int32("x", torch.zeros(1, 1, 1, 2).expand(n, 1, 1, 2))
+    with pytest.raises(gn.GnError, match="64 bits"):
+        gn._rope(torch.ones(4, dtype=torch.float64), "half", None, 2 ** 64 + 5, 1.0, 1, 1)
