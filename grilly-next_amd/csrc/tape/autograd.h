@@ -124,7 +124,9 @@ struct RopeNodeParams {
 };
 static_assert(sizeof(RopeNodeParams) == 32, "RopeNodeParams layout");
 // LinearCrossEntropy: inputs h [T,d] and targets int32 [T], outputs[0] loss fp32 [T]; saved slots {E
-// [vocab,d], lse}.  Without an upstream gradient every row's is `scale`.
+// [vocab,d], lse}.  The output is the rows' loss, not scaled.  As a root every row's gradient is `scale`; with
+// an upstream gradient (a mean or a weighted sum of the rows behind it) it is scale times the row's, so
+// that such a node takes scale 1.
 struct LinearCrossEntropyParams { uint32_t vocab; float scale; };
 struct MSELossParams { float scale; uint32_t has_scale; };      // scale default 1/n (mean)
 

@@ -108,7 +108,9 @@ def qk_norm_rope_params(heads: int, kv_heads: int, rot: int, mode: str = "half",
 
 
 def linear_cross_entropy_params(vocab: int, scale: float = 1.0) -> bytes:
-    """LinearCrossEntropy node: h [T, d] and targets [T] -> loss [T]; saved slots {E, lse}."""
+    """LinearCrossEntropy node: h [T, d] and targets [T] -> loss [T] (not scaled); saved slots {E, lse}.
+    scale: every row's gradient where the node is the root; a gradient from a node behind it (a mean of the
+    loss, say) is multiplied by scale, which is 1 there."""
     return struct.pack("<If", int(vocab), scale)
 
 

@@ -317,3 +317,29 @@ def test_sizes_past_31_bits_are_refused(gn):
         gn.rope_fwd(x, freqs(2))
     with pytest.raises(gn.GnError, match="31 bits"):
         gn.qk_norm_rope_fwd(x, None)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_the_loss_below_a_mean(gn, tape_env, dtype):
+    """LinearCrossEntropy with scale 1 and a Mean of its rows gives the gradients of the root with scale 1 / T
+    (1 / T is a power of two: the same bits); another scale multiplies what comes from behind."""
+    gc, gb, dev = tape_env
+    g = gen(12)
+    T, d, V = 64, 32, 90
+    h, E = rand(g, T, d, dtype=dtype), rand(g, V, d, dtype=dtype, std=0.3)
+    t = torch.randint(0, V, (T,), device=DEV, generator=g).to(torch.int32)
+    loss, lse = gn.linear_xent_fwd(h, E, t)
+    mean, one = loss.mean().reshape(1), torch.ones(1, device=DEV)
+    for scale in (1.0, 0.5):
+        dh, dE = gn.linear_xent_bwd(h, E, t, lse, scale=scale / T)
+        tape = gb.create_tape_context(dev)
+        tape.begin()
+        n = tape.record_op(gc.OpType.LinearCrossEntropy, [gb.tref(h, True), gb.tref(t)], [gb.tref(loss)],
+                           gb.linear_cross_entropy_params(V, scale))
+        tape.save_for_backward(n, [E.data_ptr(), lse.data_ptr()])
+        n = tape.record_op(gc.OpType.Mean, [gb.tref(loss, True)], [gb.tref(mean)])
+        tape.backward(n, one.data_ptr())
+        for x, dt, want in ((h, gb.dtype_code(h), dh), (E, gb.DTYPE_F32, dE)):
+            got = torch.from_numpy(gb.download(dev, tape.get_grad_buffer(x.data_ptr()), x.shape, dt))
+            assert torch.equal(got, want.float().cpu())
+        tape.end()
