@@ -343,3 +343,34 @@ def test_the_loss_below_a_mean(gn, tape_env, dtype):
             got = torch.from_numpy(gb.download(dev, tape.get_grad_buffer(x.data_ptr()), x.shape, dt))
             assert torch.equal(got, want.float().cpu())
         tape.end()
+
+
+@pytest.mark.parametrize("T,d", [(16, 256), (20, 512), (32, 2048), (16, 77), (64, 64), (64, 1024), (300, 72), (300, 33),
+                                 (2001, 264), (4096, 264)])
+def test_three_pieces_of_few_rows(gn, T, d):
+    """Up to 4096 rows an fp32 dE is as good as fp32's own: equal logits, p = 1 / 512, five rows with a weight,
+    three of them with one target.  lse = 9 ln 2 is off by half its step, 2^-22, and ln 2's rounding, p by
+    that, exp2's 2^-23 twice and a product's 2^-24: 2^-20.  Two pieces of G, 2^-17 of an element, do not pass."""
+    g = gen(T + d)
+    V = 512
+    h, E = rand(g, T, d), torch.zeros(V, d, device=DEV, dtype=BF)
+    t = torch.randint(0, V, (T,), device=DEV, generator=g).to(torch.int32)
+    at = torch.tensor([1, 4, T // 2, T - 3, T - 1], device=DEV)
+    t[at] = torch.tensor([7, 100, 7, 7, V - 1], device=DEV, dtype=torch.int32)
+    u = torch.zeros(T, device=DEV)
+    u[at] = torch.rand(5, device=DEV, generator=g) + 0.1
+    lse = gn.linear_xent_fwd(h, E, t)[1]
+    _, dE = gn.linear_xent_bwd(h, E, t, lse, dloss=u)
+    one = torch.ones(V, d, device=DEV)
+    gn.linear_xent_bwd(h, E, t, lse, dloss=u, need_dh=False, dE=one, accumulate=True)
+    p = (u[at].double() / V)[:, None].expand(5, V)
+    G = p.clone()
+    G[torch.arange(5), t[at].long()] -= u[at].double()
+    x = h[at].double()
+    ref = G.t() @ x
+    bound = (p * 2.0 ** -20 + G.abs() * 2.0 ** -23).t() @ x.abs() + 8 * 2.0 ** -24 * (G.t().abs() @ x.abs()) + 1e-30
+    assert bool(((dE.double() - ref).abs() <= bound).all())
+    assert bool(((one.double() - 1 - ref).abs() <= bound + 2 * 2.0 ** -24 * (1 + ref.abs() + bound)).all())
+    first = G.float().bfloat16().double()
+    two = first + (G - first).float().bfloat16().double()
+    assert bool(((two.t() @ x - ref).abs() > bound).any())
