@@ -967,12 +967,15 @@ size_t workspace_bytes(int T, int d, int V, int dtype) {
     return most;
 }
 
+// the sizes taken: the products count their tiles, and a block its k-tiles, in 31 bits
+bool within(int T, int d, int V) {
+    return T < (1 << 28) && d <= (1 << 20) && V < (1 << 30) && (int64_t)T * V < (1ll << 43) && (double)T * V * d < 0x1p58;
+}
+
 int check(const char* who, const void* h, const void* E, const int32_t* tgt, int T, int d, int V, int dtype) {
     GN_REQUIRE(dtype == GN_F32 || dtype == GN_BF16, "%s: dtype %d not supported (f32, bf16)", who, dtype);
     GN_REQUIRE(T >= 0 && d >= 1 && V >= 1, "%s: bad shape", who);
-    GN_REQUIRE(T < (1 << 28) && d <= (1 << 20) && V < (1 << 30), "%s: T below 2^28, d up to 2^20, V below 2^30", who);
-    // the products count their tiles, and a block its k-tiles, in 31 bits
-    GN_REQUIRE((int64_t)T * V < (1ll << 43) && (double)T * V * d < 0x1p58, "%s: T * V below 2^43, T * V * d below 2^58", who);
+    GN_REQUIRE(within(T, d, V), "%s: T below 2^28, d up to 2^20, V below 2^30, T * V below 2^43, T * V * d below 2^58", who);
     GN_REQUIRE(T == 0 || (h && E && tgt), "%s: null pointer", who);
     const int es = dtype == GN_F32 ? 4 : 2;
     GN_REQUIRE((((uintptr_t)h | (uintptr_t)E) & (es - 1)) == 0 && ((uintptr_t)tgt & 3u) == 0,
@@ -1072,7 +1075,7 @@ struct Call {
 using namespace gn;
 
 extern "C" size_t gn_linear_xent_workspace_bytes(int T, int d, int V, int dtype) {
-    if (T <= 0 || d <= 0 || V <= 0 || (dtype != GN_F32 && dtype != GN_BF16)) return 0;
+    if (T <= 0 || d <= 0 || V <= 0 || !within(T, d, V) || (dtype != GN_F32 && dtype != GN_BF16)) return 0;
     return workspace_bytes(T, d, V, dtype);
 }
 

@@ -320,6 +320,7 @@ int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* targets, con
                        const float* dloss, const float* dlse, float scale, void* dh, void* dE,
                        int dE_dtype, int T, int d, int V, int dtype, unsigned flags, void* ws,
                        size_t ws_bytes, void* stream);
+/* 0 for sizes that the calls refuse. */
 size_t gn_linear_xent_workspace_bytes(int T, int d, int V, int dtype);
 
 /* ---- rotary positions, per-head norms of queries and keys --------------------------------- */

@@ -206,3 +206,14 @@ def test_sizes_past_31_bits():
         gn._int32("x", torch.zeros(1, 1, 1, 2).expand(n, 1, 1, 2))
     with pytest.raises(gn.GnError, match="64 bits"):
         gn._rope(torch.ones(4, dtype=torch.float64), "half", None, 2 ** 64 + 5, 1.0, 1, 1)
+
+
+@pytest.mark.parametrize("dtype", [0, 4])
+def test_workspace_query_of_refused_sizes(dtype):
+    """0, as for other sizes that are not taken (rounding 2^31 - 1 up overflowed)."""
+    top = 2 ** 31 - 1
+    for size in ((top, 8, 8), (8, top, 8), (8, 8, top), (1 << 28, 8, 8), (8, (1 << 20) + 1, 8), (8, 8, 1 << 30),
+                 (1 << 23, 8, 1 << 20)):
+        assert gn.lib().gn_linear_xent_workspace_bytes(*size, dtype) == 0
+    assert gn.lib().gn_linear_xent_workspace_bytes((1 << 28) - 1, 8, 100, dtype) > 0
+    assert gn.lib().gn_linear_xent_workspace_bytes(8, 1 << 20, (1 << 30) - 1, dtype) > 0
