@@ -919,7 +919,8 @@ def _xent_args(h, E, targets, ws):
 def linear_xent_fwd(h, E, targets, ws=None):
     """(loss, lse), fp32 [T], of logits h E^T that are never stored: h [T, d], E [V, d] (f32 or
     bf16), targets int32 [T]; a target outside [0, V) (-100, say) marks a row without one, whose
-    loss is 0.  ws: linear_xent_workspace_bytes(T, d, V, dtype), allocated here when None."""
+    loss is 0 (its h is read all the same and has to be finite).  ws:
+    linear_xent_workspace_bytes(T, d, V, dtype), allocated here when None."""
     args, T, d, V, dt, ws = _xent_args(h, E, targets, ws)
     loss = torch.empty((T,), dtype=torch.float32, device=h.device)
     lse = torch.empty((T,), dtype=torch.float32, device=h.device)
@@ -954,7 +955,8 @@ def linear_xent_bwd(h, E, targets, lse, dloss=None, dlse=None, scale=1.0, need_d
 def rope_freqs(rot, theta=10000.0, scaling="none", factor=1.0, trained=4096, fast=32.0, slow=1.0, device="cuda:0"):
     """(freqs, mscale) for rope_fwd and qk_norm_rope_fwd: an fp64 tensor [rot / 2] of radians per
     position, kept by the caller, and the factor on cos and sin.  scaling stretches a context of
-    `trained` positions `factor` times: "linear", "ntk" or "yarn" (with its fast and slow bounds)."""
+    `trained` positions `factor` times: "linear", "ntk" or "yarn" (its ramp between the fast and slow bounds
+    is over a pair's turns; a model trained with a ramp over the pairs' index brings its own table)."""
     f = (ctypes.c_double * max(1, rot // 2))()
     m = ctypes.c_float()
     _check(lib().gn_rope_freqs(rot, theta, ROPE_SCALE[scaling], factor, trained, fast, slow,

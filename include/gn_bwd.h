@@ -299,7 +299,8 @@ int gn_xent_bwd(const void* logits, const int32_t* targets, void* dLogits, int r
  *   lse[t] = log sum_v exp l[t, v],  loss[t] = lse[t] - l[t, targets[t]]
  * h [T x d], E [V x d] in dtype; targets int32 [T]; loss, lse fp32 [T] (each may be NULL).  Outputs and the
  * workspace, here and in the backward, may share memory with nothing else of the call.  A target
- * outside [0, V) (-100, say) marks a row without one: loss 0, and no gradient from dloss.
+ * outside [0, V) (-100, say) marks a row without one: loss 0, and no gradient from dloss.  Such a row of h
+ * is read like the others: an inf or NaN in it (padding that was never written) reaches dE.
  * The logits exist a tile or a piece of the vocabulary at a time, in fp32.  T below 2^28, d up to
  * 2^20, V below 2^30, T * V below 2^43, T * V * d below 2^58.
  * ws: gn_linear_xent_workspace_bytes(T, d, V, dtype), 16-byte aligned. */
@@ -314,7 +315,8 @@ int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* targets, flo
  *   gradient, micro-batches), dh is overwritten.
  * A piece of the vocabulary at a time, its logits formed again.  On the bf16 path G enters a bf16 dE and,
  * but for its element at the target (fp32), dh rounded to bf16; an fp32 dE takes it as three bf16
- * pieces, of more than 4096 rows as two (2^-17 of each element).  Every sum's order is fixed: the same
+ * pieces, of more than 4096 rows as two (2^-17 of each element; the elements at the targets whole up to
+ * 16384 rows).  Every sum's order is fixed: the same
  * bits every time.  ws as for the forward. */
 int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* targets, const float* lse,
                        const float* dloss, const float* dlse, float scale, void* dh, void* dE,
@@ -359,12 +361,14 @@ typedef struct gn_rope {
 #define GN_ROPE_SCALE_LINEAR 1 /* positions divided by factor */
 #define GN_ROPE_SCALE_NTK 2    /* theta * factor^(rot/(rot-2)): the slowest pair slows by factor */
 #define GN_ROPE_SCALE_YARN 3   /* pairs that turn often within `trained` positions keep their frequency,
-                                  slow ones are divided by factor, a linear ramp between */
+                                  slow ones are divided by factor, a ramp linear in the turns between */
 /* freqs[i], i < rot/2, into host memory: theta^(-2i/rot), scaled for a context `factor` (>= 1) times
  * the `trained` positions.  YARN: a pair that turns r times within `trained` positions keeps
  * clamp((r - slow) / (fast - slow), 0, 1) of its own frequency (usual fast 32, slow 1), and
- * *mscale = 0.1 ln(factor) + 1; otherwise *mscale = 1.  trained, fast and slow are read by YARN
- * only. */
+ * *mscale = 0.1 ln(factor) + 1; otherwise *mscale = 1.  (Models are also trained with a ramp over the pairs'
+ * index between the two bounds, with other frequencies in between: of rot 128, theta 10000, 4096 trained,
+ * factor 32, pair 33 keeps 0.18 of its frequency here and 0.52 there.  Such frequencies are the caller's own
+ * table.)  trained, fast and slow are read by YARN only. */
 int gn_rope_freqs(int rot, double theta, int scaling, double factor, double trained, double fast,
                   double slow, double* freqs, float* mscale);
 
