@@ -10,22 +10,28 @@
 //              dh += G E_c (fp32) from it
 // A lane holds 16 columns of one row of each 32 x 32 accumulator, so the row statistics take one
 // exchange between lanes.  For an fp32 dE, G is stored as two or three bf16 pieces, whose products with h
-// are one product's longer k: two leave 2^-17 of an element (and target_rest takes the targets' rest),
-// three nothing that fp32 holds, where bf16 alone (2^-8) would be the gradient's largest error.  For dh the
-// first piece is enough but at the target: there the rounding of a row's largest element, which shows in
-// all of dh's row, is kept in fp32 and its product with E[target] added when dh is rounded (dh_finish).
+// are one product's longer k: two leave 2^-17 of an element (and up to 16384 rows target_rest takes the
+// targets' rest), three nothing that fp32 holds, where bf16 alone (2^-8) would be the gradient's largest
+// error.  For dh the first piece is enough but at the target: there the rounding of a row's largest
+// element, which shows in all of dh's row, is kept in fp32 and its product with E[target] added when dh is
+// rounded (dh_finish); dh is then off from fp64 by 1.7e-3 of its norm, what its own rounding leaves.  A
+// bf16 dE takes the first piece: a row of few targets has G's rounding beside its own, 2.3e-3 for 1.7e-3 at
+// 2001 x 1024 x 50001, and a second piece would be a product more (8190 x 768 x 32000: dE in bf16 824 us, in
+// fp32 from two pieces 1407).
 //
 // fp32.  The pieces' logits are stored (fp32, in the workspace) between the library's fp32 products
 // and row kernels, G in their place.
 //
-// Measured (rows x d x vocabulary): forward and both gradients of 8192 x 2048 x 128000 18.8 ms, of 8190 x
-// 768 x 32000 2.2 ms: five products where the formulas have three (the logits again, dE's second piece), 21.5
-// and 2.0 TFLOP at 1.14 and 0.92 PFLOP/s.  The matrix cores bound them, and on them the clock: the logits
-// with their statistics take 3.4-3.6 ms at 67 % of the matrix pipe and 1.65-1.75 GHz, the library's product
-// alone 3.3-3.9 at 76 % and 1.53.  256 x 256 tiles of four waves that issue their own loads took 2 % off
-// the larger and put 6 % onto smaller ones; staggered starts of the blocks gave nothing.  Few rows are a read
-// of E: 16 x 2048 x 32000 forward 26 us + 4 for 131 MB (5.0 TB/s).  fp32 of 1003 x 768 x 32000: 1.15-1.3 ms,
-// four products, 0.197 TFLOP at six bf16 ones each, 0.9-1.0 PFLOP/s of those.
+// Measured (rows x d x vocabulary): forward and both gradients of 8192 x 2048 x 128000 18.9-19.1 ms, of 8190 x
+// 768 x 32000 2.26-2.30 ms: five products where the formulas have three (the logits again, dE's second
+// piece), 21.5 and 2.0 TFLOP at 1.13 and 0.88 PFLOP/s.  At d = 2048 the matrix cores bound them, and on them
+// the clock: the logits with their statistics take 3.5-3.8 ms, 74 % of the matrix pipe at 1.5 GHz, the
+// library's product alone 3.5-4.1, 77 % at 1.4.  At d = 768 the epilogues do: the four compute waves run
+// them between tiles of twelve k-tiles, the pipe is busy for 54 % of the forward and 26 % of G's pieces.
+// 256 x 256 tiles of four waves that issue their own loads took 2 % off the larger and put 6 % onto smaller
+// ones; staggered starts of the blocks gave nothing.  Few rows are a read of E: 16 x 2048 x 32000 forward
+// 26 us + 4 for 131 MB (5.0 TB/s).  fp32 of 1003 x 768 x 32000: 1.14-1.17 ms, four products, 0.197 TFLOP at
+// six bf16 ones each, 1.0 PFLOP/s of those.
 //
 // Widths, row counts and vocabularies that the products' vectors do not divide: h and E's piece are
 // laid out to multiples of q = 8 (bf16) or 4 (fp32) elements first; the last V % q columns go
@@ -140,7 +146,8 @@ typedef float4 RowScale;
 
 // G of the tile, as P bf16 pieces; columns from N up to ld are zeros.  G and then what a piece left of it
 // stay in the accumulators, and the next tile's fragments are read again after the epilogue of several
-// pieces: 44 registers spilled otherwise (dE of 8190 x 768 x 32000, two pieces, 1.58 -> 1.45 ms).
+// pieces: held through it they make the compiler spill 22 registers for 2 (dE of 8190 x 768 x 32000, two pieces,
+// 1428 -> 1406 us; of 2001 x 1024 x 50001, three, 941 -> 902).
 template <int P>
 struct GradTile {
     static constexpr bool kAgain = P > 1;
@@ -476,7 +483,8 @@ __device__ __forceinline__ void finish_row(int t, float m, float s, const int32_
 }
 
 // lse and loss from the strips' statistics: R rows x 256 / R slices of the strips a block.  2 below 256 rows
-// (500 strips of 16 rows: 3.8 us, with 16 5.5), 16 from there on (782 strips of 2001 rows: 9.5 us, with 2 16).
+// (whole forwards of 16 rows: the 256 strips that logits_few leaves at d = 2048 29.8 us, with 16 30.1; the 500 of
+// the tiles at d = 4096 43.6 and 44.7), 16 from there on (782 strips of 2001 rows: 9.5 us, with 2 16).
 template <int R>
 __global__ __launch_bounds__(256) void row_stats(const float2* __restrict__ part, int strips, int T,
                                                  const int32_t* __restrict__ tgt, const float* __restrict__ lt,

@@ -19,9 +19,12 @@
 // 61.8 us (4.97 TB/s), fp32 of 49 MB 10.3 us (4.8); norms, rotation and head split of 403 MB 78.0 us
 // (5.2); their backward, which reads x again, 570 MB 126 us (4.5: two dependent row sums between a row's
 // loads and its stores, and three waves a SIMD, no more, hold two rows each); both 206 us.  Stores past the
-// caches take 17 us off the two and add 10 to them with a reader behind, so they are ordinary ones.  A token
-// a sequence: 3.4 us of kernel,
-// under the call's host time of 8.7.  16-byte pieces against elements: bf16 rotation of 4 x 4096 x 32
+// caches take 17 us off the two and add 10 to them with a reader behind, so they are ordinary ones.  fp32: norms,
+// rotation and head split of 805 MB 171 us (4.7), their backward 244.  A token a sequence: 3.4 us of kernel,
+// 5.3 with the norms, under the calls' host time of 8.7 and 21.7.  Few tokens: the backward of 3 x 777 tokens
+// (8 + 2 heads of 96, fp32, 30 MB) 20 us of kernel, a tile being two tokens there (tile()): 16 rows of q and 4 of k
+// for a block's 32 lane groups.  dw is summed in fp32 (a lane's rows, the lane groups, the blocks, in that
+// order): 2e-7 of its norm off there, where sums in fp64 leave 7e-8.  16-byte pieces against elements: bf16 rotation of 4 x 4096 x 32
 // heads, 128 wide 42.7 and 92.4 us, 64 wide 22.0 and 75.8; fp32 102 and 106, 48 and 84.
 #include <algorithm>
 #include <cmath>
@@ -62,7 +65,7 @@ struct Args {
     int accumulate;
 };
 
-// 16 / sizeof elements of one access
+// A lane's part of a row of D elements
 template <typename T, int LPR, bool VEC, bool HALF>
 struct Row {
     static constexpr int NP = VEC ? 8 : 4;          // pairs of a lane
