@@ -522,7 +522,7 @@ def attn_workspace_bytes(B, H, S, D, dtype=None):
 def _attn_like(Q, **others):
     """The kernels read and write every tensor by Q's type and size."""
     for name, t in others.items():
-        if t is not None and (t.dtype is not Q.dtype or t.shape != Q.shape):
+        if t is not None and (t.dtype is not Q.dtype or t.numel() != Q.numel()):
             raise GnError(f"{name} {list(t.shape)} {t.dtype} must be as Q, {list(Q.shape)} {Q.dtype}"
                           + (" (fewer key and value heads are repeated first)" if name in "KV" else ""))
 
