@@ -94,9 +94,12 @@ def cross_entropy_params(scale: float = 1.0) -> bytes:
 
 
 def rope_params(heads: int, rot: int, mode: str = "half", mscale: float = 1.0, positions_per_row: bool = False,
-                pos0: int = 0, kv_heads: int = 0, eps: float = 0.0) -> bytes:
+                pos0: int = 0, kv_heads: int = 0, eps: float | None = None) -> bytes:
     """Rope node: x [B, S, heads*D]; saved slots {freqs, positions (0: pos0, pos0 + 1, ...)}.
-    positions_per_row: positions are [B, S], else [S]."""
+    positions_per_row: positions are [B, S], else [S].  eps belongs to a QkNormRope node, which has
+    kv_heads (None: its 1e-6; a Rope node has none)."""
+    if eps is None:
+        eps = 1e-6 if kv_heads else 0.0
     return struct.pack("<IIIIffIi", heads, kv_heads, rot, ROPE_MODE[mode], mscale, eps, int(positions_per_row), pos0)
 
 

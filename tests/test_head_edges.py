@@ -217,3 +217,15 @@ def test_workspace_query_of_refused_sizes(dtype):
         assert gn.lib().gn_linear_xent_workspace_bytes(*size, dtype) == 0
     assert gn.lib().gn_linear_xent_workspace_bytes((1 << 28) - 1, 8, 100, dtype) > 0
     assert gn.lib().gn_linear_xent_workspace_bytes(8, 1 << 20, (1 << 30) - 1, dtype) > 0
+
+
+def test_default_eps_of_the_parameter_blocks():
+    """1e-6 where the block has key and value heads, whichever helper packs it; a given 0 stays 0."""
+    import struct
+    pytest.importorskip("grilly_core")
+    import grilly_bridge as gb
+    eps = lambda block: struct.unpack("<IIIIffIi", block)[5]
+    want = struct.unpack("<f", struct.pack("<f", 1e-6))[0]
+    assert eps(gb.rope_params(4, 64, kv_heads=2)) == eps(gb.qk_norm_rope_params(4, 2, 64)) == want
+    assert eps(gb.rope_params(4, 64, kv_heads=2, eps=0.0)) == eps(gb.qk_norm_rope_params(4, 2, 64, eps=0.0)) == 0
+    assert eps(gb.rope_params(4, 64)) == 0
