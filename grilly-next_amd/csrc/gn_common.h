@@ -168,6 +168,10 @@ inline unsigned grid_for(int64_t n, int per_block, unsigned cap = 65535u * 16u) 
     return (unsigned)g;
 }
 
+// Whether a launch may have that many blocks in one dimension: its threads there are counted in 32 bits, and
+// past them the grid wraps around without an error.
+inline bool grid_fits(int64_t blocks, int threads) { return blocks * threads < (1ll << 32); }
+
 // Zero `bytes` bytes at p with a fill kernel (gn_elementwise.hip).  The library clears memory
 // this way, never with hipMemsetAsync, so that every entry point records only kernel nodes
 // when a caller captures it into a HIP graph.

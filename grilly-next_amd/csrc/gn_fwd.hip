@@ -127,6 +127,7 @@ int norm_fwd(const void* X, const void* gamma, const void* beta, void* Y, float*
              float* stat, int rows, int F, float eps, int save_var, hipStream_t s) {
     const bool vec_ok = F % 8 == 0 && F <= 2048 && al16(X) && al16(Y) && (!gamma || al16(gamma)) &&
                         (!beta || al16(beta));
+    GN_REQUIRE(grid_fits(rows + (int64_t)kFwdWaves, vec_ok ? 64 : 256), "norm forward: %d rows are more than a launch takes", rows);
     const TX* x = (const TX*)X;
     const TY* g = (const TY*)gamma;
     const TY* b = (const TY*)beta;

@@ -363,6 +363,8 @@ int norm_bwd(const void* dY, const void* X, const void* gamma, const float* mean
     const bool vec_ok = (F % 8 == 0) && F <= 2048 && aligned16(dY) && aligned16(X) &&
                         aligned16(dX) && aligned16(gamma) && (!add || aligned16(add));
     const bool need_param = dA || dB;
+    GN_REQUIRE((vec_ok && need_param) || !dX || grid_fits(rows, 256),
+               "norm backward: %d rows are more than a launch of this form takes", rows);
     const TX* ad = (const TX*)add;
     if (partials_only && !(vec_ok && need_param)) {
         set_error("norm backward: GN_NORM_PARTIALS needs the row kernel (F %% 8 == 0, F <= 2048, "
@@ -753,6 +755,7 @@ extern "C" int gn_softmax_bwd(const void* dY, const void* Y, void* dX, int rows,
     GN_REQUIRE(rows >= 0 && C > 0, "gn_softmax_bwd: bad shape");
     if (rows == 0) return GN_OK;
     GN_REQUIRE(dY && Y && dX, "gn_softmax_bwd: null pointer");
+    GN_REQUIRE(grid_fits(rows, 256), "gn_softmax_bwd: %d rows are more than a launch takes", rows);
     hipStream_t s = as_stream(stream);
     if (dtype == GN_F32)
         softmax_bwd_kernel<float><<<rows, 256, 0, s>>>((const float*)dY, (const float*)Y, (float*)dX, C);
@@ -772,6 +775,7 @@ extern "C" int gn_xent_bwd(const void* logits, const int32_t* targets, void* dLo
     GN_REQUIRE(rows >= 0 && C > 0, "gn_xent_bwd: bad shape");
     if (rows == 0) return GN_OK;
     GN_REQUIRE(logits && targets && dLogits, "gn_xent_bwd: null pointer");
+    GN_REQUIRE(grid_fits(rows, 256), "gn_xent_bwd: %d rows are more than a launch takes", rows);
     hipStream_t s = as_stream(stream);
     if (dtype == GN_F32)
         xent_bwd_kernel<float><<<rows, 256, 0, s>>>((const float*)logits, targets, (float*)dLogits, C, scale);

@@ -284,6 +284,8 @@ int gn_rmsnorm_bwd_stat(const void* dY, int dy_dtype, const void* X, int x_dtype
                         void* stream);
 
 /* ---- softmax / cross-entropy --------------------------------------------------------- */
+/* A block a row: fewer than 2^24 rows (as the norms' passes of widths that are no multiple of 8 or above
+ * 2048, of unaligned tensors and of dX alone; more rows than a launch takes are GN_E_INVALID). */
 /* activation-softmax-backward.glsl:27-49: dX = Y * (dY - sum_c dY*Y), per row of C. */
 int gn_softmax_bwd(const void* dY, const void* Y, void* dX, int rows, int C, int dtype,
                    void* stream);

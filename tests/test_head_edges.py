@@ -229,3 +229,17 @@ def test_default_eps_of_the_parameter_blocks():
     assert eps(gb.rope_params(4, 64, kv_heads=2)) == eps(gb.qk_norm_rope_params(4, 2, 64)) == want
     assert eps(gb.rope_params(4, 64, kv_heads=2, eps=0.0)) == eps(gb.qk_norm_rope_params(4, 2, 64, eps=0.0)) == 0
     assert eps(gb.rope_params(4, 64)) == 0
+
+
+def test_rows_past_a_launch():
+    """A block of 256 threads a row: from 2^24 rows on the grid would wrap around without an error."""
+    lib = gn.lib()
+    n = 1 << 24
+    a, b, c, w = p(), p(1 << 40), p(2 << 40), p(3 << 40)
+    for dtype in (0, 4):
+        refused(lib.gn_softmax_bwd(a, b, c, n, 8, dtype, None), "rows")
+        refused(lib.gn_xent_bwd(a, w, c, n, 8, 1.0, dtype, None), "rows")
+        refused(lib.gn_layernorm_fwd(a, None, None, b, None, None, n, 12, 1e-5, dtype, 0, None), "rows")
+        refused(lib.gn_rmsnorm_fwd(a, None, b, None, 1 << 26, 64, 1e-6, dtype, None), "rows")  # a wave a row
+        refused(lib.gn_rmsnorm_bwd(a, b, w, w, c, None, n, 64, dtype, 0, None, 0, None), "rows")      # dX alone
+        refused(lib.gn_rmsnorm_bwd(a, b, w, w, c, w, n, 12, dtype, 0, None, 0, None), "rows")
