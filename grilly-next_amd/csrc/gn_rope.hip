@@ -441,8 +441,9 @@ __global__ __launch_bounds__(kThreads, 3) void norm_bwd_kernel(Args a) {
     float du[NP], dv[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i) du[i] = dv[i] = 0.f;
-    for (int tile = first; tile < a.tiles[k]; tile += step) {
-        const int t0 = tile * TB, n = min(TB, a.tokens - t0);
+    // unsigned: near 2^31 tiles the step past the last one is no int
+    for (unsigned tile = first; tile < (unsigned)a.tiles[k]; tile += step) {
+        const int t0 = (int)tile * TB, n = min(TB, a.tokens - t0);
         __syncthreads();  // the tile before has been read
         tile_angles(a, t0, n, cosv, sinv, bs);
         if (a.g[k].H) group_bwd<T, LPR, VEC, HALF>(a, a.g[k], n, cosv, sinv, bs, row, du, dv);
