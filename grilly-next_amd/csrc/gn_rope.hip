@@ -25,7 +25,9 @@
 // (8 + 2 heads of 96, fp32, 30 MB) 20 us of kernel, a tile being two tokens there (tile()): 16 rows of q and 4 of k
 // for a block's 32 lane groups.  dw is summed in fp32 (a lane's rows, the lane groups, the blocks, in that
 // order): 2e-7 of its norm off there, where sums in fp64 leave 7e-8.  16-byte pieces against elements: bf16 rotation of 4 x 4096 x 32
-// heads, 128 wide 42.7 and 92.4 us, 64 wide 22.0 and 75.8; fp32 102 and 106, 48 and 84.
+// heads, 128 wide 42.7 and 92.4 us, 64 wide 22.0 and 75.8; fp32 102 and 106, 48 and 84.  (A pair's second half
+// starts at rot / 2, and what is behind the rotation splits in two: pieces of eight elements need multiples of
+// 16.  Pieces of 8 bytes for multiples of 8 are not built.)
 #include <algorithm>
 #include <cmath>
 
