@@ -15,9 +15,8 @@
 // error.  For dh the first piece is enough but at the target: there the rounding of a row's largest
 // element, which shows in all of dh's row, is kept in fp32 and its product with E[target] added when dh is
 // rounded (dh_finish); dh is then off from fp64 by 1.7e-3 of its norm, what its own rounding leaves.  A
-// bf16 dE takes the first piece: a row of few targets has G's rounding beside its own, 2.3e-3 for 1.7e-3 at
-// 2001 x 1024 x 50001, and a second piece would be a product more (8190 x 768 x 32000: dE in bf16 824 us, in
-// fp32 from two pieces 1407).
+// bf16 dE takes two pieces up to 512 rows and the first alone above, where a second would be half a product
+// more for G's rounding beside dE's own (kWholeBf16).
 //
 // fp32.  The pieces' logits are stored (fp32, in the workspace) between the library's fp32 products
 // and row kernels, G in their place.
@@ -964,6 +963,13 @@ struct Plan {
     // rows target_rest makes the target elements whole; its reading grows with the square of the rows, and
     // beyond sqrt(16384) 2^-24 = 2^-17.
     static constexpr int kTwoPieces = 4096, kTargets = 16384;
+    // Rows up to which a bf16 dE takes two pieces.  Its norm lies in the targets' rows, each of them G's element
+    // at the target, with its rounding, times a row of h: of few rows the error is up to twice what dE's own
+    // rounding leaves (16 x 768 x 32000 3.4e-3 for 1.66e-3, 256 x 768 2.9e-3, 512 x 2048 2.6e-3), of many it
+    // is about sqrt 2 times that (2001 x 1024 x 50001 2.25e-3).  Both gradients, one piece and two, us: 16 x 2048 x 32000
+    // 98 and 102, 64 107 and 118, 128 126 and 146, 512 224 and 287; 2001 x 1024 x 50001 688 and 905, 8190 x 768 x
+    // 32000 1210 and 1812.
+    static constexpr int kWholeBf16 = 512;
     static constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 };
 
@@ -1168,24 +1174,24 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
     char* const base = (char*)ws;
     Call c{who, w, base, h, E, s, dtype};
     if (const int rc = c.start()) return rc;
-    const int planes = w.bf && dE && dE_dtype == GN_F32 ? w.planes : 1;
+    const int planes = !w.bf || !dE ? 1 : dE_dtype == GN_F32 ? w.planes : T <= Plan::kWholeBf16 ? 2 : 1;
+    const bool stacked = planes > 1 && T <= Plan::kTwoPieces;  // pieces under each other beside h as often
     const size_t plane = (size_t)T * w.vc;
     RowScale* const rows = (RowScale*)(base + w.rows);
     float* const resid = (float*)(base + w.resid);
     char* const G = base + (w.bf ? w.G : w.logits);
-    if (planes == 3) {  // three pieces are one k-segment of 3 T rows beside h three times
-        if (const int rc = c.copy(h, w.hs, T, T, 3)) return rc;
+    if (stacked) {  // one k-segment of planes T rows
+        if (const int rc = c.copy(h, w.hs, T, T, planes)) return rc;
     }
     row_scales<<<(w.Tp + 255) / 256, 256, 0, s>>>(rows, resid, T, w.Tp, targets, lse, dloss, dlse, scale, V);
     GN_LAUNCH_CHECK(who);
     // dst (+)= G's columns c0 .. c0 + M, transposed, times h: fp32 or in dE's own type
     auto weight = [&](int c0, int M, void* dst, int c_dtype, bool add) {
         GemmDesc g = product(G + (size_t)c0 * w.es, w.vc, c.hp, w.dp, w.Tp, dst, w.dp, M, w.dp);
-        if (planes == 3) {
+        if (stacked) {
             g.B[0] = (const bf16_t*)(base + w.hs);
-            g.Ks[0] = 3 * T;
-        }
-        if (planes == 2) {
+            g.Ks[0] = planes * T;
+        } else if (planes == 2) {
             g.nseg = 2;
             g.A[1] = (const bf16_t*)G + plane + c0;
             g.lda[1] = w.vc;
@@ -1217,9 +1223,7 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
             auto logits = [&](auto P_) {
                 constexpr int P = decltype(P_)::value;
                 bf16_t* const Gp = (bf16_t*)G;
-                if constexpr (P != 2) {  // two pieces: of many rows
-                    if (few_takes(g)) return launch_few(g, GradFew<P>{rows, Gp, plane, resid, w.vc, v0}, s);
-                }
+                if (few_takes(g)) return launch_few(g, GradFew<P>{rows, Gp, plane, resid, w.vc, v0}, s);
                 return launch_logits(g, GradTile<P>{rows, Gp, plane, resid, w.vc, v0}, s);
             };
             const int rc = planes == 3   ? logits(std::integral_constant<int, 3>{})
@@ -1257,7 +1261,7 @@ extern "C" int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* t
             if (const int rc = gemm_run(g, 0, 0, dtype, GN_F32, s)) return rc;
         }
     }
-    if (planes == 2 && T <= Plan::kTargets) {
+    if (planes == 2 && !stacked && T <= Plan::kTargets) {
         const auto rest = d % 8 == 0 && al16(h) && al16(dE) ? target_rest<true> : target_rest<false>;
         rest<<<T, 256, 0, s>>>(targets, resid, (const bf16_t*)h, (float*)dE, T, d, V);
         GN_LAUNCH_CHECK(who);

@@ -315,9 +315,9 @@ int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* targets, flo
  *   dh = G E [T x d] in dtype,  dE (+)= G^T h [V x d] in dE_dtype (GN_F32, or GN_BF16 on the bf16
  *   path).  dh or dE may be NULL; GN_ACCUMULATE adds onto an fp32 dE (a tied embedding's
  *   gradient, micro-batches), dh is overwritten.
- * A piece of the vocabulary at a time, its logits formed again.  On the bf16 path G enters a bf16 dE and,
- * but for its element at the target (fp32), dh rounded to bf16; an fp32 dE takes it as three bf16
- * pieces, of more than 4096 rows as two (2^-17 of each element; the elements at the targets whole up to
+ * A piece of the vocabulary at a time, its logits formed again.  On the bf16 path G enters a bf16 dE of more
+ * than 512 rows and, but for its element at the target (fp32), dh rounded to bf16; a bf16 dE of fewer rows
+ * takes it as two bf16 pieces, an fp32 dE as three, of more than 4096 rows as two (2^-17 of each element; the elements at the targets whole up to
  * 16384 rows).  Every sum's order is fixed: the same
  * bits every time.  ws as for the forward. */
 int gn_linear_xent_bwd(const void* h, const void* E, const int32_t* targets, const float* lse,

@@ -374,3 +374,29 @@ def test_three_pieces_of_few_rows(gn, T, d):
     first = G.float().bfloat16().double()
     two = first + (G - first).float().bfloat16().double()
     assert bool(((two.t() @ x - ref).abs() > bound).any())
+
+
+@pytest.mark.parametrize("T,d", [(1, 256), (16, 256), (20, 512), (32, 2048), (16, 77), (64, 64), (128, 1024), (300, 72),
+                                 (300, 33), (512, 264)])
+def test_bf16_dE_of_few_rows_is_rounded_once(gn, T, d):
+    """Up to 512 rows a bf16 dE takes two pieces of G: its own rounding (2^-8 of the value), and besides it
+    2^-16 of G, p's 2^-20 and fp32 sums.  Equal logits, five rows with a weight.  One piece does not pass."""
+    g = gen(T + d)
+    V = 512
+    h, E = rand(g, T, d), torch.zeros(V, d, device=DEV, dtype=BF)
+    t = torch.randint(0, V, (T,), device=DEV, generator=g).to(torch.int32)
+    at = torch.tensor(sorted({0, T // 3, T // 2, (3 * T) // 4, T - 1}), device=DEV)
+    u = torch.zeros(T, device=DEV)
+    u[at] = torch.rand(len(at), device=DEV, generator=g) + 0.1
+    lse = gn.linear_xent_fwd(h, E, t)[1]
+    dh, dE = gn.linear_xent_bwd(h, E, t, lse, dloss=u, dE_dtype=BF)
+    assert torch.equal(dh, gn.linear_xent_bwd(h, E, t, lse, dloss=u, need_dE=False)[0])
+    p = (u[at].double() / V)[:, None].expand(len(at), V)
+    G = p.clone()
+    G[torch.arange(len(at)), t[at].long()] -= u[at].double()
+    x = h[at].double()
+    ref = G.t() @ x
+    bound = (p * 2.0 ** -20 + G.abs() * 2.0 ** -16).t() @ x.abs() * (1 + 2.0 ** -8) + 2.0 ** -8 * ref.abs() + 1e-30
+    assert bool(((dE.double() - ref).abs() <= bound).all())
+    one = (G.float().bfloat16().double().t() @ x).float().bfloat16().double()
+    assert bool(((one - ref).abs() > bound).any())
