@@ -315,6 +315,8 @@ int gn_linear_xent_fwd(const void* h, const void* E, const int32_t* targets, flo
  *   dh = G E [T x d] in dtype,  dE (+)= G^T h [V x d] in dE_dtype (GN_F32, or GN_BF16 on the bf16
  *   path).  dh or dE may be NULL; GN_ACCUMULATE adds onto an fp32 dE (a tied embedding's
  *   gradient, micro-batches), dh is overwritten.
+ * p comes from lse as fp32 holds it, up to half a step off (2^-21 of p where lse is 8 to 16): it shows in a row certain
+ * of its target, where G is the small difference p - 1.
  * A piece of the vocabulary at a time, its logits formed again.  On the bf16 path G enters a bf16 dE of more
  * than 512 rows and, but for its element at the target (fp32), dh rounded to bf16; a bf16 dE of fewer rows
  * takes it as two bf16 pieces, an fp32 dE as three, of more than 4096 rows as two (2^-17 of each element; the elements at the targets whole up to
