@@ -25,6 +25,7 @@ ACT = {"relu": 0, "gelu_tanh": 1, "gelu_erf": 2, "silu": 3, "tanh": 4, "sigmoid"
 GLU = {"swiglu_up": 0, "swiglu_gate": 1, "geglu_up": 2, "geglu_gate": 3, "reglu_up": 4}
 ROPE = {"none": 0, "interleaved": 1, "half": 2}
 ROPE_SCALE = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+NORM = {"none": 0, "rms": 1, "layer": 2}
 
 # exported symbols, in the order include/gn_bwd.h declares them
 SYMBOLS = [
@@ -44,6 +45,7 @@ SYMBOLS = [
     "gn_rmsnorm_fwd", "gn_layernorm_fwd_ex", "gn_rmsnorm_fwd_ex", "gn_rmsnorm_fwd_stat", "gn_act_fwd", "gn_glu_fwd", "gn_linear_fwd", "gn_glu_linear_fwd", "gn_add_inplace", "gn_convert", "gn_zero",
     "gn_linear_xent_fwd", "gn_linear_xent_bwd", "gn_linear_xent_workspace_bytes", "gn_rope_freqs", "gn_rope_fwd",
     "gn_rope_bwd", "gn_qk_norm_rope_fwd", "gn_qk_norm_rope_bwd", "gn_qk_norm_rope_workspace_bytes",
+    "gn_dropout_fwd", "gn_dropout_bwd", "gn_residual_norm_fwd", "gn_residual_norm_bwd", "gn_residual_norm_workspace_bytes",
 ]
 BIN = {"sub": 0, "mul": 1, "div": 2, "neg": 3}
 RED = {"sum": 0, "mean": 1}
@@ -85,6 +87,27 @@ class Rope(ctypes.Structure):
                 ("mode", ctypes.c_int)]
 
 
+class Rng(ctypes.Structure):
+    """gn_rng (include/gn_bwd.h): where a dropout's masks come from."""
+    _fields_ = [("seed", ctypes.c_uint64), ("stream", ctypes.c_uint64), ("step", ctypes.c_uint64),
+                ("step_dev", ctypes.c_void_p)]
+
+
+class Branch(ctypes.Structure):
+    """gn_branch (include/gn_bwd.h): the norms, gate, scales and dropout of a block's residual branch."""
+    _fields_ = [("post", ctypes.c_int), ("pre", ctypes.c_int), ("post_w", ctypes.c_void_p), ("post_b", ctypes.c_void_p),
+                ("pre_w", ctypes.c_void_p), ("pre_b", ctypes.c_void_p), ("post_eps", ctypes.c_float),
+                ("pre_eps", ctypes.c_float), ("gate", ctypes.c_void_p), ("gates", ctypes.c_int),
+                ("scale", ctypes.c_float), ("res_scale", ctypes.c_float), ("p", ctypes.c_double), ("rng", Rng)]
+
+
+class BranchGrads(ctypes.Structure):
+    """gn_branch_grads (include/gn_bwd.h)."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b")]
+
+
+_RNGP = ctypes.POINTER(Rng)
+_BRANCHP = ctypes.POINTER(Branch)
 _HEADSP = ctypes.POINTER(Heads)
 _ROPEP = ctypes.POINTER(Rope)
 _D = ctypes.c_double
@@ -176,6 +199,12 @@ _SIGS = {
     "gn_qk_norm_rope_bwd": ([_HEADSP, _HEADSP, _HEADSP, _HEADSP, _HEADSP, _P, _P, _HEADSP, _HEADSP, _HEADSP, _P, _P,
                              _ROPEP, _I, _I, _I, _F, _I, _U, _P, _Z, _P], _I),
     "gn_qk_norm_rope_workspace_bytes": ([_I, _I, _I], _Z),
+    "gn_dropout_fwd": ([_P, _P, _L, _D, _RNGP, _I, _P], _I),
+    "gn_dropout_bwd": ([_P, _P, _L, _D, _RNGP, _I, _U, _P], _I),
+    "gn_residual_norm_fwd": ([_BRANCHP, _P, _I, _P, _I, _P, _P, _I, _I, _P], _I),
+    "gn_residual_norm_bwd": ([_BRANCHP, _P, _P, _P, _I, _P, _I, _P, _P, ctypes.POINTER(BranchGrads), _I, _I, _U, _P, _Z,
+                              _P], _I),
+    "gn_residual_norm_workspace_bytes": ([_I, _I, _I], _Z),
 }
 
 
@@ -1108,6 +1137,137 @@ def qk_norm_rope_bwd(dyq, dyk, q, k, wq=None, wk=None, freqs=None, dyv=None, mod
                                      _here("dwk", dwk, f32, (D,)), r, B, S, D, eps, _dt(q), ACCUMULATE if accumulate else 0, wsp, wsb, _stream()),
            "gn_qk_norm_rope_bwd")
     return (*out, dwq, dwk)
+
+
+# ---- a block's residual branch: dropout, norms with gate and residual ----------------------
+_U64 = 2 ** 64 - 1
+
+
+def _rng(seed, stream, step):
+    """gn_rng; step: a number, or an int64 tensor of one element on the GPU that the kernels read (a graph's replays
+    then draw the masks of the step that it holds)."""
+    if isinstance(step, torch.Tensor):
+        if step.numel() != 1:
+            raise GnError(f"step must have one element, not {step.numel()}")
+        return Rng(seed & _U64, stream & _U64, 0, _here("step", step, torch.int64))
+    return Rng(seed & _U64, stream & _U64, step & _U64, None)
+
+
+def _dropout(name, x, p, seed, stream, step, out, flags):
+    xp = _here("x", x)
+    y = torch.empty_like(x) if out is None else out
+    yp = _here("out", y, x.dtype, x.shape)
+    args = (xp, yp, x.numel(), p, _rng(seed, stream, step), _dt(x))
+    if flags is None:
+        _check(lib().gn_dropout_fwd(*args, _stream()), name)
+    else:
+        _check(lib().gn_dropout_bwd(*args, flags, _stream()), name)
+    return y
+
+
+def dropout_fwd(x, p, seed, stream=0, step=0, out=None):
+    """x with each element dropped with probability p, the kept ones divided by 1 - p.  The mask comes from (seed,
+    stream, step) and an element's index alone: dropout_bwd with the same three forms it again, none is stored.
+    stream: the place in the model; step: the iteration, a number or an int64 tensor on the GPU, which
+    a captured call reads at every replay.  out may be x."""
+    return _dropout("gn_dropout_fwd", x, p, seed, stream, step, out, None)
+
+
+def dropout_bwd(dy, p, seed, stream=0, step=0, out=None, accumulate=False):
+    """The gradient of dropout_fwd's x; out may be dy; accumulate adds onto a given out."""
+    if accumulate and out is None:
+        raise GnError("accumulate needs the out to add onto")
+    return _dropout("gn_dropout_bwd", dy, p, seed, stream, step, out, ACCUMULATE if accumulate else 0)
+
+
+_EPS = {"none": 0.0, "rms": 1e-6, "layer": 1e-5}
+
+
+def _branch(h, x, post, post_w, post_b, pre, pre_w, pre_b, gate, scale, res_scale, p, seed, stream, step, post_eps, pre_eps):
+    """gn_branch of checked tensors; h and x (or y) [rows, F]."""
+    if h.dim() != 2:
+        raise GnError(f"h must be [rows, F], not {list(h.shape)}")
+    _int32("h", h)
+    dt, (rows, F) = h.dtype, h.shape
+    if x.dtype is not dt and not (dt is torch.bfloat16 and x.dtype is torch.float32):
+        raise GnError(f"the stream must be {dt}" + (" or float32" if dt is torch.bfloat16 else "") + f", not {x.dtype}")
+    b = Branch(NORM[post], NORM[pre])
+    if post_w is not None:
+        b.post_w = _here("post_w", post_w, dt, (F,))
+    if post_b is not None:
+        b.post_b = _here("post_b", post_b, dt, (F,))
+    if pre_w is not None:
+        b.pre_w = _here("pre_w", pre_w, dt, (F,))
+    if pre_b is not None:
+        b.pre_b = _here("pre_b", pre_b, dt, (F,))
+    b.post_eps = _EPS[post] if post_eps is None else post_eps
+    b.pre_eps = _EPS[pre] if pre_eps is None else pre_eps
+    if gate is not None:
+        gates = 1 if gate.dim() == 1 else gate.shape[0]
+        b.gate, b.gates = _here("gate", gate, dt, (F,) if gate.dim() == 1 else (gates, F)), gates
+    b.scale, b.res_scale, b.p = scale, res_scale, p
+    if p:
+        b.rng = _rng(seed, stream, step)
+    return b
+
+
+def residual_norm_fwd(h, x, post="none", post_w=None, post_b=None, pre="none", pre_w=None, pre_b=None, gate=None,
+                      scale=1.0, res_scale=1.0, p=0.0, seed=0, stream=0, step=0, post_eps=None, pre_eps=None, out=None):
+    """(y, z) of a block's output h [rows, F] and the residual stream x [rows, F]:
+    y = res_scale x + scale gate dropout(post(h)), z = pre(y) (None without one).  post, pre: "none", "rms" or
+    "layer" (a LayerNorm), with weights and biases [F] (None: 1 and 0) and eps (None: 1e-6 and 1e-5).
+    gate: [F], or [G, F] for G sequences of rows / G rows each.  Dropout as dropout_fwd's, on element i
+    of [rows, F].  h, z, gate and weights in h's dtype; x and y may be fp32 above bf16.  out: y's tensor, may
+    be x."""
+    b = _branch(h, x, post, post_w, post_b, pre, pre_w, pre_b, gate, scale, res_scale, p, seed, stream, step, post_eps,
+                pre_eps)
+    rows, F = h.shape
+    y = torch.empty_like(x) if out is None else out
+    z = None if pre == "none" else torch.empty_like(h)
+    _check(lib().gn_residual_norm_fwd(b, _here("h", h), _dt(h), _here("x", x, None, h.shape), _dt(x),
+                                      _here("out", y, x.dtype, h.shape), _ptr(z), rows, F, _stream()),
+           "gn_residual_norm_fwd")
+    return y, z
+
+
+@functools.lru_cache(maxsize=256)
+def residual_norm_workspace_bytes(rows, F, gates=0):
+    return int(lib().gn_residual_norm_workspace_bytes(rows, F, gates))
+
+
+def residual_norm_bwd(dy, dz, h, y, post="none", post_w=None, post_b=None, pre="none", pre_w=None, pre_b=None, gate=None,
+                      scale=1.0, res_scale=1.0, p=0.0, seed=0, stream=0, step=0, post_eps=None, pre_eps=None, need_dh=True,
+                      need_dx=True, need_param=True, dx=None, grads=None, accumulate=False, ws=None):
+    """(dh, dx, dgate, dpost_w, dpost_b, dpre_w, dpre_b) of residual_norm_fwd from its h, the y it returned and the
+    gradients dy of y and dz of z (either may be None).  The parameters' gradients are fp32, None for parameters that were
+    not given; dgate has gate's shape.  grads: the five tensors to write (None in it: not wanted), which
+    accumulate adds onto; need_param False: none of them.  dx: its tensor, may be dy."""
+    b = _branch(h, y, post, post_w, post_b, pre, pre_w, pre_b, gate, scale, res_scale, p, seed, stream, step, post_eps,
+                pre_eps)
+    rows, F = shape = h.shape
+    f32, dev = torch.float32, h.device
+    args = (_here("dy", dy, y.dtype, shape), _here("dz", dz, h.dtype, shape), _here("h", h), _dt(h),
+            _here("y", y, None, shape), _dt(y))
+    dh = torch.empty_like(h) if need_dh else None
+    if need_dx and dx is None:
+        dx = torch.empty_like(y)
+    dx = dx if need_dx else None
+    params = (gate, post_w, post_b, pre_w, pre_b)
+    if not need_param:
+        grads = (None,) * 5
+    elif grads is None:
+        if accumulate:
+            raise GnError("accumulate needs the grads to add onto")
+        grads = tuple(None if t is None else torch.empty(t.shape, dtype=f32, device=dev) for t in params)
+    g = BranchGrads(*(None if t is None else _here(n, t, f32, None if q is None else q.shape)
+                      for n, t, q in zip(("dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b"), grads, params)))
+    if ws is None:
+        nb = residual_norm_workspace_bytes(rows, F, b.gates)
+        ws = workspace(nb, dev)
+    _check(lib().gn_residual_norm_bwd(b, *args, _ptr(dh), _here("dx", dx, y.dtype, shape), g, rows, F,
+                                      ACCUMULATE if accumulate else 0, _here("ws", ws), ws.numel() * ws.element_size(),
+                                      _stream()), "gn_residual_norm_bwd")
+    return (dh, dx, *grads)
 
 
 def add_inplace(out, a):

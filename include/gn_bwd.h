@@ -409,6 +409,80 @@ int gn_qk_norm_rope_bwd(const gn_heads* dyq, const gn_heads* dyk, const gn_heads
                         unsigned flags, void* ws, size_t ws_bytes, void* stream);
 size_t gn_qk_norm_rope_workspace_bytes(int B, int S, int D);
 
+/* ---- a block's residual branch: dropout, norms with gate and residual, linear epilogues ---- */
+/* The reference adds a branch with a node of its own (backward_add, autograd.cpp:611-616), norms it in
+ * another pass (fnn-layernorm.glsl:44-102, rms-norm.glsl:34-70) and has neither dropout nor a gate. */
+
+/* Where the masks of a dropout come from: a counter-based generator, so that the backward forms the mask
+ * of its forward again and none is stored.  One seed a program, one stream a place in the model, one step
+ * an iteration.  With step_dev (int64 in device memory, 8-byte aligned) the step is step + *step_dev, read when the
+ * kernel runs: a captured graph then draws another mask at every replay that the caller advances it for.
+ *   key = mix(mix(seed + phi (stream + 1)) + phi (step + 1)),  word w = mix(key + phi (w + 1))  (64 bits,
+ *   wrapping; mix: splitmix64's output function, phi 0x9E3779B97F4A7C15)
+ *   element i is dropped where half i % 2 (0: the low one) of word i / 2 is below t = round(p 2^32). */
+typedef struct gn_rng {
+    uint64_t seed, stream, step;
+    const int64_t* step_dev;
+} gn_rng;
+
+/* y[i] = x[i] / (1 - t / 2^32), or 0 where the mask drops element i (inf and NaN too); 0 <= p < 1 (t below
+ * 2^32).  The backward does the same to dY.  n elements, f32 or bf16; Y may be X, dX may be dY (the same
+ * address), otherwise they share no memory.  GN_ACCUMULATE adds onto dX (which is then not dY). */
+int gn_dropout_fwd(const void* X, void* Y, int64_t n, double p, const gn_rng* rng, int dtype,
+                   void* stream);
+int gn_dropout_bwd(const void* dY, void* dX, int64_t n, double p, const gn_rng* rng, int dtype,
+                   unsigned flags, void* stream);
+
+/* The norm after a block, its dropout, gate and scale, the scaled residual sum, and the norm before the
+ * next block, in one pass over rows of F elements:
+ *   n = post(h),  d = dropout(n) (element i of [rows x F]),  y = res_scale x + scale gate d,  z = pre(y)
+ * Norms: GN_NORM_NONE (n = h; no z), GN_NORM_RMS (v rsqrt(mean v^2 + eps) w), GN_NORM_LAYER
+ * ((v - mean) rsqrt(var + eps) w + b, the biased variance).  z is formed from y before y is rounded.
+ * gate: [gates x F], row r takes gate r / (rows / gates): one for all (a gain per channel), one a sequence, one a row;
+ * rows must be a multiple of gates.  h, z, gate and the norms' weights in h_dtype, x and y in x_dtype: (f32,
+ * f32), (bf16, bf16) or (h bf16, x f32). */
+#define GN_NORM_NONE 0
+#define GN_NORM_RMS 1
+#define GN_NORM_LAYER 2
+typedef struct gn_branch {
+    int post, pre;          /* GN_NORM_* */
+    const void* post_w;     /* [F]; NULL: 1 */
+    const void* post_b;     /* [F], GN_NORM_LAYER only; NULL: 0 */
+    const void* pre_w;
+    const void* pre_b;
+    float post_eps, pre_eps;
+    const void* gate;       /* NULL: 1 */
+    int gates;              /* rows of gate; 0 without one */
+    float scale, res_scale;
+    double p;               /* 0: no dropout, rng is not read */
+    gn_rng rng;
+} gn_branch;
+/* z: NULL without a pre norm.  y may be x (the same address); otherwise outputs share no memory with
+ * anything else of the call. */
+int gn_residual_norm_fwd(const gn_branch* branch, const void* h, int h_dtype, const void* x,
+                         int x_dtype, void* y, void* z, int rows, int F, void* stream);
+
+/* fp32 gradients of a branch's parameters, each NULL where it is not wanted. */
+typedef struct gn_branch_grads {
+    float* dgate;  /* [gates x F] */
+    float *dpost_w, *dpost_b, *dpre_w, *dpre_b;  /* [F] */
+} gn_branch_grads;
+/* Its backward from h and the stream y that the forward left (the statistics are formed again), with the
+ * gradients dy (x_dtype; NULL: none) of y and dz (h_dtype; NULL: none) of z:
+ *   dY = dy + pre'(dz) at y,  dx = res_scale dY,  dgate = sum over its rows of scale m dY n,
+ *   dn = scale gate m dY (m: the dropout's factors),  dh = post'(dn) at h
+ * and the norms' own sums over the rows.  dh (h_dtype) and dx (x_dtype) may each be NULL; dx may be dy (the
+ * same address).  GN_ACCUMULATE adds onto the parameters' gradients (dh and dx are overwritten).  The sums
+ * over rows run in a fixed order: the same bits every time.
+ * ws: gn_residual_norm_workspace_bytes, 16-byte aligned; not used where no parameter gradient is wanted
+ * and F is up to 8192. */
+int gn_residual_norm_bwd(const gn_branch* branch, const void* dy, const void* dz, const void* h,
+                         int h_dtype, const void* y, int x_dtype, void* dh, void* dx,
+                         const gn_branch_grads* grads, int rows, int F, unsigned flags, void* ws,
+                         size_t ws_bytes, void* stream);
+/* 0 for sizes that the call refuses. */
+size_t gn_residual_norm_workspace_bytes(int rows, int F, int gates);
+
 /* ---- attention ------------------------------------------------------------------------ */
 /* Attention backward (attention-backward.glsl:73-194 semantics; RoPE of
  * flash-attention2-rope.glsl:73-145 applied to Q and K inside; causal mask j <= i).
