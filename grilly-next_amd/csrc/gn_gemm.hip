@@ -569,7 +569,7 @@ int colsum_dispatch(const void* in, float* out, int M, int N, int dtype, unsigne
 // accumulating.
 int weight_grad(const void* dY, int ldy, const void* X, int ldx, int M, int N, int Kin, void* dW,
                 void* dW2, int Msplit, float* db, float* db2, int dtype, unsigned flags,
-                hipStream_t s, void* ws = nullptr, size_t ws_bytes = 0, bool beside = false) {
+                hipStream_t s, void* ws, size_t ws_bytes, bool beside) {
     GemmDesc d{};
     d.beside = beside;
     // split-K partial planes need 16-byte aligned storage; a misaligned workspace is unused

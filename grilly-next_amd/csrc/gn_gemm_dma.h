@@ -2,6 +2,7 @@
 #pragma once
 
 #include "gn_common.h"
+#include "gn_lane.h"
 #include "gn_math.h"
 
 namespace gn {
@@ -93,6 +94,8 @@ int gemm_dma_bf16(const GemmDesc& g, int transA, int transB, hipStream_t s);
 int gemm_dma_glu(const GemmDesc& g, hipStream_t s);
 // the time (us) gemm_dma_bf16's tiles are expected to take, for a choice between the kernels
 double gemm_stream_us(const GemmDesc& g);
+// and the rows of those tiles, 128 or 256 (128 columns)
+int gemm_stream_rows(const GemmDesc& g);
 // fp32 C of an unbiased weight gradient (transA, plain epilogue) on streamed tiles, where it wins
 bool gemm_stream_f32_wins(const GemmDesc& g, int transA, int transB);
 int gemm_stream_f32(const GemmDesc& g, hipStream_t s);
@@ -202,6 +205,13 @@ struct SmHyper;
 int skinny_linear_bwd(const float* dY, const float* X, const float* W, float* dX, float* dW,
                       float* db, int M, int N, int K, bool accumulate, void* ws, size_t ws_bytes,
                       hipStream_t s, float* s_bar = nullptr, const SmHyper* sm = nullptr);
+
+// When a backward call's two products run side by side (gn_gemm.hip): dx [xr x xc], dw [wr x wc], FLOP of each.
+Fork side_by_side(int dtype, double flop_dx, double flop_dw, long xr, long xc, long wr, long wc);
+// The weight gradient dW [N x Kin] = dY^T X and the bias's, db, of a Linear (gn_gemm.hip; Msplit: N, dW2: dW).
+int weight_grad(const void* dY, int ldy, const void* X, int ldx, int M, int N, int Kin, void* dW, void* dW2, int Msplit,
+                float* db, float* db2, int dtype, unsigned flags, hipStream_t s, void* ws = nullptr,
+                size_t ws_bytes = 0, bool beside = false);
 
 // Run C (+)= sum_s op(A_s) op(B_s) described by `d`.  bf16: the LDS-DMA kernels when the shape
 // allows it, else the register-staged MFMA kernel.  fp32: gemm_small, the six-product split or

@@ -72,6 +72,11 @@ double gemm_stream_us(const GemmDesc& g) {
     return us;
 }
 
+int gemm_stream_rows(const GemmDesc& g) {
+    double us;
+    return choose_rows(g, stream_blocks(), &us);
+}
+
 int gemm_dma_bf16(const GemmDesc& g, int transA, int transB, hipStream_t s) {
     if (g.Msplit < g.M) {
         set_error("gemm: a bf16 product has one destination");

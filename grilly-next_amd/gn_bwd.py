@@ -26,6 +26,7 @@ GLU = {"swiglu_up": 0, "swiglu_gate": 1, "geglu_up": 2, "geglu_gate": 3, "reglu_
 ROPE = {"none": 0, "interleaved": 1, "half": 2}
 ROPE_SCALE = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
 NORM = {"none": 0, "rms": 1, "layer": 2}
+ACT_OR_NONE = {"none": -1, **ACT}
 
 # exported symbols, in the order include/gn_bwd.h declares them
 SYMBOLS = [
@@ -46,6 +47,7 @@ SYMBOLS = [
     "gn_linear_xent_fwd", "gn_linear_xent_bwd", "gn_linear_xent_workspace_bytes", "gn_rope_freqs", "gn_rope_fwd",
     "gn_rope_bwd", "gn_qk_norm_rope_fwd", "gn_qk_norm_rope_bwd", "gn_qk_norm_rope_workspace_bytes",
     "gn_dropout_fwd", "gn_dropout_bwd", "gn_residual_norm_fwd", "gn_residual_norm_bwd", "gn_residual_norm_workspace_bytes",
+    "gn_linear_act_fwd", "gn_act_linear_bwd", "gn_linear_act_workspace_bytes",
 ]
 BIN = {"sub": 0, "mul": 1, "div": 2, "neg": 3}
 RED = {"sum": 0, "mean": 1}
@@ -205,6 +207,9 @@ _SIGS = {
     "gn_residual_norm_bwd": ([_BRANCHP, _P, _P, _P, _I, _P, _I, _P, _P, ctypes.POINTER(BranchGrads), _I, _I, _U, _P, _Z,
                               _P], _I),
     "gn_residual_norm_workspace_bytes": ([_I, _I, _I], _Z),
+    "gn_linear_act_fwd": ([_I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _Z, _P], _I),
+    "gn_act_linear_bwd": ([_I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _U, _P, _Z, _P], _I),
+    "gn_linear_act_workspace_bytes": ([_I, _I, _I, _I], _Z),
 }
 
 
@@ -1268,6 +1273,78 @@ def residual_norm_bwd(dy, dz, h, y, post="none", post_w=None, post_b=None, pre="
                                       ACCUMULATE if accumulate else 0, _here("ws", ws), ws.numel() * ws.element_size(),
                                       _stream()), "gn_residual_norm_bwd")
     return (dh, dx, *grads)
+
+
+# ---- linear layers with their activation and residual -------------------------------------
+@functools.lru_cache(maxsize=256)
+def linear_act_workspace_bytes(M, N, K, dtype):
+    """What linear_act_fwd and act_linear_bwd need of bf16 operands that 16-byte pieces do not take; dtype: a
+    GN_* code."""
+    return int(lib().gn_linear_act_workspace_bytes(M, N, K, dtype))
+
+
+def _matrix(name, t):
+    if t.dim() != 2:
+        raise GnError(f"{name} must have two dimensions, not {t.dim()}")
+    _int32(name, t)
+    return t.shape
+
+
+def linear_act_fwd(X, W, b=None, act="none", residual=None, need_pre=False, out=None, out_dtype=None, ws=None):
+    """Y = residual + act(X W^T + b), or (Y, P) when need_pre: P is what act_bwd and act_linear_bwd read (the
+    pre-activation; of tanh and sigmoid their output).  X [M, K], W [N, K], b [N] in one dtype; act: a key of ACT
+    or "none".  Y has the residual's dtype (that of out, or out_dtype, without one; default X's): it may be fp32 above
+    bf16.  out may be the residual (in fp32 only with need_pre).  ws: linear_act_workspace_bytes, allocated here
+    when None and needed."""
+    (M, K), (N, K2), dt = _matrix("X", X), _matrix("W", W), X.dtype
+    if K != K2:
+        raise GnError(f"X [M, K] and W [N, K] expected, not {list(X.shape)} and {list(W.shape)}")
+    shape = (M, N)
+    if out is None:
+        Y = torch.empty(shape, dtype=residual.dtype if residual is not None else out_dtype or dt, device=X.device)
+    else:
+        Y = out
+    xp, wp, yp, code = _here("X", X), _here("W", W, dt), _here("out", Y, None, shape), _dt(X)
+    P = torch.empty(shape, dtype=dt, device=X.device) if need_pre else None
+    if ws is None and code == BF16 and (K % 8 or (xp | wp) % 16):
+        ws = workspace(linear_act_workspace_bytes(M, N, K, code), X.device)
+    wsp, wsb = (None, 0) if ws is None else (_here("ws", ws), ws.numel() * ws.element_size())
+    _check(lib().gn_linear_act_fwd(ACT_OR_NONE[act], xp, wp, _here("b", b, dt, (N,)),
+                                   _here("residual", residual, Y.dtype, shape), _ptr(P), yp, M, N, K, code, _dt(Y), wsp,
+                                   wsb, _stream()), "gn_linear_act_fwd")
+    return (Y, P) if need_pre else Y
+
+
+def act_linear_bwd(act, dY, P, A, W, need_dp=True, need_dw=True, need_db=True, dP=None, dW=None, db=None,
+                   accumulate=False, ws=None):
+    """(dP, dW, db) of y = A W^T + b with A = act(P), the linear layer behind an activation: dP = (dY W) act'(P) in
+    P's dtype, dW = dY^T A and db the column sums of dY in fp32.  P as act_bwd takes it (of tanh and sigmoid:
+    A).  dP may be P in bf16; accumulate adds onto a given dW and db.  ws: linear_act_workspace_bytes (only where
+    needed) and linear_workspace_bytes together, allocated here when None."""
+    (M, N), (_, K), dt = _matrix("dY", dY), _matrix("W", W), dY.dtype
+    f32, dev, code = torch.float32, dY.device, _dt(dY)
+    yp, wp = _here("dY", dY), _here("W", W, dt, (N, K))
+    pp, ap = _here("P", P, dt, (M, K)), _here("A", A, dt, (M, K))
+    need_db = need_db and need_dw
+    if accumulate and ((need_dw and dW is None) or (need_db and db is None)):
+        raise GnError("accumulate needs the dW and db to add onto")
+    if need_dp and dP is None:
+        dP = torch.empty((M, K), dtype=dt, device=dev)
+    if need_dw and dW is None:
+        dW = torch.empty((N, K), dtype=f32, device=dev)
+    if need_db and db is None:
+        db = torch.empty((N,), dtype=f32, device=dev)
+    dP, dW, db = dP if need_dp else None, dW if need_dw else None, db if need_db else None
+    if ws is None:
+        nb = linear_workspace_bytes(M, N, K, code) if need_dw else 0
+        if code == BF16 and (N % 8 or K % 8 or (yp | wp) % 16):
+            nb += linear_act_workspace_bytes(M, N, K, code)
+        ws = workspace(nb, dev) if nb else None
+    wsp, wsb = (None, 0) if ws is None else (_here("ws", ws), ws.numel() * ws.element_size())
+    _check(lib().gn_act_linear_bwd(ACT[act], yp, pp, ap, wp, _here("dP", dP, dt, (M, K)), _here("dW", dW, f32, (N, K)),
+                                   _here("db", db, f32, (N,)), M, N, K, code, ACCUMULATE if accumulate else 0, wsp, wsb,
+                                   _stream()), "gn_act_linear_bwd")
+    return dP, dW, db
 
 
 def add_inplace(out, a):

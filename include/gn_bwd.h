@@ -56,6 +56,7 @@ extern "C" {
                                  the workspace, for a later gn_norm_finish (see there) */
 
 /* ---- activation kinds (gn_act_bwd) ------------------------------------------------- */
+#define GN_ACT_NONE (-1)   /* gn_linear_act_fwd: no activation */
 #define GN_ACT_RELU 0      /* dx = dy*[x>0]            activation-relu-backward.glsl:33-37 */
 #define GN_ACT_GELU_TANH 1 /* tanh-form GELU'(x)        activation-gelu-backward.glsl:38-50 */
 #define GN_ACT_GELU_ERF 2  /* erf-form GELU'(x)         autograd_core.py:529-542 */
@@ -482,6 +483,33 @@ int gn_residual_norm_bwd(const gn_branch* branch, const void* dy, const void* dz
                          size_t ws_bytes, void* stream);
 /* 0 for sizes that the call refuses. */
 size_t gn_residual_norm_workspace_bytes(int rows, int F, int gates);
+
+/* A Linear with its activation and the residual in the product's epilogue (the reference's fnn-linear.glsl:33-55,
+ * activation-*.glsl and Add are passes of their own):
+ *   v = X W^T + b,  Y = R + act(v)
+ * X [M x K], W [N x K], b [N] (NULL: 0) in dtype; R (NULL: none) and Y [M x N] in y_dtype, which is dtype, or
+ * GN_F32 over bf16 (an fp32 residual stream; Y is then not rounded at all).  P [M x N] in dtype, or NULL: what
+ * gn_act_bwd and gn_act_linear_bwd read, v or, of tanh and sigmoid, act(v).  act: GN_ACT_*.  v is fp32 up to the
+ * one rounding of P and that of Y.  Y may be R (the same address; in fp32 only with P), otherwise outputs share
+ * no memory with anything else of the call.  M, N, K below 2^28, M * N, M * K, N * K below 2^36.
+ * ws: gn_linear_act_workspace_bytes, 16-byte aligned; bf16 needs it where K is no multiple of 8 or X or W not
+ * 16-byte aligned (the operands are laid out there), otherwise it may be NULL. */
+int gn_linear_act_fwd(int act, const void* X, const void* W, const void* b, const void* R, void* P,
+                      void* Y, int M, int N, int K, int dtype, int y_dtype, void* ws,
+                      size_t ws_bytes, void* stream);
+/* The backward of y = A W^T + b with A = act(P), the Linear behind an activation, down to P:
+ *   dP = (dY W) act'(P) [M x K] in dtype (the gradient of A is not stored),
+ *   dW (+)= dY^T A [N x K],  db (+)= column sums of dY [N]  (fp32)
+ * P as gn_act_bwd takes it (of tanh and sigmoid the output: A itself).  dP may be NULL, and so may dW (with
+ * db).  In bf16 dP may be P (the same address, and then not A); otherwise outputs and the workspace share no memory with
+ * anything else of the call.  GN_ACCUMULATE adds onto dW and db (dP is overwritten).
+ * ws: bf16 needs gn_linear_act_workspace_bytes where N or K is no multiple of 8 or dY or W not 16-byte aligned;
+ * what is left of it beyond, gn_linear_workspace_bytes at best, goes to the weight gradient as in gn_linear_bwd_ws. */
+int gn_act_linear_bwd(int act, const void* dY, const void* P, const void* A, const void* W, void* dP,
+                      void* dW, void* db, int M, int N, int K, int dtype, unsigned flags, void* ws,
+                      size_t ws_bytes, void* stream);
+/* 0 in fp32 and for sizes that the calls refuse. */
+size_t gn_linear_act_workspace_bytes(int M, int N, int K, int dtype);
 
 /* ---- attention ------------------------------------------------------------------------ */
 /* Attention backward (attention-backward.glsl:73-194 semantics; RoPE of
