@@ -107,6 +107,7 @@ PYBIND11_MODULE(_grilly_core, m) {
         .value("Embedding", OpType::Embedding)
         .value("Rope", OpType::Rope).value("QkNormRope", OpType::QkNormRope)
         .value("LinearCrossEntropy", OpType::LinearCrossEntropy)
+        .value("Dropout", OpType::Dropout).value("ResidualNorm", OpType::ResidualNorm).value("LinearAct", OpType::LinearAct)
         .export_values();
 
     py::class_<TensorRef>(m, "TensorRef")

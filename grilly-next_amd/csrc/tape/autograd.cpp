@@ -171,6 +171,8 @@ void BackwardEngine::backward(TapeArena& tape, Node* loss_node, uint64_t grad_ou
     norm_pending_.clear();
     glu_node_ = nullptr;
     glu_gu_ = 0;
+    act_node_ = nullptr;
+    act_dp_ = 0;
     if (!loss_node) throw std::invalid_argument("backward: loss node is None");
     // autograd.cpp:30-31: 0 means "the loss computes its own gradient" (sentinel 1)
     loss_node->grad_output_buffer = grad_output_buffer ? grad_output_buffer : 1ULL;
@@ -201,7 +203,7 @@ void BackwardEngine::backward(TapeArena& tape, Node* loss_node, uint64_t grad_ou
             }
         }
         // a FusedGLU whose output gradient the down projection's epilogue turned into gu
-        if (cur->grad_output_buffer == 0 && cur == glu_node_) cur->grad_output_buffer = 1;
+        if (cur->grad_output_buffer == 0 && (cur == glu_node_ || cur == act_node_)) cur->grad_output_buffer = 1;
         if (cur->grad_output_buffer == 0) continue;
         stats_.nodes_with_grad++;
         std::memset(cur->grad_input_buffers, 0, sizeof(cur->grad_input_buffers));
@@ -268,6 +270,30 @@ void check_node(const Node* n, bool upstream) {
             if (upstream && (y.dtype != 0 || y.numel() != x.rows()))
                 throw std::invalid_argument("LinearCrossEntropy: an upstream gradient goes with a loss of fp32 [T]");
             break;
+        case OpType::Dropout:
+            if (!alike(x, y)) throw std::invalid_argument("Dropout: the output must have the input's type and size");
+            break;
+        case OpType::ResidualNorm: {
+            if (n->num_inputs < 2 || n->num_outputs < 1)
+                throw std::invalid_argument("ResidualNorm: inputs h and x, outputs y and z");
+            const TensorRef& s = n->inputs[1];
+            const bool pre = params_of<ResidualNormParams>(n).pre != GN_NORM_NONE;
+            if (n->params_size < sizeof(ResidualNormParams))
+                throw std::invalid_argument("ResidualNorm: params must hold the whole block");
+            if (x.numel() != s.numel() || x.last() != s.last() || !alike(s, y) || y.last() != x.last())
+                throw std::invalid_argument("ResidualNorm: h, x and y must have one size, y x's type");
+            if (pre != (n->num_outputs > 1) || (pre && !alike(n->outputs[1], x)))
+                throw std::invalid_argument("ResidualNorm: z, alike h, goes with the norm before the next block");
+            if (y.buffer_id == x.buffer_id || (pre && n->outputs[1].buffer_id == x.buffer_id))
+                throw std::invalid_argument("ResidualNorm: the backward reads h, which an output in its place overwrites");
+            break;
+        }
+        case OpType::LinearAct:
+            if (n->num_inputs > 1 && n->inputs[1].buffer_id && !alike(n->inputs[1], y))
+                throw std::invalid_argument("LinearAct: the output must have the residual's type and size");
+            if (y.dtype != x.dtype && !(x.dtype == 4 && y.dtype == 0))
+                throw std::invalid_argument("LinearAct: the output must have the input's type, or f32 above bf16");
+            break;
         default: break;
     }
 }
@@ -291,6 +317,9 @@ void BackwardEngine::dispatch(Node* n) {
         case OpType::Rope: bwd_rope(n); break;
         case OpType::QkNormRope: bwd_qk_norm_rope(n); break;
         case OpType::LinearCrossEntropy: bwd_linear_cross_entropy(n); break;
+        case OpType::Dropout: bwd_dropout(n); break;
+        case OpType::ResidualNorm: bwd_residual_norm(n); break;
+        case OpType::LinearAct: bwd_linear_act(n); break;
         case OpType::Add: bwd_add_sub(n, false); break;
         case OpType::Reshape: bwd_passthrough(n); break;
         case OpType::VSAUnpackProject: bwd_vsa_unpack_project(n); break;
@@ -385,17 +414,140 @@ void BackwardEngine::bwd_linear(Node* n) {
         if (b) contribute(b, db, 0, (size_t)N, true);
         return;
     }
-    uint64_t dX = x.requires_grad ? alloc_grad(x.size_bytes()) : 0;
+    linear_grads(n, gout(n), W, b, M, N, K, dt);
+}
+
+void BackwardEngine::linear_grads(Node* n, const void* dY, uint64_t W, uint64_t b, int M, int N, int K, int dt) {
+    const TensorRef& x = n->inputs[0];
     uint64_t dW = alloc_grad((size_t)N * K * 4);
     uint64_t db = b ? alloc_grad((size_t)N * 4) : 0;
-    const size_t wsb = gn_linear_workspace_bytes(M, N, K, dt);
-    const uint64_t ws = split_ws(wsb);
-    gn_call(gn_linear_bwd_ws(gout(n), P(x.buffer_id), P(W), P(dX), P(dW), P(db), M, N, K, dt, 0,
-                             P(ws), wsb, dev_.stream()), "Linear backward");
+    if (Node* a = act_before(n)) {
+        // x = act(P) feeds only this node: the gradient in front of the activation comes out of the
+        // input-gradient product for the LinearAct node visited next (dX never formed)
+        uint64_t dP = alloc_grad(x.size_bytes());
+        const size_t wsb = gn_linear_workspace_bytes(M, N, K, dt) + gn_linear_act_workspace_bytes(M, N, K, dt);
+        const uint64_t ws = split_ws(wsb);
+        gn_call(gn_act_linear_bwd(params_of<LinearActParams>(a).act, dY, P(a->saved_buffer_ids[2]), P(x.buffer_id), P(W), P(dP),
+                                  P(dW), P(db), M, N, K, dt, 0, P(ws), wsb, dev_.stream()),
+                "Linear backward (through the activation in front)");
+        act_node_ = a;
+        act_dp_ = dP;
+    } else {
+        uint64_t dX = x.requires_grad ? alloc_grad(x.size_bytes()) : 0;
+        const size_t wsb = gn_linear_workspace_bytes(M, N, K, dt);
+        const uint64_t ws = split_ws(wsb);
+        gn_call(gn_linear_bwd_ws(dY, P(x.buffer_id), P(W), P(dX), P(dW), P(db), M, N, K, dt, 0, P(ws), wsb, dev_.stream()),
+                "Linear backward");
+        n->grad_input_buffers[0] = dX;
+    }
     stats_.shaders_dispatched += db ? 3 : 2;
-    n->grad_input_buffers[0] = dX;
     contribute(W, dW, 0, (size_t)N * K, true);
     if (b) contribute(b, db, 0, (size_t)N, true);
+}
+
+// LinearAct: y = residual + act(x W^T + b).  The residual's gradient is the upstream one itself; the product's is that
+// times act', in x's type (an fp32 one over bf16 operands rounded first).
+void BackwardEngine::bwd_linear_act(Node* n) {
+    const TensorRef& x = n->inputs[0];
+    const TensorRef& y = n->outputs[0];
+    const int M = (int)x.rows(), K = (int)x.last(), N = (int)y.last();
+    if ((size_t)M != y.rows()) throw std::invalid_argument("LinearAct: input/output rows differ");
+    const int dt = gn_dtype(x.dtype, "LinearAct");
+    const uint64_t W = n->saved_buffer_ids[0], b = n->num_saved > 1 ? n->saved_buffer_ids[1] : 0;
+    const uint64_t pre = n->num_saved > 2 ? n->saved_buffer_ids[2] : 0;
+    const int act = n->params_size < sizeof(LinearActParams) ? GN_ACT_NONE : params_of<LinearActParams>(n).act;
+    if (!W) throw std::invalid_argument("LinearAct: saved_buffer_ids[0] must hold W");
+    if (act != GN_ACT_NONE && !pre) throw std::invalid_argument("LinearAct: saved_buffer_ids[2] must hold P");
+    uint64_t dv;
+    if (n == act_node_) {  // from the node behind (linear_grads)
+        dv = act_dp_;
+        act_node_ = nullptr;
+        act_dp_ = 0;
+        n->grad_output_buffer = 0;  // its output's gradient was never formed
+    } else {
+        const uint64_t g = reinterpret_cast<uint64_t>(gout(n));
+        dv = g;
+        if (y.dtype != x.dtype) {
+            dv = take_bf16_copy(g);
+            if (!dv) {
+                dv = alloc_grad(y.numel() * 2);
+                gn_call(gn_convert(P(g), GN_F32, P(dv), dt, (int64_t)y.numel(), dev_.stream()), "LinearAct backward (conversion)");
+                stats_.shaders_dispatched++;
+            }
+        }
+        if (act != GN_ACT_NONE) {
+            const uint64_t up = dv;
+            dv = alloc_grad(y.numel() * TensorRef::elem_size(x.dtype));
+            gn_call(gn_act_bwd(act, P(up), P(pre), P(dv), (int64_t)y.numel(), dt, 0, dev_.stream()), "LinearAct backward (activation)");
+            stats_.shaders_dispatched++;
+        }
+        if (n->num_inputs > 1 && n->inputs[1].buffer_id && n->inputs[1].requires_grad) {
+            n->grad_input_buffers[1] = g;
+            borrowed_ |= 2u;
+        }
+    }
+    linear_grads(n, P(dv), W, b, M, N, K, dt);
+}
+
+// Dropout: the mask is formed again from its counters.
+void BackwardEngine::bwd_dropout(Node* n) {
+    const TensorRef& x = n->inputs[0];
+    if (!x.requires_grad) return;
+    if (n->params_size < sizeof(DropoutParams)) throw std::invalid_argument("Dropout: params must hold p, seed, stream and step");
+    const DropoutParams p = params_of<DropoutParams>(n);
+    const gn_rng rng{p.seed, p.stream, p.step, n->num_saved ? (const int64_t*)P(n->saved_buffer_ids[0]) : nullptr};
+    uint64_t dX = alloc_grad(x.size_bytes());
+    gn_call(gn_dropout_bwd(gout(n), P(dX), (int64_t)x.numel(), p.p, &rng, gn_dtype(x.dtype, "Dropout"), 0, dev_.stream()),
+            "dropout backward");
+    stats_.shaders_dispatched++;
+    n->grad_input_buffers[0] = dX;
+}
+
+// ResidualNorm: y and z each have a gradient, or one of them; as a root the node is given y's.
+void BackwardEngine::bwd_residual_norm(Node* n) {
+    const TensorRef &h = n->inputs[0], &x = n->inputs[1], &y = n->outputs[0];
+    const ResidualNormParams p = params_of<ResidualNormParams>(n);
+    const uint64_t* s = n->saved_buffer_ids;
+    const int rows = (int)h.rows(), F = (int)h.last();
+    auto grad_of = [&](const TensorRef& t) {
+        const GradEntry* e = find(t.buffer_id);
+        if (!e || !e->grad_id) return (uint64_t)0;
+        if (e->dtype != t.dtype || e->grad_bytes != t.size_bytes())
+            throw std::runtime_error("ResidualNorm: an output's gradient has another type or size");
+        return e->grad_id;
+    };
+    uint64_t dy = grad_of(y), dz = p.pre != GN_NORM_NONE ? grad_of(n->outputs[1]) : 0;
+    if (!dy && !dz) dy = reinterpret_cast<uint64_t>(gout(n));
+    gn_branch b{};
+    b.post = (int)p.post;
+    b.pre = (int)p.pre;
+    b.post_w = P(s[0]);
+    b.post_b = P(s[1]);
+    b.pre_w = P(s[2]);
+    b.pre_b = P(s[3]);
+    b.post_eps = p.post_eps;
+    b.pre_eps = p.pre_eps;
+    b.gate = P(s[4]);
+    b.gates = (int)p.gates;
+    b.scale = p.scale;
+    b.res_scale = p.res_scale;
+    b.p = p.p;
+    b.rng = gn_rng{p.seed, p.stream, p.step, (const int64_t*)P(s[5])};
+    uint64_t dh = h.requires_grad ? alloc_grad(h.size_bytes()) : 0, dx = x.requires_grad ? alloc_grad(x.size_bytes()) : 0;
+    uint64_t g[5];  // of gate, post_w, post_b, pre_w, pre_b
+    const uint64_t of[5] = {s[4], s[0], s[1], s[2], s[3]};
+    for (int i = 0; i < 5; ++i) g[i] = of[i] ? alloc_grad((size_t)F * 4 * (i ? 1 : p.gates)) : 0;
+    const gn_branch_grads grads{(float*)P(g[0]), (float*)P(g[1]), (float*)P(g[2]), (float*)P(g[3]), (float*)P(g[4])};
+    const size_t wsb = gn_residual_norm_workspace_bytes(rows, F, b.gates);
+    const uint64_t ws = split_ws(wsb);
+    gn_call(gn_residual_norm_bwd(&b, P(dy), P(dz), P(h.buffer_id), gn_dtype(h.dtype, "ResidualNorm"), P(y.buffer_id),
+                                 gn_dtype(x.dtype, "ResidualNorm"), P(dh), P(dx), &grads, rows, F, 0, P(ws), wsb, dev_.stream()),
+            "residual norm backward");
+    stats_.shaders_dispatched += 2;
+    n->grad_input_buffers[0] = dh;
+    n->grad_input_buffers[1] = dx;
+    for (int i = 0; i < 5; ++i)
+        if (of[i]) contribute(of[i], g[i], 0, (size_t)F * (i ? 1 : p.gates), true);
 }
 
 // Elementwise activations; tanh/sigmoid read the saved output (activation-tanh-backward.glsl:33).
@@ -443,22 +595,22 @@ uint64_t BackwardEngine::norm_dx(Node* n, const void** add) {
     return alloc_grad(x.size_bytes());
 }
 
-// A pre-norm block with its residual stream in fp32 records x = Add(x_prev, y_bf16) right
-// before Norm(x): in the reverse walk the Add is the next node, and no other consumer of x is
+// A pre-norm block with its residual stream in fp32 records x = Add(x_prev, y_bf16), or a LinearAct of bf16 operands
+// with the residual x_prev, right before Norm(x): in the reverse walk the Add is the next node, and no other consumer of x is
 // visited in between, so the norm's dX (with every earlier consumer's gradient summed in by
 // norm_dx) is x's whole gradient, and the Add would convert it to bf16 for y.  The norm then
 // writes that bf16 copy in its own pass: returns the copy's buffer (0: no copy wanted).
 uint64_t BackwardEngine::bf16_copy_for(Node* n, uint64_t dX) {
     const TensorRef& x = n->inputs[0];
     const Node* a = n->prev_in_tape;
-    if (!dX || !x.requires_grad || x.dtype != 0 /* f32 */ || !a || a->op != OpType::Add || a->num_outputs < 1 ||
-        a->outputs[0].buffer_id != x.buffer_id || writes_in_place(n, x.buffer_id))
+    if (!dX || !x.requires_grad || x.dtype != 0 /* f32 */ || !a || (a->op != OpType::Add && a->op != OpType::LinearAct) ||
+        a->num_outputs < 1 || a->outputs[0].buffer_id != x.buffer_id || writes_in_place(n, x.buffer_id))
         return 0;
     // dX is x's whole gradient only when no earlier contribution is left to add after this node
     const GradEntry* e = find(x.buffer_id);
     if (!(handled_ & 1u) && e && e->grad_id) return 0;
-    bool wants = false;
-    for (uint32_t i = 0; i < a->num_inputs && i < kMaxNodeIO; ++i) {
+    bool wants = a->op == OpType::LinearAct && a->num_inputs > 0 && a->inputs[0].dtype == 4;
+    for (uint32_t i = 0; a->op == OpType::Add && i < a->num_inputs && i < kMaxNodeIO; ++i) {
         const TensorRef& in = a->inputs[i];
         wants = wants || (in.requires_grad && in.dtype == 4 /* bf16 */ && in.numel() == x.numel());
     }
@@ -484,6 +636,21 @@ Node* BackwardEngine::glu_before(Node* n) const {
         return nullptr;
     const GradEntry* e = find(x.buffer_id);
     return e && e->grad_id ? nullptr : g;
+}
+
+// The LinearAct node whose output is this Linear's or LinearAct's input, when set_glu_epilogue is on: with an activation and
+// no residual, recorded right before, and no gradient of its output yet (no other consumer).
+Node* BackwardEngine::act_before(Node* n) const {
+    const TensorRef& x = n->inputs[0];
+    Node* a = n->prev_in_tape;
+    if (!glu_epilogue_ || !a || a->op != OpType::LinearAct || !x.requires_grad || a->num_inputs < 1 ||
+        (a->num_inputs > 1 && a->inputs[1].buffer_id) || a->num_outputs < 1 || a->num_saved < 3 || !a->saved_buffer_ids[2] ||
+        a->outputs[0].buffer_id != x.buffer_id || a->inputs[0].buffer_id == x.buffer_id || a->outputs[0].dtype != x.dtype ||
+        a->inputs[0].dtype != x.dtype || a->outputs[0].numel() != x.numel() || a->outputs[0].last() != x.last() ||
+        a->params_size < sizeof(LinearActParams) || params_of<LinearActParams>(a).act == GN_ACT_NONE)
+        return nullptr;
+    const GradEntry* e = find(x.buffer_id);
+    return e && e->grad_id ? nullptr : a;
 }
 
 // saved: [0] gamma, [1] beta (or 0), [2] mean, [3] rstd (or var with stat_is_var).  x and its
@@ -769,6 +936,17 @@ void BackwardEngine::bwd_linear_cross_entropy(Node* n) {
     if (!into) contribute(E, dE, 0, (size_t)V * d, true);
 }
 
+// The bf16 copy of gradient g that a norm wrote (bf16_copy_for), once; 0: none.
+uint64_t BackwardEngine::take_bf16_copy(uint64_t g) {
+    for (auto& bc : bf16_copies_)
+        if (bc.first == g && bc.second) {
+            const uint64_t c = bc.second;
+            bc.second = 0;
+            return c;
+        }
+    return 0;
+}
+
 // Add: both inputs receive the upstream gradient itself (borrowed, copied on fan-out).  An
 // input stored in another dtype than the sum (a bf16 branch added into an fp32 residual
 // stream) receives the upstream gradient converted once to its own dtype.
@@ -783,14 +961,7 @@ void BackwardEngine::bwd_add_sub(Node* n, bool /*sub*/) {
         if (in.dtype != out.dtype) {
             // the bf16 copy the norm visited just before wrote in its pass (bf16_copy_for);
             // taken once, so a second bf16 input gets its own buffer
-            uint64_t c = 0;
-            if (in.dtype == 4 /* bf16 */)
-                for (auto& bc : bf16_copies_)
-                    if (bc.first == g && bc.second) {
-                        c = bc.second;
-                        bc.second = 0;
-                        break;
-                    }
+            uint64_t c = in.dtype == 4 /* bf16 */ ? take_bf16_copy(g) : 0;
             if (!c) {
                 c = alloc_grad(in.size_bytes());
                 gn_call(gn_convert(P(g), gn_dtype(out.dtype, "Add output"), P(c), gn_dtype(in.dtype, "Add input"),

@@ -75,6 +75,9 @@ enum class OpType : uint8_t {
     Rope,                // added by this build: heads rotated by position
     QkNormRope,          // added by this build: per-head norms of q and k with the rotation, on fused QKV rows
     LinearCrossEntropy,  // added by this build: the loss of a linear head whose logits are not kept
+    Dropout,             // added by this build: elements dropped by a counter-based mask
+    ResidualNorm,        // added by this build: norms around a block with gate, dropout and the residual sum
+    LinearAct,           // added by this build: a Linear with its activation and the residual
     _Count
 };
 static_assert(static_cast<int>(OpType::VSACosineBlendLoss) == 33, "OpType numbering");
@@ -128,6 +131,23 @@ static_assert(sizeof(RopeNodeParams) == 32, "RopeNodeParams layout");
 // an upstream gradient (a mean or a weighted sum of the rows behind it) it is scale times the row's, so
 // that such a node takes scale 1.
 struct LinearCrossEntropyParams { uint32_t vocab; float scale; };
+// Dropout: inputs[0] -> outputs[0] alike; saved slots {step counter or 0} (int64 in device memory, added to
+// step when the kernel runs).  p as the forward had it.
+struct DropoutParams { double p; uint64_t seed, stream, step; };
+// ResidualNorm: inputs h (the block's output) and x (the residual stream), [rows, F] each -> outputs y, alike x, and z,
+// alike h (none without a pre norm); saved slots {post_w, post_b, pre_w, pre_b, gate, step counter}, 0 where
+// there is none.  The backward reads h and y, which must be as the forward left them: a stream that a later
+// block updates in place is lost to this one's pre norm.
+struct ResidualNormParams {
+    double p;
+    uint64_t seed, stream, step;
+    float post_eps, pre_eps, scale, res_scale;
+    uint32_t post, pre, gates;  // GN_NORM_*; rows of the gate
+};
+static_assert(sizeof(ResidualNormParams) == 64, "ResidualNormParams layout");
+// LinearAct: inputs X and optionally the residual -> outputs[0] = residual + act(X W^T + b), in the residual's type;
+// saved slots {W, b or 0, P (what gn_linear_act_fwd left, 0 without an activation)}.
+struct LinearActParams { int32_t act; };  // GN_ACT_*, GN_ACT_NONE in a block that is empty
 struct MSELossParams { float scale; uint32_t has_scale; };      // scale default 1/n (mean)
 
 static constexpr uint32_t kMaxNodeIO = 8;
@@ -157,8 +177,8 @@ T* TapeArena::allocate_node(Args&&... args) {
     return node;
 }
 
-// Throws where the types or sizes of an attention, Rope, QkNormRope or LinearCrossEntropy node's tensors are
-// not what its backward reads and writes by (upstream: it is given a gradient of its output).  No device call.
+// Throws where the types or sizes of an attention, Rope, QkNormRope, LinearCrossEntropy, Dropout, ResidualNorm or
+// LinearAct node's tensors are not what its backward reads and writes by (upstream: it is given a gradient of its output).  No device call.
 void check_node(const Node* n, bool upstream);
 
 class BackwardEngine {
@@ -196,7 +216,10 @@ public:
     // GEMM (gn_ffn_down_glu_bwd_ws) and the FusedGLU node starts from them
     // (gn_glu_proj_bwd_ws).  The GLU output's own gradient is then never formed:
     // get_grad_buffer() for it stays 0.  bf16 only; off by default, so every gradient the
-    // reference's engine keeps is kept unless the caller asks for the fusion.
+    // reference's engine keeps is kept unless the caller asks for the fusion.  Likewise a Linear or
+    // LinearAct whose input is the output of the LinearAct node recorded right before it (with an
+    // activation, without a residual) forms the gradient in front of that activation in its own product
+    // (gn_act_linear_bwd), in fp32 as in bf16.
     void set_glu_epilogue(bool on) { glu_epilogue_ = on; }
     bool glu_epilogue() const { return glu_epilogue_; }
 
@@ -229,6 +252,10 @@ private:
     uint64_t norm_dx(Node* n, const void** add);
     uint64_t bf16_copy_for(Node* n, uint64_t dX);
     Node* glu_before(Node* n) const;
+    Node* act_before(Node* n) const;
+    // dY of a Linear-type node (in X's type) to dX or dP, dW and db
+    void linear_grads(Node* n, const void* dY, uint64_t W, uint64_t b, int M, int N, int K, int dt);
+    uint64_t take_bf16_copy(uint64_t g);
 
     void bwd_linear(Node* n);
     void bwd_act(Node* n, int kind, bool uses_output);
@@ -240,6 +267,9 @@ private:
     void bwd_rope(Node* n);
     void bwd_qk_norm_rope(Node* n);
     void bwd_linear_cross_entropy(Node* n);
+    void bwd_dropout(Node* n);
+    void bwd_residual_norm(Node* n);
+    void bwd_linear_act(Node* n);
     void bwd_add_sub(Node* n, bool sub);
     void bwd_passthrough(Node* n);
     void bwd_vsa_unpack_project(Node* n);
@@ -272,7 +302,8 @@ private:
     };
     std::vector<FusedSlot> fused_;
     // (fp32 gradient buffer, its bf16 copy) pairs a norm backward wrote in its own pass for the
-    // bf16 input of the Add visited next (bwd_layernorm, bwd_add_sub)
+    // bf16 input of the Add, or the product of the LinearAct with that residual, visited next (bwd_layernorm,
+    // bwd_add_sub, bwd_linear_act)
     std::vector<std::pair<uint64_t, uint64_t>> bf16_copies_;
     // norm backwards whose parameter gradients are still partial rows in their workspaces,
     // summed by one gn_norm_finish at the end of the pass (or before anything reads them)
@@ -282,6 +313,9 @@ private:
     bool glu_epilogue_ = false;
     const Node* glu_node_ = nullptr;
     uint64_t glu_gu_ = 0;
+    // likewise the gradient in front of a LinearAct node's activation, from the node behind it
+    const Node* act_node_ = nullptr;
+    uint64_t act_dp_ = 0;
     bool norm_pending(uint64_t buf) const;
     void flush_norms();
     FusedSlot* fused_for(uint64_t weight);

@@ -15,6 +15,12 @@ Two options replace parts of it: `qk_norm_rope` norms queries and keys per head 
 `fused_loss` takes the loss from the last norm's output and E (gn_linear_xent_fwd): no logits and no
 gradient of them are kept.
 
+Three more say how a block ends: `residual_norm` takes the residual sum and the next norm in one pass
+(gn_residual_norm_fwd), with `dropout` on each branch in it and on the embedding (gn_dropout_fwd; masks from `seed`, the
+place and the step counter `self.step`, an int64 on the GPU); `fused_linear` adds the products that end a branch into
+the stream in their epilogue (gn_linear_act_fwd); `ffn="gelu"` has a feed-forward of two products, the first with its
+activation in the epilogue.
+
 `Decoder.forward()` runs the forward on the GPU through this library's forward kernels
 (untimed: gn_layernorm_fwd saving mean/rstd, gn_linear_fwd, gn_glu_linear_fwd saving the
 gate/up caches, gn_attn_fwd saving the fp32 row logsumexp; torch only for the embedding
@@ -32,7 +38,15 @@ import gn_bwd as gn
 
 class Decoder:
     def __init__(self, layers=12, d=768, heads=12, ff=3072, vocab=32000, batch=8, seq=1024,
-                 seed=5, device="cuda:0", glu_epilogue=True, qk_norm_rope=False, fused_loss=False):
+                 seed=5, device="cuda:0", glu_epilogue=True, qk_norm_rope=False, fused_loss=False,
+                 residual_norm=False, dropout=0.0, fused_linear=False, ffn="geglu"):
+        if dropout and not residual_norm:
+            raise ValueError("dropout goes with residual_norm")
+        if fused_linear and residual_norm:
+            raise ValueError("residual_norm and fused_linear each take the residual sum")
+        if ffn not in ("geglu", "gelu"):
+            raise ValueError(f"ffn {ffn!r}: geglu or gelu")
+        self.residual_norm, self.p, self.fused_linear, self.ffn, self.seed = residual_norm, dropout, fused_linear, ffn, seed
         self.L, self.d, self.H, self.ff, self.V = layers, d, heads, ff, vocab
         self.glu_epilogue, self.qk_norm_rope, self.fused_loss = glu_epilogue, qk_norm_rope, fused_loss
         self.B, self.S, self.T = batch, seq, batch * seq
@@ -58,6 +72,7 @@ class Decoder:
                 p["qn"], p["kn"] = const(d // heads, 1), const(d // heads, 1)
             self.freqs, self.mscale = gn.rope_freqs(d // heads, device=self.dev)
         self.lnf_g, self.lnf_b = const(d, 1), const(d, 0)
+        self.step = torch.zeros(1, device=self.dev, dtype=torch.int64)
         ids = torch.randint(0, vocab, (batch, seq), device=self.dev, generator=g)
         self.ids = ids.reshape(-1).to(torch.int32).contiguous()
         self.tgt = torch.roll(ids, -1, dims=1).reshape(-1).to(torch.int32).contiguous()
@@ -72,10 +87,16 @@ class Decoder:
         bf = torch.bfloat16
         x = self.E[self.ids.long()].float().contiguous()  # fp32 residual stream
         self.x0 = x
+        if self.p:
+            x = self.x0d = gn.dropout_fwd(x, self.p, self.seed, stream=0, step=self.step)
         acts = []
-        for p in self.layers:
+        n1 = None
+        for i, p in enumerate(self.layers):
             a = {"x": x}
-            a["n1"], a["m1"], a["r1"] = gn.layernorm_fwd(x, p["ln1_g"], p["ln1_b"], out_dtype=bf)
+            if n1 is None:
+                a["n1"], a["m1"], a["r1"] = gn.layernorm_fwd(x, p["ln1_g"], p["ln1_b"], out_dtype=bf)
+            else:
+                a["n1"] = n1
             a["qkv"] = gn.linear_fwd(a["n1"], p["Wqkv"], p["bqkv"])
             if self.qk_norm_rope:
                 # the rows the attention's backward reads, and from them the forward's heads
@@ -87,22 +108,50 @@ class Decoder:
             q, k, v = (t.contiguous() for t in rows.view(B, S, 3, H, D).permute(2, 0, 3, 1, 4))
             O, a["lse"] = gn.attn_fwd(q, k, v, causal=True, rope="none", ws=ws)
             a["o"] = O.permute(0, 2, 1, 3).reshape(T, d).contiguous()
-            a["ao"] = gn.linear_fwd(a["o"], p["Wo"], p["bo"])
-            a["x2"] = (x + a["ao"].float()).contiguous()
-            a["n2"], a["m2"], a["r2"] = gn.layernorm_fwd(a["x2"], p["ln2_g"], p["ln2_b"], out_dtype=bf)
-            a["gate"], a["up"], a["h"] = gn.glu_linear_fwd("geglu_up", a["n2"], p["Wg"], p["Wu"],
-                                                           p["bg"], p["bu"])
-            a["f"] = gn.linear_fwd(a["h"], p["Wd"], p["bd"])
-            a["x3"] = (a["x2"] + a["f"].float()).contiguous()
+            if self.fused_linear:
+                a["x2"] = gn.linear_act_fwd(a["o"], p["Wo"], p["bo"], residual=x)
+            else:
+                a["ao"] = gn.linear_fwd(a["o"], p["Wo"], p["bo"])
+            if self.residual_norm:
+                a["x2"], a["n2"] = self._branch(a["ao"], x, p["ln2_g"], p["ln2_b"], 2 * i + 1)
+            else:
+                if not self.fused_linear:
+                    a["x2"] = (x + a["ao"].float()).contiguous()
+                a["n2"], a["m2"], a["r2"] = gn.layernorm_fwd(a["x2"], p["ln2_g"], p["ln2_b"], out_dtype=bf)
+            if self.ffn == "gelu":
+                a["h"], a["pre"] = gn.linear_act_fwd(a["n2"], p["Wu"], p["bu"], act="gelu_tanh", need_pre=True)
+            else:
+                a["gate"], a["up"], a["h"] = gn.glu_linear_fwd("geglu_up", a["n2"], p["Wg"], p["Wu"],
+                                                               p["bg"], p["bu"])
+            if self.fused_linear:
+                a["x3"] = gn.linear_act_fwd(a["h"], p["Wd"], p["bd"], residual=a["x2"])
+            else:
+                a["f"] = gn.linear_fwd(a["h"], p["Wd"], p["bd"])
+            if self.residual_norm:
+                a["x3"], n1 = self._branch(a["f"], a["x2"], *self._norm_after(i), 2 * i + 2)
+            elif not self.fused_linear:
+                a["x3"] = (a["x2"] + a["f"].float()).contiguous()
             acts.append(a)
             x = a["x3"]
-        self.nf, self.mf, self.rf = gn.layernorm_fwd(x, self.lnf_g, self.lnf_b, out_dtype=bf)
+        if self.residual_norm:
+            self.nf = n1
+        else:
+            self.nf, self.mf, self.rf = gn.layernorm_fwd(x, self.lnf_g, self.lnf_b, out_dtype=bf)
         if self.fused_loss:
             self.row_loss, self.lse = gn.linear_xent_fwd(self.nf, self.E, self.tgt)
         else:
             self.logits = gn.linear_fwd(self.nf, self.E)
         self.acts = acts
         torch.cuda.synchronize()
+
+    def _norm_after(self, i):
+        """The weights of the norm behind layer i: the next layer's first, or the last one."""
+        if i + 1 < self.L:
+            return self.layers[i + 1]["ln1_g"], self.layers[i + 1]["ln1_b"]
+        return self.lnf_g, self.lnf_b
+
+    def _branch(self, h, x, w, b, place):
+        return gn.residual_norm_fwd(h, x, pre="layer", pre_w=w, pre_b=b, p=self.p, seed=self.seed, stream=place, step=self.step)
 
     # ------------------------------------------------------------------ tape
     def record(self, tape):
@@ -112,9 +161,19 @@ class Decoder:
         B, S, H, d = self.B, self.S, self.H, self.d
         n = tape.record_op(op.Embedding, [t(self.ids)], [t(self.x0)], gb.embedding_params(self.V))
         tape.save_for_backward(n, [P(self.E)])
-        for p, a in zip(self.layers, self.acts):
-            n = tape.record_op(op.LayerNorm, [t(a["x"], True)], [t(a["n1"])], gb.layernorm_params())
-            tape.save_for_backward(n, [P(p["ln1_g"]), P(p["ln1_b"]), P(a["m1"]), P(a["r1"])])
+        if self.p:
+            n = tape.record_op(op.Dropout, [t(self.x0, True)], [t(self.x0d)], gb.dropout_params(self.p, self.seed))
+            tape.save_for_backward(n, [P(self.step)])
+
+        def branch(h, x, y, z, w, b, place):
+            n = tape.record_op(op.ResidualNorm, [t(h, True), t(x, True)], [t(y), t(z)],
+                               gb.residual_norm_params(pre="layer", p=self.p, seed=self.seed, stream=place))
+            tape.save_for_backward(n, [0, 0, P(w), P(b), 0, P(self.step)])
+
+        for i, (p, a) in enumerate(zip(self.layers, self.acts)):
+            if "m1" in a:
+                n = tape.record_op(op.LayerNorm, [t(a["x"], True)], [t(a["n1"])], gb.layernorm_params())
+                tape.save_for_backward(n, [P(p["ln1_g"]), P(p["ln1_b"]), P(a["m1"]), P(a["r1"])])
             n = tape.record_op(op.Linear, [t(a["n1"], True)], [t(a["qkv"])])
             tape.save_for_backward(n, [P(p["Wqkv"]), P(p["bqkv"])])
             rows = a["qkv"]
@@ -130,21 +189,38 @@ class Decoder:
             n = tape.record_op(op.FlashAttention2, [qkv], [o],
                                gb.attention_params(causal=True, rope="none", fused_qkv_heads=H))
             tape.save_for_backward(n, [P(a["lse"])])
-            n = tape.record_op(op.Linear, [t(a["o"], True)], [t(a["ao"])])
-            tape.save_for_backward(n, [P(p["Wo"]), P(p["bo"])])
-            tape.record_op(op.Add, [t(a["x"], True), t(a["ao"], True)], [t(a["x2"])])
-            n = tape.record_op(op.LayerNorm, [t(a["x2"], True)], [t(a["n2"])], gb.layernorm_params())
-            tape.save_for_backward(n, [P(p["ln2_g"]), P(p["ln2_b"]), P(a["m2"]), P(a["r2"])])
-            n = tape.record_op(op.FusedGLU, [t(a["n2"], True)], [t(a["h"])],
-                               gb.fused_glu_params("geglu_up"))
-            tape.save_for_backward(n, [P(p["Wg"]), P(p["Wu"]), P(a["gate"]), P(a["up"]),
-                                       P(p["bg"]), P(p["bu"])])
-            n = tape.record_op(op.Linear, [t(a["h"], True)], [t(a["f"])])
-            tape.save_for_backward(n, [P(p["Wd"]), P(p["bd"])])
-            tape.record_op(op.Add, [t(a["x2"], True), t(a["f"], True)], [t(a["x3"])])
+            def ends_branch(x, W, b, out, stream, y):
+                """The product that ends a branch, and the residual sum."""
+                if self.fused_linear:
+                    n = tape.record_op(op.LinearAct, [t(x, True), t(stream, True)], [t(y)], gb.linear_act_params())
+                else:
+                    n = tape.record_op(op.Linear, [t(x, True)], [t(out)])
+                tape.save_for_backward(n, [P(W), P(b)])
+                if not self.fused_linear and not self.residual_norm:
+                    tape.record_op(op.Add, [t(stream, True), t(out, True)], [t(y)])
+
+            ends_branch(a["o"], p["Wo"], p["bo"], a.get("ao"), a["x"], a["x2"])
+            if self.residual_norm:
+                branch(a["ao"], a["x"], a["x2"], a["n2"], p["ln2_g"], p["ln2_b"], 2 * i + 1)
+            else:
+                n = tape.record_op(op.LayerNorm, [t(a["x2"], True)], [t(a["n2"])], gb.layernorm_params())
+                tape.save_for_backward(n, [P(p["ln2_g"]), P(p["ln2_b"]), P(a["m2"]), P(a["r2"])])
+            if self.ffn == "gelu":
+                n = tape.record_op(op.LinearAct, [t(a["n2"], True)], [t(a["h"])], gb.linear_act_params("gelu_tanh"))
+                tape.save_for_backward(n, [P(p["Wu"]), P(p["bu"]), P(a["pre"])])
+            else:
+                n = tape.record_op(op.FusedGLU, [t(a["n2"], True)], [t(a["h"])],
+                                   gb.fused_glu_params("geglu_up"))
+                tape.save_for_backward(n, [P(p["Wg"]), P(p["Wu"]), P(a["gate"]), P(a["up"]),
+                                           P(p["bg"]), P(p["bu"])])
+            ends_branch(a["h"], p["Wd"], p["bd"], a.get("f"), a["x2"], a["x3"])
+            if self.residual_norm:
+                z = self.acts[i + 1]["n1"] if i + 1 < self.L else self.nf
+                branch(a["f"], a["x2"], a["x3"], z, *self._norm_after(i), 2 * i + 2)
         last = self.acts[-1]["x3"]
-        n = tape.record_op(op.LayerNorm, [t(last, True)], [t(self.nf)], gb.layernorm_params())
-        tape.save_for_backward(n, [P(self.lnf_g), P(self.lnf_b), P(self.mf), P(self.rf)])
+        if not self.residual_norm:
+            n = tape.record_op(op.LayerNorm, [t(last, True)], [t(self.nf)], gb.layernorm_params())
+            tape.save_for_backward(n, [P(self.lnf_g), P(self.lnf_b), P(self.mf), P(self.rf)])
         if self.fused_loss:
             n = tape.record_op(op.LinearCrossEntropy, [t(self.nf, True), t(self.tgt)], [t(self.row_loss)],
                                gb.linear_cross_entropy_params(self.V, 1.0 / self.T))
@@ -169,7 +245,8 @@ class Decoder:
         """Backward GEMM + attention FLOPs (dX and dW of every projection, causal attention
         with the P recompute counted once: 5 products over half the score matrix)."""
         T, d, ff, V, S, H = self.T, self.d, self.ff, self.V, self.S, self.H
-        per_layer = (2 * 2 * T * d * 3 * d + 2 * 2 * T * d * d + 2 * 2 * T * d * ff * 2
+        up = 2 if self.ffn == "geglu" else 1
+        per_layer = (2 * 2 * T * d * 3 * d + 2 * 2 * T * d * d + 2 * 2 * T * d * ff * up
                      + 2 * 2 * T * ff * d + 5 * 2.0 * S * S * (d // H) * 0.5 * self.B * H)
         return self.L * per_layer + 2 * 2 * T * d * V
 
@@ -177,6 +254,7 @@ class Decoder:
         """Forward GEMM + attention FLOPs: every projection once, causal attention as 2
         products over half the score matrix, the LM head."""
         T, d, ff, V, S, H = self.T, self.d, self.ff, self.V, self.S, self.H
-        per_layer = (2 * T * d * 3 * d + 2 * T * d * d + 2 * T * d * ff * 2 + 2 * T * ff * d
+        up = 2 if self.ffn == "geglu" else 1
+        per_layer = (2 * T * d * 3 * d + 2 * T * d * d + 2 * T * d * ff * up + 2 * T * ff * d
                      + 2 * 2.0 * S * S * (d // H) * 0.5 * self.B * H)
         return self.L * per_layer + 2 * T * d * V

@@ -17,6 +17,9 @@ import grilly_core
 DTYPE_F32, DTYPE_F16, DTYPE_U32, DTYPE_I32, DTYPE_BF16 = 0, 1, 2, 3, 4
 GLU_KIND = {"swiglu_up": 0, "swiglu_gate": 1, "geglu_up": 2, "geglu_gate": 3, "reglu_up": 4}
 ROPE_MODE = {"none": 0, "interleaved": 1, "half": 2}
+NORM_KIND = {"none": 0, "rms": 1, "layer": 2}
+ACT_KIND = {"none": -1, "relu": 0, "gelu_tanh": 1, "gelu_erf": 2, "silu": 3, "tanh": 4, "sigmoid": 5}
+_U64 = 2 ** 64 - 1
 
 
 def create_tape_context(device, arena_capacity: int = 64 << 20):
@@ -115,6 +118,26 @@ def linear_cross_entropy_params(vocab: int, scale: float = 1.0) -> bytes:
     scale: every row's gradient where the node is the root; a gradient from a node behind it (a mean of the
     loss, say) is multiplied by scale, which is 1 there."""
     return struct.pack("<If", int(vocab), scale)
+
+
+def dropout_params(p: float, seed: int, stream: int = 0, step: int = 0) -> bytes:
+    """Dropout node, with the forward's numbers; saved slots {step counter or 0} (a device int64, added to step)."""
+    return struct.pack("<dQQQ", p, seed & _U64, stream & _U64, step & _U64)
+
+
+def residual_norm_params(post: str = "none", pre: str = "none", gates: int = 0, scale: float = 1.0, res_scale: float = 1.0,
+                         p: float = 0.0, seed: int = 0, stream: int = 0, step: int = 0, post_eps: float | None = None,
+                         pre_eps: float | None = None) -> bytes:
+    """ResidualNorm node: inputs h and x, outputs y (and z with a pre norm), with the forward's numbers; saved slots
+    {post_w, post_b, pre_w, pre_b, gate, step counter}, 0 where there is none.  eps None: residual_norm_fwd's."""
+    eps = {"none": 0.0, "rms": 1e-6, "layer": 1e-5}
+    return struct.pack("<dQQQffffIIIxxxx", p, seed & _U64, stream & _U64, step & _U64, eps[post] if post_eps is None else post_eps,
+                       eps[pre] if pre_eps is None else pre_eps, scale, res_scale, NORM_KIND[post], NORM_KIND[pre], gates)
+
+
+def linear_act_params(act: str = "none") -> bytes:
+    """LinearAct node: inputs X and optionally the residual; saved slots {W, b or 0, P (0 without an activation)}."""
+    return struct.pack("<i", ACT_KIND[act])
 
 
 def fused_glu_params(kind: str = "swiglu_up") -> bytes:
