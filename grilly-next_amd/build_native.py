@@ -26,7 +26,8 @@ KERNEL_SOURCES = ["gn_errors.cpp", "gn_elementwise.hip", "gn_norm.hip", "gn_gemm
                   "gn_gemm_dma_f32a.hip", "gn_gemm_dma_f32b.hip", "gn_gemm_dma_glu.hip",
                   "gn_gemm_wave.hip", "gn_gemm_stream.hip", "gn_vsa.hip", "gn_attn.hip", "gn_optim.hip",
                   "gn_tapeops.hip", "gn_fwd.hip", "gn_skinny.hip", "gn_vsa_fwd.hip", "gn_gemm_f32.hip", "gn_gemm_f32mm.hip", "gn_lane.cpp",
-                  "gn_rope.hip", "gn_linear_xent.hip", "gn_residual.hip", "gn_linear_act.hip"]
+                  "gn_rope.hip", "gn_linear_xent.hip", "gn_residual.hip",
+                  "gn_linear_act.hip", "gn_linear_act_bf16.hip", "gn_linear_act_f32.hip", "gn_linear_act_bwd.hip"]
 # measurement kernels for bench.py --ceilings, kept out of the backward library
 PROBE_SOURCES = ["gn_probe.hip"]
 TAPE_SOURCES = ["tape/autograd.cpp", "tape/device.cpp", "tape/checkpoint.cpp", "tape/hypernet.cpp",

@@ -1,0 +1,67 @@
+// gn_act.h — activations and their slopes in the fewest instructions, for the epilogues of products (gn_linear_act.hip).
+#pragma once
+
+#include <type_traits>
+
+#include "gn_math.h"
+
+namespace gn {
+namespace {
+
+// With the hardware's exponential and reciprocal (1 ulp), not the correctly rounded division of six more instructions,
+// and in the fewest full-rate instructions: a 256 x 128 tile has 128 elements a lane, 0.25 us of the tile for each
+// instruction of an element.
+__device__ __forceinline__ float rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float sigmoid_of(float x) { return rcp(1.0f + __builtin_amdgcn_exp2f(x * -kLog2e)); }
+// (1 + tanh z) / 2 = sigmoid(2 z), 2 z = 2 sqrt(2 / pi) (x + 0.044715 x^3)
+constexpr float kG1 = 2.0f * kSqrt2OverPi, kG3 = 2.0f * kSqrt2OverPi * kGeluC;
+__device__ __forceinline__ float gelu_gate(float x, float xx) {
+    return rcp(1.0f + __builtin_amdgcn_exp2f(x * fmaf(xx, -kLog2e * kG3, -kLog2e * kG1)));
+}
+
+template <int KIND>
+__device__ __forceinline__ float act_of(float x) {
+    if constexpr (KIND == GN_ACT_RELU) return x > 0.f ? x : 0.f;
+    else if constexpr (KIND == GN_ACT_GELU_TANH) return x * gelu_gate(x, x * x);
+    else if constexpr (KIND == GN_ACT_GELU_ERF) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+    else if constexpr (KIND == GN_ACT_SILU) return x * sigmoid_of(x);
+    else if constexpr (KIND == GN_ACT_TANH) return fmaf(-2.0f, rcp(1.0f + __builtin_amdgcn_exp2f(x * (2.0f * kLog2e))), 1.0f);
+    else return sigmoid_of(x);
+}
+// tanh and sigmoid at their output; of x sigmoid(u): s + x s (1 - s) u' = s (1 + (1 - s) x u')
+template <int KIND>
+__device__ __forceinline__ float slope_of(float x) {
+    if constexpr (KIND == GN_ACT_GELU_TANH) {
+        const float xx = fminf(x * x, 400.f), s = gelu_gate(x, xx);  // from |x| = 20 on the gate is 0 or 1; 0 times inf is NaN
+        return s * fmaf(1.0f - s, x * fmaf(xx, 3.0f * kG3, kG1), 1.0f);
+    } else if constexpr (KIND == GN_ACT_SILU) {
+        const float s = sigmoid_of(x);
+        return s * fmaf(1.0f - s, x, 1.0f);
+    } else {
+        return act_grad<KIND>(x);
+    }
+}
+
+// f(its compile-time number) for an activation: KIND, or kAny: of the number at run time
+constexpr int kAny = -2;
+template <int KIND, bool NONE, typename F>
+__device__ __forceinline__ void by_act(int kind, F&& f) {
+    using std::integral_constant;
+    if constexpr (KIND != kAny) {
+        f(integral_constant<int, KIND>{});
+        return;
+    } else switch (kind) {
+        case GN_ACT_RELU: f(integral_constant<int, GN_ACT_RELU>{}); break;
+        case GN_ACT_GELU_TANH: f(integral_constant<int, GN_ACT_GELU_TANH>{}); break;
+        case GN_ACT_GELU_ERF: f(integral_constant<int, GN_ACT_GELU_ERF>{}); break;
+        case GN_ACT_SILU: f(integral_constant<int, GN_ACT_SILU>{}); break;
+        case GN_ACT_TANH: f(integral_constant<int, GN_ACT_TANH>{}); break;
+        default:
+            if (!NONE || kind == GN_ACT_SIGMOID) f(integral_constant<int, GN_ACT_SIGMOID>{});
+            else f(integral_constant<int, GN_ACT_NONE>{});
+    }
+}
+
+}  // namespace
+}  // namespace gn

@@ -212,6 +212,19 @@ def test_extreme_arguments(gn):
                  2 ** -20 * (1 + X.double().abs().clamp(max=128)))
 
 
+def test_extreme_slopes(gn):
+    """Derivatives far from 0: those of the activations' ends, and no NaN (W is the unit matrix: dP = dY act'(P))."""
+    x = torch.tensor([0.0, 5., -5., 19., -19., 21., -21., 90., -90., 1e4, -1e4, 1e20, -1e20, 1e30, -1e30, 1e-30], device=DEV)
+    for dtype in (BF, F32):
+        P = x.to(dtype).view(1, 16).repeat(16, 1)
+        W = torch.eye(16, device=DEV, dtype=dtype)
+        dY = torch.ones(16, 16, device=DEV, dtype=dtype)
+        for act in ("relu", "gelu_tanh", "gelu_erf", "silu"):
+            p = P.double().clamp(-600, 600)  # fp64's own 0 times inf
+            dP = gn.act_linear_bwd(act, dY, P, None, W, need_dw=False)[0]
+            near(dP, slope64(p, act), 2 ** -19 * (1 + p.abs()).clamp(max=128))
+
+
 def test_a_block_of_both(gn):
     """The feed-forward block as it is trained: up with its activation, down with the fp32 residual, and back, against
     autograd in fp64 at the saved tensors."""
