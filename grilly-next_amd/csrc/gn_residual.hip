@@ -17,6 +17,7 @@
 // LDS, and leave as one partial row a block, which a second launch adds in a fixed order: no atomics.
 // Wider rows are read three times or more (kernels at the end).
 #include <algorithm>
+#include <type_traits>
 
 #include "gn_common.h"
 #include "gn_rng.h"
@@ -114,6 +115,12 @@ struct Cols {
     int t, F;
     __device__ __forceinline__ int at(int j, int e) const { return VEC ? 8 * (t + T * j) + e : t + T * (8 * j + e); }
     __device__ __forceinline__ bool has(int j, int e) const { return at(j, VEC ? 0 : e) < F; }
+    // the place of element e in a row p: the wave's address and 32 bits of the lane's, without a vector instruction
+    template <typename E>
+    __device__ __forceinline__ E* in(E* p, int j, int e) const {
+        using B = std::conditional_t<std::is_const_v<E>, const char, char>;
+        return reinterpret_cast<E*>(reinterpret_cast<B*>(p) + (uint32_t)at(j, e) * (uint32_t)sizeof(E));
+    }
 };
 
 // Eight elements of a lane as they lie in memory (bf16 stays packed until it is used).
@@ -123,12 +130,12 @@ template <bool VEC> struct Raw<float, VEC> {
     template <typename C>
     __device__ __forceinline__ void load(const float* p, const C& c, int j) {
         if constexpr (VEC) {
-            if (c.has(j, 0)) { chunk8<float>::ld(p + c.at(j, 0), v); return; }
+            if (c.has(j, 0)) { chunk8<float>::ld(c.in(p, j, 0), v); return; }
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = 0.f;
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = c.has(j, e) ? p[c.at(j, e)] : 0.f;
+            for (int e = 0; e < 8; ++e) v[e] = c.has(j, e) ? *c.in(p, j, e) : 0.f;
         }
     }
     template <typename C>
@@ -144,12 +151,12 @@ template <bool VEC> struct Raw<bf16_t, VEC> {
     __device__ __forceinline__ void load(const bf16_t* p, const C& c, int j) {
         if constexpr (VEC) {
             uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (c.has(j, 0)) x = *reinterpret_cast<const uint4*>(p + c.at(j, 0));
+            if (c.has(j, 0)) x = *reinterpret_cast<const uint4*>(c.in(p, j, 0));
             w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
         } else {
             uint32_t q[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) q[e] = c.has(j, e) ? (uint32_t)p[c.at(j, e)] : 0u;
+            for (int e = 0; e < 8; ++e) q[e] = c.has(j, e) ? (uint32_t)*c.in(p, j, e) : 0u;
 #pragma unroll
             for (int e = 0; e < 4; ++e) w[e] = q[2 * e] | (q[2 * e + 1] << 16);
         }
@@ -168,11 +175,11 @@ template <bool VEC> struct Raw<bf16_t, VEC> {
 template <typename T, bool VEC, typename C>
 __device__ __forceinline__ void store8(T* p, const C& c, int j, const float (&v)[8]) {
     if constexpr (VEC) {
-        if (c.has(j, 0)) chunk8<T>::st(p + c.at(j, 0), v);
+        if (c.has(j, 0)) chunk8<T>::st(c.in(p, j, 0), v);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (c.has(j, e)) io<T>::st(p, c.at(j, e), v[e]);
+            if (c.has(j, e)) io<T>::st(c.in(p, j, e), 0, v[e]);
     }
 }
 
@@ -186,28 +193,51 @@ __device__ __forceinline__ void drop_piece(float (&v)[8], const C& c, int j, uin
     }
 }
 
+// The sum of a wave's lanes, in lane 63: within rows of 16 lanes as wave_sum (gn_common.h), then row 0 onto row 1 and
+// row 2 onto row 3 (row_bcast15), then the lower half onto the upper (row_bcast31).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ float wave_total(float v) {
+    v = dpp_add<0xB1, 0xF>(v);
+    v = dpp_add<0x4E, 0xF>(v);
+    v = dpp_add<0x141, 0xF>(v);
+    v = dpp_add<0x140, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    return dpp_add<0x143, 0xC>(v);
+}
+
 // Sums of N values over the lanes of a row.  Rows of several waves exchange theirs through one of two
 // LDS buffers in turn: a wave that writes a buffer again has passed the barrier of the sum in between,
-// which every wave reached after its reads of it.
+// which every wave reached after its reads of it.  Lane l reads the sums of wave l % WPR, and DPP moves among WPR
+// lanes add them up: one LDS read, whatever the number of waves.
 template <int WPR>
 struct RowSum {
-    float (*buf)[WPR][4];  // [2]
+    float4 (*buf)[WPR][2];  // [2]
     int wave, lane, turn;
     template <int N>
     __device__ __forceinline__ void operator()(float (&v)[N]) {
-        static_assert(N <= 4, "buffer");
+        static_assert(N <= 8, "buffer");
 #pragma unroll
-        for (int k = 0; k < N; ++k) v[k] = wave_sum(v[k]);
-        if constexpr (WPR > 1) {
-            if (lane == 0)
+        for (int k = 0; k < N; ++k) v[k] = wave_total(v[k]);
+        if constexpr (WPR == 1) {
 #pragma unroll
-                for (int k = 0; k < N; ++k) buf[turn][wave][k] = v[k];
+            for (int k = 0; k < N; ++k) v[k] = lane_f(v[k], 63);
+        } else {
+            auto value = [&](int k) { return k < N ? v[k < N ? k : 0] : 0.f; };
+            if (lane == 63) {
+                buf[turn][wave][0] = make_float4(value(0), value(1), value(2), value(3));
+                if constexpr (N > 4) buf[turn][wave][1] = make_float4(value(4), value(5), value(6), value(7));
+            }
             __syncthreads();
+            const float4 w = buf[turn][lane & (WPR - 1)][0], x = N > 4 ? buf[turn][lane & (WPR - 1)][1] : w;
+            const float u[8] = {w.x, w.y, w.z, w.w, x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                v[k] = buf[turn][0][k];
-#pragma unroll
-                for (int w = 1; w < WPR; ++w) v[k] += buf[turn][w][k];
+                v[k] = dpp_add<0xB1, 0xF>(u[k]);
+                if constexpr (WPR > 2) v[k] = dpp_add<0x4E, 0xF>(v[k]);
+                if constexpr (WPR > 4) v[k] = dpp_add<0x141, 0xF>(v[k]);
             }
             turn ^= 1;
         }
@@ -257,7 +287,7 @@ __device__ __forceinline__ void row_stats(const float (&v)[NC][8], int kind, flo
 template <typename TX, typename TH, int WPR, int NC, bool VEC>
 __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void residual_fwd(FwdArgs<TX, TH> a) {
     constexpr int T = 64 * WPR, RPB = WPR == 1 ? 4 : 1;  // rows of a block at a time
-    __shared__ float buf[2][WPR][4];
+    __shared__ float4 buf[2][WPR][2];
     const Cols<T, NC, VEC> c{(int)threadIdx.x & (T - 1), a.F};
     RowSum<WPR> sum{buf, (int)(threadIdx.x >> 6) & (WPR - 1), (int)threadIdx.x & 63, 0};
     const uint64_t key = a.mask.t ? a.mask.key() : 0;
@@ -278,7 +308,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void residual_fwd(FwdArg
     int at_gate = 0;
 
     const int64_t stride = (int64_t)gridDim.x * RPB;
-    int64_t r = (int64_t)blockIdx.x * RPB + (WPR == 1 ? (int)(threadIdx.x >> 6) : 0);
+    int64_t r = (int64_t)blockIdx.x * RPB + (WPR == 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) : 0);
     Raw<TH, VEC> h[NC];
     Raw<TX, VEC> x[NC];
     auto load = [&](int64_t row, Raw<TH, VEC> (&hh)[NC], Raw<TX, VEC> (&xx)[NC]) {
@@ -373,31 +403,56 @@ __device__ __forceinline__ float norm_grad(float g, float vc, float r, float u, 
     return r * (g - u - vc * (r * w));
 }
 
+// Eight weights of a lane: as they lie in memory, or as floats times a factor.
+template <typename T, bool VEC, bool FLOATS>
+struct Weights : Raw<std::conditional_t<FLOATS, float, T>, VEC> {
+    template <typename C>
+    __device__ __forceinline__ void set(const T* p, float absent, float factor, const C& c, int j) {
+        if constexpr (FLOATS) {
+            Raw<T, VEC> r;
+            if (p) r.load(p, c, j);
+            else r.fill(absent, c, j);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) this->v[e] = r[e] * factor;
+        } else {
+            if (p) this->load(p, c, j);
+            else this->fill(absent, c, j);
+        }
+    }
+};
+
 // POST: there is a norm after the block; LAYER: a LayerNorm among the norms (biases and means); GATE: the
-// gate's gradient is wanted.
+// gate's gradient is wanted.  Between a row's loads and its stores are two or three sums with barriers, which
+// something has to hide.  Where the registers of a wave leave room for four a SIMD, that is a second block a
+// CU (two_blocks); where there are three sums over rows or fewer, a wave works on two rows side by side (RP), whose sums
+// share their barriers, with weights as floats; otherwise the next row's loads alone.  Measured (us, one row and one
+// block a CU -> two blocks, two rows): 8192 x 768 LayerNorm, fp32 stream 29.4 -> 25.8, 28.2; 16001 x 4096 with both norms and a
+// gate 185 -> 226 (spills), 178.
+__host__ __device__ constexpr bool two_blocks(bool vec, bool post, bool layer, bool gate, size_t x_size) {
+    return vec && !gate && (!post || (!layer && x_size == 2));
+}
 template <typename TX, typename TH, int WPR, int NC, bool VEC, bool POST, bool LAYER, bool GATE>
-__global__ __launch_bounds__(512) void residual_bwd(BwdArgs<TX, TH> a) {
-    constexpr int T = 64 * WPR, RG = 512 / T;  // rows of a block at a time
-    constexpr bool AHEAD = NC == 1;             // the next row's loads before this row's work
-    __shared__ float rbuf[RG][2][WPR][4];
+__global__ __launch_bounds__(512, NC == 1 && two_blocks(VEC, POST, LAYER, GATE, sizeof(TX)) ? 4 : 2) void residual_bwd(BwdArgs<TX, TH> a) {
+    constexpr int T = 64 * WPR, RG = 512 / T;  // rows of a block side by side, times RP
+    constexpr int SUMS = GATE + (POST ? 1 + LAYER : 0) + 1 + LAYER;
+    constexpr int RP = NC == 1 && SUMS <= 3 && !two_blocks(VEC, POST, LAYER, GATE, sizeof(TX)) ? 2 : 1;
+    constexpr bool AHEAD = NC == 1, FW = RP == 2;  // AHEAD: the next rows' loads before these rows' work
+    constexpr int NS = POST ? 3 : 2;
+    __shared__ float4 rbuf[RG][2][WPR][2];
     __shared__ __align__(16) float acc_lds[RG > 1 ? RG * T * NC * 8 : 4];
-    const int rg = threadIdx.x / T;
+    const int rg = __builtin_amdgcn_readfirstlane((int)threadIdx.x / T);  // the wave's
     const Cols<T, NC, VEC> c{(int)threadIdx.x & (T - 1), a.F};
     RowSum<WPR> sum{rbuf[rg], (int)(threadIdx.x >> 6) & (WPR - 1), (int)threadIdx.x & 63, 0};
     const uint64_t key = a.mask.t ? a.mask.key() : 0;
-    const float inv = 1.0f / (float)a.F;
+    const float inv = 1.0f / (float)a.F, gate_scale = FW ? 1.f : a.scale;  // of the gate's weights as they are held
 
-    Raw<TH, VEC> wp[POST ? NC : 1], bp[POST && LAYER && GATE ? NC : 1], wn[NC], gate[NC];
+    Weights<TH, VEC, FW> wp[POST ? NC : 1], bp[POST && LAYER && GATE ? NC : 1], wn[NC], gate[NC];
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-        auto weights = [&](Raw<TH, VEC>& to, const TH* p, float absent) {
-            if (p) to.load(p, c, j);
-            else to.fill(absent, c, j);
-        };
-        if constexpr (POST) weights(wp[j], a.post_w, 1.f);
-        if constexpr (POST && LAYER && GATE) weights(bp[j], a.post_b, 0.f);
-        weights(wn[j], a.pre_w, 1.f);
-        weights(gate[j], a.gate, 1.f);
+        if constexpr (POST) wp[j].set(a.post_w, 1.f, 1.f, c, j);
+        if constexpr (POST && LAYER && GATE) bp[j].set(a.post_b, 0.f, 1.f, c, j);
+        wn[j].set(a.pre_w, 1.f, 1.f, c, j);
+        gate[j].set(a.gate, 1.f, a.scale, c, j);
     }
     int at_gate = 0;
 
@@ -417,7 +472,7 @@ __global__ __launch_bounds__(512) void residual_bwd(BwdArgs<TX, TH> a) {
         Raw<TH, VEC> h[NC], dz[NC];
         Raw<TX, VEC> y[NC], dy[NC];
     };
-    auto load = [&](int64_t r, Row& w) {
+    auto load = [&](int64_t r, Row& w) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < NC; ++j) {
             if (a.dz) w.dz[j].load(a.dz + r * a.F, c, j), w.y[j].load(a.y + r * a.F, c, j);
@@ -425,6 +480,23 @@ __global__ __launch_bounds__(512) void residual_bwd(BwdArgs<TX, TH> a) {
             if (a.dy) w.dy[j].load(a.dy + r * a.F, c, j);
             else w.dy[j].fill(0.f, c, j);
             if (POST || GATE) w.h[j].load(a.h + r * a.F, c, j);
+        }
+    };
+    // a wave's rows of a turn, from r on, of those below r1; past them zeros, which add nothing to any sum
+    auto load_turn = [&](int r, int r1, Row (&w)[RP]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < RP; ++k) {
+            if (r + k * RG < r1) {
+                load(r + k * RG, w[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NC; ++j) {
+                    w[k].h[j].fill(0.f, c, j);
+                    w[k].dz[j].fill(0.f, c, j);
+                    w[k].y[j].fill(0.f, c, j);
+                    w[k].dy[j].fill(0.f, c, j);
+                }
+            }
         }
     };
 
@@ -465,128 +537,159 @@ __global__ __launch_bounds__(512) void residual_bwd(BwdArgs<TX, TH> a) {
     for (int g = g0; g < g1; ++g) {
         int r0, r1;
         a.split.rows(blockIdx.x, g, r0, r1);
-        const int turns = (r1 - r0 + RG - 1) / RG;  // the same for all waves: they meet at barriers
-        Row cur;
-        if (r0 + rg < r1) load(r0 + rg, cur);
+        const int turns = (r1 - r0 + RP * RG - 1) / (RP * RG);  // the same for all waves: they meet at barriers
+        Row cur[RP];
+        load_turn(r0 + rg, r1, cur);
         for (int i = 0; i < turns; ++i) {
-            const int r = r0 + i * RG + rg;
-            const bool on = r < r1;
-            Row nxt;
-            if (AHEAD && r + RG < r1) load(r + RG, nxt);
-            if (a.gates > 1 && on) {
-                const int q = r / a.gate_rows;
-                if (q != at_gate) {
-                    at_gate = q;
+            const int r = r0 + i * RP * RG + rg;
+            Row nxt[RP];
+            if (AHEAD && i + 1 < turns) load_turn(r + RP * RG, r1, nxt);
+            // statistics: h's, y's and the sums of the pre norm's gradient, together
+            float mp[RP] = {}, rp[RP], mn[RP] = {}, rn[RP], u[RP] = {}, w[RP], q[RP * NS] = {};
+            if constexpr (LAYER) {
+                float s[RP * NS] = {};
 #pragma unroll
-                    for (int j = 0; j < NC; ++j) gate[j].load(a.gate + (size_t)q * a.F, c, j);
-                }
-            }
-            if (WPR > 1 || on) {
-                // statistics: h's, y's and the sums of the pre norm's gradient, together
-                float mp = 0.f, rp = 1.f, mn = 0.f, rn = 1.f, u = 0.f;
-                if constexpr (LAYER) {
-                    float s[3] = {0.f, 0.f, 0.f};
+                for (int k = 0; k < RP; ++k)
 #pragma unroll
                     for (int j = 0; j < NC; ++j)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            s[0] += cur.y[j][e];
-                            s[1] += wn[j][e] * cur.dz[j][e];
-                            if constexpr (POST) s[2] += cur.h[j][e];
+                            s[NS * k] += cur[k].y[j][e];
+                            s[NS * k + 1] += wn[j][e] * cur[k].dz[j][e];
+                            if constexpr (POST) s[NS * k + 2] += cur[k].h[j][e];
                         }
-                    sum(s);
-                    if (a.pre == GN_NORM_LAYER) mn = s[0] * inv, u = s[1] * inv;
-                    if (a.post == GN_NORM_LAYER) mp = s[2] * inv;
+                sum(s);
+#pragma unroll
+                for (int k = 0; k < RP; ++k) {
+                    if (a.pre == GN_NORM_LAYER) mn[k] = s[NS * k] * inv, u[k] = s[NS * k + 1] * inv;
+                    if constexpr (POST)
+                        if (a.post == GN_NORM_LAYER) mp[k] = s[NS * k + 2] * inv;
                 }
-                float q[3] = {0.f, 0.f, 0.f};
+            }
+            // v - mu, 0 in the places that the row does not have
+            auto centred = [&](float v, float mu, int j, int e) __attribute__((always_inline)) {
+                if constexpr (LAYER) return c.has(j, e) ? v - mu : 0.f;
+                return v;
+            };
+#pragma unroll
+            for (int k = 0; k < RP; ++k)
 #pragma unroll
                 for (int j = 0; j < NC; ++j)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float yc = c.has(j, e) ? cur.y[j][e] - mn : 0.f;
-                        q[0] += yc * yc;
-                        q[1] += wn[j][e] * cur.dz[j][e] * yc;
+                        const float yc = centred(cur[k].y[j][e], mn[k], j, e);
+                        q[NS * k] += yc * yc;
+                        q[NS * k + 1] += wn[j][e] * cur[k].dz[j][e] * yc;
                         if constexpr (POST) {
-                            const float hc = c.has(j, e) ? cur.h[j][e] - mp : 0.f;
-                            q[2] += hc * hc;
+                            const float hc = centred(cur[k].h[j][e], mp[k], j, e);
+                            q[NS * k + 2] += hc * hc;
                         }
                     }
-                sum(q);
-                if (a.dz) rn = rsqrtf(q[0] * inv + a.pre_eps);
-                if constexpr (POST) rp = rsqrtf(q[2] * inv + a.post_eps);
-                const float w = q[1] * inv * rn;
-                float d[NC][8], s[2] = {0.f, 0.f};
+            sum(q);
+            float d[RP][NC][8], s[RP * (1 + LAYER)] = {};
+#pragma unroll
+            for (int k = 0; k < RP; ++k) {
+                const int row = r + k * RG;
+                const bool on = row < r1;
+                // (of no row: 1, not the 1 / sqrt(eps) that may be inf and make its zeros NaN)
+                rn[k] = on && a.dz ? rsqrtf(q[NS * k] * inv + a.pre_eps) : 1.f;
+                rp[k] = 1.f;
+                if constexpr (POST) rp[k] = on ? rsqrtf(q[NS * k + 2] * inv + a.post_eps) : 1.f;
+                w[k] = q[NS * k + 1] * inv * rn[k];
+                if (a.gates > 1 && on) {
+                    const int at = row / a.gate_rows;
+                    if (at != at_gate) {
+                        at_gate = at;
+#pragma unroll
+                        for (int j = 0; j < NC; ++j) gate[j].set(a.gate + (size_t)at * a.F, 1.f, a.scale, c, j);
+                    }
+                }
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
+                    float (&dk)[8] = d[k][j];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float yc = cur.y[j][e] - mn, dz = cur.dz[j][e];
-                        d[j][e] = cur.dy[j][e];
-                        if (a.dz) d[j][e] += norm_grad(wn[j][e] * dz, yc, rn, u, w);
-                        if (on) {
-                            dwn[j][e] += dz * yc * rn;
-                            if constexpr (LAYER) dbn[j][e] += dz;
-                        }
+                        const float yh = centred(cur[k].y[j][e], mn[k], j, e) * rn[k], dz = cur[k].dz[j][e];
+                        float gr = wn[j][e] * dz;
+                        if constexpr (LAYER) gr -= u[k];
+                        dk[e] = cur[k].dy[j][e] + rn[k] * (gr - yh * w[k]);
+                        dwn[j][e] += dz * yh;
+                        if constexpr (LAYER) dbn[j][e] += dz;
                     }
                     if (on && a.dx) {
                         float o[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) o[e] = a.res_scale * d[j][e];
-                        store8<TX, VEC>(a.dx + (int64_t)r * a.F, c, j, o);
+                        for (int e = 0; e < 8; ++e) o[e] = a.res_scale * dk[e];
+                        store8<TX, VEC>(a.dx + (int64_t)row * a.F, c, j, o);
                     }
-                    if (a.mask.t) drop_piece<VEC>(d[j], c, j, key, (uint64_t)r * a.F, a.mask);
-                    if constexpr (GATE) {
+                    if (a.mask.t) drop_piece<VEC>(dk, c, j, key, (uint64_t)row * a.F, a.mask);
+                    if constexpr (GATE) {  // dgate / scale
                         float o[8];
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            float n = cur.h[j][e];
+                            float n = cur[k].h[j][e];
                             if constexpr (POST) {
-                                n = (n - mp) * rp * wp[j][e];
+                                n = centred(n, mp[k], j, e) * rp[k] * wp[j][e];
                                 if constexpr (LAYER) n += bp[j][e];
                             }
-                            o[e] = a.scale * d[j][e] * n;
-                            if (on) dg[j][e] += o[e];
+                            o[e] = dk[e] * n;
+                            dg[j][e] += o[e];
                         }
                         if (a.gate_rows == 1 && a.gates > 1 && on) {  // a gate a row: its gradient has no sum
-                            float* const to = a.grad[kGate] + (int64_t)r * a.F;
+                            float* const to = a.grad[kGate] + (int64_t)row * a.F;
 #pragma unroll
                             for (int e = 0; e < 8; ++e)
-                                if (c.has(j, e)) to[c.at(j, e)] = a.accumulate ? to[c.at(j, e)] + o[e] : o[e];
+                                if (c.has(j, e)) to[c.at(j, e)] = a.accumulate ? to[c.at(j, e)] + a.scale * o[e] : a.scale * o[e];
                         }
                     }
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        d[j][e] *= a.scale * gate[j][e];
+                        dk[e] *= FW ? gate[j][e] : gate_scale * gate[j][e];
                         if constexpr (POST) {
-                            const float hc = cur.h[j][e] - mp;
-                            if (on) {
-                                dwp[j][e] += d[j][e] * hc * rp;
-                                if constexpr (LAYER) dbp[j][e] += d[j][e];
-                            }
-                            d[j][e] *= wp[j][e];
-                            s[0] += d[j][e];
-                            s[1] += d[j][e] * hc;
+                            const float hh = centred(cur[k].h[j][e], mp[k], j, e) * rp[k];
+                            dwp[j][e] += dk[e] * hh;
+                            if constexpr (LAYER) dbp[j][e] += dk[e];
+                            dk[e] *= wp[j][e];
+                            s[k * (1 + LAYER)] += dk[e] * hh;
+                            if constexpr (LAYER) s[k * (1 + LAYER) + 1] += dk[e];
                         }
                     }
                 }
+            }
+            if constexpr (POST) sum(s);
+#pragma unroll
+            for (int k = 0; k < RP; ++k) {
                 if constexpr (POST) {
-                    sum(s);
-                    const float pu = a.post == GN_NORM_LAYER ? s[0] * inv : 0.f, pw = s[1] * inv * rp;
+                    const float pw = s[k * (1 + LAYER)] * inv;
+                    float pu = 0.f;
+                    if constexpr (LAYER)
+                        if (a.post == GN_NORM_LAYER) pu = s[k * (1 + LAYER) + 1] * inv;
 #pragma unroll
                     for (int j = 0; j < NC; ++j)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) d[j][e] = norm_grad(d[j][e], cur.h[j][e] - mp, rp, pu, pw);
+                        for (int e = 0; e < 8; ++e) {
+                            const float hh = (LAYER ? cur[k].h[j][e] - mp[k] : cur[k].h[j][e]) * rp[k];
+                            if constexpr (LAYER) d[k][j][e] -= pu;
+                            d[k][j][e] = rp[k] * (d[k][j][e] - hh * pw);
+                        }
                 }
-                if (on && a.dh)
+                const int row = r + k * RG;
+                if (row < r1 && a.dh)
 #pragma unroll
-                    for (int j = 0; j < NC; ++j) store8<TH, VEC>(a.dh + (int64_t)r * a.F, c, j, d[j]);
+                    for (int j = 0; j < NC; ++j) store8<TH, VEC>(a.dh + (int64_t)row * a.F, c, j, d[k][j]);
             }
-            if constexpr (AHEAD) cur = nxt;
-            else if (r + RG < r1) load(r + RG, cur);
+#pragma unroll
+            for (int k = 0; k < RP; ++k)
+                if constexpr (AHEAD) cur[k] = nxt[k];
+            if (!AHEAD && i + 1 < turns) load_turn(r + RP * RG, r1, cur);
         }
         if constexpr (GATE)
             if (a.gate_rows > 1 || a.gates <= 1) {
                 const bool whole = a.split.per <= 1;  // the group's rows are all this block's
+#pragma unroll
+                for (int j = 0; j < NC; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dg[j][e] *= a.scale;
                 emit(dg, whole ? a.grad[kGate] + (size_t)g * a.F : a.part + ((size_t)kGate * a.split.blocks + blockIdx.x) * a.F,
                      whole && a.accumulate);
                 clear(dg);
@@ -623,7 +726,7 @@ __global__ __launch_bounds__(1024) void residual_finish(FinishArgs a) {
         const int n = is_gate ? a.per : a.blocks;
         float s = 0.f;
         if (f < a.F) {
-#pragma unroll 8
+#pragma unroll 16
             for (int k = wave; k < n; k += 16) s += part[(size_t)k * a.F + f];
         }
         sh[wave][lane] = s;
@@ -856,11 +959,11 @@ void launch_kinds(const BwdArgs<TX, TH>& a, hipStream_t s) {
     else gate ? launch_rows<TX, TH, VEC, false, false, true>(a, s) : launch_rows<TX, TH, VEC, false, false, false>(a, s);
 }
 
-// Blocks of the backward for rows of F elements in `groups`: a block a CU, with two turns of rows each
+// Blocks of the backward for rows of F elements in `groups`: a block a CU, or two, with two turns of rows each
 // or more.
-Split make_split(int rows, int F, int groups) {
+Split make_split(int rows, int F, int groups, bool two) {
     const int turn = F > kMaxF ? 16 : 8 / waves_of(F);
-    const int most = F > kMaxF ? 64 : 256;
+    const int most = F > kMaxF ? 64 : two && F <= kMaxF / 2 ? 512 : 256;
     const int blocks = std::max(1, std::min(most, rows / (2 * turn)));
     Split s;
     s.groups = std::max(groups, 1);
@@ -874,7 +977,8 @@ size_t stats_bytes(int rows, int F) { return F > kMaxF ? (size_t)rows * sizeof(W
 
 // Partial rows for any of the groupings that a call of these sizes may take.
 size_t workspace_bytes(int rows, int F, int gates) {
-    const int b = std::max(make_split(rows, F, gates).blocks, make_split(rows, F, 1).blocks);
+    // (the gate's groups with its gradient, and then one block a CU)
+    const int b = std::max(make_split(rows, F, gates, false).blocks, make_split(rows, F, 1, true).blocks);
     return stats_bytes(rows, F) + (size_t)kPlanes * b * F * 4;
 }
 
@@ -1001,11 +1105,13 @@ int bwd(const gn_branch* b, const Mask& m, const void* dy, const void* dz, const
     a.post_eps = b->post_eps;
     a.pre_eps = b->pre_eps;
     a.mask = m;
-    a.split = make_split(rows, F, grad[kGate] && a.gate_rows > 1 ? b->gates : 1);
     a.stats = (float*)ws;
     a.part = (float*)((char*)ws + stats_bytes(rows, F));
     const bool vec = F % 8 == 0 && al16(dy) && al16(dz) && al16(h) && al16(y) && al16(dh) && al16(dx) && al16(b->post_w) &&
                      al16(b->post_b) && al16(b->pre_w) && al16(b->gate);
+    const bool layer = a.post == GN_NORM_LAYER || a.pre == GN_NORM_LAYER;
+    a.split = make_split(rows, F, grad[kGate] && a.gate_rows > 1 ? b->gates : 1,
+                         two_blocks(vec, a.post != GN_NORM_NONE, layer, grad[kGate] != nullptr, sizeof(TX)));
     return launch_bwd<TX, TH>(a, vec, s);
 }
 

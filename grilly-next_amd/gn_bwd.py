@@ -1145,29 +1145,38 @@ def qk_norm_rope_bwd(dyq, dyk, q, k, wq=None, wk=None, freqs=None, dyv=None, mod
 
 
 # ---- a block's residual branch: dropout, norms with gate and residual ----------------------
+def _arg(name, t, dtype, shape, dev):
+    """_here for a call of many tensors on device dev (the current one), in one step where all is well."""
+    if t is None:
+        return None
+    if t.dtype is dtype and t.get_device() == dev >= 0 and t.is_contiguous() and t.shape == shape:
+        return t.data_ptr()
+    return _here(name, t, dtype, shape)
+
+
 _U64 = 2 ** 64 - 1
 
 
-def _rng(seed, stream, step):
+def _rng(seed, stream, step, dev):
     """gn_rng; step: a number, or an int64 tensor of one element on the GPU that the kernels read (a graph's replays
     then draw the masks of the step that it holds)."""
     if isinstance(step, torch.Tensor):
         if step.numel() != 1:
             raise GnError(f"step must have one element, not {step.numel()}")
-        return Rng(seed & _U64, stream & _U64, 0, _here("step", step, torch.int64))
+        return Rng(seed & _U64, stream & _U64, 0, _arg("step", step, torch.int64, step.shape, dev))
     return Rng(seed & _U64, stream & _U64, step & _U64, None)
 
 
-def _dropout(name, x, p, seed, stream, step, out, flags):
-    xp = _here("x", x)
-    y = torch.empty_like(x) if out is None else out
-    yp = _here("out", y, x.dtype, x.shape)
-    args = (xp, yp, x.numel(), p, _rng(seed, stream, step), _dt(x))
-    if flags is None:
-        _check(lib().gn_dropout_fwd(*args, _stream()), name)
+def _dropout(fn, name, x, p, seed, stream, step, out, *flags):
+    dev = _device()
+    code, xp = _dt(x), _arg("x", x, x.dtype, x.shape, dev)
+    if out is None:
+        out = torch.empty_like(x)
+        yp = out.data_ptr()
     else:
-        _check(lib().gn_dropout_bwd(*args, flags, _stream()), name)
-    return y
+        yp = _arg("out", out, x.dtype, x.shape, dev)
+    _check(fn(xp, yp, x.numel(), p, _rng(seed, stream, step, dev), code, *flags, _stream()), name)
+    return out
 
 
 def dropout_fwd(x, p, seed, stream=0, step=0, out=None):
@@ -1175,45 +1184,41 @@ def dropout_fwd(x, p, seed, stream=0, step=0, out=None):
     stream, step) and an element's index alone: dropout_bwd with the same three forms it again, none is stored.
     stream: the place in the model; step: the iteration, a number or an int64 tensor on the GPU, which
     a captured call reads at every replay.  out may be x."""
-    return _dropout("gn_dropout_fwd", x, p, seed, stream, step, out, None)
+    return _dropout(lib().gn_dropout_fwd, "gn_dropout_fwd", x, p, seed, stream, step, out)
 
 
 def dropout_bwd(dy, p, seed, stream=0, step=0, out=None, accumulate=False):
     """The gradient of dropout_fwd's x; out may be dy; accumulate adds onto a given out."""
     if accumulate and out is None:
         raise GnError("accumulate needs the out to add onto")
-    return _dropout("gn_dropout_bwd", dy, p, seed, stream, step, out, ACCUMULATE if accumulate else 0)
+    return _dropout(lib().gn_dropout_bwd, "gn_dropout_bwd", dy, p, seed, stream, step, out, ACCUMULATE if accumulate else 0)
 
 
 _EPS = {"none": 0.0, "rms": 1e-6, "layer": 1e-5}
+_GRADS = ("dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b")
 
 
-def _branch(h, x, post, post_w, post_b, pre, pre_w, pre_b, gate, scale, res_scale, p, seed, stream, step, post_eps, pre_eps):
+def _branch(h, x, post, post_w, post_b, pre, pre_w, pre_b, gate, scale, res_scale, p, seed, stream, step, post_eps, pre_eps, dev):
     """gn_branch of checked tensors; h and x (or y) [rows, F]."""
     if h.dim() != 2:
         raise GnError(f"h must be [rows, F], not {list(h.shape)}")
-    _int32("h", h)
     dt, (rows, F) = h.dtype, h.shape
+    if rows > _INT or F > _INT:
+        _int32("h", h)
     if x.dtype is not dt and not (dt is torch.bfloat16 and x.dtype is torch.float32):
         raise GnError(f"the stream must be {dt}" + (" or float32" if dt is torch.bfloat16 else "") + f", not {x.dtype}")
-    b = Branch(NORM[post], NORM[pre])
-    if post_w is not None:
-        b.post_w = _here("post_w", post_w, dt, (F,))
-    if post_b is not None:
-        b.post_b = _here("post_b", post_b, dt, (F,))
-    if pre_w is not None:
-        b.pre_w = _here("pre_w", pre_w, dt, (F,))
-    if pre_b is not None:
-        b.pre_b = _here("pre_b", pre_b, dt, (F,))
-    b.post_eps = _EPS[post] if post_eps is None else post_eps
-    b.pre_eps = _EPS[pre] if pre_eps is None else pre_eps
+    w, gates = (F,), 0
     if gate is not None:
-        gates = 1 if gate.dim() == 1 else gate.shape[0]
-        b.gate, b.gates = _here("gate", gate, dt, (F,) if gate.dim() == 1 else (gates, F)), gates
-    b.scale, b.res_scale, b.p = scale, res_scale, p
-    if p:
-        b.rng = _rng(seed, stream, step)
-    return b
+        if gate.dim() == 1:
+            gates = 1
+            gate = _arg("gate", gate, dt, w, dev)
+        else:
+            gates = gate.shape[0]
+            gate = _arg("gate", gate, dt, (gates, F), dev)
+    return Branch(NORM[post], NORM[pre], _arg("post_w", post_w, dt, w, dev), _arg("post_b", post_b, dt, w, dev),
+                  _arg("pre_w", pre_w, dt, w, dev), _arg("pre_b", pre_b, dt, w, dev),
+                  _EPS[post] if post_eps is None else post_eps, _EPS[pre] if pre_eps is None else pre_eps, gate, gates, scale,
+                  res_scale, p, _rng(seed, stream, step, dev) if p else Rng())
 
 
 def residual_norm_fwd(h, x, post="none", post_w=None, post_b=None, pre="none", pre_w=None, pre_b=None, gate=None,
@@ -1224,15 +1229,20 @@ def residual_norm_fwd(h, x, post="none", post_w=None, post_b=None, pre="none", p
     gate: [F], or [G, F] for G sequences of rows / G rows each.  Dropout as dropout_fwd's, on element i
     of [rows, F].  h, z, gate and weights in h's dtype; x and y may be fp32 above bf16.  out: y's tensor, may
     be x."""
+    dev = _device()
     b = _branch(h, x, post, post_w, post_b, pre, pre_w, pre_b, gate, scale, res_scale, p, seed, stream, step, post_eps,
-                pre_eps)
-    rows, F = h.shape
-    y = torch.empty_like(x) if out is None else out
+                pre_eps, dev)
+    rows, F = shape = h.shape
+    hc, xc, hp, xp = _dt(h), _dt(x), _arg("h", h, h.dtype, shape, dev), _arg("x", x, x.dtype, shape, dev)
+    if out is None:
+        out = torch.empty_like(x)
+        yp = out.data_ptr()
+    else:
+        yp = _arg("out", out, x.dtype, shape, dev)
     z = None if pre == "none" else torch.empty_like(h)
-    _check(lib().gn_residual_norm_fwd(b, _here("h", h), _dt(h), _here("x", x, None, h.shape), _dt(x),
-                                      _here("out", y, x.dtype, h.shape), _ptr(z), rows, F, _stream()),
+    _check(lib().gn_residual_norm_fwd(b, hp, hc, xp, xc, yp, None if z is None else z.data_ptr(), rows, F, _stream()),
            "gn_residual_norm_fwd")
-    return y, z
+    return out, z
 
 
 @functools.lru_cache(maxsize=256)
@@ -1247,29 +1257,30 @@ def residual_norm_bwd(dy, dz, h, y, post="none", post_w=None, post_b=None, pre="
     gradients dy of y and dz of z (either may be None).  The parameters' gradients are fp32, None for parameters that were
     not given; dgate has gate's shape.  grads: the five tensors to write (None in it: not wanted), which
     accumulate adds onto; need_param False: none of them.  dx: its tensor, may be dy."""
+    dev = _device()
     b = _branch(h, y, post, post_w, post_b, pre, pre_w, pre_b, gate, scale, res_scale, p, seed, stream, step, post_eps,
-                pre_eps)
+                pre_eps, dev)
     rows, F = shape = h.shape
-    f32, dev = torch.float32, h.device
-    args = (_here("dy", dy, y.dtype, shape), _here("dz", dz, h.dtype, shape), _here("h", h), _dt(h),
-            _here("y", y, None, shape), _dt(y))
+    f32, ht, xt = torch.float32, h.dtype, y.dtype
+    args = (_arg("dy", dy, xt, shape, dev), _arg("dz", dz, ht, shape, dev), _arg("h", h, ht, shape, dev), _dt(h),
+            _arg("y", y, xt, shape, dev), _dt(y))
     dh = torch.empty_like(h) if need_dh else None
-    if need_dx and dx is None:
+    if not need_dx:
+        dx = None
+    elif dx is None:
         dx = torch.empty_like(y)
-    dx = dx if need_dx else None
     params = (gate, post_w, post_b, pre_w, pre_b)
     if not need_param:
         grads = (None,) * 5
     elif grads is None:
         if accumulate:
             raise GnError("accumulate needs the grads to add onto")
-        grads = tuple(None if t is None else torch.empty(t.shape, dtype=f32, device=dev) for t in params)
-    g = BranchGrads(*(None if t is None else _here(n, t, f32, None if q is None else q.shape)
-                      for n, t, q in zip(("dgate", "dpost_w", "dpost_b", "dpre_w", "dpre_b"), grads, params)))
+        grads = tuple([None if t is None else torch.empty_like(t, dtype=f32) for t in params])
+    g = BranchGrads(*[None if t is None else _arg(n, t, f32, t.shape if q is None else q.shape, dev)
+                      for n, t, q in zip(_GRADS, grads, params)])
     if ws is None:
-        nb = residual_norm_workspace_bytes(rows, F, b.gates)
-        ws = workspace(nb, dev)
-    _check(lib().gn_residual_norm_bwd(b, *args, _ptr(dh), _here("dx", dx, y.dtype, shape), g, rows, F,
+        ws = workspace(residual_norm_workspace_bytes(rows, F, b.gates), h.device)
+    _check(lib().gn_residual_norm_bwd(b, *args, None if dh is None else dh.data_ptr(), _arg("dx", dx, xt, shape, dev), g, rows, F,
                                       ACCUMULATE if accumulate else 0, _here("ws", ws), ws.numel() * ws.element_size(),
                                       _stream()), "gn_residual_norm_bwd")
     return (dh, dx, *grads)

@@ -372,6 +372,17 @@ def test_rows_do_not_touch_each_other(gn):
         assert bool(torch.isfinite(b[[11, 12, 13]]).all())
 
 
+@pytest.mark.parametrize("rows", [1, 3, 9, 17, 33])
+def test_no_eps(gn, rows):
+    """Norms without an eps: lanes that have no row add nothing, not 0 / 0."""
+    for F in (64, 1000, 4096, 9000):
+        c = Case(rows, F, "rms", "rms", 1, 0.0, F32, BF)
+        kw = dict(c.kw, post_eps=0.0, pre_eps=0.0)
+        ref = gn.residual_norm_bwd(c.dy, c.dz, c.h, c.x, **c.kw)
+        for a, b in zip(gn.residual_norm_bwd(c.dy, c.dz, c.h, c.x, **kw), ref):
+            assert a is b is None or float((a.double() - b.double()).norm()) <= 2 ** -7 * float(b.double().norm())
+
+
 def test_no_rows(gn):
     c = Case(4, 64, "layer", "layer", 2)
     cut = lambda t: t[:0]  # noqa: E731
