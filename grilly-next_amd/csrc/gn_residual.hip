@@ -431,6 +431,9 @@ struct Weights : Raw<std::conditional_t<FLOATS, float, T>, VEC> {
 __host__ __device__ constexpr bool two_blocks(bool vec, bool post, bool layer, bool gate, size_t x_size) {
     return vec && !gate && (!post || (!layer && x_size == 2));
 }
+constexpr bool lds_sums(int nc, bool post, bool layer, bool gate) {
+    return nc > 1 && gate + (post ? 1 + layer : 0) + 1 + layer >= 3;
+}
 template <typename TX, typename TH, int WPR, int NC, bool VEC, bool POST, bool LAYER, bool GATE>
 __global__ __launch_bounds__(512, NC == 1 && two_blocks(VEC, POST, LAYER, GATE, sizeof(TX)) ? 4 : 2) void residual_bwd(BwdArgs<TX, TH> a) {
     constexpr int T = 64 * WPR, RG = 512 / T;  // rows of a block side by side, times RP
@@ -438,6 +441,13 @@ __global__ __launch_bounds__(512, NC == 1 && two_blocks(VEC, POST, LAYER, GATE, 
     constexpr int RP = NC == 1 && SUMS <= 3 && !two_blocks(VEC, POST, LAYER, GATE, sizeof(TX)) ? 2 : 1;
     constexpr bool AHEAD = NC == 1, FW = RP == 2;  // AHEAD: the next rows' loads before these rows' work
     constexpr int NS = POST ? 3 : 2;
+    // Sixteen elements a lane and three sums or more do not fit the registers beside the row: all sums but pre_w's are
+    // then in LDS, where every lane has columns of its own (one row a block).  8192 x 6144, both LayerNorms and a
+    // gate: 331 us with what the registers spilled.
+    constexpr bool IN_LDS = lds_sums(NC, POST, LAYER, GATE);
+    constexpr int L_GATE = 0, L_PW = GATE, L_PB = GATE + POST, L_NB = GATE + POST + (POST && LAYER);
+    extern __shared__ __align__(16) float lds_sum[];  // [SUMS - 1][F up to a multiple of 8]
+    const int pitch = (a.F + 7) & ~7;
     __shared__ float4 rbuf[RG][2][WPR][2];
     __shared__ __align__(16) float acc_lds[RG > 1 ? RG * T * NC * 8 : 4];
     const int rg = __builtin_amdgcn_readfirstlane((int)threadIdx.x / T);  // the wave's
@@ -456,17 +466,61 @@ __global__ __launch_bounds__(512, NC == 1 && two_blocks(VEC, POST, LAYER, GATE, 
     }
     int at_gate = 0;
 
-    float dg[GATE ? NC : 1][8], dwp[POST ? NC : 1][8], dbp[POST && LAYER ? NC : 1][8], dwn[NC][8], dbn[LAYER ? NC : 1][8];
-    auto clear = [](auto& v) {
-        for (auto& p : v)
+    constexpr int NR = IN_LDS ? 1 : NC;
+    float dg[GATE ? NR : 1][8], dwp[POST ? NR : 1][8], dbp[POST && LAYER ? NR : 1][8], dwn[NC][8], dbn[LAYER ? NR : 1][8];
+    // a lane's eight sums of plane p in LDS, f(place, e) each
+    auto lds_each = [&](int p, int j, auto f) __attribute__((always_inline)) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = 0.f;
+        for (int e = 0; e < 8; ++e)
+            if (c.has(j, e)) f(lds_sum + p * pitch + c.at(j, e), e);
     };
-    clear(dg);
-    clear(dwp);
-    clear(dbp);
-    clear(dwn);
-    clear(dbn);
+    auto clear = [&](auto& v, int p) {
+        if constexpr (IN_LDS) {
+#pragma unroll
+            for (int j = 0; j < NC; ++j) lds_each(p, j, [](float* to, int) { *to = 0.f; });
+        } else {
+            for (auto& r : v)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) r[e] = 0.f;
+        }
+    };
+    auto add = [&](auto& v, int p, int j, const float (&x)[8]) __attribute__((always_inline)) {
+        if constexpr (IN_LDS) {
+            if constexpr (VEC) {
+                if (c.has(j, 0)) {
+                    float4* to = reinterpret_cast<float4*>(lds_sum + p * pitch + c.at(j, 0));
+                    const float4 u = to[0], w = to[1];
+                    to[0] = make_float4(u.x + x[0], u.y + x[1], u.z + x[2], u.w + x[3]);
+                    to[1] = make_float4(w.x + x[4], w.y + x[5], w.z + x[6], w.w + x[7]);
+                }
+            } else {
+                lds_each(p, j, [&](float* to, int e) { *to += x[e]; });
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[j][e] += x[e];
+        }
+    };
+    // what add() added up, for emit()
+    auto summed = [&](auto& v, int p, float (&out)[NC][8]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            if constexpr (IN_LDS) {
+                lds_each(p, j, [&](float* from, int e) { out[j][e] = *from; });
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) out[j][e] = v[j][e];
+            }
+        }
+    };
+    if constexpr (GATE) clear(dg, L_GATE);
+    if constexpr (POST) clear(dwp, L_PW);
+    if constexpr (POST && LAYER) clear(dbp, L_PB);
+    if constexpr (LAYER) clear(dbn, L_NB);
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dwn[j][e] = 0.f;
 
     struct Row {
         Raw<TH, VEC> h[NC], dz[NC];
@@ -607,6 +661,7 @@ __global__ __launch_bounds__(512, NC == 1 && two_blocks(VEC, POST, LAYER, GATE, 
 #pragma unroll
                 for (int j = 0; j < NC; ++j) {
                     float (&dk)[8] = d[k][j];
+                    float x[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float yh = centred(cur[k].y[j][e], mn[k], j, e) * rn[k], dz = cur[k].dz[j][e];
@@ -614,8 +669,9 @@ __global__ __launch_bounds__(512, NC == 1 && two_blocks(VEC, POST, LAYER, GATE, 
                         if constexpr (LAYER) gr -= u[k];
                         dk[e] = cur[k].dy[j][e] + rn[k] * (gr - yh * w[k]);
                         dwn[j][e] += dz * yh;
-                        if constexpr (LAYER) dbn[j][e] += dz;
+                        x[e] = dz;
                     }
+                    if constexpr (LAYER) add(dbn, L_NB, j, x);
                     if (on && a.dx) {
                         float o[8];
 #pragma unroll
@@ -633,8 +689,8 @@ __global__ __launch_bounds__(512, NC == 1 && two_blocks(VEC, POST, LAYER, GATE, 
                                 if constexpr (LAYER) n += bp[j][e];
                             }
                             o[e] = dk[e] * n;
-                            dg[j][e] += o[e];
                         }
+                        add(dg, L_GATE, j, o);
                         if (a.gate_rows == 1 && a.gates > 1 && on) {  // a gate a row: its gradient has no sum
                             float* const to = a.grad[kGate] + (int64_t)row * a.F;
 #pragma unroll
@@ -647,12 +703,16 @@ __global__ __launch_bounds__(512, NC == 1 && two_blocks(VEC, POST, LAYER, GATE, 
                         dk[e] *= FW ? gate[j][e] : gate_scale * gate[j][e];
                         if constexpr (POST) {
                             const float hh = centred(cur[k].h[j][e], mp[k], j, e) * rp[k];
-                            dwp[j][e] += dk[e] * hh;
-                            if constexpr (LAYER) dbp[j][e] += dk[e];
-                            dk[e] *= wp[j][e];
-                            s[k * (1 + LAYER)] += dk[e] * hh;
-                            if constexpr (LAYER) s[k * (1 + LAYER) + 1] += dk[e];
+                            x[e] = dk[e] * hh;
+                            s[k * (1 + LAYER)] += x[e] * wp[j][e];
+                            if constexpr (LAYER) s[k * (1 + LAYER) + 1] += dk[e] * wp[j][e];
                         }
+                    }
+                    if constexpr (POST) {
+                        add(dwp, L_PW, j, x);
+                        if constexpr (LAYER) add(dbp, L_PB, j, dk);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) dk[e] *= wp[j][e];
                     }
                 }
             }
@@ -686,24 +746,31 @@ __global__ __launch_bounds__(512, NC == 1 && two_blocks(VEC, POST, LAYER, GATE, 
         if constexpr (GATE)
             if (a.gate_rows > 1 || a.gates <= 1) {
                 const bool whole = a.split.per <= 1;  // the group's rows are all this block's
+                float all[NC][8];
+                summed(dg, L_GATE, all);
 #pragma unroll
                 for (int j = 0; j < NC; ++j)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) dg[j][e] *= a.scale;
-                emit(dg, whole ? a.grad[kGate] + (size_t)g * a.F : a.part + ((size_t)kGate * a.split.blocks + blockIdx.x) * a.F,
+                    for (int e = 0; e < 8; ++e) all[j][e] *= a.scale;
+                emit(all, whole ? a.grad[kGate] + (size_t)g * a.F : a.part + ((size_t)kGate * a.split.blocks + blockIdx.x) * a.F,
                      whole && a.accumulate);
-                clear(dg);
+                clear(dg, L_GATE);
             }
     }
-    auto plane = [&](auto& v, int p) {
+    auto plane = [&](auto& v, int l, int p) {
         if (!a.grad[p]) return;
         const bool one = a.split.blocks == 1;
-        emit(v, one ? a.grad[p] : a.part + ((size_t)p * a.split.blocks + blockIdx.x) * a.F, one && a.accumulate);
+        float all[NC][8];
+        summed(v, l, all);
+        emit(all, one ? a.grad[p] : a.part + ((size_t)p * a.split.blocks + blockIdx.x) * a.F, one && a.accumulate);
     };
-    if constexpr (POST) plane(dwp, kPostW);
-    if constexpr (POST && LAYER) plane(dbp, kPostB);
-    plane(dwn, kPreW);
-    if constexpr (LAYER) plane(dbn, kPreB);
+    if constexpr (POST) plane(dwp, L_PW, kPostW);
+    if constexpr (POST && LAYER) plane(dbp, L_PB, kPostB);
+    if constexpr (LAYER) plane(dbn, L_NB, kPreB);
+    if (a.grad[kPreW]) {
+        const bool one = a.split.blocks == 1;
+        emit(dwn, one ? a.grad[kPreW] : a.part + ((size_t)kPreW * a.split.blocks + blockIdx.x) * a.F, one && a.accumulate);
+    }
 }
 
 // out[f] (+)= the sum of `count` partial rows.  16 waves of 64 columns, each a share of the rows, added in
@@ -937,26 +1004,40 @@ int launch_fwd(const FwdArgs<TX, TH>& a, hipStream_t s) {
 }
 
 template <typename TX, typename TH, bool VEC, bool POST, bool LAYER, bool GATE>
-void launch_rows(const BwdArgs<TX, TH>& a, hipStream_t s) {
+int launch_rows(const BwdArgs<TX, TH>& a, hipStream_t s) {
     const dim3 grid((unsigned)a.split.blocks);
     switch (waves_of(a.F)) {
         case 1: residual_bwd<TX, TH, 1, 1, VEC, POST, LAYER, GATE><<<grid, 512, 0, s>>>(a); break;
         case 2: residual_bwd<TX, TH, 2, 1, VEC, POST, LAYER, GATE><<<grid, 512, 0, s>>>(a); break;
         case 4: residual_bwd<TX, TH, 4, 1, VEC, POST, LAYER, GATE><<<grid, 512, 0, s>>>(a); break;
         default:
-            if (a.F <= 4096) residual_bwd<TX, TH, 8, 1, VEC, POST, LAYER, GATE><<<grid, 512, 0, s>>>(a);
-            else residual_bwd<TX, TH, 8, 2, VEC, POST, LAYER, GATE><<<grid, 512, 0, s>>>(a);
+            if (a.F <= 4096) {
+                residual_bwd<TX, TH, 8, 1, VEC, POST, LAYER, GATE><<<grid, 512, 0, s>>>(a);
+            } else {
+                constexpr int planes = lds_sums(2, POST, LAYER, GATE) ? GATE + (POST ? 1 + LAYER : 0) + LAYER : 0;
+                if constexpr (planes > 0) {
+                    static const bool ok = hipFuncSetAttribute(reinterpret_cast<const void*>(&residual_bwd<TX, TH, 8, 2, VEC, POST, LAYER, GATE>),
+                                                               hipFuncAttributeMaxDynamicSharedMemorySize, planes * kMaxF * 4) == hipSuccess;
+                    if (!ok) {
+                        (void)hipGetLastError();
+                        set_error("gn_residual_norm_bwd: cannot reserve %d B of LDS", planes * kMaxF * 4);
+                        return GN_E_HIP;
+                    }
+                }
+                residual_bwd<TX, TH, 8, 2, VEC, POST, LAYER, GATE><<<grid, 512, (size_t)planes * ((a.F + 7) & ~7) * 4, s>>>(a);
+            }
     }
+    return GN_OK;
 }
 
 template <typename TX, typename TH, bool VEC>
-void launch_kinds(const BwdArgs<TX, TH>& a, hipStream_t s) {
+int launch_kinds(const BwdArgs<TX, TH>& a, hipStream_t s) {
     const bool post = a.post != GN_NORM_NONE, layer = a.post == GN_NORM_LAYER || a.pre == GN_NORM_LAYER;
     const bool gate = a.grad[kGate] != nullptr;
-    if (post && layer) gate ? launch_rows<TX, TH, VEC, true, true, true>(a, s) : launch_rows<TX, TH, VEC, true, true, false>(a, s);
-    else if (post) gate ? launch_rows<TX, TH, VEC, true, false, true>(a, s) : launch_rows<TX, TH, VEC, true, false, false>(a, s);
-    else if (layer) gate ? launch_rows<TX, TH, VEC, false, true, true>(a, s) : launch_rows<TX, TH, VEC, false, true, false>(a, s);
-    else gate ? launch_rows<TX, TH, VEC, false, false, true>(a, s) : launch_rows<TX, TH, VEC, false, false, false>(a, s);
+    if (post && layer) return gate ? launch_rows<TX, TH, VEC, true, true, true>(a, s) : launch_rows<TX, TH, VEC, true, true, false>(a, s);
+    if (post) return gate ? launch_rows<TX, TH, VEC, true, false, true>(a, s) : launch_rows<TX, TH, VEC, true, false, false>(a, s);
+    if (layer) return gate ? launch_rows<TX, TH, VEC, false, true, true>(a, s) : launch_rows<TX, TH, VEC, false, true, false>(a, s);
+    return gate ? launch_rows<TX, TH, VEC, false, false, true>(a, s) : launch_rows<TX, TH, VEC, false, false, false>(a, s);
 }
 
 // Blocks of the backward for rows of F elements in `groups`: a block a CU, or two, with two turns of rows each
@@ -988,10 +1069,8 @@ int launch_bwd(BwdArgs<TX, TH>& a, bool vec, hipStream_t s) {
         residual_bwd_stats<TX, TH><<<std::min(a.rows, 1 << 20), kWide, 0, s>>>(a);
         GN_LAUNCH_CHECK("gn_residual_norm_bwd");
         residual_bwd_cols<TX, TH><<<dim3((a.F + 255) / 256, a.split.blocks), 256, 0, s>>>(a);
-    } else if (vec) {
-        launch_kinds<TX, TH, true>(a, s);
-    } else {
-        launch_kinds<TX, TH, false>(a, s);
+    } else if (const int rc = vec ? launch_kinds<TX, TH, true>(a, s) : launch_kinds<TX, TH, false>(a, s)) {
+        return rc;
     }
     GN_LAUNCH_CHECK("gn_residual_norm_bwd");
     FinishArgs f{};
