@@ -293,7 +293,7 @@ int launch_wave(const GemmDesc& g, const E& e, hipStream_t s) {
 }
 
 // The tiles are the plain product's (gemm_wave_shape, gemm_stream_rows), whose time the epilogues change little.  The
-// streamed tiles' kernels are an activation's each, but for odd widths and addresses.
+// streamed tiles' kernels are an activation's each.
 template <bool TB, typename E, typename F>
 int launch(const GemmDesc& g, const E& any, F&& of_act, hipStream_t s) {
     switch (gemm_wave_shape(g, 0, TB, GN_BF16)) {
@@ -307,8 +307,7 @@ int launch(const GemmDesc& g, const E& any, F&& of_act, hipStream_t s) {
     auto go = [&](const auto& e) {
         return gemm_stream_rows(g) == 128 ? launch_stream<TB, 128>(g, e, blocks, s) : launch_stream<TB, 256>(g, e, blocks, s);
     };
-    if constexpr (!E::kVec) return go(any);
-    else return of_act(go);
+    return of_act(go);
 }
 
 template <typename TY, bool VEC>

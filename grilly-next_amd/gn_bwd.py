@@ -1346,13 +1346,14 @@ def act_linear_bwd(act, dY, P, A, W, need_dp=True, need_dw=True, need_db=True, d
     if need_db and db is None:
         db = torch.empty((N,), dtype=f32, device=dev)
     dP, dW, db = dP if need_dp else None, dW if need_dw else None, db if need_db else None
+    dwp = _here("dW", dW, f32, (N, K))
     if ws is None:
         nb = linear_workspace_bytes(M, N, K, code) if need_dw else 0
-        if code == BF16 and (N % 8 or K % 8 or (yp | wp) % 16):
+        if code == BF16 and (N % 8 or K % 8 or (yp | wp | (ap or 0) | (dwp or 0)) % 16):
             nb += linear_act_workspace_bytes(M, N, K, code)
         ws = workspace(nb, dev) if nb else None
     wsp, wsb = (None, 0) if ws is None else (_here("ws", ws), ws.numel() * ws.element_size())
-    _check(lib().gn_act_linear_bwd(ACT[act], yp, pp, ap, wp, _here("dP", dP, dt, (M, K)), _here("dW", dW, f32, (N, K)),
+    _check(lib().gn_act_linear_bwd(ACT[act], yp, pp, ap, wp, _here("dP", dP, dt, (M, K)), dwp,
                                    _here("db", db, f32, (N,)), M, N, K, code, ACCUMULATE if accumulate else 0, wsp, wsb,
                                    _stream()), "gn_act_linear_bwd")
     return dP, dW, db
