@@ -183,13 +183,14 @@ __device__ __forceinline__ void store8(T* p, const C& c, int j, const float (&v)
     }
 }
 
-template <bool VEC, typename C>
-__device__ __forceinline__ void drop_piece(float (&v)[8], const C& c, int j, uint64_t key, uint64_t row0, const Mask& m) {
+template <bool VEC, typename C, typename F = NoMore>
+__device__ __forceinline__ void drop_piece(float (&v)[8], const C& c, int j, uint64_t key, uint64_t row0, const Mask& m, F&& f = F{}) {
     if constexpr (VEC) {
-        drop8(v, key, row0 + (uint64_t)c.at(j, 0), m.t, m.keep);
+        drop8(v, key, row0 + (uint64_t)c.at(j, 0), m.t, m.keep, f);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = drop1(v[e], key, row0 + (uint64_t)c.at(j, e), m.t, m.keep);
+        for (int e = 0; e < 8; ++e)
+            v[e] = drop1(v[e], key, row0 + (uint64_t)c.at(j, e), m.t, m.keep, [&](int, bool kept) { f(e, kept); });
     }
 }
 
@@ -678,18 +679,24 @@ __global__ __launch_bounds__(512, NC == 1 && two_blocks(VEC, POST, LAYER, GATE, 
                         for (int e = 0; e < 8; ++e) o[e] = a.res_scale * dk[e];
                         store8<TX, VEC>(a.dx + (int64_t)row * a.F, c, j, o);
                     }
-                    if (a.mask.t) drop_piece<VEC>(dk, c, j, key, (uint64_t)row * a.F, a.mask);
-                    if constexpr (GATE) {  // dgate / scale
-                        float o[8];
+                    float o[8];  // n, then dgate / scale: drop(n)'s terms, so that a dropped inf or NaN adds 0
+                    if constexpr (GATE) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            float n = cur[k].h[j][e];
+                            o[e] = cur[k].h[j][e];
                             if constexpr (POST) {
-                                n = centred(n, mp[k], j, e) * rp[k] * wp[j][e];
-                                if constexpr (LAYER) n += bp[j][e];
+                                o[e] = centred(o[e], mp[k], j, e) * rp[k] * wp[j][e];
+                                if constexpr (LAYER) o[e] += bp[j][e];
                             }
-                            o[e] = dk[e] * n;
                         }
+                    }
+                    if (a.mask.t)
+                        drop_piece<VEC>(dk, c, j, key, (uint64_t)row * a.F, a.mask, [&](int e, bool kept) __attribute__((always_inline)) {
+                            if constexpr (GATE) o[e] = kept ? o[e] : 0.f;
+                        });
+                    if constexpr (GATE) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] *= dk[e];
                         add(dg, L_GATE, j, o);
                         if (a.gate_rows == 1 && a.gates > 1 && on) {  // a gate a row: its gradient has no sum
                             float* const to = a.grad[kGate] + (int64_t)row * a.F;
@@ -936,10 +943,11 @@ __global__ __launch_bounds__(256) void residual_bwd_cols(BwdArgs<TX, TH> a) {
                 dbn += dz;
             }
             if (a.dx) io<TX>::st(a.dx, i, a.res_scale * d);
-            if (a.mask.t) d = drop1(d, key, (uint64_t)i, a.mask.t, a.mask.keep);
-            d *= a.scale;
             const float hc = io<TH>::ld(a.h, i) - s.mp;
-            const float n = hc * s.rp * wp + bp;
+            float n = hc * s.rp * wp + bp;
+            if (a.mask.t)  // (dgate takes drop(n): a dropped inf or NaN adds 0)
+                d = drop1(d, key, (uint64_t)i, a.mask.t, a.mask.keep, [&](int, bool kept) { n = kept ? n : 0.f; });
+            d *= a.scale;
             dg += d * n;
             if (a.grad[kGate] && a.gate_rows == 1 && a.gates > 1) {
                 float* to = a.grad[kGate] + i;

@@ -36,19 +36,30 @@ struct Mask {
     }
 };
 
-// Eight elements from i0 (a multiple of 8) on: kept times the factor, or 0.  A dropped inf or NaN is 0.
-__device__ __forceinline__ void drop8(float (&v)[8], uint64_t key, uint64_t i0, uint32_t t, float keep) {
+// Eight elements from i0 (a multiple of 8) on, or one: kept times the factor, or 0.  A dropped inf or NaN is 0.  f(e, kept) follows
+// what becomes of element e.
+struct NoMore {
+    __device__ __forceinline__ void operator()(int, bool) const {}
+};
+template <typename F = NoMore>
+__device__ __forceinline__ void drop8(float (&v)[8], uint64_t key, uint64_t i0, uint32_t t, float keep, F&& f = F{}) {
     uint64_t z = key + kPhi * ((i0 >> 1) + 1);
 #pragma unroll
     for (int k = 0; k < 4; ++k, z += kPhi) {
         const uint64_t w = mix64(z);
-        v[2 * k] = (uint32_t)w >= t ? v[2 * k] * keep : 0.f;
-        v[2 * k + 1] = (uint32_t)(w >> 32) >= t ? v[2 * k + 1] * keep : 0.f;
+        const bool k0 = (uint32_t)w >= t, k1 = (uint32_t)(w >> 32) >= t;
+        v[2 * k] = k0 ? v[2 * k] * keep : 0.f;
+        v[2 * k + 1] = k1 ? v[2 * k + 1] * keep : 0.f;
+        f(2 * k, k0);
+        f(2 * k + 1, k1);
     }
 }
-__device__ __forceinline__ float drop1(float v, uint64_t key, uint64_t i, uint32_t t, float keep) {
+template <typename F = NoMore>
+__device__ __forceinline__ float drop1(float v, uint64_t key, uint64_t i, uint32_t t, float keep, F&& f = F{}) {
     const uint64_t w = mix64(key + kPhi * ((i >> 1) + 1));
-    return ((i & 1) ? (uint32_t)(w >> 32) : (uint32_t)w) >= t ? v * keep : 0.f;
+    const bool kept = ((i & 1) ? (uint32_t)(w >> 32) : (uint32_t)w) >= t;
+    f(0, kept);
+    return kept ? v * keep : 0.f;
 }
 
 // A probability below 1 as the mask takes it; false: not one.

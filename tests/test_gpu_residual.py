@@ -372,6 +372,23 @@ def test_rows_do_not_touch_each_other(gn):
         assert bool(torch.isfinite(b[[11, 12, 13]]).all())
 
 
+@pytest.mark.parametrize("gates", [0, 1, 5, 40])
+@pytest.mark.parametrize("F", [64, 1001, 2048, 6000, 9000])
+def test_dropped_inf_and_nan_add_nothing(gn, F, gates):
+    """Without a norm after the block, what the mask drops reaches no output, the gate's gradient included."""
+    c = Case(40, F, "none", "layer", gates, 0.4, F32, BF)
+    off = (c.m == 0).view(40, F)
+    h0, h = c.h.masked_fill(off, 0.0), c.h.masked_fill(off, float("nan"))
+    h[::2] = c.h.masked_fill(off, float("-inf"))[::2]
+    y, z = gn.residual_norm_fwd(h0, c.x, **c.kw)
+    for a, b in zip(gn.residual_norm_fwd(h, c.x, **c.kw), (y, z)):
+        assert torch.equal(a, b)
+    ref = gn.residual_norm_bwd(c.dy, c.dz, h0, y, **c.kw)
+    for a, b in zip(gn.residual_norm_bwd(c.dy, c.dz, h, y, **c.kw), ref):
+        assert a is b is None or torch.equal(a, b)
+    assert (ref[2] is not None) == (gates > 0)
+
+
 @pytest.mark.parametrize("rows", [1, 3, 9, 17, 33])
 def test_no_eps(gn, rows):
     """Norms without an eps: lanes that have no row add nothing, not 0 / 0."""
