@@ -440,7 +440,7 @@ int gn_dropout_bwd(const void* dY, void* dX, int64_t n, double p, const gn_rng* 
  * Norms: GN_NORM_NONE (n = h; no z), GN_NORM_RMS (v rsqrt(mean v^2 + eps) w), GN_NORM_LAYER
  * ((v - mean) rsqrt(var + eps) w + b, the biased variance).  z is formed from y before y is rounded.
  * gate: [gates x F], row r takes gate r / (rows / gates): one for all (a gain per channel), one a sequence, one a row;
- * rows must be a multiple of gates.  h, z, gate and the norms' weights in h_dtype, x and y in x_dtype: (f32,
+ * rows (below 2^30) must be a multiple of gates.  h, z, gate and the norms' weights in h_dtype, x and y in x_dtype: (f32,
  * f32), (bf16, bf16) or (h bf16, x f32). */
 #define GN_NORM_NONE 0
 #define GN_NORM_RMS 1

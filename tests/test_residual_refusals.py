@@ -66,6 +66,8 @@ def bwd(b=None, dy=DY, dz=DZ, h=H, hd=gn.BF16, y=Y, xd=gn.F32, dh=DH, dx=DX, g=N
 def test_residual_norm_refuses_a_branch(call):
     refused(call(rows=-1), "rows")
     refused(call(f=0), "rows of 0")
+    refused(call(rows=1 << 30), "2^30")
+    refused(call(rows=(1 << 31) - 1), "2^30")
     refused(call(f=(1 << 24) + 1), "2^24")
     refused(call(hd=gn.F16), "dtype")
     refused(call(hd=gn.F32, xd=gn.BF16), "dtype")
@@ -114,7 +116,7 @@ def test_residual_norm_refuses_outputs():
 
 def test_workspace_query_of_refused_sizes():
     q = gn.lib().gn_residual_norm_workspace_bytes
-    assert q(0, 8, 0) == q(4, 0, 0) == q(4, (1 << 24) + 1, 0) == q(4, 8, 3) == q(4, 8, -1) == 0
+    assert q(0, 8, 0) == q(4, 0, 0) == q(4, (1 << 24) + 1, 0) == q(4, 8, 3) == q(4, 8, -1) == q(1 << 30, 1, 0) == 0
     assert q(4, 8, 2) > 0
 
 
