@@ -168,6 +168,33 @@ def test_linear_act_node(env, act, dtype, res):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+def test_one_tensor_as_both_inputs(env, dtype):
+    """The residual that is the product's or the block's own input: one gradient, the sum of both (its terms rounded once
+    each, and the sum: within a step of the terms' magnitudes)."""
+    gc, gb, dev, gn = env
+    M, K = 24, 64
+    X, W, w = rand(1, M, K, dtype=dtype), rand(2, K, K, dtype=dtype, std=0.1), 1 + rand(3, K, dtype=dtype, std=0.1)
+    op, t = gc.OpType, gb.tref
+    dY = rand(5, M, K, dtype=dtype)
+    Y, pre = gn.linear_act_fwd(X, W, act="silu", residual=X, need_pre=True)
+    y, z = gn.residual_norm_fwd(X, X, post="layer", pre="rms", pre_w=w, p=0.2, seed=4)
+    product = gn.linear_bwd(gn.act_bwd("silu", dY, pre), X, W)[0]
+    dh, dx = gn.residual_norm_bwd(dY, None, X, y, post="layer", pre="rms", pre_w=w, p=0.2, seed=4)[:2]
+    for node, inputs, outputs, params, saved, terms in (
+            (op.LinearAct, [t(X, True), t(X, True)], [t(Y)], gb.linear_act_params("silu"), [W.data_ptr(), 0, pre.data_ptr()], (product, dY)),
+            (op.ResidualNorm, [t(X, True), t(X, True)], [t(y), t(z)], gb.residual_norm_params(post="layer", pre="rms", p=0.2, seed=4),
+             [0, 0, w.data_ptr()], (dh, dx))):
+        tape = gb.create_tape_context(dev)
+        tape.begin()
+        n = tape.record_op(node, inputs, outputs, params)
+        tape.save_for_backward(n, saved)
+        tape.backward(n, dY.data_ptr())
+        got, (a, b) = grad(gb, dev, tape, X).astype(np.float64), (host(v).astype(np.float64) for v in terms)
+        assert (np.abs(got - a - b) <= torch.finfo(dtype).eps * (np.abs(a) + np.abs(b))).all()
+        tape.end()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("behind", ["Linear", "LinearAct"])
 @pytest.mark.parametrize("fused", [False, True])
 def test_two_layers(env, dtype, behind, fused):
