@@ -639,7 +639,7 @@ Node* BackwardEngine::glu_before(Node* n) const {
 }
 
 // The LinearAct node whose output is this Linear's or LinearAct's input, when set_glu_epilogue is on: with an activation and
-// no residual, recorded right before, and no gradient of its output yet (no other consumer).
+// no residual, recorded right before, and no gradient of its output yet nor from this node's residual (no other consumer).
 Node* BackwardEngine::act_before(Node* n) const {
     const TensorRef& x = n->inputs[0];
     Node* a = n->prev_in_tape;
@@ -649,6 +649,8 @@ Node* BackwardEngine::act_before(Node* n) const {
         a->inputs[0].dtype != x.dtype || a->outputs[0].numel() != x.numel() || a->outputs[0].last() != x.last() ||
         a->params_size < sizeof(LinearActParams) || params_of<LinearActParams>(a).act == GN_ACT_NONE)
         return nullptr;
+    for (uint32_t i = 1; i < n->num_inputs && i < kMaxNodeIO; ++i)  // x is the node's residual too
+        if (n->inputs[i].buffer_id == x.buffer_id) return nullptr;
     const GradEntry* e = find(x.buffer_id);
     return e && e->grad_id ? nullptr : a;
 }

@@ -251,6 +251,30 @@ def test_activation_with_two_consumers_is_not_fused(env):
     tape.end()
 
 
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_activation_that_is_its_consumers_residual_is_not_fused(env, dtype, fused):
+    gc, gb, dev, gn = env
+    M, d = 24, 64
+    X, W1, W2 = rand(1, M, d, dtype=dtype), rand(2, d, d, dtype=dtype, std=0.1), rand(3, d, d, dtype=dtype, std=0.1)
+    A, pre = gn.linear_act_fwd(X, W1, act="silu", need_pre=True)
+    Y = gn.linear_act_fwd(A, W2, residual=A)
+    dY = rand(5, M, d, dtype=dtype)
+    op, t = gc.OpType, gb.tref
+    tape = gb.create_tape_context(dev)
+    tape.set_glu_epilogue(fused)
+    tape.begin()
+    n = tape.record_op(op.LinearAct, [t(X, True)], [t(A)], gb.linear_act_params("silu"))
+    tape.save_for_backward(n, [W1.data_ptr(), 0, pre.data_ptr()])
+    n = tape.record_op(op.LinearAct, [t(A, True), t(A, True)], [t(Y)])
+    tape.save_for_backward(n, [W2.data_ptr()])
+    tape.backward(n, dY.data_ptr())
+    dA = gn.linear_bwd(dY, A, W2)[0] + dY
+    same(gb, dev, tape, A, dA)
+    same(gb, dev, tape, X, gn.linear_bwd(gn.act_bwd("silu", dA, pre), X, W1)[0])
+    tape.end()
+
+
 def test_nodes_refuse(env):
     gc, gb, dev, gn = env
     x, y = rand(1, 4, 8), rand(2, 4, 8)
