@@ -206,7 +206,8 @@ extern "C" int gn_linear_act_fwd(int act, const void* X, const void* W, const vo
         float* const v = (float*)(P ? P : Y);
         if (const int rc = gn_linear_fwd(X, W, b, v, M, N, K, dtype, stream)) return rc;
         if (P || R || act != GN_ACT_NONE) {
-            finish_forward<float, float><<<grid, 256, 0, s>>>(v, nullptr, (const float*)R, (float*)Y, (float*)P, n, N, act, out_is_pre);
+            // (a P of the sums themselves is the product's, and complete)
+            finish_forward<float, float><<<grid, 256, 0, s>>>(v, nullptr, (const float*)R, (float*)Y, out_is_pre ? (float*)P : nullptr, n, N, act, out_is_pre);
             GN_LAUNCH_CHECK(who);
         }
         return GN_OK;
