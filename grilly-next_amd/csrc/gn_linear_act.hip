@@ -142,13 +142,14 @@ int check_spans(const char* who, const Span (&t)[N]) {
     return GN_OK;
 }
 
+// (a tile's loads are 32 bits of bytes from its first row: 255 rows of 2^23 bf16 elements at most)
 bool sizes_fit(int M, int N, int K) {
-    return M < (1 << 28) && N < (1 << 26) && K < (1 << 26) && (int64_t)M * std::max(N, K) < (1ll << 36) && (int64_t)N * K < (1ll << 36);
+    return M < (1 << 28) && N < (1 << 23) && K < (1 << 23) && (int64_t)M * std::max(N, K) < (1ll << 36) && (int64_t)N * K < (1ll << 36);
 }
 int check_sizes(const char* who, int M, int N, int K, int dtype) {
     GN_REQUIRE(M >= 0 && N >= 0 && K >= 0, "%s: negative size", who);
     GN_REQUIRE(dtype == GN_F32 || dtype == GN_BF16, "%s: dtype %d not supported (f32, bf16)", who, dtype);
-    GN_REQUIRE(sizes_fit(M, N, K), "%s: M below 2^28, N and K below 2^26, M * N, M * K and N * K below 2^36", who);
+    GN_REQUIRE(sizes_fit(M, N, K), "%s: M below 2^28, N and K below 2^23, M * N, M * K and N * K below 2^36", who);
     return GN_OK;
 }
 int check_ws(const char* who, const void* ws, size_t ws_bytes, size_t need) {

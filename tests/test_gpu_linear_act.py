@@ -225,6 +225,49 @@ def test_extreme_slopes(gn):
             near(dP, slope64(p, act), 2 ** -19 * (1 + p.abs()).clamp(max=128))
 
 
+def test_rows_as_long_as_they_may_be(gn):
+    """Rows of 2^23 - 8 elements: a tile's last ones begin 2^32 bytes behind its first, less some.  Whole numbers in four columns,
+    0 elsewhere: every sum is exact."""
+    M, K, L = 512, 512, 2 ** 23 - 8
+    cols = [0, 5, L // 2 + 3, L - 1]
+    small = torch.randint(-3, 4, (M, 4), device=DEV).to(BF), torch.randint(-3, 4, (K, 4), device=DEV).to(BF)
+
+    def long(t):
+        out = torch.zeros(len(t), L, dtype=BF, device=DEV)
+        out[:, cols] = t
+        return out
+
+    X, W = long(small[0]), long(small[1])
+    want = small[0].double() @ small[1].double().T
+    assert torch.equal(gn.linear_act_fwd(X, W, act="relu").double(), want.clamp(min=0))
+    del W
+    K = 128
+    P, A = torch.ones(M, K, dtype=BF, device=DEV), torch.randint(-3, 4, (M, K), device=DEV).to(BF)
+    W = torch.zeros(L, K, dtype=BF, device=DEV)
+    W[cols] = small[1][:K].T.contiguous()
+    dP, dW, db = gn.act_linear_bwd("relu", X, P, A, W)
+    assert torch.equal(dP.double(), want[:, :K])
+    assert torch.equal(dW[cols].double(), small[0].double().T @ A.double()) and torch.equal(db[cols].double(), small[0].double().sum(0))
+    dW[cols] = 0
+    assert not bool(dW.any()) and int(db.count_nonzero()) <= 4
+
+
+def test_elements_past_31_bits(gn):
+    """Outputs, residuals and stored sums of more than 2^31 elements, of small whole numbers: every sum is exact."""
+    M, N, K = 270001, 8008, 16
+    whole = lambda *shape: torch.randint(-3, 4, shape, device=DEV, dtype=torch.int8).to(BF)  # noqa: E731
+    X, W, R = whole(M, K), whole(N, K), whole(M, N)
+    Y, P = gn.linear_act_fwd(X, W, act="relu", residual=R, need_pre=True)
+    rows = [0, 1, M // 2, M - 300, M - 1]
+    v = X[rows].double() @ W.double().T
+    assert torch.equal(P[rows].double(), v) and torch.equal(Y[rows].double(), v.clamp(min=0) + R[rows].double())
+    dY, W2 = whole(M, K), whole(K, N)
+    dP, dW, db = gn.act_linear_bwd("relu", dY, P, R, W2, dP=Y)
+    assert torch.equal(dP[rows].double(), dY[rows].double() @ W2.double() * (P[rows] > 0))
+    at = [0, 3, N // 2, N - 1]
+    assert torch.equal(dW[:, at].double(), dY.double().T @ R[:, at].double()) and torch.equal(db.double(), dY.double().sum(0))
+
+
 def test_a_block_of_both(gn):
     """The feed-forward block as it is trained: up with its activation, down with the fp32 residual, and back, against
     autograd in fp64 at the saved tensors."""
