@@ -20,13 +20,20 @@ __device__ __forceinline__ float gelu_gate(float x, float xx) {
     return rcp(1.0f + __builtin_amdgcn_exp2f(x * fmaf(xx, -kLog2e * kG3, -kLog2e * kG1)));
 }
 
+// 1 - 2 / (1 + e^2x), which is good to 2^-22 of 1: towards 0, where that is too little of x, the series, whose next term is 62/2835 x^8
+// (4096 x 5632 x 2048: 104 us for 99 without)
+__device__ __forceinline__ float tanh_of(float x) {
+    const float xx = x * x, far = fmaf(-2.0f, rcp(1.0f + __builtin_amdgcn_exp2f(x * (2.0f * kLog2e))), 1.0f);
+    return fabsf(x) < 0.25f ? x * fmaf(xx, fmaf(xx, fmaf(xx, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f) : far;
+}
+
 template <int KIND>
 __device__ __forceinline__ float act_of(float x) {
     if constexpr (KIND == GN_ACT_RELU) return x > 0.f ? x : 0.f;
     else if constexpr (KIND == GN_ACT_GELU_TANH) return x * gelu_gate(x, x * x);
     else if constexpr (KIND == GN_ACT_GELU_ERF) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
     else if constexpr (KIND == GN_ACT_SILU) return x * sigmoid_of(x);
-    else if constexpr (KIND == GN_ACT_TANH) return fmaf(-2.0f, rcp(1.0f + __builtin_amdgcn_exp2f(x * (2.0f * kLog2e))), 1.0f);
+    else if constexpr (KIND == GN_ACT_TANH) return tanh_of(x);
     else return sigmoid_of(x);
 }
 // tanh and sigmoid at their output; of x sigmoid(u): s + x s (1 - s) u' = s (1 + (1 - s) x u')

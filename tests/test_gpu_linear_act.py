@@ -212,6 +212,18 @@ def test_extreme_arguments(gn):
                  2 ** -20 * (1 + X.double().abs().clamp(max=128)))
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("act", ["tanh", "silu", "gelu_tanh", "gelu_erf"])
+def test_small_arguments(gn, act, dtype):
+    """Towards 0 an activation is good to a part of itself, not of 1: its terms of x have at most 2^-20 of themselves as error, and tanh
+    from 0.245 on 2^-22 of 1 (W is the unit matrix)."""
+    x = torch.tensor([1e-30, -1e-20, 1e-10, 1e-7, -1e-6, 1e-5, 1e-4, -1e-3, 0.01, 0.06, -0.1, 0.2, 0.249, 0.251, -0.3, 0.5], device=DEV)
+    X = x.to(dtype).view(1, 16).repeat(16, 1)
+    Y = gn.linear_act_fwd(X, torch.eye(16, device=DEV, dtype=dtype), act=act)
+    ref = act64(X.double(), act)
+    near(Y, ref, 2 ** -19 * ref.abs())
+
+
 def test_extreme_slopes(gn):
     """Derivatives far from 0: those of the activations' ends, and no NaN (W is the unit matrix: dP = dY act'(P))."""
     x = torch.tensor([0.0, 5., -5., 19., -19., 21., -21., 90., -90., 1e4, -1e4, 1e20, -1e20, 1e30, -1e30, 1e-30], device=DEV)
