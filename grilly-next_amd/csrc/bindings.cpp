@@ -280,6 +280,35 @@ PYBIND11_MODULE(_grilly_core, m) {
           },
           py::arg("op"), py::arg("inputs"), py::arg("outputs"), py::arg("params") = py::bytes(), py::arg("upstream") = false,
           "The backward's check of a node's types and sizes, without a device");
+    using Tensors = std::vector<TensorRef>;
+    m.def("_check_kept",
+          [](OpType op, const Tensors& inputs, const Tensors& outputs, const std::vector<uint64_t>& saved, py::bytes params,
+             const std::vector<std::tuple<OpType, Tensors, Tensors>>& behind, bool dz) {
+              auto node = [](OpType o, const Tensors& in, const Tensors& out) {
+                  Node n{};
+                  n.op = o;
+                  n.num_inputs = (uint32_t)std::min<size_t>(in.size(), kMaxNodeIO);
+                  n.num_outputs = (uint32_t)std::min<size_t>(out.size(), kMaxNodeIO);
+                  std::copy_n(in.begin(), n.num_inputs, n.inputs);
+                  std::copy_n(out.begin(), n.num_outputs, n.outputs);
+                  return n;
+              };
+              Node n = node(op, inputs, outputs);
+              n.num_saved = (uint32_t)std::min<size_t>(saved.size(), kMaxNodeIO);
+              std::copy_n(saved.begin(), n.num_saved, n.saved_buffer_ids);
+              const std::string p = params;
+              n.params_size = (uint32_t)std::min(p.size(), sizeof(n.params));
+              std::copy_n(p.data(), n.params_size, n.params);
+              std::vector<uint64_t> written;
+              for (const auto& [o, in, out] : behind) {
+                  const Node b = node(o, in, out);
+                  add_written(&b, written);
+              }
+              check_kept(&n, dz, written);
+          },
+          py::arg("op"), py::arg("inputs"), py::arg("outputs"), py::arg("saved"), py::arg("params"), py::arg("behind"),
+          py::arg("dz") = false,
+          "The backward's check that the nodes behind a node wrote none of the buffers it reads, without a device");
 
     // ---- GRLY v3 hypernetwork checkpoint (bindings.cpp:2965-3039) + optimizer section ----
     // dims = (d_model, vsa_dim, K, router_hidden); opt = None or dict(kind, n_states, step,

@@ -173,6 +173,7 @@ void BackwardEngine::backward(TapeArena& tape, Node* loss_node, uint64_t grad_ou
     glu_gu_ = 0;
     act_node_ = nullptr;
     act_dp_ = 0;
+    written_.clear();
     if (!loss_node) throw std::invalid_argument("backward: loss node is None");
     // autograd.cpp:30-31: 0 means "the loss computes its own gradient" (sentinel 1)
     loss_node->grad_output_buffer = grad_output_buffer ? grad_output_buffer : 1ULL;
@@ -191,7 +192,10 @@ void BackwardEngine::backward(TapeArena& tape, Node* loss_node, uint64_t grad_ou
         f.eligible = linear_uses == 1 && other_uses == 0;
         f.u.applied = false;
     }
+    const Node* behind = nullptr;
     for (Node* cur = tape.tail<Node>(); cur != nullptr; cur = cur->prev_in_tape) {
+        if (behind) add_written(behind, written_);
+        behind = cur;
         stats_.nodes_visited++;
         if (cur->grad_output_buffer == 0) {
             for (uint32_t i = 0; i < cur->num_outputs && i < kMaxNodeIO; ++i) {
@@ -295,6 +299,28 @@ void check_node(const Node* n, bool upstream) {
                 throw std::invalid_argument("LinearAct: the output must have the input's type, or f32 above bf16");
             break;
         default: break;
+    }
+}
+
+void add_written(const Node* n, std::vector<uint64_t>& written) {
+    const bool through = n->op == OpType::Reshape || n->op == OpType::CubeMindSurprise || n->op == OpType::TemporalSurprise;
+    for (uint32_t o = 0; o < n->num_outputs && o < kMaxNodeIO; ++o)
+        if (n->outputs[o].buffer_id && !(through && n->num_inputs > 0 && n->outputs[o].buffer_id == n->inputs[0].buffer_id))
+            written.push_back(n->outputs[o].buffer_id);
+}
+
+void check_kept(const Node* n, bool dz, const std::vector<uint64_t>& written) {
+    auto kept = [&](uint64_t id, const char* what) {
+        if (id && std::find(written.begin(), written.end(), id) != written.end())
+            throw std::invalid_argument(std::string(what) + ", which a later node of the tape overwrote");
+    };
+    if (n->op == OpType::ResidualNorm) {
+        if (dz) kept(n->outputs[0].buffer_id, "ResidualNorm: the gradient of z needs the stream y");
+        if (params_of<ResidualNormParams>(n).post != GN_NORM_NONE || (n->num_saved > 4 && n->saved_buffer_ids[4]))
+            kept(n->inputs[0].buffer_id, "ResidualNorm: the backward reads h");
+    } else if (n->op == OpType::LinearAct) {
+        kept(n->inputs[0].buffer_id, "LinearAct: the backward reads X");
+        if (n->num_saved > 2) kept(n->saved_buffer_ids[2], "LinearAct: the backward reads P");
     }
 }
 
@@ -458,6 +484,7 @@ void BackwardEngine::bwd_linear_act(Node* n) {
     const int act = n->params_size < sizeof(LinearActParams) ? GN_ACT_NONE : params_of<LinearActParams>(n).act;
     if (!W) throw std::invalid_argument("LinearAct: saved_buffer_ids[0] must hold W");
     if (act != GN_ACT_NONE && !pre) throw std::invalid_argument("LinearAct: saved_buffer_ids[2] must hold P");
+    check_kept(n, false, written_);
     uint64_t dv;
     if (n == act_node_) {  // from the node behind (linear_grads)
         dv = act_dp_;
@@ -517,6 +544,7 @@ void BackwardEngine::bwd_residual_norm(Node* n) {
         return e->grad_id;
     };
     uint64_t dy = grad_of(y), dz = p.pre != GN_NORM_NONE ? grad_of(n->outputs[1]) : 0;
+    check_kept(n, dz != 0, written_);
     if (!dy && !dz) dy = reinterpret_cast<uint64_t>(gout(n));
     gn_branch b{};
     b.post = (int)p.post;

@@ -136,8 +136,8 @@ struct LinearCrossEntropyParams { uint32_t vocab; float scale; };
 struct DropoutParams { double p; uint64_t seed, stream, step; };
 // ResidualNorm: inputs h (the block's output) and x (the residual stream), [rows, F] each -> outputs y, alike x, and z,
 // alike h (none without a pre norm); saved slots {post_w, post_b, pre_w, pre_b, gate, step counter}, 0 where
-// there is none.  The backward reads h and y, which must be as the forward left them: a stream that a later
-// block updates in place is lost to this one's pre norm.
+// there is none.  The backward reads y where z has a gradient, and h under a post norm or a gate, as the forward left
+// them: it throws where a node behind this one wrote either buffer again (a stream updated in place by two blocks).
 struct ResidualNormParams {
     double p;
     uint64_t seed, stream, step;
@@ -180,6 +180,12 @@ T* TapeArena::allocate_node(Args&&... args) {
 // Throws where the types or sizes of an attention, Rope, QkNormRope, LinearCrossEntropy, Dropout, ResidualNorm or
 // LinearAct node's tensors are not what its backward reads and writes by (upstream: it is given a gradient of its output).  No device call.
 void check_node(const Node* n, bool upstream);
+
+// Throws where a buffer that a ResidualNorm's or LinearAct's backward reads is among those that the nodes behind it
+// wrote (dz: z has a gradient): the values that it needs are gone.  No device call.
+void check_kept(const Node* n, bool dz, const std::vector<uint64_t>& written);
+// Adds the buffers that n wrote: its outputs, but not a view's (a pass-through's output in its input's place).
+void add_written(const Node* n, std::vector<uint64_t>& written);
 
 class BackwardEngine {
 public:
@@ -316,6 +322,7 @@ private:
     // likewise the gradient in front of a LinearAct node's activation, from the node behind it
     const Node* act_node_ = nullptr;
     uint64_t act_dp_ = 0;
+    std::vector<uint64_t> written_;  // the buffers that the nodes behind the one being visited wrote
     bool norm_pending(uint64_t buf) const;
     void flush_norms();
     FusedSlot* fused_for(uint64_t weight);
