@@ -40,8 +40,10 @@ __device__ __forceinline__ float act_of(float x) {
 template <int KIND>
 __device__ __forceinline__ float slope_of(float x) {
     if constexpr (KIND == GN_ACT_GELU_TANH) {
-        const float xx = fminf(x * x, 400.f), s = gelu_gate(x, xx);  // from |x| = 20 on the gate is 0 or 1; 0 times inf is NaN
-        return s * fmaf(1.0f - s, x * fmaf(xx, 3.0f * kG3, kG1), 1.0f);
+        // from |x| = 20 on the gate is 0 or 1, and the slope: without the limit x u' overflows, and 0 times inf is NaN.  The gate
+        // takes x itself, so that a NaN stays one.
+        const float c = __builtin_amdgcn_fmed3f(x, -20.f, 20.f), xx = c * c, s = gelu_gate(x, xx);
+        return s * fmaf(1.0f - s, c * fmaf(xx, 3.0f * kG3, kG1), 1.0f);
     } else if constexpr (KIND == GN_ACT_SILU) {
         const float s = sigmoid_of(x);
         return s * fmaf(1.0f - s, x, 1.0f);
