@@ -29,7 +29,7 @@ __device__ __forceinline__ float tanh_of(float x) {
 
 template <int KIND>
 __device__ __forceinline__ float act_of(float x) {
-    if constexpr (KIND == GN_ACT_RELU) return x > 0.f ? x : 0.f;
+    if constexpr (KIND == GN_ACT_RELU) return x < 0.f ? 0.f : x;  // a NaN stays
     else if constexpr (KIND == GN_ACT_GELU_TANH) return x * gelu_gate(x, x * x);
     else if constexpr (KIND == GN_ACT_GELU_ERF) return 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
     else if constexpr (KIND == GN_ACT_SILU) return x * sigmoid_of(x);

@@ -489,9 +489,9 @@ size_t gn_residual_norm_workspace_bytes(int rows, int F, int gates);
  *   v = X W^T + b,  Y = R + act(v)
  * X [M x K], W [N x K], b [N] (NULL: 0) in dtype; R (NULL: none) and Y [M x N] in y_dtype, which is dtype, or
  * GN_F32 over bf16 (an fp32 residual stream; Y is then not rounded at all).  P [M x N] in dtype, or NULL: what
- * gn_act_bwd and gn_act_linear_bwd read, v or, of tanh and sigmoid, act(v).  act: GN_ACT_*.  v is fp32 up to the
- * one rounding of P and that of Y.  Y may be R (the same address; in fp32 only with P), otherwise outputs share
- * no memory with anything else of the call.  M below 2^28, N and K below 2^23, M * N, M * K, N * K below 2^36.
+ * gn_act_bwd and gn_act_linear_bwd read, v or, of tanh and sigmoid, act(v).  act: GN_ACT_*; a NaN v stays one, also under
+ * relu (gn_act_fwd's relu gives 0 there).  v is fp32 up to the one rounding of P and that of Y.  Y may be R (the
+ * same address; in fp32 only with P), otherwise outputs share no memory with anything else of the call.  M below 2^28, N and K below 2^23, M * N, M * K, N * K below 2^36.
  * ws: gn_linear_act_workspace_bytes, 16-byte aligned; bf16 needs it where K is no multiple of 8 or X or W not
  * 16-byte aligned (the operands are laid out there), otherwise it may be NULL. */
 int gn_linear_act_fwd(int act, const void* X, const void* W, const void* b, const void* R, void* P,
