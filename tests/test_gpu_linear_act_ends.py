@@ -1,4 +1,8 @@
-"""GPU tests of linear_act_fwd and act_linear_bwd where the numbers end: slopes of the largest P, NaN in a sum."""
+"""GPU tests of linear_act_fwd and act_linear_bwd where the numbers end: slopes of the largest P, NaN in a sum, fp32 activations to a
+few units in the last place.
+
+u = 2^-24.  The math library's exponential is good to one step (2 u of itself), its tanh to two (4 u), erfc to four (8 u);
+a sum, product or quotient to u."""
 import math
 
 import pytest
@@ -6,7 +10,9 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from test_gpu_linear_act import ACTS, BF, DEV, F32, near, rand  # noqa: E402
+from test_gpu_linear_act import ACTS, BF, DEV, F32, act64, near, rand, slope64  # noqa: E402
+
+U = 2.0 ** -24
 
 
 @pytest.fixture(scope="module")
@@ -51,3 +57,50 @@ def test_nan_in_a_sum_stays(gn, act, dtype, res):
                 assert bool(torch.isnan(g[3]).all()), (M, pre)
                 rest = torch.arange(M, device=DEV) != 3
                 assert torch.equal(g[rest], c[rest])
+
+
+def z2(x):
+    """gelu_tanh's 2 z and its derivative."""
+    k = 2 * math.sqrt(2 / math.pi)
+    return k * (x + 0.044715 * x ** 3), k * (1 + 3 * 0.044715 * x * x)
+
+
+@pytest.mark.parametrize("M,N,K", [(40, 64, 48), (500, 256, 256)])
+@pytest.mark.parametrize("act", ACTS)
+def test_fp32_activations(gn, act, M, N, K):
+    """At the very sums (the same call without an activation).  silu, sigmoid: e^-x 2 u, 1 + it, the quotient.  tanh: the
+    library's.  gelu_tanh: 2 z, of a square, two constants, a sum and a product, to 4 u of itself, which e^-2z hands on.  gelu_erf:
+    erfc's argument to 2 u, and erfc hands on at most x^2 times that."""
+    X, W, b = rand(1, M, K, dtype=F32), rand(2, N, K, dtype=F32, std=K ** -0.5), rand(3, N, dtype=F32)
+    v = gn.linear_act_fwd(X, W, b).double()
+    Y = gn.linear_act_fwd(X, W, b, act=act)
+    # (1 + tanh and 1 + erf of fp64 cancel where v is far below 0)
+    ref = v * torch.special.erfc(-v / math.sqrt(2)) / 2 if act == "gelu_erf" else v * torch.sigmoid(z2(v)[0]) if act == "gelu_tanh" else act64(v, act)
+    size = dict(relu=0 * v, silu=4 + 0 * v, sigmoid=4 + 0 * v, tanh=4 + 0 * v, gelu_tanh=4 + 4 * z2(v)[0].abs(), gelu_erf=12 + 2 * v * v)[act]
+    near(Y, ref, size * U * ref.abs())
+    kept = gn.linear_act_fwd(X, W, b, act=act, need_pre=True)
+    assert torch.equal(kept[0], Y) and torch.equal(kept[1], Y if act in ("tanh", "sigmoid") else v.float())
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_fp32_slopes(gn, act):
+    """At P (W is the unit matrix, dY 1).  s + x s (1 - s) z' with s as above: its two terms' magnitudes to 8 + 4 |z| steps of u;
+    the normal density's exponent to 2 u of x^2 / 2."""
+    M, K = 300, 64
+    P = rand(1, M, K, dtype=F32, std=2)
+    if act in ("tanh", "sigmoid"):
+        P = act64(P.double(), act).float()
+    dP = gn.act_linear_bwd(act, torch.ones(M, K, device=DEV), P, None, torch.eye(K, device=DEV), need_dw=False)[0]
+    x = P.double()
+    if act in ("silu", "gelu_tanh"):
+        z, dz = (x, torch.ones_like(x)) if act == "silu" else z2(x)
+        s = torch.sigmoid(z)
+        size = (8 + 4 * z.abs()) * (s + (x * s * torch.sigmoid(-z) * dz).abs())
+        ref = s + x * s * torch.sigmoid(-z) * dz
+    elif act == "gelu_erf":
+        phi, t = torch.special.erfc(-x / math.sqrt(2)) / 2, x * torch.exp(-x * x / 2) / math.sqrt(2 * math.pi)
+        ref, size = phi + t, (12 + 2 * x * x) * phi + (8 + x * x) * t.abs()
+    else:
+        ref = slope64(x, act)
+        size = 2 * ref
+    near(dP, ref, size * U)
