@@ -208,6 +208,9 @@ int skinny_linear_bwd(const float* dY, const float* X, const float* W, float* dX
 
 // When a backward call's two products run side by side (gn_gemm.hip): dx [xr x xc], dw [wr x wc], FLOP of each.
 Fork side_by_side(int dtype, double flop_dx, double flop_dw, long xr, long xc, long wr, long wc);
+// gn_gemm with a workspace for the fp32 path's ranges of terms (gn_gemm.hip).
+int gemm_dispatch(const void* A0, const void* B0, int K0, const void* A1, const void* B1, int K1, void* C, int M, int N, int transA,
+                  int transB, int dtype, int c_dtype, unsigned flags, hipStream_t s, void* ws, size_t ws_bytes, bool beside);
 // The weight gradient dW [N x Kin] = dY^T X and the bias's, db, of a Linear (gn_gemm.hip; Msplit: N, dW2: dW).
 int weight_grad(const void* dY, int ldy, const void* X, int ldx, int M, int N, int Kin, void* dW, void* dW2, int Msplit,
                 float* db, float* db2, int dtype, unsigned flags, hipStream_t s, void* ws = nullptr,

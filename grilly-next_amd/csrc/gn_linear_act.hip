@@ -84,14 +84,26 @@ __global__ __launch_bounds__(256) void finish_forward(const float* v, const TB* 
         io<TR>::st(Y, i, R ? x + io<TR>::ld(R, i) : x);
     }
 }
-// dP *= act'(P), fp32
-__global__ __launch_bounds__(256) void finish_backward(float* dP, const float* P, int64_t n, int act) {
-    for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const float p = P[i];
-        float d = dP[i];
-        by_act<kAny, false>(act, [&](auto A) { d *= slope_f32<decltype(A)::value>(p); });
-        dP[i] = d;
-    }
+// dP *= act'(P), fp32: n4 pieces of four elements, or (V 1) n4 elements
+template <int V>
+__global__ __launch_bounds__(256) void finish_backward(float* dP, const float* P, int64_t n4, int act) {
+    by_act<kAny, false>(act, [&](auto A) {
+        for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
+            float p[V], d[V];
+            if constexpr (V == 4) {
+                const float4 x = reinterpret_cast<const float4*>(P)[i], y = reinterpret_cast<const float4*>(dP)[i];
+                p[0] = x.x; p[1] = x.y; p[2] = x.z; p[3] = x.w;
+                d[0] = y.x; d[1] = y.y; d[2] = y.z; d[3] = y.w;
+            } else {
+                p[0] = P[i];
+                d[0] = dP[i];
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) d[e] *= slope_f32<decltype(A)::value>(p[e]);
+            if constexpr (V == 4) reinterpret_cast<float4*>(dP)[i] = make_float4(d[0], d[1], d[2], d[3]);
+            else dP[i] = d[0];
+        }
+    });
 }
 
 // dst [Rp x dp] = src [R x d], zeros around it; dp a multiple of 8, dst 16-byte aligned: eight elements a thread
@@ -301,18 +313,28 @@ extern "C" int gn_act_linear_bwd(int act, const void* dY, const void* P, const v
     }
     if (need)
         if (const int rc = check_ws(who, ws, ws_bytes, need)) return rc;
-    char* const rest = ws ? (char*)ws + need : nullptr;  // the weight gradient's partial sums
+    char* const rest = ws ? (char*)ws + need : nullptr;  // the products' partial sums
     const size_t rest_bytes = ws && ws_bytes > need ? ws_bytes - need : 0;
     const int64_t nk = (int64_t)m * K;
-    const unsigned grid = grid_for(nk, 1024, 16384);
     if (dtype == GN_F32) {
-        if (dP)
-            if (const int rc = gn_gemm(dY, W, N, nullptr, nullptr, 0, dP, M, K, 0, 0, dtype, dtype, 0, stream)) return rc;
-        if (dP) {
-            finish_backward<<<grid, 256, 0, s>>>((float*)dP, (const float*)P, nk, act);
+        // dP's product and dW's as the plain layer's backward has them: one pass over W for up to 8 rows, one launch for small
+        // layers, ranges of the terms in the workspace (us, silu, with two products of their own and no ranges -> so; the plain
+        // layer and gn_act_bwd: 8 x 5632 x 2048 148 -> 41, 41; 128 x 4096 x 1024 110 -> 38, 39; 64 x 10 x 256 7.4 -> 4.8, 4.9;
+        // 64 x 256 x 784 17.3 -> 18.7, 18.6).  Without the workspace the few rows' sums would be atomics, and where dW is
+        // added onto, dP would be too: then dP's product by itself.
+        const bool both = dP && dW && !(flags & GN_ACCUMULATE) &&
+                          (skinny_bwd_ws_bytes(M, N, K) == 0 || (al16(rest) && rest_bytes >= skinny_bwd_ws_bytes(M, N, K)));
+        int rc = GN_OK;
+        if (dW) rc = gn_linear_bwd_ws(dY, A, W, both ? dP : nullptr, dW, db, M, N, K, dtype, flags, rest, rest_bytes, stream);
+        if (rc == GN_OK && dP && !both) rc = gemm_dispatch(dY, W, N, nullptr, nullptr, 0, dP, M, K, 0, 0, dtype, dtype, 0, s, rest, rest_bytes, false);
+        if (rc == GN_OK && dP) {
+            if (nk % 4 == 0 && al16(dP) && al16(P))
+                finish_backward<4><<<grid_for(nk / 4, 256, 8192), 256, 0, s>>>((float*)dP, (const float*)P, nk / 4, act);
+            else
+                finish_backward<1><<<grid_for(nk, 256, 8192), 256, 0, s>>>((float*)dP, (const float*)P, nk, act);
             GN_LAUNCH_CHECK(who);
         }
-        return dW ? gn_linear_bwd_ws(dY, A, W, nullptr, dW, db, M, N, K, dtype, flags, rest, rest_bytes, stream) : GN_OK;
+        return rc;
     }
     char* const base = (char*)ws;
     const bool accumulate = flags & GN_ACCUMULATE;

@@ -1348,7 +1348,7 @@ def act_linear_bwd(act, dY, P, A, W, need_dp=True, need_dw=True, need_db=True, d
     dP, dW, db = dP if need_dp else None, dW if need_dw else None, db if need_db else None
     dwp = _here("dW", dW, f32, (N, K))
     if ws is None:
-        nb = linear_workspace_bytes(M, N, K, code) if need_dw else 0
+        nb = linear_workspace_bytes(M, N, K, code) if need_dw or code == F32 else 0
         if code == BF16 and (N % 8 or K % 8 or (yp | wp | (ap or 0) | (dwp or 0)) % 16):
             nb += linear_act_workspace_bytes(M, N, K, code)
         ws = workspace(nb, dev) if nb else None

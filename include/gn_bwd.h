@@ -504,8 +504,8 @@ int gn_linear_act_fwd(int act, const void* X, const void* W, const void* b, cons
  * db).  In bf16 dP may be P (the same address, and then not A); otherwise outputs and the workspace share no memory with
  * anything else of the call.  GN_ACCUMULATE adds onto dW and db (dP is overwritten).
  * ws, 16-byte aligned: bf16 needs gn_linear_act_workspace_bytes where N or K is no multiple of 8 or dY, W, A or dW not
- * 16-byte aligned; what is left of it beyond, gn_linear_workspace_bytes at best, goes to the weight gradient as
- * in gn_linear_bwd_ws. */
+ * 16-byte aligned; what is left of it beyond, gn_linear_workspace_bytes at best, goes to the weight gradient (fp32: to
+ * dP's product too) as in gn_linear_bwd_ws. */
 int gn_act_linear_bwd(int act, const void* dY, const void* P, const void* A, const void* W, void* dP,
                       void* dW, void* db, int M, int N, int K, int dtype, unsigned flags, void* ws,
                       size_t ws_bytes, void* stream);

@@ -1,5 +1,5 @@
 """GPU tests of linear_act_fwd and act_linear_bwd where the numbers end: slopes of the largest P, NaN in a sum, fp32 activations to a
-few units in the last place.
+few units in the last place, and the fp32 backward against the plain linear layer's.
 
 u = 2^-24.  The math library's exponential is good to one step (2 u of itself), its tanh to two (4 u), erfc to four (8 u);
 a sum, product or quotient to u."""
@@ -10,7 +10,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from test_gpu_linear_act import ACTS, BF, DEV, F32, act64, near, rand, slope64  # noqa: E402
+from test_gpu_linear_act import ACTS, BF, DEV, F32, act64, check_bwd, near, rand, slope64  # noqa: E402
 
 U = 2.0 ** -24
 
@@ -104,3 +104,40 @@ def test_fp32_slopes(gn, act):
         ref = slope64(x, act)
         size = 2 * ref
     near(dP, ref, size * U)
+
+
+# few rows (one pass over W), one launch, ranges of the terms, and tiles that need neither
+FP32 = [(1, 256, 784), (8, 1000, 512), (3, 10, 256), (64, 10, 256), (64, 256, 784), (128, 4096, 1024), (256, 6144, 768), (2000, 512, 256), (77, 33, 51)]
+
+
+@pytest.mark.parametrize("M,N,K", FP32)
+def test_fp32_backward_takes_the_linear_layers_products(gn, M, N, K):
+    """With relu, whose slopes are 0 and 1: dP, dW and db are linear_bwd's, bit for bit."""
+    dY, P, W = rand(1, M, N, dtype=F32, std=0.01), rand(2, M, K, dtype=F32), rand(3, N, K, dtype=F32, std=0.05)
+    A = P.clamp(min=0)
+    dX, dW, db = gn.linear_bwd(dY, A, W)
+    got = gn.act_linear_bwd("relu", dY, P, A, W)
+    assert torch.equal(got[0], dX * (P > 0)) and torch.equal(got[1], dW) and torch.equal(got[2], db)
+    again = gn.act_linear_bwd("relu", dY, P, A, W)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    check_bwd(gn, M, N, K, "silu", F32, accumulate=True)
+    only = gn.act_linear_bwd("relu", dY, P, None, W, need_dw=False)[0]
+    ref = dY.double() @ W.double() * (P > 0)
+    near(only, ref, 2 ** -23 * (N ** 0.5 + 8) * (dY.double().abs() @ W.double().abs()))
+
+
+@pytest.mark.parametrize("M,N,K", FP32)
+def test_fp32_backward_without_workspace(gn, M, N, K):
+    """The call takes none: the same bits every time then too."""
+    dY, P, W = rand(1, M, N, dtype=F32, std=0.01), rand(2, M, K, dtype=F32), rand(3, N, K, dtype=F32, std=0.05)
+    A = P.clamp(min=0)
+    out = []
+    for _ in range(3):
+        dP, dW, db = (torch.empty(*s, device=DEV) for s in ((M, K), (N, K), (N,)))
+        rc = gn.lib().gn_act_linear_bwd(gn.ACT["relu"], dY.data_ptr(), P.data_ptr(), A.data_ptr(), W.data_ptr(), dP.data_ptr(),
+                                        dW.data_ptr(), db.data_ptr(), M, N, K, gn.F32, 0, None, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        out.append((dP, dW, db))
+    assert all(torch.equal(a, b) for o in out[1:] for a, b in zip(o, out[0]))
+    ref = dY.double() @ W.double() * (P > 0)
+    near(out[0][0], ref, 2 ** -23 * (N ** 0.5 + 8) * (dY.double().abs() @ W.double().abs()))
