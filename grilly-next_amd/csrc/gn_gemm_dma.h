@@ -215,6 +215,7 @@ int gemm_dispatch(const void* A0, const void* B0, int K0, const void* A1, const 
 int weight_grad(const void* dY, int ldy, const void* X, int ldx, int M, int N, int Kin, void* dW, void* dW2, int Msplit,
                 float* db, float* db2, int dtype, unsigned flags, hipStream_t s, void* ws = nullptr,
                 size_t ws_bytes = 0, bool beside = false);
+size_t weight_grad_ws_bytes(int M, int N, int Kin, int dtype);
 
 // Run C (+)= sum_s op(A_s) op(B_s) described by `d`.  bf16: the LDS-DMA kernels when the shape
 // allows it, else the register-staged MFMA kernel.  fp32: gemm_small, the six-product split or

@@ -509,7 +509,8 @@ int gn_linear_act_fwd(int act, const void* X, const void* W, const void* b, cons
 int gn_act_linear_bwd(int act, const void* dY, const void* P, const void* A, const void* W, void* dP,
                       void* dW, void* db, int M, int N, int K, int dtype, unsigned flags, void* ws,
                       size_t ws_bytes, void* stream);
-/* 0 in fp32 and for sizes that the calls refuse. */
+/* 0 in fp32 and for sizes that the calls refuse.  Where N or K is no multiple of 8 it has room for the partial sums of
+ * the weight gradient, which the call does without in less. */
 size_t gn_linear_act_workspace_bytes(int M, int N, int K, int dtype);
 
 /* ---- attention ------------------------------------------------------------------------ */

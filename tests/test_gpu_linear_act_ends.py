@@ -1,5 +1,5 @@
 """GPU tests of linear_act_fwd and act_linear_bwd where the numbers end: slopes of the largest P, NaN in a sum, fp32 activations to a
-few units in the last place, and the fp32 backward against the plain linear layer's.
+few units in the last place, and the fp32 and odd-sized backward against the plain linear layer's.
 
 u = 2^-24.  The math library's exponential is good to one step (2 u of itself), its tanh to two (4 u), erfc to four (8 u);
 a sum, product or quotient to u."""
@@ -141,3 +141,13 @@ def test_fp32_backward_without_workspace(gn, M, N, K):
     assert all(torch.equal(a, b) for o in out[1:] for a, b in zip(o, out[0]))
     ref = dY.double() @ W.double() * (P > 0)
     near(out[0][0], ref, 2 ** -23 * (N ** 0.5 + 8) * (dY.double().abs() @ W.double().abs()))
+
+
+@pytest.mark.parametrize("M,N,K", [(8192, 1027, 1031), (8192, 513, 519), (4100, 767, 769), (3000, 64, 100), (5000, 100, 64)])
+def test_odd_weight_gradients_over_ranges_of_rows(gn, M, N, K):
+    """Sizes whose laid-out weight gradient is a sum of partial planes, with their room in the workspace."""
+    check_bwd(gn, M, N, K, "silu")
+    check_bwd(gn, M, N, K, "gelu_tanh", accumulate=True, seed=7)
+    dY, P, W = rand(1, M, N, std=0.01), rand(2, M, K), rand(3, N, K, std=0.05)
+    first, second = (gn.act_linear_bwd("relu", dY, P, P, W) for _ in range(2))
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
