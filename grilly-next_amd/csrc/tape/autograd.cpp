@@ -451,7 +451,9 @@ void BackwardEngine::linear_grads(Node* n, const void* dY, uint64_t W, uint64_t 
         // x = act(P) feeds only this node: the gradient in front of the activation comes out of the
         // input-gradient product for the LinearAct node visited next (dX never formed)
         uint64_t dP = alloc_grad(x.size_bytes());
-        const size_t wsb = gn_linear_workspace_bytes(M, N, K, dt) + gn_linear_act_workspace_bytes(M, N, K, dt);
+        // operands are laid out only where 16-byte pieces do not take them
+        const bool lay = dt == GN_BF16 && (N % 8 || K % 8 || ((reinterpret_cast<uint64_t>(dY) | x.buffer_id | W | dW) & 15u));
+        const size_t wsb = gn_linear_workspace_bytes(M, N, K, dt) + (lay ? gn_linear_act_workspace_bytes(M, N, K, dt) : 0);
         const uint64_t ws = split_ws(wsb);
         gn_call(gn_act_linear_bwd(params_of<LinearActParams>(a).act, dY, P(a->saved_buffer_ids[2]), P(x.buffer_id), P(W), P(dP),
                                   P(dW), P(db), M, N, K, dt, 0, P(ws), wsb, dev_.stream()),
@@ -472,7 +474,8 @@ void BackwardEngine::linear_grads(Node* n, const void* dY, uint64_t W, uint64_t 
 }
 
 // LinearAct: y = residual + act(x W^T + b).  The residual's gradient is the upstream one itself; the product's is that
-// times act', in x's type (an fp32 one over bf16 operands rounded first).
+// times act', in x's type.  An fp32 one over bf16 operands is rounded first, before act' too: the norm behind
+// the stream has written that copy in its own pass, and gn_act_bwd has one type for all of its tensors.
 void BackwardEngine::bwd_linear_act(Node* n) {
     const TensorRef& x = n->inputs[0];
     const TensorRef& y = n->outputs[0];
