@@ -1214,6 +1214,8 @@ def _branch(h, x, post, post_w, post_b, pre, pre_w, pre_b, gate, scale, res_scal
             gate = _arg("gate", gate, dt, w, dev)
         else:
             gates = gate.shape[0]
+            if not gates and rows:  # (an empty tensor has no address, and would be no gate at all)
+                raise GnError(f"gate must have a row, not {list(gate.shape)}")
             gate = _arg("gate", gate, dt, (gates, F), dev)
     return Branch(NORM[post], NORM[pre], _arg("post_w", post_w, dt, w, dev), _arg("post_b", post_b, dt, w, dev),
                   _arg("pre_w", pre_w, dt, w, dev), _arg("pre_b", pre_b, dt, w, dev),
