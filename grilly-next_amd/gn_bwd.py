@@ -1160,11 +1160,12 @@ _U64 = 2 ** 64 - 1
 def _rng(seed, stream, step, dev):
     """gn_rng; step: a number, or an int64 tensor of one element on the GPU that the kernels read (a graph's replays
     then draw the masks of the step that it holds)."""
+    seed, stream = int(seed) & _U64, int(stream) & _U64  # (numpy's whole numbers too)
     if isinstance(step, torch.Tensor):
         if step.numel() != 1:
             raise GnError(f"step must have one element, not {step.numel()}")
-        return Rng(seed & _U64, stream & _U64, 0, _arg("step", step, torch.int64, step.shape, dev))
-    return Rng(seed & _U64, stream & _U64, step & _U64, None)
+        return Rng(seed, stream, 0, _arg("step", step, torch.int64, step.shape, dev))
+    return Rng(seed, stream, int(step) & _U64, None)
 
 
 def _dropout(fn, name, x, p, seed, stream, step, out, *flags):

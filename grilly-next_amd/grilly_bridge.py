@@ -122,7 +122,7 @@ def linear_cross_entropy_params(vocab: int, scale: float = 1.0) -> bytes:
 
 def dropout_params(p: float, seed: int, stream: int = 0, step: int = 0) -> bytes:
     """Dropout node, with the forward's numbers; saved slots {step counter or 0} (a device int64, added to step)."""
-    return struct.pack("<dQQQ", p, seed & _U64, stream & _U64, step & _U64)
+    return struct.pack("<dQQQ", p, int(seed) & _U64, int(stream) & _U64, int(step) & _U64)
 
 
 def residual_norm_params(post: str = "none", pre: str = "none", gates: int = 0, scale: float = 1.0, res_scale: float = 1.0,
@@ -131,7 +131,7 @@ def residual_norm_params(post: str = "none", pre: str = "none", gates: int = 0, 
     """ResidualNorm node: inputs h and x, outputs y (and z with a pre norm), with the forward's numbers; saved slots
     {post_w, post_b, pre_w, pre_b, gate, step counter}, 0 where there is none.  eps None: residual_norm_fwd's."""
     eps = {"none": 0.0, "rms": 1e-6, "layer": 1e-5}
-    return struct.pack("<dQQQffffIIIxxxx", p, seed & _U64, stream & _U64, step & _U64, eps[post] if post_eps is None else post_eps,
+    return struct.pack("<dQQQffffIIIxxxx", p, int(seed) & _U64, int(stream) & _U64, int(step) & _U64, eps[post] if post_eps is None else post_eps,
                        eps[pre] if pre_eps is None else pre_eps, scale, res_scale, NORM_KIND[post], NORM_KIND[pre], gates)
 
 
