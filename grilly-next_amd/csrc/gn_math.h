@@ -33,7 +33,8 @@ __device__ __forceinline__ float silu_grad_f(float x) {
 template <int KIND>
 __device__ __forceinline__ float act_grad(float x) {
     if constexpr (KIND == GN_ACT_RELU) return x > 0.0f ? 1.0f : 0.0f;
-    else if constexpr (KIND == GN_ACT_GELU_TANH) return gelu_tanh_grad_f(x);
+    else if constexpr (KIND == GN_ACT_GELU_TANH)  // (0 or 1 from |x| = 20 on; further out x^2 overflows, and 0 times inf is NaN)
+        return gelu_tanh_grad_f(fabsf(x) > 20.0f ? copysignf(20.0f, x) : x);
     else if constexpr (KIND == GN_ACT_GELU_ERF) return gelu_erf_grad_f(x);
     else if constexpr (KIND == GN_ACT_SILU) return silu_grad_f(x);
     else if constexpr (KIND == GN_ACT_TANH) return 1.0f - x * x;  // x = saved tanh output
