@@ -1,4 +1,5 @@
-// gn_act.h — activations and their slopes in the fewest instructions, for the epilogues of products (gn_linear_act.hip).
+// gn_act.h — activations and their slopes in the fewest instructions, for the epilogues of bf16 products (gn_linear_act_core.h; the
+// passes behind fp32 ones, gn_linear_act.hip, have forms of their own).
 #pragma once
 
 #include <type_traits>

@@ -7,13 +7,13 @@
 // bf16 products run on the streamed tiles (gn_gemm_stream_core.h) or, where those would leave compute units
 // idle, on the small ones (gn_gemm_wave_core.h), with the epilogues of gn_linear_act_core.h: the sums stay in fp32 until Y, P or dP
 // is rounded once.  Sizes and addresses that the products' 16-byte pieces do not take are laid out first in the
-// workspace.  fp32 products are gn_linear_fwd's and gn_gemm's, with a pass behind them where there is an
+// workspace.  fp32 products are gn_linear_fwd's and gn_linear_bwd_ws's, with a pass behind them where there is an
 // activation or a residual.
 //
 // Measured (us, bf16; in brackets the library's products alone, without bias, activation, residual or stored P):
 //   4096 x 5632 x 2048 with bias, gelu and P   107 (89)   0.88 PFLOP/s
 //   4001 x 2048 x 5632, bias, fp32 residual     95 (81)   0.97
-//   backward of 4096 x 2048 x 5632, gelu, db   212 (99 + 110)   0.89 over both products
+//   backward of 4096 x 2048 x 5632, gelu, db   209 (99 + 110)   0.90 over both products
 //   8 x 5632 x 2048 with bias and silu         8.3, 7.3 of it the kernel: 3.2 TB/s of W
 // The matrix cores bound the large ones; beside them stand the epilogue's reads of R or P and its stores, which a tile's compute waves do
 // themselves with the matrix pipe idle, and dW's 176 tiles of 256 x 256 on 256 CUs.  A few rows are bound by the latency of

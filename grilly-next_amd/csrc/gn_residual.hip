@@ -17,12 +17,14 @@
 // LDS, and leave as one partial row a block, which a second launch adds in a fixed order: no atomics.
 // Wider rows are read three times or more (kernels at the end).
 //
-// Measured (us; a large copy reaches 4.8 TB/s on the card, reads alone 6.0): dropout of 8192 x 5632 bf16 34.9, 5.3 TB/s; forward
-// 8192 x 768, RMS norm, dropout, LayerNorm, fp32 stream 14.0, 5.4 TB/s, and 16001 x 4096 bf16, two RMS norms and a gate 96, 5.5;
-// backward of the first 24.8, 4.6, of the second 178, 4.4: 4 us of either are the second launch, and what the loads ahead do
-// not cover of two or three dependent sums a row is the rest.  Rows that vectors do not divide hold an element's mask word
-// each, not eight elements' four: 2107 x 1027 fp32 backward 33, 1.6 TB/s, bound by vector instructions.  A token's
-// row costs its launch: 3.7 of 9.4 with the call.
+// Measured (us; a large copy reaches 5.1 to 5.2 TB/s on the card, reads alone 6.0): dropout of 8192 x 5632 bf16 34.9, 5.3 TB/s; forward
+// 8192 x 768, dropout, LayerNorm before the next block, fp32 stream 14.0, 5.4 TB/s, and 16001 x 4096 bf16, two RMS norms and a gate 96, 5.5;
+// backward of the first, which without a norm after the block or a gate does not read h, 25.2, 4.0 TB/s, of the second 178, 4.4: 4 us of
+// either are the second launch, and what the loads ahead do not cover of two or three dependent sums a row is the rest (with an
+// RMS norm after the block the first takes 15.9 and 35.6).  Rows that vectors do not divide hold an element's mask word each, not
+// eight elements' four: 2107 x 1027 fp32 backward 33, 1.6 TB/s; its waves, two a SIMD, compute 28 % of their time and wait for loads
+// and the sums' barriers 44 %.  A token's row costs its launch: 3.7 of 9.4 with the call.  Past 8192 elements the passes are far from HBM's
+// rate: 4096 x 12288 bf16 with two RMS norms 342 forward, 908 backward (4096 x 8192: 51, 99).
 #include <algorithm>
 #include <type_traits>
 

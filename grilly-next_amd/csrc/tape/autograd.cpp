@@ -451,7 +451,7 @@ void BackwardEngine::linear_grads(Node* n, const void* dY, uint64_t W, uint64_t 
         // x = act(P) feeds only this node: the gradient in front of the activation comes out of the
         // input-gradient product for the LinearAct node visited next (dX never formed)
         uint64_t dP = alloc_grad(x.size_bytes());
-        // operands are laid out only where 16-byte pieces do not take them
+        // operands are laid out only where 16-byte pieces do not take them (131 MB at 8192 x 768 x 5632)
         const bool lay = dt == GN_BF16 && (N % 8 || K % 8 || ((reinterpret_cast<uint64_t>(dY) | x.buffer_id | W | dW) & 15u));
         const size_t wsb = gn_linear_workspace_bytes(M, N, K, dt) + (lay ? gn_linear_act_workspace_bytes(M, N, K, dt) : 0);
         const uint64_t ws = split_ws(wsb);
