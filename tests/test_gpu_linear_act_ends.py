@@ -151,3 +151,40 @@ def test_odd_weight_gradients_over_ranges_of_rows(gn, M, N, K):
     dY, P, W = rand(1, M, N, std=0.01), rand(2, M, K), rand(3, N, K, std=0.05)
     first, second = (gn.act_linear_bwd("relu", dY, P, P, W) for _ in range(2))
     assert all(torch.equal(a, b) for a, b in zip(first, second))
+
+
+@pytest.mark.parametrize("shift", [1, 2])
+@pytest.mark.parametrize("M,N,K", [(5, 64, 256), (64, 36, 100), (128, 512, 1024), (900, 264, 136)])
+def test_fp32_backward_of_unaligned_views(gn, M, N, K, shift):
+    check_bwd(gn, M, N, K, "gelu_tanh", F32, shift=shift)
+    check_bwd(gn, M, N, K, "tanh", F32, shift=shift, accumulate=True)
+
+
+@pytest.mark.parametrize("M,N,K", [(8, 1000, 512), (64, 10, 256), (128, 4096, 1024), (700, 513, 519)])
+def test_fp32_two_at_once_and_replays(gn, M, N, K):
+    dY, P, W = rand(1, M, N, dtype=F32, std=0.01), rand(2, M, K, dtype=F32), rand(3, N, K, dtype=F32, std=0.05)
+    A = act64(P.double(), "silu").float()
+
+    def call():
+        return (gn.linear_act_fwd(P, W, act="gelu_erf"),) + gn.act_linear_bwd("silu", dY, P, A, W)
+
+    ref = call()
+    torch.cuda.synchronize()
+    got = []
+    for s in (torch.cuda.Stream(), torch.cuda.Stream()):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, ref))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    for k in range(4):
+        dY.copy_(rand(20 + k, M, N, dtype=F32, std=0.01))
+        P.copy_(rand(30 + k, M, K, dtype=F32))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), k
